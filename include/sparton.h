@@ -291,6 +291,93 @@ int sparton_loss_bwd_terms(const void* q, const void* d, const float* probs,
                            int dtype, void* stream);
 
 /*
+ * Attention of a backbone layer. No counterpart in the reference, whose backbones run torch's
+ * (training/model.py:88-139); the operator in front of the transform above.
+ *     s_ij = scale q_i . k_j;  p_ij = softmax over the keys j that row i may look at;  o_i = sum_j p_ij v_j
+ * q and o are [B, Hq, Sq, D], k and v [B, Hk, Sk, D]; query head h reads key head h / (Hq / Hk).
+ * A key takes part where mask[b, j] is nonzero (mask may be NULL: every key) and, with `causal`,
+ * where j <= i + Sk - Sq. A row without keys gives zeros, and zero gradients. Values of keys that
+ * take no part reach no output, whatever they are. Sums, maxima and log sums are fp32.
+ * Strides are in elements; the innermost is 1. Bases are 16-byte aligned, and so are the strides
+ * (multiples of 8 elements, 4 for fp32) of dimensions larger than 1. D * element size is a multiple
+ * of 16 bytes and D <= 128; 0 < scale < infinity. Sizes whose rows or workgroups pass 32 bits are
+ * SPARTON_EUNSUPPORTED; offsets are 64-bit.
+ */
+typedef struct sparton_attention_desc {
+  int64_t B, Hq, Hk, Sq, Sk, D;
+  int64_t q[3], k[3], v[3], o[3];           /* strides of batch, head and row */
+  int64_t d_o[3], d_q[3], d_k[3], d_v[3];   /* the same of the gradients (backward only) */
+  int64_t mask_batch;                       /* batch stride of the mask [B, Sk] */
+  float scale;
+  int causal;                               /* 0 or 1 */
+  int dtype;                                /* enum sparton_dtype */
+  int mask_dtype;                           /* SPARTON_MASK_I64, _I32 or _U8 */
+} sparton_attention_desc;
+
+/* Bytes of device scratch sparton_attention_fwd needs (partial outputs where few rows look at many
+ * keys, which are then split; 0 otherwise), and sparton_attention_bwd (do . o of each row). */
+size_t sparton_attention_workspace_bytes(const sparton_attention_desc* desc);
+size_t sparton_attention_bwd_workspace_bytes(const sparton_attention_desc* desc);
+
+/* Forward: out, and lse [B, Hq, Sq] (fp32, the base-2 logarithm of each row's sum of exponentials;
+ * may be NULL if no backward follows). */
+int sparton_attention_fwd(const sparton_attention_desc* desc, const void* q, const void* k,
+                          const void* v, const void* mask, void* out, float* lse, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Backward: d_q, d_k and d_v (every element is written) from d_out and the forward's inputs, out and
+ * lse; the probabilities are recomputed. Deterministic: no atomics, every sum in a fixed order. */
+int sparton_attention_bwd(const sparton_attention_desc* desc, const void* q, const void* k,
+                          const void* v, const void* mask, const void* out, const float* lse,
+                          const void* d_out, void* d_q, void* d_k, void* d_v, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
+ * LayerNorm of a backbone's rows with the residual sum in front, y = LayerNorm(x + residual) weight + bias
+ * over rows of D elements (1 <= D <= 16384; any alignment of whole elements). No counterpart in the
+ * reference, whose backbones run torch's. `dtype` is the type of x, residual, y and their gradients,
+ * `vec_dtype` that of weight, bias and theirs: SPARTON_F32 or `dtype`. residual and bias may be NULL.
+ * The sum x + residual is formed in fp32 and not rounded.
+ */
+size_t sparton_layer_norm_workspace_bytes(int64_t M, int64_t D); /* of the backward: column partial sums */
+
+/* Forward: y, and each row's mean and 1/sqrt(var + eps) (fp32 [M]; both or neither may be NULL). */
+int sparton_layer_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias,
+                           int vec_dtype, float eps, void* y, float* mean, float* rstd, int64_t M,
+                           int64_t D, int dtype, void* stream);
+
+/* Backward: dx (the gradient of x and of residual alike), and the sums over rows d_weight and d_bias
+ * (each may be NULL), added in fp32 and rounded once. Deterministic. */
+int sparton_layer_norm_bwd(const void* dy, const void* x, const void* residual, const void* weight,
+                           int vec_dtype, const float* mean, const float* rstd, void* dx, void* d_weight,
+                           void* d_bias, void* workspace, size_t workspace_bytes, int64_t M, int64_t D,
+                           int dtype, void* stream);
+
+/*
+ * Preference loss on pairs: for each of B rows a query's reps q, a preferred document's pos and a
+ * rejected one's neg, [B, V] row-major of any alignment of whole elements. A retriever gives a document
+ * the probability softmax over scores q.d / temperature, so a pair's log ratio is its score margin:
+ *     m = (q.pos - q.neg) / temperature;   z = beta (m - ref_margin)
+ *     loss = mean over rows of -(1 - smoothing) log sigma(z) - smoothing log sigma(-z)
+ * ref_margin [B] (fp32; NULL: zeros) holds the reference model's margins. temperature and beta are
+ * positive and finite, 0 <= smoothing <= 0.5. Sums are fp32, deterministic. No counterpart in the
+ * reference, which trains on the in-batch loss above alone (training/train.py:164-197).
+ */
+size_t sparton_preference_workspace_bytes(int64_t B, int64_t V, int dtype);
+
+/* margin [B], and with loss (one fp32) coef [B], d loss / d(q.pos) of each row, for the backward; loss
+ * and coef may both be NULL (a reference model's margins). */
+int sparton_preference_fwd(const void* q, const void* pos, const void* neg, const float* ref_margin,
+                           int64_t B, int64_t V, float temperature, float beta, float smoothing,
+                           float* loss, float* margin, float* coef, void* workspace,
+                           size_t workspace_bytes, int dtype, void* stream);
+
+/* The reps' gradients from the device scalar grad_loss. */
+int sparton_preference_bwd(const void* q, const void* pos, const void* neg, const float* coef,
+                           const float* grad_loss, int64_t B, int64_t V, void* d_q, void* d_pos,
+                           void* d_neg, int dtype, void* stream);
+
+/*
  * Measurement probe, no counterpart in the reference: `grid` workgroups (one per CU) of 4
  * waves each run `iters` rounds of 16 independent v_mfma_f32_32x32x16_{bf16,f16} on random
  * register operands (dtype SPARTON_BF16 or SPARTON_F16). clk[2*w] receives workgroup w's

@@ -61,6 +61,16 @@ EXPORTED_SYMBOLS = (
     "sparton_loss_bwd",
     "sparton_loss_bwd_terms",
     "sparton_loss_workspace_bytes",
+    "sparton_attention_fwd",
+    "sparton_attention_bwd",
+    "sparton_attention_workspace_bytes",
+    "sparton_attention_bwd_workspace_bytes",
+    "sparton_layer_norm_fwd",
+    "sparton_layer_norm_bwd",
+    "sparton_layer_norm_workspace_bytes",
+    "sparton_preference_fwd",
+    "sparton_preference_bwd",
+    "sparton_preference_workspace_bytes",
     "sparton_mfma_probe",
     "sparton_strerror",
     "sparton_limits",
@@ -72,6 +82,14 @@ _lib = None
 
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
+
+
+class AttentionDesc(ctypes.Structure):
+    """struct sparton_attention_desc (include/sparton.h)."""
+    _fields_ = ([(n, _i64) for n in ("B", "Hq", "Hk", "Sq", "Sk", "D")]
+                + [(n, _i64 * 3) for n in ("q", "k", "v", "o", "d_o", "d_q", "d_k", "d_v")]
+                + [("mask_batch", _i64), ("scale", ctypes.c_float), ("causal", ctypes.c_int),
+                   ("dtype", ctypes.c_int), ("mask_dtype", ctypes.c_int)])
 
 
 def lib_path() -> str:
@@ -138,6 +156,29 @@ def load() -> ctypes.CDLL:
                                              ctypes.c_float, ctypes.c_float, ctypes.c_float, _vp, _vp,
                                              ctypes.c_int, _vp]
         L.sparton_loss_bwd_terms.restype = ctypes.c_int
+        desc = ctypes.POINTER(AttentionDesc)
+        L.sparton_attention_fwd.argtypes = [desc] + [_vp] * 7 + [ctypes.c_size_t, _vp]
+        L.sparton_attention_fwd.restype = ctypes.c_int
+        L.sparton_attention_bwd.argtypes = [desc] + [_vp] * 11 + [ctypes.c_size_t, _vp]
+        L.sparton_attention_bwd.restype = ctypes.c_int
+        for size in (L.sparton_attention_workspace_bytes, L.sparton_attention_bwd_workspace_bytes):
+            size.argtypes = [desc]
+            size.restype = ctypes.c_size_t
+        L.sparton_layer_norm_fwd.argtypes = [_vp] * 4 + [ctypes.c_int, ctypes.c_float, _vp, _vp, _vp, _i64, _i64,
+                                                          ctypes.c_int, _vp]
+        L.sparton_layer_norm_fwd.restype = ctypes.c_int
+        L.sparton_layer_norm_bwd.argtypes = ([_vp] * 4 + [ctypes.c_int] + [_vp] * 6
+                                             + [ctypes.c_size_t, _i64, _i64, ctypes.c_int, _vp])
+        L.sparton_layer_norm_bwd.restype = ctypes.c_int
+        L.sparton_layer_norm_workspace_bytes.argtypes = [_i64, _i64]
+        L.sparton_layer_norm_workspace_bytes.restype = ctypes.c_size_t
+        L.sparton_preference_fwd.argtypes = ([_vp] * 4 + [_i64, _i64] + [ctypes.c_float] * 3 + [_vp] * 4
+                                             + [ctypes.c_size_t, ctypes.c_int, _vp])
+        L.sparton_preference_fwd.restype = ctypes.c_int
+        L.sparton_preference_bwd.argtypes = [_vp] * 5 + [_i64, _i64] + [_vp] * 3 + [ctypes.c_int, _vp]
+        L.sparton_preference_bwd.restype = ctypes.c_int
+        L.sparton_preference_workspace_bytes.argtypes = [_i64, _i64, ctypes.c_int]
+        L.sparton_preference_workspace_bytes.restype = ctypes.c_size_t
         L.sparton_mfma_probe.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]
         L.sparton_mfma_probe.restype = ctypes.c_int
         L.sparton_strerror.argtypes = [ctypes.c_int]

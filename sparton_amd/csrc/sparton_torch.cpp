@@ -19,6 +19,11 @@
 //       LayerNorm(gelu(x W^T + b)) (training/model.py:14-40)
 //   sparton_eager::splade_loss(q, d?, temperature, w_ce, w_l1, w_flops) -> out[6]
 //       (total, CE, L1 q, L1 d, FLOPS q, FLOPS d)  (training/train.py:73-94, :164-197)
+//   sparton_eager::attention(q, k, v, mask?, causal, scale) -> out   (a backbone layer's attention)
+//   sparton_eager::layer_norm(x, residual?, weight, bias?, eps) -> y   LayerNorm(x + residual)
+//   sparton_eager::preference_loss(q, pos, neg, ref_margin?, temperature, beta, smoothing) -> (loss, margin)
+//   sparton_eager::{attention,layer_norm,preference}_{fwd,bwd}: their halves, which the torch.library
+//       ops call; preference_margin: the margins alone
 //
 // The Python callers validate shapes and dtypes first (the same checks, and error types, as
 // the torch.library ops); here only what the C ABI needs is enforced.
@@ -613,6 +618,315 @@ Loss6 loss_cuda(const Tensor& q, const c10::optional<Tensor>& d, double T, doubl
   return split6(std::get<0>(loss_fwd(q.contiguous(), dd, T, w_ce, w_l1, w_flops)));
 }
 
+// ---- attention ----------------------------------------------------------------------------
+
+// [B, H, S, D] with unit inner stride and rows that start on 16 bytes, as the C ABI reads it: the
+// tensor itself where it is so (a view of a projection's output, or of a cache), else a copy. A head
+// size that is not a multiple of 16 bytes is padded with zero columns, which change no product.
+Tensor attention_rows(const Tensor& t) {
+  const int64_t unit = 16 / t.element_size(), pad = (unit - t.size(3) % unit) % unit;
+  if (pad > 0) return at::constant_pad_nd(t, {0, pad});
+  bool ok = t.stride(3) == 1 || t.size(3) == 1;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) % unit == 0 && t.stride(i) >= 0));
+  Tensor c = ok ? t : t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 != 0 ? c.clone(at::MemoryFormat::Contiguous) : c;
+}
+
+// [B, S, H, D] in memory, as the projection behind it reads it, seen as [B, H, S, D].
+Tensor attention_like(const Tensor& t) {
+  return at::empty({t.size(0), t.size(2), t.size(1), t.size(3)}, t.options()).transpose(1, 2);
+}
+
+void set_strides(int64_t* to, const Tensor& t) {
+  for (int i = 0; i < 3; ++i) to[i] = t.stride(i);
+}
+
+sparton_attention_desc attention_desc(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask,
+                                      const Tensor& out, bool causal, double scale) {
+  sparton_attention_desc d;
+  std::memset(&d, 0, sizeof(d));
+  d.B = q.size(0);
+  d.Hq = q.size(1);
+  d.Hk = k.size(1);
+  d.Sq = q.size(2);
+  d.Sk = k.size(2);
+  d.D = q.size(3);
+  set_strides(d.q, q);
+  set_strides(d.k, k);
+  set_strides(d.v, v);
+  set_strides(d.o, out);
+  d.scale = (float)scale;
+  d.causal = causal;
+  d.dtype = dtype_code(q.scalar_type());
+  if (mask.defined()) {
+    d.mask_batch = mask.stride(0);
+    d.mask_dtype = mask_code(mask.scalar_type());
+  }
+  return d;
+}
+
+// The mask [B, Sk] with unit inner stride (a row may be shared: stride 0 of an expanded batch).
+Tensor attention_mask(const c10::optional<Tensor>& m) {
+  if (!m.has_value()) return Tensor();
+  return m->size(1) <= 1 || m->stride(1) == 1 ? *m : m->contiguous();
+}
+
+// out on the rows as they are (padded head size), and the rows' log sums if asked for.
+std::tuple<Tensor, Tensor> attention_run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask,
+                                         bool causal, double scale, bool with_lse) {
+  Tensor out = attention_like(q);
+  Tensor lse = with_lse ? at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat)) : Tensor();
+  const sparton_attention_desc d = attention_desc(q, k, v, mask, out, causal, scale);
+  const size_t ws_bytes = sparton_attention_workspace_bytes(&d);
+  Tensor ws = workspace(ws_bytes, q);
+  check(sparton_attention_fwd(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(mask), out.data_ptr(),
+                              with_lse ? lse.data_ptr<float>() : nullptr, ws.data_ptr(), ws_bytes, stream_of(q)),
+        "sparton_attention_fwd");
+  return {out, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> attention_grads(const Tensor& dout, const Tensor& q, const Tensor& k,
+                                                   const Tensor& v, const Tensor& mask, const Tensor& out,
+                                                   const Tensor& lse, bool causal, double scale) {
+  Tensor go = attention_rows(dout.to(q.scalar_type()));
+  Tensor dq = attention_like(q), dk = attention_like(k), dv = attention_like(v);
+  sparton_attention_desc d = attention_desc(q, k, v, mask, out, causal, scale);
+  set_strides(d.d_o, go);
+  set_strides(d.d_q, dq);
+  set_strides(d.d_k, dk);
+  set_strides(d.d_v, dv);
+  const size_t ws_bytes = sparton_attention_bwd_workspace_bytes(&d);
+  Tensor ws = workspace(ws_bytes, q);
+  check(sparton_attention_bwd(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(mask), out.data_ptr(),
+                              lse.data_ptr<float>(), go.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                              ws.data_ptr(), ws_bytes, stream_of(q)),
+        "sparton_attention_bwd");
+  return {dq, dk, dv};
+}
+
+Tensor head_cols(const Tensor& t, int64_t D) { return t.size(3) == D ? t : t.narrow(3, 0, D); }
+
+// The pair that the torch.library ops run on (sparton::attention_fwd / _bwd).
+std::tuple<Tensor, Tensor> attention_fwd_cuda(const Tensor& q, const Tensor& k, const Tensor& v,
+                                              const c10::optional<Tensor>& mask, bool causal, double scale) {
+  c10::OptionalDeviceGuard guard(q.device());
+  auto [out, lse] = attention_run(attention_rows(q), attention_rows(k), attention_rows(v), attention_mask(mask),
+                                  causal, scale, true);
+  return {head_cols(out, q.size(3)), lse};
+}
+std::tuple<Tensor, Tensor, Tensor> attention_bwd_cuda(const Tensor& dout, const Tensor& q, const Tensor& k,
+                                                      const Tensor& v, const c10::optional<Tensor>& mask,
+                                                      const Tensor& out, const Tensor& lse, bool causal,
+                                                      double scale) {
+  c10::OptionalDeviceGuard guard(q.device());
+  auto [dq, dk, dv] = attention_grads(dout, attention_rows(q), attention_rows(k), attention_rows(v),
+                                      attention_mask(mask), attention_rows(out), lse, causal, scale);
+  const int64_t D = q.size(3);
+  return {head_cols(dq, D), head_cols(dk, D), head_cols(dv, D)};
+}
+
+struct AttentionFn : public torch::autograd::Function<AttentionFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+                        const Tensor& mask_in, bool has_mask, bool causal, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::OptionalDeviceGuard guard(q_in.device());
+    Tensor q = attention_rows(q_in), k = attention_rows(k_in), v = attention_rows(v_in);
+    Tensor mask = has_mask ? attention_mask(mask_in) : Tensor();
+    auto [out, lse] = attention_run(q, k, v, mask, causal, scale, true);
+    ctx->save_for_backward({q, k, v, mask, out, lse});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["D"] = q_in.size(3);
+    return head_cols(out, q_in.size(3));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return variable_list(7);
+    auto s = ctx->get_saved_variables();
+    c10::OptionalDeviceGuard guard(s[0].device());
+    auto [dq, dk, dv] = attention_grads(grads[0], s[0], s[1], s[2], s[3], s[4], s[5],
+                                        ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+    const int64_t D = ctx->saved_data["D"].toInt();
+    return {head_cols(dq, D), head_cols(dk, D), head_cols(dv, D), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& mask,
+                          bool causal, double scale) {
+  return AttentionFn::apply(q, k, v, present(mask, q), mask.has_value(), causal, scale);
+}
+Tensor attention_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& mask,
+                      bool causal, double scale) {
+  c10::OptionalDeviceGuard guard(q.device());
+  return head_cols(std::get<0>(attention_run(attention_rows(q), attention_rows(k), attention_rows(v),
+                                             attention_mask(mask), causal, scale, false)),
+                   q.size(3));
+}
+
+// ---- LayerNorm ----------------------------------------------------------------------------
+
+struct NormOut {
+  Tensor y, mean, rstd;
+};
+
+NormOut norm_run(const Tensor& x, const Tensor& r, const Tensor& w, const Tensor& b, double eps, bool with_stats) {
+  const int64_t D = x.size(-1), M = D == 0 ? 0 : x.numel() / D;
+  NormOut o;
+  o.y = at::empty(x.sizes(), x.options());
+  if (with_stats) {
+    o.mean = at::empty({M}, x.options().dtype(at::kFloat));
+    o.rstd = at::empty_like(o.mean);
+  }
+  check(sparton_layer_norm_fwd(x.data_ptr(), ptr(r), w.data_ptr(), ptr(b), dtype_code(w.scalar_type()), (float)eps,
+                               o.y.data_ptr(), with_stats ? o.mean.data_ptr<float>() : nullptr,
+                               with_stats ? o.rstd.data_ptr<float>() : nullptr, M, D, dtype_code(x.scalar_type()),
+                               stream_of(x)),
+        "sparton_layer_norm_fwd");
+  return o;
+}
+
+std::tuple<Tensor, Tensor, Tensor> norm_grads(const Tensor& dy_in, const Tensor& x, const Tensor& r, const Tensor& w,
+                                              bool has_bias, const Tensor& mean, const Tensor& rstd) {
+  const int64_t D = x.size(-1), M = mean.size(0);
+  Tensor dy = dy_in.to(x.scalar_type()).contiguous();
+  Tensor dx = at::empty(x.sizes(), x.options());
+  Tensor dw = at::empty({D}, w.options());
+  Tensor db = at::empty({has_bias ? D : 0}, w.options());
+  const size_t ws_bytes = sparton_layer_norm_workspace_bytes(M, D);
+  Tensor ws = workspace(ws_bytes, x);
+  check(sparton_layer_norm_bwd(dy.data_ptr(), x.data_ptr(), ptr(r), w.data_ptr(), dtype_code(w.scalar_type()),
+                               mean.data_ptr<float>(), rstd.data_ptr<float>(), dx.data_ptr(), dw.data_ptr(),
+                               has_bias ? db.data_ptr() : nullptr, ws.data_ptr(), ws_bytes, M, D,
+                               dtype_code(x.scalar_type()), stream_of(x)),
+        "sparton_layer_norm_bwd");
+  return {dx, dw, db};
+}
+
+Tensor whole(const c10::optional<Tensor>& t) { return t.has_value() ? t->contiguous() : Tensor(); }
+
+std::tuple<Tensor, Tensor, Tensor> norm_fwd_cuda(const Tensor& x, const c10::optional<Tensor>& r, const Tensor& w,
+                                                 const c10::optional<Tensor>& b, double eps) {
+  c10::OptionalDeviceGuard guard(x.device());
+  NormOut o = norm_run(x.contiguous(), whole(r), w.contiguous(), whole(b), eps, true);
+  return {o.y, o.mean, o.rstd};
+}
+std::tuple<Tensor, Tensor, Tensor> norm_bwd_cuda(const Tensor& dy, const Tensor& x, const c10::optional<Tensor>& r,
+                                                 const Tensor& w, bool has_bias, const Tensor& mean,
+                                                 const Tensor& rstd) {
+  c10::OptionalDeviceGuard guard(x.device());
+  return norm_grads(dy, x.contiguous(), whole(r), w.contiguous(), has_bias, mean, rstd);
+}
+
+struct NormFn : public torch::autograd::Function<NormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& r_in, const Tensor& w_in,
+                        const Tensor& b_in, bool has_r, bool has_b, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::OptionalDeviceGuard guard(x_in.device());
+    Tensor x = x_in.contiguous(), r = has_r ? r_in.contiguous() : Tensor(), w = w_in.contiguous();
+    NormOut o = norm_run(x, r, w, has_b ? b_in.contiguous() : Tensor(), eps, true);
+    ctx->save_for_backward({x, r, w, o.mean, o.rstd});
+    ctx->saved_data["has_b"] = has_b;
+    return o.y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return variable_list(7);
+    auto s = ctx->get_saved_variables();
+    c10::OptionalDeviceGuard guard(s[0].device());
+    const bool has_b = ctx->saved_data["has_b"].toBool();
+    auto [dx, dw, db] = norm_grads(grads[0], s[0], s[1], s[2], has_b, s[3], s[4]);
+    return {dx, s[1].defined() ? dx : Tensor(), dw, has_b ? db : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor norm_autograd(const Tensor& x, const c10::optional<Tensor>& r, const Tensor& w, const c10::optional<Tensor>& b,
+                     double eps) {
+  return NormFn::apply(x, present(r, x), w, present(b, w), r.has_value(), b.has_value(), eps);
+}
+Tensor norm_cuda(const Tensor& x, const c10::optional<Tensor>& r, const Tensor& w, const c10::optional<Tensor>& b,
+                 double eps) {
+  c10::OptionalDeviceGuard guard(x.device());
+  return norm_run(x.contiguous(), whole(r), w.contiguous(), whole(b), eps, false).y;
+}
+
+// ---- the preference loss -------------------------------------------------------------------
+
+// loss (undefined without `with_loss`), margin [B] and the backward's coefficients [B].
+std::tuple<Tensor, Tensor, Tensor> preference_run(const Tensor& q, const Tensor& p, const Tensor& n, const Tensor& ref,
+                                                  double T, double beta, double smoothing, bool with_loss) {
+  const int64_t B = q.size(0), V = q.size(1);
+  const auto f32 = q.options().dtype(at::kFloat);
+  Tensor margin = at::empty({B}, f32);
+  Tensor loss = with_loss ? at::empty({}, f32) : Tensor(), coef = with_loss ? at::empty({B}, f32) : Tensor();
+  const int dt = dtype_code(q.scalar_type());
+  const size_t ws_bytes = sparton_preference_workspace_bytes(B, V, dt);
+  Tensor ws = workspace(ws_bytes, q);
+  check(sparton_preference_fwd(q.data_ptr(), p.data_ptr(), n.data_ptr(), ref.defined() ? ref.data_ptr<float>() : nullptr,
+                               B, V, (float)T, (float)beta, (float)smoothing,
+                               with_loss ? loss.data_ptr<float>() : nullptr, margin.data_ptr<float>(),
+                               with_loss ? coef.data_ptr<float>() : nullptr, ws.data_ptr(), ws_bytes, dt, stream_of(q)),
+        "sparton_preference_fwd");
+  return {loss, margin, coef};
+}
+
+std::tuple<Tensor, Tensor, Tensor> preference_grads(const Tensor& grad, const Tensor& q, const Tensor& p,
+                                                    const Tensor& n, const Tensor& coef) {
+  Tensor g = grad.to(at::kFloat).contiguous();
+  Tensor dq = at::empty(q.sizes(), q.options()), dp = at::empty_like(dq), dn = at::empty_like(dq);
+  check(sparton_preference_bwd(q.data_ptr(), p.data_ptr(), n.data_ptr(), coef.data_ptr<float>(), g.data_ptr<float>(),
+                               q.size(0), q.size(1), dq.data_ptr(), dp.data_ptr(), dn.data_ptr(),
+                               dtype_code(q.scalar_type()), stream_of(q)),
+        "sparton_preference_bwd");
+  return {dq, dp, dn};
+}
+
+std::tuple<Tensor, Tensor, Tensor> preference_fwd_cuda(const Tensor& q, const Tensor& p, const Tensor& n,
+                                                       const c10::optional<Tensor>& ref, double T, double beta,
+                                                       double smoothing) {
+  c10::OptionalDeviceGuard guard(q.device());
+  return preference_run(q.contiguous(), p.contiguous(), n.contiguous(), whole(ref), T, beta, smoothing, true);
+}
+std::tuple<Tensor, Tensor, Tensor> preference_bwd_cuda(const Tensor& grad, const Tensor& q, const Tensor& p,
+                                                       const Tensor& n, const Tensor& coef) {
+  c10::OptionalDeviceGuard guard(q.device());
+  return preference_grads(grad, q.contiguous(), p.contiguous(), n.contiguous(), coef);
+}
+Tensor preference_margin_cuda(const Tensor& q, const Tensor& p, const Tensor& n, double T) {
+  c10::OptionalDeviceGuard guard(q.device());
+  return std::get<1>(preference_run(q.contiguous(), p.contiguous(), n.contiguous(), Tensor(), T, 1.0, 0.0, false));
+}
+
+struct PreferenceFn : public torch::autograd::Function<PreferenceFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& p_in, const Tensor& n_in,
+                               const Tensor& ref, bool has_ref, double T, double beta, double smoothing) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::OptionalDeviceGuard guard(q_in.device());
+    Tensor q = q_in.contiguous(), p = p_in.contiguous(), n = n_in.contiguous();
+    auto [loss, margin, coef] = preference_run(q, p, n, has_ref ? ref.contiguous() : Tensor(), T, beta, smoothing, true);
+    ctx->save_for_backward({q, p, n, coef});
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({margin});
+    return {loss, margin};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return variable_list(8);
+    auto s = ctx->get_saved_variables();
+    c10::OptionalDeviceGuard guard(s[0].device());
+    auto [dq, dp, dn] = preference_grads(grads[0], s[0], s[1], s[2], s[3]);
+    return {dq, dp, dn, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> preference_autograd(const Tensor& q, const Tensor& p, const Tensor& n,
+                                               const c10::optional<Tensor>& ref, double T, double beta,
+                                               double smoothing) {
+  auto o = PreferenceFn::apply(q, p, n, present(ref, q), ref.has_value(), T, beta, smoothing);
+  return {o[0], o[1]};
+}
+std::tuple<Tensor, Tensor> preference_cuda(const Tensor& q, const Tensor& p, const Tensor& n,
+                                           const c10::optional<Tensor>& ref, double T, double beta, double smoothing) {
+  auto [loss, margin, coef] = preference_fwd_cuda(q, p, n, ref, T, beta, smoothing);
+  return {loss, margin};
+}
+
 // CPU tensors: the same refusal as the reference's `assert hidden.is_cuda`
 // (sparton_kernel.py:650), as a RuntimeError.
 [[noreturn]] void cpu_refused(const char* op) {
@@ -632,6 +946,21 @@ TORCH_LIBRARY(sparton_eager, m) {
         "Tensor ln_bias, float eps) -> Tensor");
   m.def("splade_loss(Tensor q, Tensor? d, float temperature, float w_ce, float w_l1, "
         "float w_flops) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? mask, bool causal, float scale) -> Tensor");
+  m.def("attention_fwd(Tensor q, Tensor k, Tensor v, Tensor? mask, bool causal, float scale) -> (Tensor, Tensor)");
+  m.def("attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor? mask, Tensor out, Tensor lse, "
+        "bool causal, float scale) -> (Tensor, Tensor, Tensor)");
+  m.def("layer_norm(Tensor x, Tensor? residual, Tensor weight, Tensor? bias, float eps) -> Tensor");
+  m.def("layer_norm_fwd(Tensor x, Tensor? residual, Tensor weight, Tensor? bias, float eps) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("layer_norm_bwd(Tensor dy, Tensor x, Tensor? residual, Tensor weight, bool has_bias, Tensor mean, "
+        "Tensor rstd) -> (Tensor, Tensor, Tensor)");
+  m.def("preference_loss(Tensor q, Tensor pos, Tensor neg, Tensor? ref_margin, float temperature, float beta, "
+        "float smoothing) -> (Tensor, Tensor)");
+  m.def("preference_fwd(Tensor q, Tensor pos, Tensor neg, Tensor? ref_margin, float temperature, float beta, "
+        "float smoothing) -> (Tensor, Tensor, Tensor)");
+  m.def("preference_bwd(Tensor grad, Tensor q, Tensor pos, Tensor neg, Tensor coef) -> (Tensor, Tensor, Tensor)");
+  m.def("preference_margin(Tensor q, Tensor pos, Tensor neg, float temperature) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(sparton_eager, CUDA, m) {
@@ -641,6 +970,16 @@ TORCH_LIBRARY_IMPL(sparton_eager, CUDA, m) {
   m.impl("mlm_transform", &transform_cuda);
   m.impl("mlm_transform_typed", &transform_typed_cuda);
   m.impl("splade_loss", &loss_cuda);
+  m.impl("attention", &attention_cuda);
+  m.impl("attention_fwd", &attention_fwd_cuda);
+  m.impl("attention_bwd", &attention_bwd_cuda);
+  m.impl("layer_norm", &norm_cuda);
+  m.impl("layer_norm_fwd", &norm_fwd_cuda);
+  m.impl("layer_norm_bwd", &norm_bwd_cuda);
+  m.impl("preference_loss", &preference_cuda);
+  m.impl("preference_fwd", &preference_fwd_cuda);
+  m.impl("preference_bwd", &preference_bwd_cuda);
+  m.impl("preference_margin", &preference_margin_cuda);
 }
 
 TORCH_LIBRARY_IMPL(sparton_eager, AutogradCUDA, m) {
@@ -649,6 +988,9 @@ TORCH_LIBRARY_IMPL(sparton_eager, AutogradCUDA, m) {
   m.impl("mlm_transform", &transform_autograd);
   m.impl("mlm_transform_typed", &transform_typed_autograd);
   m.impl("splade_loss", &loss_autograd);
+  m.impl("attention", &attention_autograd);
+  m.impl("layer_norm", &norm_autograd);
+  m.impl("preference_loss", &preference_autograd);
 }
 
 TORCH_LIBRARY_IMPL(sparton_eager, CPU, m) {
@@ -667,4 +1009,10 @@ TORCH_LIBRARY_IMPL(sparton_eager, CPU, m) {
                                    double) -> Tensor { cpu_refused("sparton_eager::mlm_transform_typed"); });
   m.impl("splade_loss", [](const Tensor&, const c10::optional<Tensor>&, double, double, double,
                            double) -> Loss6 { cpu_refused("sparton_eager::splade_loss"); });
+  m.impl("attention", [](const Tensor&, const Tensor&, const Tensor&, const c10::optional<Tensor>&, bool,
+                         double) -> Tensor { cpu_refused("sparton_eager::attention"); });
+  m.impl("layer_norm", [](const Tensor&, const c10::optional<Tensor>&, const Tensor&, const c10::optional<Tensor>&,
+                          double) -> Tensor { cpu_refused("sparton_eager::layer_norm"); });
+  m.impl("preference_loss", [](const Tensor&, const Tensor&, const Tensor&, const c10::optional<Tensor>&, double, double,
+                               double) -> std::tuple<Tensor, Tensor> { cpu_refused("sparton_eager::preference_loss"); });
 }

@@ -25,9 +25,17 @@ split-vocabulary score GEMM with a fixed-order sum of its partials, per-slice ro
 statistics, a row softmax, and a backward that recomputes each vocabulary slice's column sums
 and forms both gradients tile by tile (sparton_loss.hip). Limits: 1 <= Bq <= Bd when documents are given (the labels
 arange(Bq) index d's rows); the C ABI reports sizes past its int offsets as unsupported.
+
+preference_loss is the objective of a second training stage, on pairs that a frozen reference model
+scores too (the reference has none; its losses above see only positives and in-batch negatives):
+
+    sparton::preference_fwd(q, pos, neg, ref_margin?, temperature, beta, smoothing)
+        -> (loss, margin [B] fp32, coef [B] fp32)
+    sparton::preference_bwd(grad, q, pos, neg, coef) -> (dq, dpos, dneg)
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -211,3 +219,111 @@ def splade_training_loss(query_reps: Tensor, doc_reps: Tensor, step: int, temper
     return splade_loss(query_reps, doc_reps, temperature,
                        get_reg_weight(step, reg_warmup_steps, lambda_l1),
                        get_reg_weight(step, reg_warmup_steps, lambda_flops))
+
+
+class PreferenceLossOutput(NamedTuple):
+    """loss is back-propagated; margin [B] (fp32, not differentiable) is each pair's log ratio, for
+    logging, or as another model's ref_margin."""
+    loss: Tensor
+    margin: Tensor
+
+
+def _check_pairs(q: Tensor, pos: Tensor, neg: Tensor, ref: Optional[Tensor], temperature: float, beta: float,
+                 smoothing: float, op: str) -> None:
+    if q.dim() != 2 or q.dtype not in _FLOAT_DTYPES or q.shape[0] < 1 or q.shape[1] < 1:
+        raise ValueError(f"{op}: query reps must be a 2-D float tensor [B, V], B and V at least 1, got {q.dtype} "
+                         f"{tuple(q.shape)}")
+    for t, name in ((pos, "preferred"), (neg, "rejected")):
+        if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{op}: {name} document reps must be {tuple(q.shape)} {q.dtype} on {q.device}, got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    if ref is not None:
+        if tuple(ref.shape) != (q.shape[0],) or ref.dtype != torch.float32 or ref.device != q.device:
+            raise ValueError(f"{op}: ref_margin must be float32 [{q.shape[0]}] on {q.device}, got {ref.dtype} "
+                             f"{tuple(ref.shape)} on {ref.device}")
+        if ref.requires_grad:
+            raise ValueError(f"{op}: ref_margin is the frozen reference model's and gets no gradient; detach it")
+    for v, name in ((temperature, "temperature"), (beta, "beta")):
+        if not (v > 0.0 and math.isfinite(v)):
+            raise ValueError(f"{op}: {name} must be positive and finite, got {v}")
+    if not 0.0 <= smoothing <= 0.5:
+        raise ValueError(f"{op}: label_smoothing must lie in [0, 0.5], got {smoothing}")
+    if not q.is_cuda:
+        raise RuntimeError(f"{op} only supports ROCm/HIP device tensors (got device {q.device})")
+
+
+@torch.library.custom_op("sparton::preference_fwd", mutates_args=())
+def preference_fwd(q: Tensor, pos: Tensor, neg: Tensor, ref_margin: Optional[Tensor], temperature: float, beta: float,
+                   smoothing: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """(loss, margin [B], coef [B]) in fp32; coef = d loss / d(q.pos) of each row, which the backward uses."""
+    _check_pairs(q, pos, neg, ref_margin, temperature, beta, smoothing, "sparton::preference_fwd")
+    return _eager.load().preference_fwd(q, pos, neg, ref_margin, temperature, beta, smoothing)
+
+
+@preference_fwd.register_fake
+def _(q, pos, neg, ref_margin, temperature, beta, smoothing):
+    row = q.new_empty((q.shape[0],), dtype=torch.float32)
+    return q.new_empty((), dtype=torch.float32), row, row.clone()
+
+
+@torch.library.custom_op("sparton::preference_bwd", mutates_args=())
+def preference_bwd(grad: Tensor, q: Tensor, pos: Tensor, neg: Tensor, coef: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dq, dpos, dneg) in the reps dtype, from the loss's upstream gradient (a scalar)."""
+    op = "sparton::preference_bwd"
+    _check_pairs(q, pos, neg, None, 1.0, 1.0, 0.0, op)
+    if grad.numel() != 1 or tuple(coef.shape) != (q.shape[0],) or coef.dtype != torch.float32 or not coef.is_contiguous():
+        raise ValueError(f"{op}: grad must be a scalar and coef contiguous float32 [{q.shape[0]}], got "
+                         f"{tuple(grad.shape)} and {coef.dtype} {tuple(coef.shape)}")
+    for t in (grad, coef):
+        if t.device != q.device:
+            raise ValueError(f"{op}: all tensors must be on {q.device}, got {t.device}")
+    return _eager.load().preference_bwd(grad, q, pos, neg, coef)
+
+
+@preference_bwd.register_fake
+def _(grad, q, pos, neg, coef):
+    return q.new_empty(q.shape), q.new_empty(q.shape), q.new_empty(q.shape)
+
+
+def _preference_setup(ctx, inputs, output):
+    q, pos, neg = inputs[:3]
+    _loss, margin, coef = output
+    ctx.mark_non_differentiable(margin, coef)
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(q, pos, neg, coef)
+
+
+def _preference_backward(ctx, g_loss, _g_margin, _g_coef):
+    q, pos, neg, coef = ctx.saved_tensors
+    if g_loss is None:  # the loss did not reach what is differentiated
+        return None, None, None, None, None, None, None
+    return (*torch.ops.sparton.preference_bwd(g_loss, q, pos, neg, coef), None, None, None, None)
+
+
+preference_fwd.register_autograd(_preference_backward, setup_context=_preference_setup)
+
+
+def preference_loss(query_reps: Tensor, pos_reps: Tensor, neg_reps: Tensor, ref_margin: Optional[Tensor] = None, *,
+                    beta: float = 1.0, temperature: float = 1.0, label_smoothing: float = 0.0) -> PreferenceLossOutput:
+    """Preference loss on pairs: row i of the reps [B, V] is a query, the document preferred for it and
+    one rejected. A retriever gives documents the probabilities softmax(q.d / temperature), so a pair's
+    log ratio log P(pos) - log P(neg) is its score margin m = (q.pos - q.neg) / temperature, and with
+    the reference model's margins r (preference_margin of its reps; default zeros)
+
+        loss = mean of -(1 - label_smoothing) log sigma(z) - label_smoothing log sigma(-z),  z = beta (m - r)
+
+    Scores and sums are fp32 whatever the reps dtype, over the difference pos - neg, so that close
+    scores do not cancel."""
+    args = (query_reps, pos_reps, neg_reps, ref_margin, float(temperature), float(beta), float(label_smoothing))
+    if torch.compiler.is_compiling() or not query_reps.is_cuda:  # the registered op: fake + autograd
+        loss, margin, _ = torch.ops.sparton.preference_fwd(*args)
+        return PreferenceLossOutput(loss, margin)
+    _check_pairs(*args, "preference_loss")
+    return PreferenceLossOutput(*_eager.load().preference_loss(*args))
+
+
+@torch.no_grad()
+def preference_margin(query_reps: Tensor, pos_reps: Tensor, neg_reps: Tensor, temperature: float = 1.0) -> Tensor:
+    """The margins [B] (fp32) of a reference model's reps, for preference_loss's ref_margin."""
+    _check_pairs(query_reps, pos_reps, neg_reps, None, float(temperature), 1.0, 0.0, "preference_margin")
+    return _eager.load().preference_margin(query_reps, pos_reps, neg_reps, float(temperature))

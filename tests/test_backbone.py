@@ -1,0 +1,189 @@
+"""The attention and norm kernels in transformers backbones of the reference's families (bert,
+distilbert, roberta, xlm-roberta; training/model.py:14-40), tiny and built offline, and a whole
+training step on them: backbone -> transform -> head -> SPLADE loss and preference loss -> every
+parameter's gradient, against the same model with torch's attention and norms.
+
+Tolerances, fp32 throughout: hidden states rtol 1e-4, atol 1e-5; gradients by the measure of
+test_hf_integration.py (error against the gradient's largest magnitude, with a floor of 1e-4 of the
+largest of all, at most 1e-3; torch's fp32 CPU result sits within 1e-6 of float64 by it)."""
+import copy
+
+import pytest
+import torch
+from torch import nn
+
+import sparton_amd
+from _parity import say
+from sparton_amd.backbone import attention_forward, key_mask, use_in_backbone
+from sparton_amd.loss import preference_loss, preference_margin, splade_loss
+from test_hf_integration import backbone_and_head, batch, sparton_projection, tiny_mlm
+
+
+def tiny(kind, seed=0):
+    if kind in ("bert", "xlm-roberta"):
+        return tiny_mlm(kind, seed).eval()
+    from transformers import DistilBertConfig, DistilBertForMaskedLM, RobertaConfig, RobertaForMaskedLM
+    torch.manual_seed(seed)
+    if kind == "roberta":
+        return RobertaForMaskedLM(RobertaConfig(vocab_size=3001, hidden_size=128, num_hidden_layers=2, num_attention_heads=4,
+                                                intermediate_size=256, max_position_embeddings=130,
+                                                attn_implementation="eager", hidden_dropout_prob=0.0,
+                                                attention_probs_dropout_prob=0.0)).eval()
+    return DistilBertForMaskedLM(DistilBertConfig(vocab_size=3001, dim=128, n_layers=2, n_heads=4, hidden_dim=256,
+                                                  max_position_embeddings=128, attn_implementation="eager", dropout=0.0,
+                                                  attention_dropout=0.0)).eval()
+
+
+def base(llm):
+    return getattr(llm, llm.base_model_prefix)
+
+
+KINDS = ["bert", "distilbert", "roberta", "xlm-roberta"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_switching_keeps_parameters_and_names(kind):
+    llm = tiny(kind)
+    names, own = list(llm.state_dict()), {n: id(p) for n, p in llm.named_parameters()}
+    norms = sum(type(m) is nn.LayerNorm for m in llm.modules())
+    assert use_in_backbone(llm) is llm and llm.config._attn_implementation == "sparton"
+    assert list(llm.state_dict()) == names and {n: id(p) for n, p in llm.named_parameters()} == own
+    assert sum(type(m) is sparton_amd.SpartonLayerNorm for m in llm.modules()) == norms > 0
+    assert not any(type(m) is nn.LayerNorm for m in llm.modules())
+    use_in_backbone(llm)  # a second time changes nothing
+    assert list(llm.state_dict()) == names
+    twin = copy.deepcopy(llm)  # the copy's blocks run on the copy's own parameters
+    for a, b in zip(llm.modules(), twin.modules()):
+        if "forward" in a.__dict__:
+            assert b.forward.__self__ is b
+
+
+def test_refusals():
+    q = torch.zeros(1, 2, 4, 8)
+    with pytest.raises(ValueError, match="dropout"):
+        attention_forward(nn.Module(), q, q, q, None, dropout=0.1)
+    with pytest.raises(ValueError, match="sliding_window"):
+        attention_forward(nn.Module(), q, q, q, None, sliding_window=16)
+    with pytest.raises(ValueError, match="output_attentions"):
+        attention_forward(nn.Module(), q, q, q, None, output_attentions=True)
+    with pytest.raises(ValueError, match="per key"):
+        attention_forward(nn.Module(), q, q, q, torch.zeros(1, 1, 4, 4))
+    from transformers.masking_utils import causal_mask_function, sliding_window_overlay
+    with pytest.raises(ValueError, match="pattern"):
+        key_mask(1, 4, 4, mask_function=sliding_window_overlay(2))
+    with pytest.raises(ValueError, match="room"):
+        key_mask(1, 1, 16, q_offset=3, mask_function=causal_mask_function)
+    m = torch.ones(1, 4, dtype=torch.long)
+    assert key_mask(1, 4, 4, mask_function=causal_mask_function, attention_mask=m) is m
+    assert key_mask(1, 4, 4) is None
+
+
+def test_training_with_attention_dropout_is_refused():
+    from transformers import BertConfig, BertModel
+    model = use_in_backbone(BertModel(BertConfig(vocab_size=50, hidden_size=32, num_hidden_layers=1, num_attention_heads=2,
+                                                 intermediate_size=64)))
+    model.embeddings.LayerNorm = nn.LayerNorm(32)  # lets a CPU run reach the attention
+    with pytest.raises(ValueError, match="dropout"):
+        model.train()(torch.ones(1, 4, dtype=torch.long))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("padded", [True, False])
+def test_backbone_matches_torch(kind, padded, device):
+    say(f"backbone {kind} padded={padded}")
+    llm = tiny(kind, seed=3).to(device)
+    ours = use_in_backbone(copy.deepcopy(llm))
+    ids, mask = batch(5, 47, seed=4, device=device)
+    mask = mask if padded else torch.ones_like(mask)
+    with torch.no_grad():
+        ref, got = base(llm)(ids, mask).last_hidden_state, base(ours)(ids, mask).last_hidden_state
+        bare = base(ours)(ids).last_hidden_state
+    # every position but the padding, whose queries see the same keys and are compared too
+    torch.testing.assert_close(got, ref, rtol=1e-4, atol=1e-5)
+    if not padded:
+        torch.testing.assert_close(bare, ref, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.gpu
+def test_decoder_backbone_is_causal(device):
+    """A decoder-only backbone with shared key heads (random, tiny): the registry hands its attention over."""
+    from transformers import LlamaConfig, LlamaModel
+    torch.manual_seed(0)
+    cfg = LlamaConfig(vocab_size=300, hidden_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                      intermediate_size=256, attn_implementation="eager", use_cache=False)
+    ref = LlamaModel(cfg).to(device).eval()
+    ours = use_in_backbone(copy.deepcopy(ref))
+    ids, mask = batch(3, 40, seed=1, device=device)
+    ids = ids % 300
+    with torch.no_grad():
+        a, b = ref(ids, mask).last_hidden_state, ours(ids, mask).last_hidden_state
+    on = mask.bool()
+    torch.testing.assert_close(b[on], a[on], rtol=1e-4, atol=1e-5)
+    # token by token over a cache: the rows are the last ones of the keys
+    with torch.no_grad():
+        whole = ours(ids[:1, :30]).last_hidden_state
+        first = ours(ids[:1, :25], use_cache=True)
+        last = ours(ids[:1, 25:30], past_key_values=first.past_key_values, use_cache=True).last_hidden_state
+    torch.testing.assert_close(last, whole[:, 25:], rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bert", "xlm-roberta"])
+def test_training_step_with_every_operator(kind, device):
+    say(f"training step {kind}")
+    llm = tiny(kind, seed=6).to(device)
+    ours = use_in_backbone(copy.deepcopy(llm))
+    q_ids, q_mask = batch(6, 16, seed=7, device=device)
+    d_ids, d_mask = batch(12, 60, seed=8, device=device)
+    T = 100.0
+
+    def step(model):
+        """Gradients of the SPLADE loss over (query, preferred) plus the preference loss over the pairs."""
+        backbone, transform, decoder = backbone_and_head(model)
+        xf, head = sparton_projection(transform, decoder)
+        encode = lambda ids, mask: head(xf(backbone(ids, mask).last_hidden_state), mask)
+        q, d = encode(q_ids, q_mask), encode(d_ids, d_mask)
+        with torch.no_grad():
+            ref = preference_margin(q * 0.9, d[:6], d[6:] * 1.1, T)
+        pairs = preference_loss(q, d[:6], d[6:], ref, beta=0.5, temperature=T)
+        loss = splade_loss(q, d[:6], T, 1e-3, 1e-3).total + pairs.loss
+        model.zero_grad()
+        loss.backward()
+        return loss.detach(), {n: p.grad for n, p in model.named_parameters() if p.grad is not None}
+
+    (la, ga), (lb, gb) = step(llm), step(ours)
+    torch.testing.assert_close(lb, la, rtol=1e-4, atol=1e-6)
+    assert ga.keys() == gb.keys()
+    floor = 1e-4 * max(g.abs().max().item() for g in ga.values())
+    worst = max((gb[n] - g).abs().max().item() / max(g.abs().max().item(), floor) for n, g in ga.items())
+    say(f"   loss {lb.item():.6f} (torch's backbone {la.item():.6f}), worst gradient error {worst:.2e}")
+    assert worst <= 1e-3
+
+
+@pytest.mark.gpu
+def test_training_step_in_bf16(device):
+    """The same under bf16 autocast over fp32 parameters, and held in bf16: it runs, its loss is near the
+    fp32 one, and every gradient is finite."""
+    say("training step, bf16")
+    llm = use_in_backbone(tiny("bert", seed=9).to(device))
+    ids, mask = batch(4, 33, seed=10, device=device)
+    backbone, transform, decoder = backbone_and_head(llm)
+    xf, head = sparton_projection(transform, decoder)
+
+    def reps():
+        return head(xf(backbone(ids, mask).last_hidden_state), mask)
+
+    with torch.no_grad():
+        want = reps()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = reps()
+    assert got.dtype == torch.bfloat16 and (got.float() - want).abs().max() <= 5e-2 * want.abs().max()
+    got.float().sum().backward()
+    assert all(torch.isfinite(p.grad).all() for p in llm.parameters() if p.grad is not None)
+    llm.zero_grad()
+    llm.to(torch.bfloat16)
+    got = reps()
+    assert got.dtype == torch.bfloat16 and (got.float() - want).abs().max() <= 5e-2 * want.abs().max()
+    got.float().sum().backward()
+    assert all(torch.isfinite(p.grad).all() for p in llm.parameters() if p.grad is not None)
