@@ -60,16 +60,17 @@ template <typename T, int DH> struct Geo {
   static constexpr int DB = DH / 32;        // 32-row blocks of a transposed output
 };
 
-// LDS rows are ROW bytes; the chunks of row r are permuted by XOR with f(r), so that the 32 lanes
-// that read one chunk of 32 rows spread over all banks.
-template <int ROW, int CPR> __device__ __forceinline__ int swz(int r) {
-  constexpr int SH = ROW >= 128 ? 0 : ROW >= 64 ? 1 : 2;
-  constexpr int MASK = (CPR < 16 ? CPR : 16) - 1;
-  return (r >> SH) & MASK;
+// LDS rows are ROW bytes; the chunks of row r are permuted by XOR with f(r), which has period 16 at
+// most. It serves both reads: one chunk of 8 consecutive rows (a row operand) and 64 bytes of 4
+// consecutive rows (a column operand) each fall on different banks.
+template <int ROW> __device__ __forceinline__ int swz(int r) {
+  if constexpr (ROW == 64) return (r >> 1) & 3;
+  else if constexpr (ROW == 128) return ((r & 2) << 1) | ((r & 4) >> 1) | (r & 1);
+  else return ((r & 3) << 2) | ((r >> 2) & 3);
 }
 template <typename T, int DH> __device__ __forceinline__ int lds_at(int row, int chunk) {
   typedef Geo<T, DH> Gm;
-  return row * Gm::ROW + ((chunk ^ swz<Gm::ROW, Gm::CPR>(row)) << 4);
+  return row * Gm::ROW + ((chunk ^ swz<Gm::ROW>(row)) << 4);
 }
 
 template <typename T> struct Frag;
@@ -145,11 +146,25 @@ __device__ __forceinline__ float other_half_sum(float x) {
   return __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
 }
 
-// Consecutive workgroups go to the eight XCDs in turn; this numbering gives each XCD a contiguous
-// range instead, so that the tiles of one head share their keys and values in that XCD's L2.
-__device__ __forceinline__ int xcd_range(int w, int n) {
-  const int x = w & 7, base = n >> 3, rem = n & 7;
-  return x * base + min(x, rem) + (w >> 3);
+// Workgroup w's place among `pairs` (batch row, key head) pairs of `tiles` workgroups each. Consecutive
+// workgroups go to the eight XCDs in turn. A pair's tiles stay on one XCD, whose L2 then holds its keys
+// and values, and the pairs go round the XCDs, so that long and short rows of a padded batch spread
+// evenly; what is left of pairs after whole rounds is cut into eight runs of tiles.
+struct Place {
+  int pair, tile;
+};
+__device__ __forceinline__ Place place_of(int w, int pairs, int tiles) {
+  const int x = w & 7, k = w >> 3, rounds = pairs >> 3, whole = rounds * tiles;
+  Place p;
+  if (k < whole) {
+    p.pair = k / tiles * 8 + x;
+    p.tile = k % tiles;
+  } else {
+    const int n = (pairs & 7) * tiles, i = x * (n >> 3) + min(x, n & 7) + (k - whole);
+    p.pair = rounds * 8 + i / tiles;
+    p.tile = i % tiles;
+  }
+  return p;
 }
 
 __device__ __forceinline__ bool key_on(const void* mask, int mask_dtype, int64_t off) {
@@ -175,19 +190,31 @@ struct KeyBits {
     chunk = -1;
     word = 0;
   }
-  __device__ __forceinline__ void load(int c) {  // keys [2048 c, 2048 (c + 1))
+  // Eight loads are in flight at a time: one after the other would cost a round trip per 64 keys.
+  template <typename M> __device__ __forceinline__ void gather(int k0, int n) {
     const int lane = threadIdx.x & 63;
-    const int k0 = c * 2048;
-    const int n = min(32, (kend - k0 + 63) >> 6);
+    for (int x0 = 0; x0 < n; x0 += 8) {
+      M v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = ((const M*)mask)[row + min(k0 + (x0 + i) * 64 + lane, kend - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int x = x0 + i;
+        const uint64_t bits = __ballot(v[i] != 0 && k0 + x * 64 + lane < kend);
+        word = lane == 2 * x ? (uint32_t)bits : lane == 2 * x + 1 ? (uint32_t)(bits >> 32) : word;
+      }
+    }
+  }
+  __device__ __forceinline__ void load(int c) {  // keys [2048 c, 2048 (c + 1)), below kend
+    const int k0 = c * 2048, n = min(32, (kend - k0 + 63) >> 6);
     chunk = c;
     word = 0;
-    for (int x = 0; x < n; ++x) {
-      const int key = k0 + x * 64 + lane;
-      bool on = key < kend;
-      if (mask != nullptr) on = key_on(mask, dtype, row + min(key, kend - 1)) && on;
-      const uint64_t bits = __ballot(on);
-      word = lane == 2 * x ? (uint32_t)bits : lane == 2 * x + 1 ? (uint32_t)(bits >> 32) : word;
-    }
+    if (mask == nullptr) {
+      const int left = kend - k0 - (threadIdx.x & 63) * 32;
+      word = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+    } else if (dtype == SPARTON_MASK_I64) gather<int64_t>(k0, n);
+    else if (dtype == SPARTON_MASK_I32) gather<int32_t>(k0, n);
+    else gather<uint8_t>(k0, n);
   }
   // word of keys [32 blk, 32 blk + 32); blk < cdiv(kend, 32) rounded up to a tile
   __device__ __forceinline__ uint32_t at(int blk) {
@@ -207,31 +234,53 @@ struct KeyBits {
   }
 };
 
-// One thread's share of a [rows][DH] tile on its way from memory to LDS: chunk id = tid + u threads.
+// What a staged chunk is read from past the last row and past D: every load is then unconditional.
+__device__ u32x4 zero_chunk;
+
+// One thread's share of a [ROWS][DH] tile on its way from memory to LDS: chunk `ch` of rows row0 + u RPU.
 template <typename T, int DH, int ROWS, int THREADS> struct Stage {
   typedef Geo<T, DH> Gm;
   static constexpr int N = ROWS * Gm::CPR / THREADS;
-  static_assert(ROWS * Gm::CPR % THREADS == 0, "a thread stages whole chunks");
+  static constexpr int RPU = THREADS / Gm::CPR;
+  static_assert(ROWS * Gm::CPR % THREADS == 0 && THREADS % Gm::CPR == 0, "a thread stages whole chunks of one column");
   u32x4 r[N];
-  // Rows past `rows` load the last one, chunks past D the first: in range, and zeroed by put().
-  __device__ __forceinline__ void get(const T* base, int64_t stride, int row0, int rows, int D) {
+  const T* mine;
+  int64_t stride;
+  int row0, ch, rows;  // rows: how many there are for this chunk (none past D)
+  __device__ __forceinline__ void init(const T* base, int64_t stride_, int rows_, int D) {
+    row0 = threadIdx.x / Gm::CPR;
+    ch = threadIdx.x % Gm::CPR;
+    rows = ch * Gm::EPC < D ? rows_ : 0;
+    stride = stride_;
+    mine = base + row0 * stride + ch * Gm::EPC;
+  }
+  __device__ __forceinline__ void get(int first) {
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int id = threadIdx.x + u * THREADS, row = id / Gm::CPR, ch = id % Gm::CPR;
-      const int64_t off = (int64_t)min(row0 + row, rows - 1) * stride + (ch * Gm::EPC < D ? ch * Gm::EPC : 0);
-      r[u] = *(const u32x4*)(base + off);
+      const T* at = mine + (int64_t)(first + u * RPU) * stride;
+      r[u] = *(first + row0 + u * RPU < rows ? (const u32x4*)at : &zero_chunk);
     }
   }
-  // Rows whose bit in `w` is clear, and chunks past D, as zeros.
-  template <int NW> __device__ __forceinline__ void put(char* tile, const uint32_t (&w)[NW], int D) const {
+  __device__ __forceinline__ int to(int u) const {
+    return RPU % 16 == 0 ? lds_at<T, DH>(row0, ch) + u * RPU * Gm::ROW : lds_at<T, DH>(row0 + u * RPU, ch);
+  }
+  __device__ __forceinline__ void put(char* tile) const {
+#pragma unroll
+    for (int u = 0; u < N; ++u) *(u32x4*)(tile + to(u)) = r[u];
+  }
+  // Rows whose bit in `w` is clear become zeros.
+  template <int NW> __device__ __forceinline__ void clear(const uint32_t (&w)[NW]) {
+    uint32_t all = w[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) all &= w[i];
+    if (all == 0xffffffffu) return;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int id = threadIdx.x + u * THREADS, row = id / Gm::CPR, ch = id % Gm::CPR;
+      const int row = row0 + u * RPU;
       uint32_t bits = w[0];
 #pragma unroll
       for (int i = 1; i < NW; ++i) bits = (row >> 5) == i ? w[i] : bits;
-      const bool on = ((bits >> (row & 31)) & 1) && ch * Gm::EPC < D;
-      *(u32x4*)(tile + lds_at<T, DH>(row, ch)) = on ? r[u] : u32x4{0, 0, 0, 0};
+      if (!((bits >> (row & 31)) & 1)) r[u] = u32x4{0, 0, 0, 0};
     }
   }
 };
@@ -299,30 +348,29 @@ __device__ __forceinline__ void pos_range(const Params& p, int r0, int r1, int* 
 }
 
 // ---- forward -----------------------------------------------------------------------------
-// WR x WK waves: wave (wr, wk) holds 32 NB rows and takes the 32 JB keys wk of each tile of 32 JB WK.
-// Each wave keeps its rows' running maximum and sum; where WK > 1 the waves' results are joined
+// WR x WK waves: wave (wr, wk) holds 32 rows and takes the 32 JB keys wk of each tile of 32 JB WK.
+// Each wave keeps its rows' running maximum and sum; where WK > 1 the results of a row's waves are joined
 // through LDS at the end, and with SPLIT each workgroup takes tiles_per_split tiles of the keys and
 // writes its normalised result and log sum for attn_join_kernel.
-template <typename T, int DH, int NB, int WR, int WK, int JB, int NBUF, bool SPLIT>
-__global__ __launch_bounds__(64 * WR * WK, NB * DH > 128 ? 1 : 2) void attn_fwd_kernel(Params p) {
+template <typename T, int DH, int WR, int WK, int JB, int NBUF, bool SPLIT>
+__global__ __launch_bounds__(64 * WR * WK, sizeof(T) * DH <= 256 ? 2 : 1) void attn_fwd_kernel(Params p) {
   typedef Geo<T, DH> Gm;
   constexpr int THREADS = 64 * WR * WK, BK = 32 * JB * WK, NW = JB * WK;
   constexpr int TILE = BK * Gm::ROW;
-  static_assert(WK == 1 || (NB == 1 && WR == 1 && NBUF * 2 * TILE >= WK * 32 * DH * 4), "joining waves reuse the tiles");
+  static_assert(WK == 1 || NBUF * 2 * TILE >= WR * WK * 32 * DH * 4, "joining waves reuse the tiles");
   __shared__ __attribute__((aligned(16))) char smem[NBUF * 2 * TILE];
-  __shared__ float wave_stat[WK > 1 ? 2 * WK * 32 : 1];
+  __shared__ float wave_stat[WK > 1 ? WR * WK * 64 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wr = wave % WR, wk = wave / WR;
-  const int row_tiles = (p.R + 32 * NB * WR - 1) / (32 * NB * WR);
-  int id = xcd_range(blockIdx.x, gridDim.x);
-  const int split = SPLIT ? id % p.splits : 0;
-  if (SPLIT) id /= p.splits;
-  const int bh = id / row_tiles, tile = row_tiles - 1 - id % row_tiles;  // causal: longest first
+  const int row_tiles = (p.R + 32 * WR - 1) / (32 * WR);
+  const Place at = place_of(blockIdx.x, p.B * p.Hk, SPLIT ? row_tiles * p.splits : row_tiles);
+  const int split = SPLIT ? at.tile % p.splits : 0;
+  const int bh = at.pair, tile = row_tiles - 1 - (SPLIT ? at.tile / p.splits : at.tile);  // causal: longest first
   const int b = bh / p.Hk, hk = bh % p.Hk;
-  const int r0 = tile * 32 * NB * WR;
+  const int r0 = tile * 32 * WR;
 
   int i_lo, i_hi;
-  pos_range(p, r0, r0 + 32 * NB * WR, &i_lo, &i_hi);
+  pos_range(p, r0, r0 + 32 * WR, &i_lo, &i_hi);
   const int off = p.Sk - p.Sq;
   const int kend = p.causal ? max(0, min(p.Sk, i_hi + off + 1)) : p.Sk;
   int t_end = (kend + BK - 1) / BK, t = -1;
@@ -331,59 +379,58 @@ __global__ __launch_bounds__(64 * WR * WK, NB * DH > 128 ? 1 : 2) void attn_fwd_
     t_end = min(t_end, t + 1 + p.tiles_per_split);
   }
 
-  Row row[NB];
-  frag_t<T> qf[NB][Gm::NC];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    row[n] = row_of(p, r0 + (wr * NB + n) * 32 + (lane & 31));
-    load_row<T, DH>(qf[n], (const T*)p.q + b * p.sq.b + (int64_t)(hk * p.G + row[n].g) * p.sq.h + row[n].i * p.sq.s,
-                    half, p.D, true);
-  }
+  const Row row = row_of(p, r0 + wr * 32 + (lane & 31));
+  frag_t<T> qf[Gm::NC];
+  load_row<T, DH>(qf, (const T*)p.q + b * p.sq.b + (int64_t)(hk * p.G + row.g) * p.sq.h + row.i * p.sq.s, half, p.D, true);
   const T* kb = (const T*)p.k + b * p.sk.b + hk * p.sk.h;
   const T* vb = (const T*)p.v + b * p.sv.b + hk * p.sv.h;
 
-  f32x16 acc[NB][Gm::DB];
-  float m[NB], l[NB];  // the running maximum (times c) and this half's part of the sum
+  f32x16 acc[Gm::DB];
+  float m = -INFINITY, l = 0.0f;  // the running maximum (times c) and this half's part of the sum
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.0f;
-#pragma unroll
-    for (int db = 0; db < Gm::DB; ++db) acc[n][db] = zero16();
-  }
+  for (int db = 0; db < Gm::DB; ++db) acc[db] = zero16();
 
+  // The first tile is on its way before the mask is known, which seldom leaves it out.
+  Stage<T, DH, BK, THREADS> ks, vs;
+  ks.init(kb, p.sk.s, p.Sk, p.D);
+  vs.init(vb, p.sv.s, p.Sk, p.D);
+  const int ahead = t + 1;
+  ks.get(ahead * BK);
+  vs.get(ahead * BK);
   KeyBits bits;
   bits.init(p, b, kend);
   uint32_t w[NW], wn[NW];
   t = bits.next<NW>(t, t_end, w);
-  Stage<T, DH, BK, THREADS> ks, vs;
   if (t < t_end) {
-    ks.get(kb, p.sk.s, t * BK, p.Sk, p.D);
-    vs.get(vb, p.sv.s, t * BK, p.Sk, p.D);
-    ks.template put<NW>(smem, w, p.D);
-    vs.template put<NW>(smem + TILE, w, p.D);
+    if (t != ahead) {
+      ks.get(t * BK);
+      vs.get(t * BK);
+    }
+    ks.template clear<NW>(w);
+    vs.template clear<NW>(w);
+    ks.put(smem);
+    vs.put(smem + TILE);
     __syncthreads();
   }
   int buf = 0;
   while (t < t_end) {
     const int tn = bits.next<NW>(t, t_end, wn);
     if (tn < t_end) {
-      ks.get(kb, p.sk.s, tn * BK, p.Sk, p.D);
-      vs.get(vb, p.sv.s, tn * BK, p.Sk, p.D);
+      ks.get(tn * BK);
+      vs.get(tn * BK);
     }
     const char* kt = smem + buf * 2 * TILE;
     const char* vt = kt + TILE;
-    f32x16 s[NB][JB];
+    f32x16 s[JB];
 #pragma unroll
     for (int jb = 0; jb < JB; ++jb) {
+      s[jb] = zero16();
+      frag_t<T> kf[Gm::NC];
 #pragma unroll
-      for (int n = 0; n < NB; ++n) s[n][jb] = zero16();
+      for (int c = 0; c < Gm::NC; ++c)
+        kf[c] = lds_frag<T>(kt + lds_at<T, DH>((wk * JB + jb) * 32 + (lane & 31), 2 * c + half));
 #pragma unroll
-      for (int c = 0; c < Gm::NC; ++c) {
-        const frag_t<T> kf = lds_frag<T>(kt + lds_at<T, DH>((wk * JB + jb) * 32 + (lane & 31), 2 * c + half));
-#pragma unroll
-        for (int n = 0; n < NB; ++n) s[n][jb] = mma(kf, qf[n][c], s[n][jb]);
-      }
+      for (int c = 0; c < Gm::NC; ++c) s[jb] = mma(kf[c], qf[c], s[jb]);
     }
     uint32_t wj[JB];
     bool part = false;
@@ -399,72 +446,67 @@ __global__ __launch_bounds__(64 * WR * WK, NB * DH > 128 ? 1 : 2) void attn_fwd_
       for (int jb = 0; jb < JB; ++jb) {
         const uint32_t mine = wj[jb] >> (4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-          for (int n = 0; n < NB; ++n) s[n][jb][r] = (mine >> reg_row(r)) & 1 ? s[n][jb][r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) s[jb][r] = (mine >> reg_row(r)) & 1 ? s[jb][r] : -INFINITY;
       }
     }
     if (p.causal && (t + 1) * BK - 1 > i_lo + off) {
 #pragma unroll
-      for (int jb = 0; jb < JB; ++jb)
+      for (int jb = 0; jb < JB; ++jb) {
+        const int lim = row.i + off - (t * BK + (wk * JB + jb) * 32 + 4 * half);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const int lim = row[n].i + off - (t * BK + (wk * JB + jb) * 32 + 4 * half);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[n][jb][r] = reg_row(r) <= lim ? s[n][jb][r] : -INFINITY;
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      float top = s[n][0][0];
-#pragma unroll
-      for (int jb = 0; jb < JB; ++jb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][jb][r]);
-      top = other_half_max(top) * p.c;
-      // The maximum follows only where it has grown by more than 2^8 (p stays below 2^8, and sums
-      // have room for that): after the first tiles the output's rescaling is hardly ever taken.
-      const bool up = top > m[n] + 8.0f;
-      if (__any(up)) {
-        const float mn = up ? top : m[n];
-        const float a = up ? __builtin_amdgcn_exp2f(m[n] - mn) : 1.0f;
-        l[n] *= a;
-#pragma unroll
-        for (int db = 0; db < Gm::DB; ++db)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[n][db][r] *= a;
-        m[n] = mn;
+        for (int r = 0; r < 16; ++r) s[jb][r] = reg_row(r) <= lim ? s[jb][r] : -INFINITY;
       }
-      const float mm = m[n] == -INFINITY ? 0.0f : m[n];
-      float sum = 0.0f;
-#pragma unroll
-      for (int jb = 0; jb < JB; ++jb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[n][jb][r] = __builtin_amdgcn_exp2f(fmaf(s[n][jb][r], p.c, -mm));
-          sum += s[n][jb][r];
-        }
-      l[n] += sum;
     }
+    // From here to the tile's end a wave goes before the CU's others: they are then in their products
+    // while this one is in its exponentials, where equal waves keep step and wait for the same unit
+    // (8192 x 8192, 12 heads of 64: 291 -> 270 us).
+    __builtin_amdgcn_s_setprio(1);
+    float top = s[0][0];
+#pragma unroll
+    for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[jb][r]);
+    top = other_half_max(top) * p.c;
+    // The maximum follows only where it has grown by more than 2^8 (p stays below 2^8, and sums
+    // have room for that): after the first tiles the output's rescaling is hardly ever taken.
+    const bool up = top > m + 8.0f;
+    if (__any(up)) {
+      const float mn = up ? top : m;
+      const float a = up ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+      l *= a;
+#pragma unroll
+      for (int db = 0; db < Gm::DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[db][r] *= a;
+      m = mn;
+    }
+    const float mm = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[jb][r] = __builtin_amdgcn_exp2f(fmaf(s[jb][r], p.c, -mm));
+        sum += s[jb][r];
+      }
+    l += sum;
 #pragma unroll
     for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
       for (int c = 0; c < Gm::PB; ++c) {
-        frag_t<T> pf[NB];
+        const frag_t<T> pf = pack<T>(s[jb], c);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) pf[n] = pack<T>(s[n][jb], c);
-#pragma unroll
-        for (int db = 0; db < Gm::DB; ++db) {
-          const frag_t<T> vf = lds_cols<T, DH>(vt, (wk * JB + jb) * 32 + c * Gm::KC, db, lane);
-#pragma unroll
-          for (int n = 0; n < NB; ++n) acc[n][db] = mma(vf, pf[n], acc[n][db]);
-        }
+        for (int db = 0; db < Gm::DB; ++db)
+          acc[db] = mma(lds_cols<T, DH>(vt, (wk * JB + jb) * 32 + c * Gm::KC, db, lane), pf, acc[db]);
       }
+    __builtin_amdgcn_s_setprio(0);
     if (NBUF == 1) __syncthreads();
     if (tn < t_end) {
       if (NBUF == 2) buf ^= 1;
-      ks.template put<NW>(smem + buf * 2 * TILE, wn, p.D);
-      vs.template put<NW>(smem + buf * 2 * TILE + TILE, wn, p.D);
+      ks.template clear<NW>(wn);
+      vs.template clear<NW>(wn);
+      ks.put(smem + buf * 2 * TILE);
+      vs.put(smem + buf * 2 * TILE + TILE);
     }
     __syncthreads();
     t = tn;
@@ -472,32 +514,31 @@ __global__ __launch_bounds__(64 * WR * WK, NB * DH > 128 ? 1 : 2) void attn_fwd_
     for (int i = 0; i < NW; ++i) w[i] = wn[i];
   }
 
-#pragma unroll
-  for (int n = 0; n < NB; ++n) l[n] = other_half_sum(l[n]);
+  l = other_half_sum(l);
 
   if constexpr (WK > 1) {
-    // acc, m and l of the WK waves, each for the same 32 rows, to LDS; wave 0 joins them.
+    // acc, m and l of the WK waves that hold the same 32 rows, to LDS; the first joins them.
     __syncthreads();
     float* mine = (float*)smem + wave * 32 * DH;
 #pragma unroll
     for (int db = 0; db < Gm::DB; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mine[(db * 16 + r) * 64 + lane] = acc[0][db][r];
+      for (int r = 0; r < 16; ++r) mine[(db * 16 + r) * 64 + lane] = acc[db][r];
     if (half == 0) {
-      wave_stat[wave * 64 + lane] = m[0];
-      wave_stat[wave * 64 + 32 + lane] = l[0];
+      wave_stat[wave * 64 + lane] = m;
+      wave_stat[wave * 64 + 32 + lane] = l;
     }
     __syncthreads();
-    if (wave > 0) return;
-    float top = m[0];
+    if (wk > 0) return;
+    float top = m;
 #pragma unroll
-    for (int x = 1; x < WK; ++x) top = fmaxf(top, wave_stat[x * 64 + (lane & 31)]);
+    for (int x = 1; x < WK; ++x) top = fmaxf(top, wave_stat[(wr + x * WR) * 64 + (lane & 31)]);
     const float mm = top == -INFINITY ? 0.0f : top;
     float wt[WK], sum = 0.0f;
 #pragma unroll
     for (int x = 0; x < WK; ++x) {
-      wt[x] = __builtin_amdgcn_exp2f(wave_stat[x * 64 + (lane & 31)] - mm);
-      sum += wt[x] * wave_stat[x * 64 + 32 + (lane & 31)];
+      wt[x] = __builtin_amdgcn_exp2f(wave_stat[(wr + x * WR) * 64 + (lane & 31)] - mm);
+      sum += wt[x] * wave_stat[(wr + x * WR) * 64 + 32 + (lane & 31)];
     }
 #pragma unroll
     for (int db = 0; db < Gm::DB; ++db)
@@ -505,27 +546,24 @@ __global__ __launch_bounds__(64 * WR * WK, NB * DH > 128 ? 1 : 2) void attn_fwd_
       for (int r = 0; r < 16; ++r) {
         float a = 0.0f;
 #pragma unroll
-        for (int x = 0; x < WK; ++x) a += wt[x] * ((const float*)smem)[x * 32 * DH + (db * 16 + r) * 64 + lane];
-        acc[0][db][r] = a;
+        for (int x = 0; x < WK; ++x) a += wt[x] * ((const float*)smem)[(wr + x * WR) * 32 * DH + (db * 16 + r) * 64 + lane];
+        acc[db][r] = a;
       }
-    m[0] = top;
-    l[0] = sum;
+    m = top;
+    l = sum;
   }
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    if (!row[n].in) continue;
-    const bool none = l[n] == 0.0f;
-    const float inv = none ? 0.0f : 1.0f / l[n];
-    const float lse = none ? -INFINITY : m[n] + __builtin_amdgcn_logf(l[n]);
-    if constexpr (SPLIT) {
-      const int64_t at = ((int64_t)bh * p.splits + split) * p.R + r0 + (wr * NB + n) * 32 + (lane & 31);
-      store_col<float, Gm::DB>(p.part + at * p.D, acc[n], inv, half, p.D);
-      if (half == 0) p.part_lse[at] = lse;
-    } else {
-      const int64_t h = hk * p.G + row[n].g;
-      store_col<T, Gm::DB>((T*)p.out + b * p.so.b + h * p.so.h + row[n].i * p.so.s, acc[n], inv, half, p.D);
-      if (half == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + row[n].i] = lse;
-    }
+  if (!row.in) return;
+  const bool none = l == 0.0f;
+  const float inv = none ? 0.0f : 1.0f / l;
+  const float lse = none ? -INFINITY : m + __builtin_amdgcn_logf(l);
+  if constexpr (SPLIT) {
+    const int64_t to = ((int64_t)bh * p.splits + split) * p.R + r0 + wr * 32 + (lane & 31);
+    store_col<float, Gm::DB>(p.part + to * p.D, acc, inv, half, p.D);
+    if (half == 0) p.part_lse[to] = lse;
+  } else {
+    const int64_t h = hk * p.G + row.g;
+    store_col<T, Gm::DB>((T*)p.out + b * p.so.b + h * p.so.h + row.i * p.so.s, acc, inv, half, p.D);
+    if (half == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Sq + row.i] = lse;
   }
 }
 
@@ -601,222 +639,231 @@ template <> struct ColScale<f16> {
 template <typename T> constexpr float kLog2Up = 0.0f;
 template <> constexpr float kLog2Up<f16> = 10.0f;
 
-// dq, and delta for the next kernel. Four waves of 32 NB rows each; the tiles as in the forward.
-template <typename T, int DH, int NB, int JB, int NBUF>
-__global__ __launch_bounds__(kThreads, 1) void attn_dq_kernel(Params p) {
+// Sums of the waves of a workgroup that hold the same rows (or keys) added in order, through LDS, into
+// the first's. Wave w's place in it is `mine` of `step` apart, N in all; every wave calls it.
+template <int DB, int N>
+__device__ __forceinline__ void join_sums(f32x16 (&acc)[DB], char* smem, int wave, int step, bool first) {
+  const int lane = threadIdx.x & 63;
+  float* mine = (float*)smem + wave * DB * 1024;
+  __syncthreads();
+  if (!first)
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[(db * 16 + r) * 64 + lane] = acc[db][r];
+  __syncthreads();
+  if (first)
+#pragma unroll
+    for (int x = 1; x < N; ++x)
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[db][r] += mine[x * step * DB * 1024 + (db * 16 + r) * 64 + lane];
+}
+
+// dq, and delta for the next kernel. WR x WK = 4 waves, rows and tiles as in the forward; a row's waves
+// add their dq at the end.
+template <typename T, int DH, int WR, int WK, int JB, int NBUF>
+__global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_dq_kernel(Params p) {
   typedef Geo<T, DH> Gm;
-  constexpr int BK = 32 * JB, TILE = BK * Gm::ROW;
+  constexpr int BK = 32 * JB * WK, NW = JB * WK, TILE = BK * Gm::ROW, RB = 32 * WR;
+  static_assert(WR * WK * 64 == kThreads && (WK == 1 || NBUF * 2 * TILE >= kThreads / 2 * DH * 4), "joining waves reuse the tiles");
   __shared__ __attribute__((aligned(16))) char smem[NBUF * 2 * TILE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int row_tiles = (p.R + 128 * NB - 1) / (128 * NB);
-  const int id = xcd_range(blockIdx.x, gridDim.x);
-  const int bh = id / row_tiles, tile = row_tiles - 1 - id % row_tiles;
+  const int wr = wave % WR, wk = wave / WR;
+  const int row_tiles = (p.R + RB - 1) / RB;
+  const Place at = place_of(blockIdx.x, p.B * p.Hk, row_tiles);
+  const int bh = at.pair, tile = row_tiles - 1 - at.tile;
   const int b = bh / p.Hk, hk = bh % p.Hk;
-  const int r0 = tile * 128 * NB;
+  const int r0 = tile * RB;
   int i_lo, i_hi;
-  pos_range(p, r0, r0 + 128 * NB, &i_lo, &i_hi);
+  pos_range(p, r0, r0 + RB, &i_lo, &i_hi);
   const int off = p.Sk - p.Sq;
   const int kend = p.causal ? max(0, min(p.Sk, i_hi + off + 1)) : p.Sk;
   const int t_end = (kend + BK - 1) / BK;
 
-  Row row[NB];
-  frag_t<T> qf[NB][Gm::NC], gf[NB][Gm::NC];
-  float lse[NB], delta[NB];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    row[n] = row_of(p, r0 + (wave * NB + n) * 32 + (lane & 31));
-    const int64_t h = hk * p.G + row[n].g;
-    load_row<T, DH>(qf[n], (const T*)p.q + b * p.sq.b + h * p.sq.h + row[n].i * p.sq.s, half, p.D, true);
-    load_row<T, DH>(gf[n], (const T*)p.dout + b * p.sdo.b + h * p.sdo.h + row[n].i * p.sdo.s, half, p.D, true);
+  Row row;
+  frag_t<T> qf[Gm::NC], gf[Gm::NC];
+  float lse, delta;
+  {
+    row = row_of(p, r0 + wr * 32 + (lane & 31));
+    const int64_t h = hk * p.G + row.g;
+    load_row<T, DH>(qf, (const T*)p.q + b * p.sq.b + h * p.sq.h + row.i * p.sq.s, half, p.D, true);
+    load_row<T, DH>(gf, (const T*)p.dout + b * p.sdo.b + h * p.sdo.h + row.i * p.sdo.s, half, p.D, true);
     frag_t<T> of[Gm::NC];
-    load_row<T, DH>(of, (const T*)p.o + b * p.so.b + h * p.so.h + row[n].i * p.so.s, half, p.D, true);
+    load_row<T, DH>(of, (const T*)p.o + b * p.so.b + h * p.so.h + row.i * p.so.s, half, p.D, true);
     float a = 0.0f;
 #pragma unroll
     for (int c = 0; c < Gm::NC; ++c)
 #pragma unroll
-      for (int e = 0; e < Gm::EPC; ++e) a += to_f32(gf[n][c][e]) * to_f32(of[c][e]);
-    delta[n] = other_half_sum(a);
-    const int64_t at = ((int64_t)b * p.Hq + h) * p.Sq + row[n].i;
-    lse[n] = p.lse[at];
-    if (!row[n].in || lse[n] == -INFINITY) lse[n] = INFINITY;  // exp2(s - lse) = 0
-    if (half == 0 && row[n].in) p.delta[at] = delta[n];
+      for (int e = 0; e < Gm::EPC; ++e) a += to_f32(gf[c][e]) * to_f32(of[c][e]);
+    delta = other_half_sum(a);
+    const int64_t to = ((int64_t)b * p.Hq + h) * p.Sq + row.i;
+    lse = p.lse[to];
+    if (!row.in || lse == -INFINITY) lse = INFINITY;  // exp2(s - lse) = 0
+    if (half == 0 && wk == 0 && row.in) p.delta[to] = delta;
   }
   const T* kb = (const T*)p.k + b * p.sk.b + hk * p.sk.h;
   const T* vb = (const T*)p.v + b * p.sv.b + hk * p.sv.h;
-  f32x16 acc[NB][Gm::DB];
-  ColScale<T> cs[NB];
+  f32x16 acc[Gm::DB];
+  ColScale<T> cs;
 #pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int db = 0; db < Gm::DB; ++db) acc[n][db] = zero16();
+  for (int db = 0; db < Gm::DB; ++db) acc[db] = zero16();
 
+  Stage<T, DH, BK, kThreads> ks, vs;
+  ks.init(kb, p.sk.s, p.Sk, p.D);
+  vs.init(vb, p.sv.s, p.Sk, p.D);
+  ks.get(0);
+  vs.get(0);
   KeyBits bits;
   bits.init(p, b, kend);
-  uint32_t w[JB], wn[JB];
-  int t = bits.next<JB>(-1, t_end, w);
-  Stage<T, DH, BK, kThreads> ks, vs;
+  uint32_t w[NW], wn[NW];
+  int t = bits.next<NW>(-1, t_end, w);
   if (t < t_end) {
-    ks.get(kb, p.sk.s, t * BK, p.Sk, p.D);
-    vs.get(vb, p.sv.s, t * BK, p.Sk, p.D);
-    ks.template put<JB>(smem, w, p.D);
-    vs.template put<JB>(smem + TILE, w, p.D);
+    if (t != 0) {
+      ks.get(t * BK);
+      vs.get(t * BK);
+    }
+    ks.template clear<NW>(w);
+    vs.template clear<NW>(w);
+    ks.put(smem);
+    vs.put(smem + TILE);
     __syncthreads();
   }
   int buf = 0;
   while (t < t_end) {
-    const int tn = bits.next<JB>(t, t_end, wn);
+    const int tn = bits.next<NW>(t, t_end, wn);
     if (tn < t_end) {
-      ks.get(kb, p.sk.s, tn * BK, p.Sk, p.D);
-      vs.get(vb, p.sv.s, tn * BK, p.Sk, p.D);
+      ks.get(tn * BK);
+      vs.get(tn * BK);
     }
     const char* kt = smem + buf * 2 * TILE;
     const char* vt = kt + TILE;
 #pragma unroll
     for (int jb = 0; jb < JB; ++jb) {
-      f32x16 s[NB], dp[NB];
-#pragma unroll
-      for (int n = 0; n < NB; ++n) s[n] = dp[n] = zero16();
+      f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int c = 0; c < Gm::NC; ++c) {
-        const int at = lds_at<T, DH>(jb * 32 + (lane & 31), 2 * c + half);
+        const int at = lds_at<T, DH>((wk * JB + jb) * 32 + (lane & 31), 2 * c + half);
         const frag_t<T> kf = lds_frag<T>(kt + at), vf = lds_frag<T>(vt + at);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          s[n] = mma(kf, qf[n][c], s[n]);
-          dp[n] = mma(vf, gf[n][c], dp[n]);
-        }
+        s = mma(kf, qf[c], s);
+        dp = mma(vf, gf[c], dp);
       }
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.c, -lse));
+      uint32_t word = w[jb];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], p.c, -lse[n]));
-      if (w[jb] != 0xffffffffu) {
-        const uint32_t mine = w[jb] >> (4 * half);
+      for (int x = 1; x < WK; ++x) word = wk == x ? w[x * JB + jb] : word;
+      if (word != 0xffffffffu) {
+        const uint32_t mine = word >> (4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-          for (int n = 0; n < NB; ++n) s[n][r] = (mine >> reg_row(r)) & 1 ? s[n][r] : 0.0f;
+        for (int r = 0; r < 16; ++r) s[r] = (mine >> reg_row(r)) & 1 ? s[r] : 0.0f;
       }
-      if (p.causal && t * BK + jb * 32 + 31 > i_lo + off) {
+      const int j0 = t * BK + (wk * JB + jb) * 32;
+      if (p.causal && j0 + 31 > i_lo + off) {
+        const int lim = row.i + off - (j0 + 4 * half);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const int lim = row[n].i + off - (t * BK + jb * 32 + 4 * half);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[n][r] = reg_row(r) <= lim ? s[n][r] : 0.0f;
-        }
+        for (int r = 0; r < 16; ++r) s[r] = reg_row(r) <= lim ? s[r] : 0.0f;
       }
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] *= dp[n][r] - delta[n];
-        cs[n].template apply<Gm::DB>(s[n], acc[n]);
-      }
+      for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
+      cs.template apply<Gm::DB>(s, acc);
 #pragma unroll
       for (int c = 0; c < Gm::PB; ++c) {
-        frag_t<T> df[NB];
+        const frag_t<T> df = pack<T>(s, c);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) df[n] = pack<T>(s[n], c);
-#pragma unroll
-        for (int db = 0; db < Gm::DB; ++db) {
-          const frag_t<T> kf = lds_cols<T, DH>(kt, jb * 32 + c * Gm::KC, db, lane);
-#pragma unroll
-          for (int n = 0; n < NB; ++n) acc[n][db] = mma(kf, df[n], acc[n][db]);
-        }
+        for (int db = 0; db < Gm::DB; ++db)
+          acc[db] = mma(lds_cols<T, DH>(kt, (wk * JB + jb) * 32 + c * Gm::KC, db, lane), df, acc[db]);
       }
     }
     if (NBUF == 1) __syncthreads();
     if (tn < t_end) {
       if (NBUF == 2) buf ^= 1;
-      ks.template put<JB>(smem + buf * 2 * TILE, wn, p.D);
-      vs.template put<JB>(smem + buf * 2 * TILE + TILE, wn, p.D);
+      ks.template clear<NW>(wn);
+      vs.template clear<NW>(wn);
+      ks.put(smem + buf * 2 * TILE);
+      vs.put(smem + buf * 2 * TILE + TILE);
     }
     __syncthreads();
     t = tn;
 #pragma unroll
-    for (int i = 0; i < JB; ++i) w[i] = wn[i];
+    for (int i = 0; i < NW; ++i) w[i] = wn[i];
   }
+  float f = p.scale * cs.inv();
+  if constexpr (WK > 1) {
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    if (!row[n].in) continue;
-    const int64_t h = hk * p.G + row[n].g;
-    store_col<T, Gm::DB>((T*)p.dq + b * p.sdq.b + h * p.sdq.h + row[n].i * p.sdq.s, acc[n], p.scale * cs[n].inv(), half,
-                         p.D);
+    for (int db = 0; db < Gm::DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[db][r] *= f;
+    f = 1.0f;
+    join_sums<Gm::DB, WK>(acc, smem, wave, WR, wk == 0);
   }
+  if (wk > 0 || !row.in) return;
+  store_col<T, Gm::DB>((T*)p.dq + b * p.sdq.b + (int64_t)(hk * p.G + row.g) * p.sdq.h + row.i * p.sdq.s, acc, f, half, p.D);
 }
 
-// dk and dv. Four waves hold 32 NB keys each (K and V as right operands, in registers) and walk the
-// rows of every query head of the group in tiles of 32 IB. A key that takes no part has its own
+// dk and dv. KG x RG = 4 waves: wave (kg, rg) holds 32 keys (K and V as right operands, in registers) and
+// walks the rows of every query head of the group in tiles of 32 IB RG, of which it takes the 32 IB
+// rows rg; a key's waves add their sums at the end. A key that takes no part has its own
 // column throughout, which is written as zeros: no element needs the key mask here.
-template <typename T, int DH, int NB, int IB, int NBUF>
-__global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(Params p) {
+template <typename T, int DH, int KG, int RG, int IB, int NBUF>
+__global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 128 ? 2 : 1) void attn_dkv_kernel(Params p) {
   typedef Geo<T, DH> Gm;
-  constexpr int BR = 32 * IB, TILE = BR * Gm::ROW;
+  constexpr int BR = 32 * IB * RG, KB = 32 * KG, TILE = BR * Gm::ROW;
+  static_assert(KG * RG * 64 == kThreads && (RG == 1 || NBUF * 2 * TILE >= kThreads / 2 * DH * 4), "joining waves reuse the tiles");
   __shared__ __attribute__((aligned(16))) char smem[NBUF * 2 * TILE];
-  __shared__ __attribute__((aligned(16))) float stat[NBUF * 2 * BR];  // lse, delta of the tile's rows
+  __shared__ __attribute__((aligned(16))) float stat[NBUF * 2 * BR];  // lse, -delta of the tile's rows
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int key_tiles = (p.Sk + 128 * NB - 1) / (128 * NB);
-  const int id = xcd_range(blockIdx.x, gridDim.x);
-  const int bh = id / key_tiles;
+  const int kg = wave % KG, rg = wave / KG;
+  const int key_tiles = (p.Sk + KB - 1) / KB;
+  const Place at = place_of(blockIdx.x, p.B * p.Hk, key_tiles);
+  const int bh = at.pair;
   const int b = bh / p.Hk, hk = bh % p.Hk;
-  const int j0 = (id % key_tiles) * 128 * NB;
+  const int j0 = at.tile * KB;
   const int off = p.Sk - p.Sq;
 
   // This workgroup's keys: which take part, and whether any does.
-  int key[NB];
-  bool on[NB];
-  bool any = false;
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    key[n] = j0 + (wave * NB + n) * 32 + (lane & 31);
-    on[n] = key[n] < p.Sk;
-    if (p.mask != nullptr) on[n] = key_on(p.mask, p.mask_dtype, b * p.mask_b + min(key[n], p.Sk - 1)) && on[n];
-    any |= on[n];
-  }
-  const bool wave_any = __any(any);
-  const bool wg_any = __syncthreads_or(any);
+  const int key = j0 + kg * 32 + (lane & 31);
+  bool on = key < p.Sk;
+  if (p.mask != nullptr) on = key_on(p.mask, p.mask_dtype, b * p.mask_b + min(key, p.Sk - 1)) && on;
+  const bool wave_any = __any(on);
+  const bool wg_any = __syncthreads_or(on);
 
-  f32x16 dk[NB][Gm::DB], dv[NB][Gm::DB];
-  ColScale<T> cs[NB];
+  f32x16 dk[Gm::DB], dv[Gm::DB];
+  ColScale<T> cs;
 #pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int db = 0; db < Gm::DB; ++db) dk[n][db] = dv[n][db] = zero16();
+  for (int db = 0; db < Gm::DB; ++db) dk[db] = dv[db] = zero16();
 
   // Row tiles (g, it) of the group's heads; with `causal` those whose last row sees key j0.
   const int ntile = (p.Sq + BR - 1) / BR;
   const int first = p.causal ? min(ntile, max(0, j0 - off) / BR) : 0;
   if (wg_any && first < ntile) {
-    frag_t<T> kf[NB][Gm::NC], vf[NB][Gm::NC];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const int64_t j = min(key[n], p.Sk - 1);
-      load_row<T, DH>(kf[n], (const T*)p.k + b * p.sk.b + hk * p.sk.h + j * p.sk.s, half, p.D, on[n]);
-      load_row<T, DH>(vf[n], (const T*)p.v + b * p.sv.b + hk * p.sv.h + j * p.sv.s, half, p.D, on[n]);
-    }
+    frag_t<T> kf[Gm::NC], vf[Gm::NC];
+    const int64_t j = min(key, p.Sk - 1);
+    load_row<T, DH>(kf, (const T*)p.k + b * p.sk.b + hk * p.sk.h + j * p.sk.s, half, p.D, on);
+    load_row<T, DH>(vf, (const T*)p.v + b * p.sv.b + hk * p.sv.h + j * p.sv.s, half, p.D, on);
     Stage<T, DH, BR, kThreads> qs, gs;
-    float st = 0.0f;  // threads [0, BR): lse, [BR, 2 BR): delta of the staged rows
+    float st = 0.0f;  // threads [0, BR): lse, [BR, 2 BR): -delta of the staged rows
     const auto get = [&](int g, int it) {
       const int64_t h = hk * p.G + g;
-      qs.get((const T*)p.q + b * p.sq.b + h * p.sq.h, p.sq.s, it * BR, p.Sq, p.D);
-      gs.get((const T*)p.dout + b * p.sdo.b + h * p.sdo.h, p.sdo.s, it * BR, p.Sq, p.D);
+      qs.init((const T*)p.q + b * p.sq.b + h * p.sq.h, p.sq.s, p.Sq, p.D);
+      gs.init((const T*)p.dout + b * p.sdo.b + h * p.sdo.h, p.sdo.s, p.Sq, p.D);
+      qs.get(it * BR);
+      gs.get(it * BR);
       if (threadIdx.x < 2 * BR) {
         const int i = it * BR + (threadIdx.x & (BR - 1));
         const float* src = threadIdx.x < BR ? p.lse : p.delta;
-        st = src[((int64_t)b * p.Hq + h) * p.Sq + min(i, p.Sq - 1)];
-        if (threadIdx.x < BR) st = i >= p.Sq || st == -INFINITY ? INFINITY : st - kLog2Up<T>;
-        else st = i >= p.Sq ? 0.0f : st;
+        st = src[((int64_t)b * p.Hq + h) * p.Sq + min(i, p.Sq - 1)];  // used by put() alone: nothing waits for it here
       }
     };
     const auto put = [&](int buf, int it) {
-      uint32_t w[IB];
-#pragma unroll
-      for (int i = 0; i < IB; ++i) {
-        const int left = p.Sq - it * BR - i * 32;
-        w[i] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+      qs.put(smem + buf * 2 * TILE);
+      gs.put(smem + buf * 2 * TILE + TILE);
+      if (threadIdx.x < 2 * BR) {
+        const bool in = it * BR + (int)(threadIdx.x & (BR - 1)) < p.Sq;
+        stat[buf * 2 * BR + threadIdx.x] =
+            threadIdx.x >= BR ? (in ? -st : 0.0f) : in && st != -INFINITY ? st - kLog2Up<T> : INFINITY;
       }
-      qs.template put<IB>(smem + buf * 2 * TILE, w, p.D);
-      gs.template put<IB>(smem + buf * 2 * TILE + TILE, w, p.D);
-      if (threadIdx.x < 2 * BR) stat[buf * 2 * BR + threadIdx.x] = st;
     };
     int g = 0, it = first, buf = 0;
     get(g, it);
@@ -833,73 +880,53 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(Params p) {
         const char* qt = smem + buf * 2 * TILE;
         const char* gt = qt + TILE;
 #pragma unroll
-        for (int ib = 0; ib < IB; ++ib) {
-          f32x16 s[NB], dp[NB];
-#pragma unroll
-          for (int n = 0; n < NB; ++n) s[n] = dp[n] = zero16();
-#pragma unroll
-          for (int c = 0; c < Gm::NC; ++c) {
-            const int at = lds_at<T, DH>(ib * 32 + (lane & 31), 2 * c + half);
-            const frag_t<T> qf = lds_frag<T>(qt + at), gf = lds_frag<T>(gt + at);
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-              s[n] = mma(qf, kf[n][c], s[n]);
-              dp[n] = mma(gf, vf[n][c], dp[n]);
-            }
-          }
+        for (int i = 0; i < IB; ++i) {
+          const int ib = rg * IB + i;
           const float* lse = stat + buf * 2 * BR + ib * 32 + 4 * half;
           const float* del = lse + BR;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x4 l4 = *(const f32x4*)(lse + 8 * q);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int n = 0; n < NB; ++n)
-                s[n][4 * q + e] = __builtin_amdgcn_exp2f(fmaf(s[n][4 * q + e], p.c, -l4[e]));
-          }
-          const int i0 = it * BR + ib * 32 + 4 * half;
-          if (p.causal && it * BR + ib * 32 < j0 + 128 * NB - 1 - off) {
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-              const int lim = key[n] - off - i0;  // rows from here on see the key
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[n][r] = reg_row(r) >= lim ? s[n][r] : 0.0f;
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < Gm::PB; ++c) {
-            frag_t<T> pf[NB];
-#pragma unroll
-            for (int n = 0; n < NB; ++n) pf[n] = pack<T>(s[n], c);
-#pragma unroll
-            for (int db = 0; db < Gm::DB; ++db) {
-              const frag_t<T> gf = lds_cols<T, DH>(gt, ib * 32 + c * Gm::KC, db, lane);
-#pragma unroll
-              for (int n = 0; n < NB; ++n) dv[n][db] = mma(gf, pf[n], dv[n][db]);
-            }
-          }
+          f32x16 start;  // do . v - delta: the sums start at -delta
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const f32x4 d4 = *(const f32x4*)(del + 8 * q);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 4; ++e) start[4 * q + e] = d4[e];
+          }
+          f32x16 s = zero16(), dp = start;
 #pragma unroll
-              for (int n = 0; n < NB; ++n) s[n][4 * q + e] *= dp[n][4 * q + e] - d4[e];
+          for (int c = 0; c < Gm::NC; ++c) {
+            const int at = lds_at<T, DH>(ib * 32 + (lane & 31), 2 * c + half);
+            const frag_t<T> qf = lds_frag<T>(qt + at), gf = lds_frag<T>(gt + at);
+            s = mma(qf, kf[c], s);
+            dp = mma(gf, vf[c], dp);
           }
 #pragma unroll
-          for (int n = 0; n < NB; ++n) cs[n].template apply<Gm::DB>(s[n], dk[n]);
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 l4 = *(const f32x4*)(lse + 8 * q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], p.c, -l4[e]));
+          }
+          const int i0 = it * BR + ib * 32 + 4 * half;
+          if (p.causal && it * BR + ib * 32 < j0 + KB - 1 - off) {
+            const int lim = key - off - i0;  // rows from here on see the key
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = reg_row(r) >= lim ? s[r] : 0.0f;
+          }
 #pragma unroll
           for (int c = 0; c < Gm::PB; ++c) {
-            frag_t<T> df[NB];
+            const frag_t<T> pf = pack<T>(s, c);
 #pragma unroll
-            for (int n = 0; n < NB; ++n) df[n] = pack<T>(s[n], c);
+            for (int db = 0; db < Gm::DB; ++db)
+              dv[db] = mma(lds_cols<T, DH>(gt, ib * 32 + c * Gm::KC, db, lane), pf, dv[db]);
+          }
 #pragma unroll
-            for (int db = 0; db < Gm::DB; ++db) {
-              const frag_t<T> qf = lds_cols<T, DH>(qt, ib * 32 + c * Gm::KC, db, lane);
+          for (int r = 0; r < 16; ++r) s[r] *= dp[r];
+          cs.template apply<Gm::DB>(s, dk);
 #pragma unroll
-              for (int n = 0; n < NB; ++n) dk[n][db] = mma(qf, df[n], dk[n][db]);
-            }
+          for (int c = 0; c < Gm::PB; ++c) {
+            const frag_t<T> df = pack<T>(s, c);
+#pragma unroll
+            for (int db = 0; db < Gm::DB; ++db)
+              dk[db] = mma(lds_cols<T, DH>(qt, ib * 32 + c * Gm::KC, db, lane), df, dk[db]);
           }
         }
       }
@@ -913,38 +940,47 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(Params p) {
       it = itn;
     }
   }
-  const float up = __builtin_amdgcn_exp2f(-kLog2Up<T>);
+  const float fv = __builtin_amdgcn_exp2f(-kLog2Up<T>), fk = on ? p.scale * fv * cs.inv() : 0.0f;
+  // A key that takes no part: zeros, whatever its column held.
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    if (key[n] >= p.Sk) continue;
-    if (!on[n]) {
+  for (int db = 0; db < Gm::DB; ++db)
 #pragma unroll
-      for (int db = 0; db < Gm::DB; ++db) dk[n][db] = dv[n][db] = zero16();
+    for (int r = 0; r < 16; ++r) {
+      dk[db][r] = on ? dk[db][r] * fk : 0.0f;
+      dv[db][r] = on ? dv[db][r] * fv : 0.0f;
     }
-    store_col<T, Gm::DB>((T*)p.dk + b * p.sdk.b + hk * p.sdk.h + key[n] * p.sdk.s, dk[n], p.scale * up * cs[n].inv(), half,
-                         p.D);
-    store_col<T, Gm::DB>((T*)p.dv + b * p.sdv.b + hk * p.sdv.h + key[n] * p.sdv.s, dv[n], up, half, p.D);
+  if constexpr (RG > 1) {
+    join_sums<Gm::DB, RG>(dk, smem, wave, KG, rg == 0);
+    join_sums<Gm::DB, RG>(dv, smem, wave, KG, rg == 0);
   }
+  if (rg > 0 || key >= p.Sk) return;
+  store_col<T, Gm::DB>((T*)p.dk + b * p.sdk.b + hk * p.sdk.h + key * p.sdk.s, dk, 1.0f, half, p.D);
+  store_col<T, Gm::DB>((T*)p.dv + b * p.sdv.b + hk * p.sdv.h + key * p.sdv.s, dv, 1.0f, half, p.D);
 }
 
 // ---- launches ----------------------------------------------------------------------------
 constexpr int64_t kTargetGroups = 512;  // workgroups that fill the chip twice
+constexpr int64_t kFewGroups = 192;     // fewer than that: keys are split
 
 struct FwdPlan {
-  bool few;  // at most 32 rows look at a key head: waves share the keys
-  int nb, splits, tiles_per_split;
+  int rows;  // of a workgroup: 32 (four waves share each tile's keys), 64 (two pairs of waves do) or 128
+  int splits, tiles_per_split;
   int64_t groups;
 };
 
-// Keys are split where there are few workgroups and each has many tiles.
+// fp32 products take long enough that a workgroup of 64 rows (or keys), whose waves share the other
+// side, beats one of 128 where those are few; in 16 bits the joining costs more than it gives (8 x 12
+// heads, 512 x 512: dk and dv 27 us with 128 keys, 33 with 64; fp32, 7 x 12 heads, 181 x 181: 34 and 23).
+bool small_groups(int64_t pairs, int64_t n, int es) { return es == 4 && pairs * cdiv(n, 128) < kTargetGroups; }
+
+// Keys are split over workgroups where those are few and each has many tiles.
 FwdPlan fwd_plan(int64_t B, int64_t Hk, int64_t R, int64_t Sk, int64_t D, int es) {
   FwdPlan f;
-  f.few = R <= 32;
-  f.nb = !f.few && es == 2 && D <= 64 && B * Hk * cdiv(R, 256) >= kTargetGroups ? 2 : 1;
-  const int64_t rows = f.few ? 32 : 128 * f.nb;
-  f.groups = B * Hk * cdiv(R, rows);
-  const int64_t tiles = cdiv(Sk, f.few ? 128 : 64);
-  int64_t n = std::min<int64_t>({cdiv(kTargetGroups, std::max<int64_t>(f.groups, 1)), std::max<int64_t>(tiles / 4, 1), kMaxSplits});
+  f.rows = R <= 32 ? 32 : small_groups(B * Hk, R, es) ? 64 : 128;
+  f.groups = B * Hk * cdiv(R, f.rows);
+  const int64_t tiles = cdiv(Sk, f.rows == 32 ? 128 : f.rows == 64 || D <= 64 ? 64 : 32);
+  const int64_t n = f.groups >= kFewGroups ? 1 : std::min<int64_t>({cdiv(kTargetGroups, std::max<int64_t>(f.groups, 1)),
+                                                                    std::max<int64_t>(tiles / 4, 1), kMaxSplits});
   f.tiles_per_split = (int)cdiv(tiles, n);
   f.splits = (int)cdiv(tiles, f.tiles_per_split);
   return f;
@@ -954,30 +990,42 @@ size_t fwd_bytes(const FwdPlan& f, int64_t B, int64_t Hk, int64_t R, int64_t D) 
   return f.splits > 1 ? (size_t)(B * Hk * f.splits * R) * (size_t)(D + 1) * 4 : 0;
 }
 
+template <typename T, int DH, int WR, int WK, int JB, int NBUF>
+void launch_fwd_rows(const FwdPlan& f, const Params& p, hipStream_t st) {
+  const dim3 grid((unsigned)(f.groups * f.splits)), block(kThreads);
+  if (f.splits > 1) hipLaunchKernelGGL((attn_fwd_kernel<T, DH, WR, WK, JB, NBUF, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((attn_fwd_kernel<T, DH, WR, WK, JB, NBUF, false>), grid, block, 0, st, p);
+}
+
 template <typename T, int DH>
 void launch_fwd(const FwdPlan& f, const Params& p, hipStream_t st) {
-  const dim3 grid((unsigned)(f.groups * f.splits)), block(kThreads);
-  if (f.few) {
-    if (f.splits > 1) hipLaunchKernelGGL((attn_fwd_kernel<T, DH, 1, 1, 4, 1, 1, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((attn_fwd_kernel<T, DH, 1, 1, 4, 1, 1, false>), grid, block, 0, st, p);
-  } else if (f.nb == 1) {
-    if (f.splits > 1) hipLaunchKernelGGL((attn_fwd_kernel<T, DH, 1, 4, 1, 2, 2, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((attn_fwd_kernel<T, DH, 1, 4, 1, 2, 2, false>), grid, block, 0, st, p);
-  } else if constexpr (sizeof(T) == 2 && DH <= 64) {
-    hipLaunchKernelGGL((attn_fwd_kernel<T, DH, 2, 4, 1, 2, 2, false>), grid, block, 0, st, p);
-  }
+  constexpr int JB = DH == 128 ? 1 : 2;  // 32 or 64 keys a tile: what leaves a SIMD two waves' registers
+  if (f.rows == 32) launch_fwd_rows<T, DH, 1, 4, 1, 1>(f, p, st);
+  else if (f.rows == 128) launch_fwd_rows<T, DH, 4, 1, JB, 2>(f, p, st);
+  else if constexpr (sizeof(T) == 4) launch_fwd_rows<T, DH, 2, 2, 1, 2>(f, p, st);
   if (f.splits > 1)
-    hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)cdiv((int64_t)p.B * p.Hk * p.R, kThreads / 64)), block, 0, st, p);
+    hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)cdiv((int64_t)p.B * p.Hk * p.R, kThreads / 64)), dim3(kThreads),
+                       0, st, p);
 }
 
 template <typename T, int DH>
 void launch_bwd(const Params& p, hipStream_t st) {
   const int64_t bh = (int64_t)p.B * p.Hk;
   const dim3 block(kThreads);
-  if (p.R > 0)
-    hipLaunchKernelGGL((attn_dq_kernel<T, DH, 1, 2, 2>), dim3((unsigned)(bh * cdiv(p.R, 128))), block, 0, st, p);
-  if (p.Sk > 0)
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DH, 1, 2, 2>), dim3((unsigned)(bh * cdiv(p.Sk, 128))), block, 0, st, p);
+  constexpr int JB = DH == 128 ? 1 : 2;
+  constexpr int ES = sizeof(T);
+  if (p.R > 0) {
+    if (!small_groups(bh, p.R, ES))
+      hipLaunchKernelGGL((attn_dq_kernel<T, DH, 4, 1, JB, 2>), dim3((unsigned)(bh * cdiv(p.R, 128))), block, 0, st, p);
+    else if constexpr (ES == 4)
+      hipLaunchKernelGGL((attn_dq_kernel<T, DH, 2, 2, 1, 2>), dim3((unsigned)(bh * cdiv(p.R, 64))), block, 0, st, p);
+  }
+  if (p.Sk > 0) {
+    if (!small_groups(bh, p.Sk, ES))
+      hipLaunchKernelGGL((attn_dkv_kernel<T, DH, 4, 1, 2, 2>), dim3((unsigned)(bh * cdiv(p.Sk, 128))), block, 0, st, p);
+    else if constexpr (ES == 4)
+      hipLaunchKernelGGL((attn_dkv_kernel<T, DH, 2, 2, 1, 2>), dim3((unsigned)(bh * cdiv(p.Sk, 64))), block, 0, st, p);
+  }
 }
 
 template <typename T> void fwd_t(const FwdPlan& f, const Params& p, hipStream_t st) {
@@ -1061,8 +1109,7 @@ SPARTON_EXPORT size_t sparton_attention_workspace_bytes(const sparton_attention_
   attn::Params p;
   bool empty;
   if (attn::read_desc(d, nullptr, &p, &empty) != SPARTON_OK || empty || p.R == 0 || p.Sk == 0) return 0;
-  const int es = d->dtype == SPARTON_F32 ? 4 : 2;
-  return attn::fwd_bytes(attn::fwd_plan(p.B, p.Hk, p.R, p.Sk, p.D, es), p.B, p.Hk, p.R, p.D);
+  return attn::fwd_bytes(attn::fwd_plan(p.B, p.Hk, p.R, p.Sk, p.D, d->dtype == SPARTON_F32 ? 4 : 2), p.B, p.Hk, p.R, p.D);
 }
 
 SPARTON_EXPORT int sparton_attention_fwd(const sparton_attention_desc* d, const void* q, const void* k, const void* v,
