@@ -69,9 +69,21 @@ template <int VE> struct Place {
   }
 };
 
-template <int VE> __device__ __forceinline__ void vec_param(float* out, const void* p, int dt, int at) {
+// A lane's elements of weight or bias, in fp32 or in the rows' type.
+template <typename T, int VE> __device__ __forceinline__ void vec_param(float* out, const void* p, int dt, int at) {
+  if (dt == SPARTON_F32) {  // uniform
+    constexpr int N = VE < 4 ? VE : 4;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) out[e] = load_float(p, dt, at + e);
+    for (int i = 0; i < VE; i += N) {
+      const vec_t<float, N> v = load_any<float, N>((const float*)p + at + i);
+#pragma unroll
+      for (int e = 0; e < N; ++e) out[i + e] = v[e];
+    }
+  } else {
+    const vec_t<T, VE> v = load_any<T, VE>((const T*)p + at);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) out[e] = to_f32(v[e]);
+  }
 }
 
 // Sum over the WPR waves of a row, in wave order; result in every lane. `slot` is the row group's
@@ -107,8 +119,8 @@ __global__ __launch_bounds__(64 * (WPR > kFwdWaves ? WPR : kFwdWaves)) void norm
       nx[q] = load_any<T, VE>((const T*)p.x + row * p.D + pl.at);
       if (p.r != nullptr) nr[q] = load_any<T, VE>((const T*)p.r + row * p.D + pl.at);
     }
-    vec_param<VE>(ga[q], p.gamma, p.vec_dtype, pl.at);
-    if (p.beta != nullptr) vec_param<VE>(be[q], p.beta, p.vec_dtype, pl.at);
+    vec_param<T, VE>(ga[q], p.gamma, p.vec_dtype, pl.at);
+    if (p.beta != nullptr) vec_param<T, VE>(be[q], p.beta, p.vec_dtype, pl.at);
     else
 #pragma unroll
       for (int e = 0; e < VE; ++e) be[q][e] = 0.0f;
@@ -194,7 +206,7 @@ __global__ __launch_bounds__(64 * kBwdWaves) void norm_bwd_kernel(Params p) {
 #pragma unroll
   for (int q = 0; q < NP; ++q) {
     const Place<VE> pl(VE * (t + 64 * WPR * q), p.D);
-    vec_param<VE>(ga[q], p.gamma, p.vec_dtype, pl.at);
+    vec_param<T, VE>(ga[q], p.gamma, p.vec_dtype, pl.at);
 #pragma unroll
     for (int e = 0; e < VE; ++e) pg[q][e] = pb[q][e] = 0.0f;
   }
@@ -324,8 +336,8 @@ template <typename T, int VE, int NP, int WPR> void launch(const Params& p, bool
     return;
   }
   constexpr int WAVES = WPR > kFwdWaves ? WPR : kFwdWaves;
-  // Eight workgroups of four waves fill a CU; past that a wave takes several rows.
-  const int64_t groups = std::min<int64_t>(cdiv(p.M, WAVES / WPR), 2048 * kFwdWaves / WAVES);
+  // Past four workgroups of four waves a CU a wave takes several rows: it loads weight and bias once.
+  const int64_t groups = std::min<int64_t>(cdiv(p.M, WAVES / WPR), 1024 * kFwdWaves / WAVES);
   hipLaunchKernelGGL((norm_fwd_kernel<T, VE, NP, WPR>), dim3((unsigned)groups), dim3(64 * WAVES), 0, st, p);
 }
 

@@ -20,8 +20,8 @@ namespace pref {
 
 constexpr int NT = 256;
 constexpr int FIN = 1024;             // threads of the finishing workgroup
-constexpr int64_t kTargetGroups = 2048;
 constexpr int kMaxChunks = 64;
+constexpr int64_t kMaxParts = 16384;
 
 template <typename T> struct Vec {
   static constexpr int N = 16 / sizeof(T);
@@ -36,17 +36,23 @@ template <typename T> __device__ __forceinline__ void store_any(T* p, typename V
 }
 
 struct Plan {
-  int chunks;
-  int64_t span;  // elements of a chunk, a multiple of a workgroup's step
+  int64_t chunks;  // of a row, at most `cap`
+  int64_t span;    // elements of a chunk, a multiple of a workgroup's step
 };
-Plan plan(int64_t B, int64_t V, int es) {
+Plan plan(int64_t V, int es, int64_t cap) {
   const int64_t step = NT * (16 / es);
-  const int64_t want = std::min<int64_t>(kMaxChunks, cdiv(kTargetGroups, B));
   Plan p;
-  p.span = round_up(cdiv(V, want), step);
-  p.chunks = (int)cdiv(V, p.span);
+  p.span = std::max(2 * step, round_up(cdiv(V, cap), step));
+  p.chunks = cdiv(V, p.span);
   return p;
 }
+// Short chunks in the rows' order keep the memory's open pages few: at 500 rows of 250002 in 16 bits
+// margins took 157 us by 2 steps a chunk, 160 by 4, 164 by 8, 176 by 25; gradients 273, 256, 258 us by
+// 1, 2, 4 steps and 302 by 25. One workgroup adds the margins' chunks, so there they are limited.
+Plan margin_plan(int64_t B, int64_t V, int es) {
+  return plan(V, es, std::min<int64_t>(kMaxChunks, std::max<int64_t>(1, kMaxParts / B)));
+}
+Plan grad_plan(int64_t B, int64_t V, int es) { return plan(V, es, INT32_MAX / B); }
 
 // Sum over the workgroup in a fixed order; result in thread 0.
 template <int THREADS> __device__ __forceinline__ float group_sum(float x, float* lds) {
@@ -62,7 +68,7 @@ template <int THREADS> __device__ __forceinline__ float group_sum(float x, float
 // Rows shorter than a vector (V < N) are read element by element.
 template <typename T>
 __global__ __launch_bounds__(NT) void pref_margin_kernel(const T* __restrict__ q, const T* __restrict__ p,
-                                                         const T* __restrict__ n, int64_t V, int chunks, int64_t span,
+                                                         const T* __restrict__ n, int64_t V, int64_t chunks, int64_t span,
                                                          float* __restrict__ part) {
   constexpr int N = Vec<T>::N;
   __shared__ float lds[NT / 64];
@@ -70,7 +76,7 @@ __global__ __launch_bounds__(NT) void pref_margin_kernel(const T* __restrict__ q
   const int64_t base = b * V;
   float a = 0.0f;
   if (V >= N) {
-#pragma unroll 2
+#pragma unroll 4
     for (int64_t v = v0 + threadIdx.x * N; v < v1; v += NT * N) {
       const int64_t at = min(v, V - N);
       const int own = (int)(v - at);
@@ -97,6 +103,7 @@ __global__ __launch_bounds__(FIN) void pref_finish_kernel(const float* __restric
   float total = 0.0f;
   for (int64_t b = threadIdx.x; b < B; b += FIN) {
     float m = 0.0f;
+#pragma unroll 8
     for (int c = 0; c < chunks; ++c) m += part[b * chunks + c];
     m *= inv_t;
     margin[b] = m;
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(FIN) void pref_finish_kernel(const float* __restric
 template <typename T>
 __global__ __launch_bounds__(NT) void pref_grad_kernel(const T* __restrict__ q, const T* __restrict__ p,
                                                        const T* __restrict__ n, const float* __restrict__ coef,
-                                                       const float* __restrict__ grad, int64_t V, int chunks,
+                                                       const float* __restrict__ grad, int64_t V, int64_t chunks,
                                                        int64_t span, T* __restrict__ dq, T* __restrict__ dp,
                                                        T* __restrict__ dn) {
   constexpr int N = Vec<T>::N;
@@ -181,7 +188,7 @@ using namespace sparton;
 
 SPARTON_EXPORT size_t sparton_preference_workspace_bytes(int64_t B, int64_t V, int dtype) {
   if (pref::check(B, V, dtype) != SPARTON_OK) return 0;
-  return (size_t)B * pref::plan(B, V, pref::elem(dtype)).chunks * 4;
+  return (size_t)B * pref::margin_plan(B, V, pref::elem(dtype)).chunks * 4;
 }
 
 SPARTON_EXPORT int sparton_preference_fwd(const void* q, const void* pos, const void* neg, const float* ref_margin,
@@ -200,7 +207,7 @@ SPARTON_EXPORT int sparton_preference_fwd(const void* q, const void* pos, const 
   if (!pref::aligned(q, es) || !pref::aligned(pos, es) || !pref::aligned(neg, es) || !pref::aligned(ref_margin, 4) ||
       !pref::aligned(loss, 4) || !pref::aligned(margin, 4) || !pref::aligned(coef, 4))
     return SPARTON_EALIGN;
-  const pref::Plan pl = pref::plan(B, V, es);
+  const pref::Plan pl = pref::margin_plan(B, V, es);
   if (workspace == nullptr || workspace_bytes < (size_t)B * pl.chunks * 4) return SPARTON_EWORKSPACE;
   if (!pref::aligned(workspace, 256)) return SPARTON_EALIGN;
   hipStream_t st = (hipStream_t)stream;
@@ -210,7 +217,7 @@ SPARTON_EXPORT int sparton_preference_fwd(const void* q, const void* pos, const 
   else pref::margins<float>(q, pos, neg, B, V, pl, part, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL(pref::pref_finish_kernel, dim3(1), dim3(pref::FIN), 0, st, (const float*)part, pl.chunks,
+  hipLaunchKernelGGL(pref::pref_finish_kernel, dim3(1), dim3(pref::FIN), 0, st, (const float*)part, (int)pl.chunks,
                      ref_margin, B, 1.0f / temperature, beta, smoothing, loss, margin, coef);
   return (int)hipGetLastError();
 }
@@ -228,7 +235,7 @@ SPARTON_EXPORT int sparton_preference_bwd(const void* q, const void* pos, const 
   if (!pref::aligned(q, es) || !pref::aligned(pos, es) || !pref::aligned(neg, es) || !pref::aligned(d_q, es) ||
       !pref::aligned(d_pos, es) || !pref::aligned(d_neg, es) || !pref::aligned(coef, 4) || !pref::aligned(grad_loss, 4))
     return SPARTON_EALIGN;
-  const pref::Plan pl = pref::plan(B, V, es);
+  const pref::Plan pl = pref::grad_plan(B, V, es);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == SPARTON_BF16) pref::grads<bf16>(q, pos, neg, coef, grad_loss, B, V, pl, d_q, d_pos, d_neg, st);
   else if (dtype == SPARTON_F16) pref::grads<f16>(q, pos, neg, coef, grad_loss, B, V, pl, d_q, d_pos, d_neg, st);
