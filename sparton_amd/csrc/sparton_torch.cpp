@@ -31,6 +31,8 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <hipblaslt/hipblaslt.h>
@@ -164,6 +166,9 @@ Tensor opt(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(
 Tensor present(const c10::optional<Tensor>& t, const Tensor& like) {
   return t.has_value() ? *t : at::empty({0}, like.options());
 }
+
+// (The operators below the head's pass another argument twice instead, which costs no allocation: its
+// gradient at the absent place is undefined.)
 
 // The forward's dispatch bodies: inference (no autograd) reps.
 Tensor head_encode_cuda(const Tensor& hidden, const Tensor& weight, const c10::optional<Tensor>& bias,
@@ -618,6 +623,21 @@ Loss6 loss_cuda(const Tensor& q, const c10::optional<Tensor>& d, double T, doubl
   return split6(std::get<0>(loss_fwd(q.contiguous(), dd, T, w_ce, w_l1, w_flops)));
 }
 
+// A backward's results where the caller keeps a graph of them (create_graph): the kernels have no
+// second derivative, so that graph raises when it is run, instead of losing a term.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::edge_list inputs = torch::autograd::get_current_node()->next_edges();  // the forward's
+  auto node = std::make_shared<torch::autograd::Error>("sparton: gradients of this operator cannot be differentiated "
+                                                       "again", std::move(inputs));
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach();
+    torch::autograd::set_history(g, node);
+  }
+  return grads;
+}
+
 // ---- attention ----------------------------------------------------------------------------
 
 // [B, H, S, D] with unit inner stride and rows that start on 16 bytes, as the C ABI reads it: the
@@ -634,7 +654,8 @@ Tensor attention_rows(const Tensor& t) {
 
 // [B, S, H, D] in memory, as the projection behind it reads it, seen as [B, H, S, D].
 Tensor attention_like(const Tensor& t) {
-  return at::empty({t.size(0), t.size(2), t.size(1), t.size(3)}, t.options()).transpose(1, 2);
+  const int64_t B = t.size(0), H = t.size(1), S = t.size(2), D = t.size(3);
+  return at::empty_strided({B, H, S, D}, {S * H * D, D, H * D, 1}, t.options());
 }
 
 void set_strides(int64_t* to, const Tensor& t) {
@@ -746,13 +767,13 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
     auto [dq, dk, dv] = attention_grads(grads[0], s[0], s[1], s[2], s[3], s[4], s[5],
                                         ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
     const int64_t D = ctx->saved_data["D"].toInt();
-    return {head_cols(dq, D), head_cols(dk, D), head_cols(dv, D), Tensor(), Tensor(), Tensor(), Tensor()};
+    return once({head_cols(dq, D), head_cols(dk, D), head_cols(dv, D), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
 Tensor attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& mask,
                           bool causal, double scale) {
-  return AttentionFn::apply(q, k, v, present(mask, q), mask.has_value(), causal, scale);
+  return AttentionFn::apply(q, k, v, mask.has_value() ? *mask : q, mask.has_value(), causal, scale);
 }
 Tensor attention_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& mask,
                       bool causal, double scale) {
@@ -833,13 +854,13 @@ struct NormFn : public torch::autograd::Function<NormFn> {
     c10::OptionalDeviceGuard guard(s[0].device());
     const bool has_b = ctx->saved_data["has_b"].toBool();
     auto [dx, dw, db] = norm_grads(grads[0], s[0], s[1], s[2], has_b, s[3], s[4]);
-    return {dx, s[1].defined() ? dx : Tensor(), dw, has_b ? db : Tensor(), Tensor(), Tensor(), Tensor()};
+    return once({dx, s[1].defined() ? dx : Tensor(), dw, has_b ? db : Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
 Tensor norm_autograd(const Tensor& x, const c10::optional<Tensor>& r, const Tensor& w, const c10::optional<Tensor>& b,
                      double eps) {
-  return NormFn::apply(x, present(r, x), w, present(b, w), r.has_value(), b.has_value(), eps);
+  return NormFn::apply(x, r.has_value() ? *r : x, w, b.has_value() ? *b : w, r.has_value(), b.has_value(), eps);
 }
 Tensor norm_cuda(const Tensor& x, const c10::optional<Tensor>& r, const Tensor& w, const c10::optional<Tensor>& b,
                  double eps) {
@@ -911,14 +932,14 @@ struct PreferenceFn : public torch::autograd::Function<PreferenceFn> {
     auto s = ctx->get_saved_variables();
     c10::OptionalDeviceGuard guard(s[0].device());
     auto [dq, dp, dn] = preference_grads(grads[0], s[0], s[1], s[2], s[3]);
-    return {dq, dp, dn, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return once({dq, dp, dn, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
 std::tuple<Tensor, Tensor> preference_autograd(const Tensor& q, const Tensor& p, const Tensor& n,
                                                const c10::optional<Tensor>& ref, double T, double beta,
                                                double smoothing) {
-  auto o = PreferenceFn::apply(q, p, n, present(ref, q), ref.has_value(), T, beta, smoothing);
+  auto o = PreferenceFn::apply(q, p, n, ref.has_value() ? *ref : q, ref.has_value(), T, beta, smoothing);
   return {o[0], o[1]};
 }
 std::tuple<Tensor, Tensor> preference_cuda(const Tensor& q, const Tensor& p, const Tensor& n,
