@@ -585,7 +585,6 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(Params p) {
   const int d = lane * 2;
   float a0 = 0.0f, a1 = 0.0f;
   const float* src = p.part + (bh * p.splits * p.R + r) * p.D + (d < p.D ? d : 0);
-#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float f = lane_f(wt, s);
     const float2 v = *(const float2*)(src + (int64_t)s * p.R * p.D);
@@ -968,15 +967,19 @@ struct FwdPlan {
   int64_t groups;
 };
 
-// fp32 products take long enough that a workgroup of 64 rows (or keys), whose waves share the other
-// side, beats one of 128 where those are few; in 16 bits the joining costs more than it gives (8 x 12
-// heads, 512 x 512: dk and dv 27 us with 128 keys, 33 with 64; fp32, 7 x 12 heads, 181 x 181: 34 and 23).
-bool small_groups(int64_t pairs, int64_t n, int es) { return es == 4 && pairs * cdiv(n, 128) < kTargetGroups; }
+// Workgroups of 64 rows (or keys), whose waves share the other side and join at the end, where those of
+// 128 do not fill the chip once (in fp32, whose products take longer, twice). 12 heads of 1024 x 1024,
+// bf16, 96 groups of 128 rows: dq 26.5 us with 128, 20.3 with 64; dk and dv 27.8 and 20.4.
+// 4 x 12 heads of 512 x 512, 192 groups: 18.6 and 17.6, 18.6 and 18.8; 8 x 12 heads, 384 groups: dk and
+// dv 27 and 33. fp32, 7 x 12 heads of 181 x 181, 168 groups: dk and dv 34 and 23.
+bool small_groups(int64_t pairs, int64_t n, int es) { return pairs * cdiv(n, 128) < (es == 4 ? kTargetGroups : 200); }
 
-// Keys are split over workgroups where those are few and each has many tiles.
+// Keys are split over workgroups where those are few and each has many tiles. In 16 bits long keys are
+// rather split than walked by small groups: 4 heads of 4096 x 4096, split 34 us and 8 to join, by small
+// groups 58; 12 heads of 1024 x 1024, 16 and 7, and 18.
 FwdPlan fwd_plan(int64_t B, int64_t Hk, int64_t R, int64_t Sk, int64_t D, int es) {
   FwdPlan f;
-  f.rows = R <= 32 ? 32 : small_groups(B * Hk, R, es) ? 64 : 128;
+  f.rows = R <= 32 ? 32 : small_groups(B * Hk, R, es) && (es == 4 || Sk <= 2048) ? 64 : 128;
   f.groups = B * Hk * cdiv(R, f.rows);
   const int64_t tiles = cdiv(Sk, f.rows == 32 ? 128 : f.rows == 64 || D <= 64 ? 64 : 32);
   const int64_t n = f.groups >= kFewGroups ? 1 : std::min<int64_t>({cdiv(kTargetGroups, std::max<int64_t>(f.groups, 1)),
@@ -1002,7 +1005,7 @@ void launch_fwd(const FwdPlan& f, const Params& p, hipStream_t st) {
   constexpr int JB = DH == 128 ? 1 : 2;  // 32 or 64 keys a tile: what leaves a SIMD two waves' registers
   if (f.rows == 32) launch_fwd_rows<T, DH, 1, 4, 1, 1>(f, p, st);
   else if (f.rows == 128) launch_fwd_rows<T, DH, 4, 1, JB, 2>(f, p, st);
-  else if constexpr (sizeof(T) == 4) launch_fwd_rows<T, DH, 2, 2, 1, 2>(f, p, st);
+  else launch_fwd_rows<T, DH, 2, 2, 1, 2>(f, p, st);
   if (f.splits > 1)
     hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)cdiv((int64_t)p.B * p.Hk * p.R, kThreads / 64)), dim3(kThreads),
                        0, st, p);
@@ -1013,17 +1016,16 @@ void launch_bwd(const Params& p, hipStream_t st) {
   const int64_t bh = (int64_t)p.B * p.Hk;
   const dim3 block(kThreads);
   constexpr int JB = DH == 128 ? 1 : 2;
-  constexpr int ES = sizeof(T);
   if (p.R > 0) {
-    if (!small_groups(bh, p.R, ES))
+    if (!small_groups(bh, p.R, sizeof(T)))
       hipLaunchKernelGGL((attn_dq_kernel<T, DH, 4, 1, JB, 2>), dim3((unsigned)(bh * cdiv(p.R, 128))), block, 0, st, p);
-    else if constexpr (ES == 4)
+    else
       hipLaunchKernelGGL((attn_dq_kernel<T, DH, 2, 2, 1, 2>), dim3((unsigned)(bh * cdiv(p.R, 64))), block, 0, st, p);
   }
   if (p.Sk > 0) {
-    if (!small_groups(bh, p.Sk, ES))
+    if (!small_groups(bh, p.Sk, sizeof(T)))
       hipLaunchKernelGGL((attn_dkv_kernel<T, DH, 4, 1, 2, 2>), dim3((unsigned)(bh * cdiv(p.Sk, 128))), block, 0, st, p);
-    else if constexpr (ES == 4)
+    else
       hipLaunchKernelGGL((attn_dkv_kernel<T, DH, 2, 2, 1, 2>), dim3((unsigned)(bh * cdiv(p.Sk, 64))), block, 0, st, p);
   }
 }

@@ -361,3 +361,18 @@ def test_rows_outside_a_slice_are_left_alone(device):
     for (n, t), r in zip(bufs.items(), ("out", "dq", "dk", "dv")):
         assert bool((t[:, S:] == 5.0).all()) and bool((t[..., D:] == 5.0).all()), n
         assert torch.equal(t[:, :S, :, :D].transpose(1, 2), want[r]), n
+
+
+@pytest.mark.parametrize("case", [
+    # B, Hq, Hk, Sq, Sk, D, dtype, mask, causal: few and many workgroups on either side
+    (1, 2, 2, 300, 2100, 64, "bf16", "int64", False),
+    (1, 4, 2, 150, 1500, 128, "fp16", "int64 holes", True),
+    (1, 3, 3, 1100, 90, 32, "bf16", "bool", False),
+    (2, 2, 1, 257, 400, 96, "bf16", "int64 left", True),
+    (20, 12, 12, 129, 131, 64, "bf16", "int64 holes empty", True),
+    (17, 12, 12, 140, 70, 128, "fp16", "none", False),
+], ids=str)
+def test_attention_group_sizes(case, device):
+    say(f"case {case}")
+    B, Hq, Hk, Sq, Sk, D, dt, mask, causal = case
+    check(*make(B, Hq, Hk, Sq, Sk, D, dt, mask, device), causal)
