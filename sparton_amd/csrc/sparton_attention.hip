@@ -352,6 +352,15 @@ __device__ __forceinline__ void pos_range(const Params& p, int r0, int r1, int* 
 // Each wave keeps its rows' running maximum and sum; where WK > 1 the results of a row's waves are joined
 // through LDS at the end, and with SPLIT each workgroup takes tiles_per_split tiles of the keys and
 // writes its normalised result and log sum for attn_join_kernel.
+//
+// What bounds it. Long rows (12 heads of 8192 x 8192 x 64, bf16): 270 us, 760 TFLOP/s, half of what a
+// large library product reaches on the card: 32 x 32 scores take eight MFMAs of 32 cycles, 16
+// exponentials of 8, and some 60 maxima, multiply-adds, sums and conversions of 4 cycles or less, and
+// two waves a SIMD overlap the matrix and the vector unit only in part. Short rows (padded 32 x 12 heads
+// of 256 x 256: 18 us) pay for the way to the first tile, four tiles being all there are. A
+// token against a long cache (4 x 8 key heads of 20001 x 128, 9000 or more in use) is bound by memory:
+// 54 us, 4.4 TB/s. The tile's keys pass from memory through registers to two LDS buffers, so that the
+// next tile's loads run under this one's products and a masked key's memory can be replaced by zeros.
 template <typename T, int DH, int WR, int WK, int JB, int NBUF, bool SPLIT>
 __global__ __launch_bounds__(64 * WR * WK, sizeof(T) * DH <= 256 ? 2 : 1) void attn_fwd_kernel(Params p) {
   typedef Geo<T, DH> Gm;
@@ -670,6 +679,9 @@ __device__ __forceinline__ void join_sums(f32x16 (&acc)[DB], char* smem, int wav
 
 // dq, and delta for the next kernel. WR x WK = 4 waves, rows and tiles as in the forward; a row's waves
 // add their dq at the end.
+// The scores come again from q and k rather than from memory: at 12 heads of 8192 x 8192 they would be
+// 1.6 GB to write and read. There it takes 355 us, 870 TFLOP/s, products and vector work overlapping as
+// in the forward; 32 x 12 heads of 256 x 256, padded, 24 us.
 template <typename T, int DH, int WR, int WK, int JB, int NBUF>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_dq_kernel(Params p) {
   typedef Geo<T, DH> Gm;
@@ -813,6 +825,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_
 // walks the rows of every query head of the group in tiles of 32 IB RG, of which it takes the 32 IB
 // rows rg; a key's waves add their sums at the end. A key that takes no part has its own
 // column throughout, which is written as zeros: no element needs the key mask here.
+// A kernel of its own, so that both sums stay in registers and nothing is added by atomics: the price is
+// a second pass over the scores. Every operand but the keys' comes from LDS, twice over: its reads are
+// 73% busy at 12 heads of 8192 x 8192 x 64, 480 us, 860 TFLOP/s. Head size 128 takes the registers of a
+// whole SIMD for one wave: 16 x 32 heads over 8 key heads, 512 x 512 x 128 causal and padded, 202 us,
+// where the forward takes 90 and dq 115 (tiles of 32 rows in place of 64: 248).
 template <typename T, int DH, int KG, int RG, int IB, int NBUF>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 128 ? 2 : 1) void attn_dkv_kernel(Params p) {
   typedef Geo<T, DH> Gm;

