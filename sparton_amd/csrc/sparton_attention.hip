@@ -149,16 +149,21 @@ __device__ __forceinline__ float other_half_sum(float x) {
 // Workgroup w's place among `pairs` (batch row, key head) pairs of `tiles` workgroups each. Consecutive
 // workgroups go to the eight XCDs in turn. A pair's tiles stay on one XCD, whose L2 then holds its keys
 // and values, and the pairs go round the XCDs, so that long and short rows of a padded batch spread
-// evenly; what is left of pairs after whole rounds is cut into eight runs of tiles.
+// evenly; what is left of pairs after whole rounds is cut into eight runs of tiles. With `causal` tiles
+// differ in length: an XCD then takes all its pairs' longest tiles first (by_tile), which leaves the
+// short ones for the end, and what is shared is read from beyond the L2. 16 x 32 heads over 8 key heads,
+// 512 x 512 x 128, padded: forward 95 -> 82 us, dq 120 -> 106, dk and dv 214 -> 148; 8 x 16 heads of
+// 2048 x 2048 x 64: 142 -> 123, 174 -> 150, 223 -> 192. Tiles of one length lose by it: 8 x 12 heads of
+// 512 x 512, dq 23.4 -> 25.5.
 struct Place {
   int pair, tile;
 };
-__device__ __forceinline__ Place place_of(int w, int pairs, int tiles) {
+__device__ __forceinline__ Place place_of(int w, int pairs, int tiles, bool by_tile) {
   const int x = w & 7, k = w >> 3, rounds = pairs >> 3, whole = rounds * tiles;
   Place p;
   if (k < whole) {
-    p.pair = k / tiles * 8 + x;
-    p.tile = k % tiles;
+    p.pair = (by_tile ? k % rounds : k / tiles) * 8 + x;
+    p.tile = by_tile ? k / rounds : k % tiles;
   } else {
     const int n = (pairs & 7) * tiles, i = x * (n >> 3) + min(x, n & 7) + (k - whole);
     p.pair = rounds * 8 + i / tiles;
@@ -372,7 +377,7 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) * DH <= 256 ? 2 : 1) void a
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wr = wave % WR, wk = wave / WR;
   const int row_tiles = (p.R + 32 * WR - 1) / (32 * WR);
-  const Place at = place_of(blockIdx.x, p.B * p.Hk, SPLIT ? row_tiles * p.splits : row_tiles);
+  const Place at = place_of(blockIdx.x, p.B * p.Hk, SPLIT ? row_tiles * p.splits : row_tiles, p.causal);
   const int split = SPLIT ? at.tile % p.splits : 0;
   const int bh = at.pair, tile = row_tiles - 1 - (SPLIT ? at.tile / p.splits : at.tile);  // causal: longest first
   const int b = bh / p.Hk, hk = bh % p.Hk;
@@ -691,7 +696,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wr = wave % WR, wk = wave / WR;
   const int row_tiles = (p.R + RB - 1) / RB;
-  const Place at = place_of(blockIdx.x, p.B * p.Hk, row_tiles);
+  const Place at = place_of(blockIdx.x, p.B * p.Hk, row_tiles, p.causal);
   const int bh = at.pair, tile = row_tiles - 1 - at.tile;
   const int b = bh / p.Hk, hk = bh % p.Hk;
   const int r0 = tile * RB;
@@ -826,10 +831,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_
 // rows rg; a key's waves add their sums at the end. A key that takes no part has its own
 // column throughout, which is written as zeros: no element needs the key mask here.
 // A kernel of its own, so that both sums stay in registers and nothing is added by atomics: the price is
-// a second pass over the scores. Every operand but the keys' comes from LDS, twice over: its reads are
-// 73% busy at 12 heads of 8192 x 8192 x 64, 480 us, 860 TFLOP/s. Head size 128 takes the registers of a
-// whole SIMD for one wave: 16 x 32 heads over 8 key heads, 512 x 512 x 128 causal and padded, 202 us,
-// where the forward takes 90 and dq 115 (tiles of 32 rows in place of 64: 248).
+// a second pass over the scores. At 12 heads of 8192 x 8192 x 64 it takes 480 us, 860 TFLOP/s: the
+// matrix unit is busy 42% of the time and the LDS 59%, conflicts among that 11. Head size 128 takes the
+// registers of a whole SIMD for one wave: 16 x 32 heads over 8 key heads, 512 x 512 x 128 causal and
+// padded, 148 us, where the forward takes 82 and dq 106 (tiles of 32 rows in place of 64 were slower by
+// a quarter).
 template <typename T, int DH, int KG, int RG, int IB, int NBUF>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 128 ? 2 : 1) void attn_dkv_kernel(Params p) {
   typedef Geo<T, DH> Gm;
@@ -840,7 +846,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 128 ? 2 : 1) void attn_
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int kg = wave % KG, rg = wave / KG;
   const int key_tiles = (p.Sk + KB - 1) / KB;
-  const Place at = place_of(blockIdx.x, p.B * p.Hk, key_tiles);
+  const Place at = place_of(blockIdx.x, p.B * p.Hk, key_tiles, p.causal);
   const int bh = at.pair;
   const int b = bh / p.Hk, hk = bh % p.Hk;
   const int j0 = at.tile * KB;
