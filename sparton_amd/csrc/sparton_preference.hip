@@ -6,8 +6,8 @@
 // Both passes are bound by memory. Forward: each workgroup sums one chunk of one row's q (p - n) (the
 // difference first: two close scores would cancel), and one workgroup adds the chunks in order and
 // forms margins, loss and c. Backward: one pass over the rows. At 500 rows of 250002 in bf16 the margins
-// take 148 to 160 us (4.7 TB/s or more; a copy reaches 4.9), the one workgroup 7, and the gradients 237 to
-// 257 (5.8 or more); at 32 rows of 30522, 3.5, 2.1 and 4.2 us, mostly launches.
+// take 164 us (4.6 TB/s; a copy reaches 4.9), the one workgroup 5.6, and the gradients 257 (5.8); at 32 rows
+// of 30522, 3.4, 2.2 and 4.2 us, mostly launches.
 // Rows of V elements need no alignment (V = 30522 in 16 bits: rows start on 4 bytes): global vector
 // accesses take any address, and a row's last vector is moved back to end with the row.
 
@@ -23,7 +23,7 @@ namespace pref {
 constexpr int NT = 256;
 constexpr int FIN = 1024;             // threads of the finishing workgroup
 constexpr int kMaxChunks = 64;
-constexpr int64_t kMaxParts = 16384;
+constexpr int64_t kMaxParts = 8192;
 
 template <typename T> struct Vec {
   static constexpr int N = 16 / sizeof(T);
@@ -50,7 +50,8 @@ Plan plan(int64_t V, int es, int64_t cap) {
 }
 // Short chunks in the rows' order keep the memory's open pages few: at 500 rows of 250002 in 16 bits
 // margins took 157 us by 2 steps a chunk, 160 by 4, 164 by 8, 176 by 25; gradients 273, 256, 258 us by
-// 1, 2, 4 steps and 302 by 25. One workgroup adds the margins' chunks, so there they are limited.
+// 1, 2, 4 steps and 302 by 25. One workgroup adds the margins' chunks (4.8, 5.6, 7,
+// 9.5 us at 25, 8, 4 and 2 steps), so there they are limited.
 Plan margin_plan(int64_t B, int64_t V, int es) {
   return plan(V, es, std::min<int64_t>(kMaxChunks, std::max<int64_t>(1, kMaxParts / B)));
 }
