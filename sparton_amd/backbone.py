@@ -14,7 +14,7 @@ attention probabilities, sliding windows, position biases, masks that are not on
 """
 from __future__ import annotations
 
-import types
+import functools
 from typing import Optional
 
 import torch
@@ -67,7 +67,8 @@ def key_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_func
 
 
 def register() -> None:
-    """Make attn_implementation="sparton" known to transformers."""
+    """Make attn_implementation="sparton" known to transformers: once per process, before a switched model
+    that was pickled elsewhere, or saved with its config, runs there."""
     from transformers import AttentionInterface
     from transformers.masking_utils import AttentionMaskInterface
     AttentionInterface.register(NAME, attention_forward)
@@ -78,16 +79,29 @@ def _residual_norm(self, hidden_states: Tensor, input_tensor: Tensor) -> Tensor:
     return self.LayerNorm(self.dropout(self.dense(hidden_states)), input_tensor)
 
 
+class _BlockForward(functools.partial):
+    """A block's forward bound to it. A method of a function that its class does not have could not be pickled."""
+
+    @property
+    def __self__(self):
+        return self.args[0]
+
+
 def use_in_backbone(model: nn.Module) -> nn.Module:
-    """Switch a transformers model (or a masked LM with its head) in place; returns it."""
+    """Switch a transformers model (or a masked LM with its head) in place; returns it. A model that
+    cannot be switched raises and stays as it was."""
+    norms = [(module, name, SpartonLayerNorm.of(child)) for module in model.modules()
+             for name, child in module.named_children()
+             if type(child) is nn.LayerNorm and len(child.normalized_shape) == 1 and child.weight is not None]
     register()
+    before = model.config._attn_implementation
     model.set_attn_implementation(NAME)
     if model.config._attn_implementation != NAME:
+        model.set_attn_implementation(before)
         raise ValueError(f"{type(model).__name__} does not take its attention from transformers' registry")
-    for module in list(model.modules()):
-        for name, child in list(module.named_children()):
-            if type(child) is nn.LayerNorm and len(child.normalized_shape) == 1 and child.weight is not None:
-                setattr(module, name, SpartonLayerNorm.of(child))
+    for module, name, norm in norms:
+        setattr(module, name, norm)
+    for module in model.modules():
         if type(module).__name__ in _RESIDUAL_BLOCKS:
-            module.forward = types.MethodType(_residual_norm, module)
+            module.forward = _BlockForward(_residual_norm, module)
     return model

@@ -50,8 +50,8 @@ Plan plan(int64_t V, int es, int64_t cap) {
 }
 // Short chunks in the rows' order keep the memory's open pages few: at 500 rows of 250002 in 16 bits
 // margins took 157 us by 2 steps a chunk, 160 by 4, 164 by 8, 176 by 25; gradients 273, 256, 258 us by
-// 1, 2, 4 steps and 302 by 25. One workgroup adds the margins' chunks (4.8, 5.6, 7,
-// 9.5 us at 25, 8, 4 and 2 steps), so there they are limited.
+// 1, 2, 4 steps and 302 by 25. One workgroup adds the margins' chunks (5 of a row
+// in 4.8 us, 16 in 5.6, 31 in 7), so there they are limited.
 Plan margin_plan(int64_t B, int64_t V, int es) {
   return plan(V, es, std::min<int64_t>(kMaxChunks, std::max<int64_t>(1, kMaxParts / B)));
 }

@@ -7,6 +7,7 @@ Tolerances, fp32 throughout: hidden states rtol 1e-4, atol 1e-5; gradients by th
 test_hf_integration.py (error against the gradient's largest magnitude, with a floor of 1e-4 of the
 largest of all, at most 1e-3; torch's fp32 CPU result sits within 1e-6 of float64 by it)."""
 import copy
+import pickle
 
 import pytest
 import torch
@@ -56,6 +57,29 @@ def test_switching_keeps_parameters_and_names(kind):
     for a, b in zip(llm.modules(), twin.modules()):
         if "forward" in a.__dict__:
             assert b.forward.__self__ is b
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_switched_model_pickles(kind):
+    llm = use_in_backbone(tiny(kind))
+    twin = pickle.loads(pickle.dumps(llm))
+    assert list(twin.state_dict()) == list(llm.state_dict())
+    blocks = 0
+    for a, b in zip(llm.modules(), twin.modules()):
+        assert type(a) is type(b)
+        if "forward" in a.__dict__:
+            assert b.forward.__self__ is b and b is not a
+            blocks += 1
+    assert blocks == (0 if kind == "distilbert" else 4)
+
+
+def test_a_refused_model_stays_as_it_was():
+    llm = tiny("bert")
+    llm.extra = nn.LayerNorm(16385)  # wider than the kernel's rows
+    with pytest.raises(ValueError, match="16384"):
+        use_in_backbone(llm)
+    assert llm.config._attn_implementation == "eager"
+    assert not any(type(m) is sparton_amd.SpartonLayerNorm or "forward" in m.__dict__ for m in llm.modules())
 
 
 def test_refusals():
