@@ -627,7 +627,9 @@ Loss6 loss_cuda(const Tensor& q, const c10::optional<Tensor>& d, double T, doubl
 // second derivative, so that graph raises when it is run, instead of losing a term.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
-  torch::autograd::edge_list inputs = torch::autograd::get_current_node()->next_edges();  // the forward's
+  const auto current = torch::autograd::get_current_node();  // none where grad_fn is called by hand
+  torch::autograd::edge_list inputs;                         // the forward's
+  if (current != nullptr) inputs = current->next_edges();
   auto node = std::make_shared<torch::autograd::Error>("sparton: gradients of this operator cannot be differentiated "
                                                        "again", std::move(inputs));
   for (Tensor& g : grads) {

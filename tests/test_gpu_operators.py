@@ -59,6 +59,20 @@ def test_a_second_derivative_is_refused(name, device):
         torch.autograd.grad(grads[0].float().sum(), leaves[0])
 
 
+@pytest.mark.parametrize("name", NAMES)
+def test_a_backward_called_by_hand(name, device):
+    """Outside the autograd engine, with and without grad mode."""
+    say(f"grad_fn of {name}")
+    f, leaves = calls(device)[name]
+    want = both(f, leaves)[1:]
+    out = f(*[t.detach().requires_grad_() for t in leaves])
+    grads = [torch.ones_like(out)] + [None] * (name == "preference_loss")  # that node's second output: the margins
+    for mode in (False, True):
+        with torch.set_grad_enabled(mode):
+            got = [g for g in out.grad_fn(*grads) if g is not None]
+        assert all(torch.equal(g.detach(), w) for g, w in zip(got, want)) and len(got) >= len(want)
+
+
 def test_calls_at_once_on_two_streams(device):
     say("two streams")
     first, second = calls(device, 0), calls(device, 100)
