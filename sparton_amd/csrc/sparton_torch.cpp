@@ -760,7 +760,8 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["D"] = q_in.size(3);
-    return head_cols(out, q_in.size(3));
+    // A narrower result is a copy: autograd would not see `out` change with a view of it made here.
+    return out.size(3) == q_in.size(3) ? out : head_cols(out, q_in.size(3)).clone();
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return variable_list(7);

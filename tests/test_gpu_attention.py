@@ -376,3 +376,20 @@ def test_attention_group_sizes(case, device):
     say(f"case {case}")
     B, Hq, Hk, Sq, Sk, D, dt, mask, causal = case
     check(*make(B, Hq, Hk, Sq, Sk, D, dt, mask, device), causal)
+
+
+@pytest.mark.parametrize("D", [20, 64])
+def test_output_changed_in_place(D, device):
+    """An output that its user overwrites: the gradients are right, or the backward says what happened."""
+    say(f"in place, {D}")
+    q, k, v, m, do = make(2, 2, 2, 33, 40, D, "bf16", "int64", device)
+    want = run(q, k, v, m, do, False)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention(*leaves, m)
+    out.mul_(0.5)
+    try:
+        grads = torch.autograd.grad(out, leaves, do * 2)  # powers of two: the same bits
+    except RuntimeError as e:
+        assert "inplace" in str(e)
+    else:
+        assert all(torch.equal(g, want[n]) for g, n in zip(grads, ("dq", "dk", "dv")))
