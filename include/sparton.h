@@ -300,7 +300,8 @@ int sparton_loss_bwd_terms(const void* q, const void* d, const float* probs,
  * take no part reach no output, whatever they are. Sums, maxima and log sums are fp32.
  * Strides are in elements; the innermost is 1. Bases are 16-byte aligned, and so are the strides
  * (multiples of 8 elements, 4 for fp32) of dimensions larger than 1. D * element size is a multiple
- * of 16 bytes and D <= 128; 0 < scale < infinity. Sizes whose rows or workgroups pass 32 bits are
+ * of 16 bytes and D <= 128; 0 < scale < infinity. Sizes whose rows pass 32 bits, or whose workgroups (one
+ * for up to 128 packed rows of a key head, in the backward also for 128 keys) reach 2^24, are
  * SPARTON_EUNSUPPORTED; offsets are 64-bit.
  */
 typedef struct sparton_attention_desc {

@@ -27,6 +27,8 @@ namespace attn {
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kThreads = 256;
 constexpr int kMaxSplits = 64;  // the combining wave holds one split's weight per lane
+// A launch holds fewer than 2^32 threads (past that, workgroups were left out without an error).
+constexpr int64_t kMaxGroups = (((int64_t)1 << 32) - 1) / kThreads;
 
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 
@@ -1084,7 +1086,7 @@ bool tensor_ok(const void* p, const int64_t* s, int64_t B, int64_t H, int64_t S,
 }
 
 // Status of a description, and its parameters: SPARTON_OK with *empty set where there is nothing to do.
-int read_desc(const sparton_attention_desc* d, const void* mask, Params* p, bool* empty) {
+int read_desc(const sparton_attention_desc* d, const void* mask, bool bwd, Params* p, bool* empty) {
   *empty = false;
   if (d == nullptr) return SPARTON_EINVAL;
   if (d->B < 0 || d->Hq < 0 || d->Hk < 0 || d->Sq < 0 || d->Sk < 0 || d->D <= 0) return SPARTON_EINVAL;
@@ -1104,6 +1106,10 @@ int read_desc(const sparton_attention_desc* d, const void* mask, Params* p, bool
   if (d->B > lim || d->Hq > lim || d->Sq > lim / 2 || d->Sk > lim / 2 || G > (lim / 2) / std::max<int64_t>(d->Sq, 1))
     return SPARTON_EUNSUPPORTED;
   if (d->B > lim / d->Hq || d->B * d->Hk > (lim / kMaxSplits) / std::max({cdiv(G * d->Sq, 32), cdiv(d->Sk, 128), (int64_t)1}))
+    return SPARTON_EUNSUPPORTED;
+  // Workgroups of 128 rows, and of 128 keys for dk and dv; of 64 there are less than a thousand. Up to 32
+  // packed rows are one workgroup either way.
+  if (d->B * d->Hk > kMaxGroups / std::max({cdiv(G * d->Sq, 128), bwd ? cdiv(d->Sk, 128) : 1, (int64_t)1}))
     return SPARTON_EUNSUPPORTED;
   p->mask = mask;
   p->sq = strides(d->q);
@@ -1141,7 +1147,7 @@ using namespace sparton;
 SPARTON_EXPORT size_t sparton_attention_workspace_bytes(const sparton_attention_desc* d) {
   attn::Params p;
   bool empty;
-  if (attn::read_desc(d, nullptr, &p, &empty) != SPARTON_OK || empty || p.R == 0 || p.Sk == 0) return 0;
+  if (attn::read_desc(d, nullptr, false, &p, &empty) != SPARTON_OK || empty || p.R == 0 || p.Sk == 0) return 0;
   return attn::fwd_bytes(attn::fwd_plan(p.B, p.Hk, p.R, p.Sk, p.D, d->dtype == SPARTON_F32 ? 4 : 2), p.B, p.Hk, p.R, p.D);
 }
 
@@ -1150,7 +1156,7 @@ SPARTON_EXPORT int sparton_attention_fwd(const sparton_attention_desc* d, const 
                                          size_t workspace_bytes, void* stream) {
   attn::Params p = {};
   bool empty;
-  const int rc = attn::read_desc(d, mask, &p, &empty);
+  const int rc = attn::read_desc(d, mask, false, &p, &empty);
   if (rc != SPARTON_OK || empty || p.R == 0) return rc;
   if (q == nullptr || out == nullptr || (p.Sk > 0 && (k == nullptr || v == nullptr))) return SPARTON_EINVAL;
   const int es = d->dtype == SPARTON_F32 ? 4 : 2;
@@ -1182,7 +1188,7 @@ SPARTON_EXPORT int sparton_attention_fwd(const sparton_attention_desc* d, const 
 SPARTON_EXPORT size_t sparton_attention_bwd_workspace_bytes(const sparton_attention_desc* d) {
   attn::Params p;
   bool empty;
-  if (attn::read_desc(d, nullptr, &p, &empty) != SPARTON_OK || empty) return 0;
+  if (attn::read_desc(d, nullptr, true, &p, &empty) != SPARTON_OK || empty) return 0;
   return (size_t)p.B * p.Hq * p.Sq * 4;
 }
 
@@ -1192,7 +1198,7 @@ SPARTON_EXPORT int sparton_attention_bwd(const sparton_attention_desc* d, const 
                                          void* stream) {
   attn::Params p = {};
   bool empty;
-  const int rc = attn::read_desc(d, mask, &p, &empty);
+  const int rc = attn::read_desc(d, mask, true, &p, &empty);
   if (rc != SPARTON_OK || empty) return rc;
   if ((p.R > 0 && (q == nullptr || out == nullptr || lse == nullptr || d_out == nullptr || d_q == nullptr)) ||
       (p.Sk > 0 && (k == nullptr || v == nullptr || d_k == nullptr || d_v == nullptr)))

@@ -81,6 +81,38 @@ def test_attention_sizes_with_nothing_to_do():
     assert L.sparton_attention_workspace_bytes(desc(B=1, q=(7, 64, 256))) >= 0
 
 
+THREADS = 1 << 32  # a launch of as many threads leaves workgroups out, and reports nothing
+MOST = THREADS // 256 - 1
+
+
+@pytest.mark.parametrize("sizes", [
+    dict(B=1 << 24, Hq=1, Hk=1, Sq=1, Sk=1),             # a workgroup a (batch row, key head)
+    dict(B=1 << 12, Hq=1 << 12, Hk=1 << 12, Sq=1, Sk=1),
+    dict(B=1 << 23, Hq=2, Hk=1, Sq=100, Sk=1),           # two workgroups of 128 rows each
+    dict(B=1 << 22, Hq=1, Hk=1, Sq=385, Sk=1),
+], ids=str)
+def test_attention_launches_hold_fewer_than_32_bits_of_threads(sizes):
+    assert fwd(sizes) == -3 and bwd(sizes) == -3
+    assert _lib.load().sparton_attention_workspace_bytes(desc(**sizes)) == 0
+    assert _lib.load().sparton_attention_bwd_workspace_bytes(desc(**sizes)) == 0
+
+
+def test_attention_backward_launches_over_keys():
+    """dk and dv take a workgroup for 128 keys, where the forward walks any number of keys in one."""
+    d = dict(B=1 << 22, Hq=1, Hk=1, Sq=1, Sk=385)
+    assert bwd(d) == -3 and _lib.load().sparton_attention_bwd_workspace_bytes(desc(**d)) == 0
+    assert fwd(d, ws=None, q=P + 8) == -2                # accepted so far: the next check is what answers
+    assert bwd(dict(d, Sk=384, B=(1 << 22) + ((1 << 22) - 1) // 3), q=P + 8) == -2
+
+
+@pytest.mark.parametrize("sizes", [
+    dict(B=MOST, Hq=1, Hk=1, Sq=1, Sk=1), dict(B=MOST, Hq=1, Hk=1, Sq=32, Sk=128),
+    dict(B=1, Hq=1, Hk=1, Sq=1 << 29, Sk=1), dict(B=1, Hq=1, Hk=1, Sq=1, Sk=(1 << 30) - 1),
+], ids=str)
+def test_attention_sizes_below_that_are_taken(sizes):
+    assert fwd(sizes, q=P + 8) == -2 and bwd(sizes, q=P + 8) == -2
+
+
 def test_attention_workspace():
     L = _lib.load()
     need = lambda **kw: L.sparton_attention_workspace_bytes(desc(**kw))
