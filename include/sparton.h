@@ -361,7 +361,7 @@ int sparton_layer_norm_bwd(const void* dy, const void* x, const void* residual, 
  *     m = (q.pos - q.neg) / temperature;   z = beta (m - ref_margin)
  *     loss = mean over rows of -(1 - smoothing) log sigma(z) - smoothing log sigma(-z)
  * ref_margin [B] (fp32; NULL: zeros) holds the reference model's margins. temperature and beta are
- * positive and finite, 0 <= smoothing <= 0.5. Sums are fp32, deterministic. No counterpart in the
+ * positive and finite, 0 <= smoothing <= 0.5. B is below 2^24. Sums are fp32, deterministic. No counterpart in the
  * reference, which trains on the in-batch loss above alone (training/train.py:164-197).
  */
 size_t sparton_preference_workspace_bytes(int64_t B, int64_t V, int dtype);

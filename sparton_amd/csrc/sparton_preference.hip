@@ -24,6 +24,9 @@ constexpr int NT = 256;
 constexpr int FIN = 1024;             // threads of the finishing workgroup
 constexpr int kMaxChunks = 64;
 constexpr int64_t kMaxParts = 8192;
+// A launch holds fewer than 2^32 threads (past that, workgroups were left out without an error), and a
+// row takes at least one workgroup.
+constexpr int64_t kMaxGroups = (((int64_t)1 << 32) - 1) / NT;
 
 template <typename T> struct Vec {
   static constexpr int N = 16 / sizeof(T);
@@ -55,7 +58,7 @@ Plan plan(int64_t V, int es, int64_t cap) {
 Plan margin_plan(int64_t B, int64_t V, int es) {
   return plan(V, es, std::min<int64_t>(kMaxChunks, std::max<int64_t>(1, kMaxParts / B)));
 }
-Plan grad_plan(int64_t B, int64_t V, int es) { return plan(V, es, INT32_MAX / B); }
+Plan grad_plan(int64_t B, int64_t V, int es) { return plan(V, es, kMaxGroups / B); }
 
 // Sum over the workgroup in a fixed order; result in thread 0.
 template <int THREADS> __device__ __forceinline__ float group_sum(float x, float* lds) {
@@ -165,7 +168,7 @@ __global__ __launch_bounds__(NT) void pref_grad_kernel(const T* __restrict__ q, 
 
 int check(int64_t B, int64_t V, int dtype) {
   if (B < 1 || V < 1 || dtype < SPARTON_F32 || dtype > SPARTON_F16) return SPARTON_EINVAL;
-  return B > INT32_MAX / kMaxChunks || V > INT32_MAX ? SPARTON_EUNSUPPORTED : SPARTON_OK;
+  return B > kMaxGroups || V > INT32_MAX ? SPARTON_EUNSUPPORTED : SPARTON_OK;
 }
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int elem(int dtype) { return dtype == SPARTON_F32 ? 4 : 2; }

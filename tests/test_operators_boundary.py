@@ -257,6 +257,14 @@ def test_preference_bwd_checks(kw, code):
     assert pbwd(**kw) == code
 
 
+def test_preference_launches_hold_fewer_than_32_bits_of_threads():
+    size = _lib.load().sparton_preference_workspace_bytes
+    for B in (MOST + 1, (1 << 25) - 1):
+        assert pfwd(B=B) == -3 and pbwd(B=B) == -3 and size(B, 100, 1) == 0
+    assert pfwd(B=MOST, q=P + 1) == -2 and pbwd(B=MOST, q=P + 1) == -2
+    assert size(MOST, 100, 1) == MOST * 4
+
+
 def test_preference_workspace():
     size = _lib.load().sparton_preference_workspace_bytes
     assert size(0, 10, 1) == 0 and size(4, 0, 1) == 0 and size(4, 10, 9) == 0
