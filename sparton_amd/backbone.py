@@ -50,8 +50,9 @@ def attention_forward(module: nn.Module, query: Tensor, key: Tensor, value: Tens
 
 
 def key_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function=None, attention_mask=None, **kwargs):
-    """The registry's mask: the tokenizer's [B, kv_length] as it is, or None. What is causal is known to the
-    attention itself."""
+    """The registry's mask: the tokenizer's values of the keys, [B, kv_length], or None. Its column j is
+    position j, and the keys are the positions from kv_offset on; a position past its last column takes no
+    part. What is causal is known to the attention itself."""
     from transformers.masking_utils import bidirectional_mask_function, causal_mask_function
     if mask_function not in (None, bidirectional_mask_function, causal_mask_function):
         raise ValueError("sparton attention supports plain bidirectional and causal attention over padded batches; "
@@ -61,8 +62,9 @@ def key_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_func
         raise ValueError("sparton attention's causal rows are the last ones of the keys; this cache has room behind them")
     if attention_mask is None:
         return None
-    if attention_mask.shape[-1] > kv_length:
-        attention_mask = attention_mask[:, -kv_length:]
+    if kv_offset != 0 or attention_mask.shape[-1] != kv_length:
+        attention_mask = attention_mask[:, kv_offset:kv_offset + kv_length]
+        attention_mask = nn.functional.pad(attention_mask, (0, kv_length - attention_mask.shape[-1]))
     return attention_mask
 
 

@@ -111,6 +111,49 @@ def test_training_with_attention_dropout_is_refused():
         model.train()(torch.ones(1, 4, dtype=torch.long))
 
 
+def plain_attention(q, k, v, mask=None, *, causal=False, scale=None):
+    """The kernels' formula in torch, for CPU runs."""
+    from _attention_ref import allowed_pairs
+    G = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+    on = allowed_pairs(q.shape[0], q.shape[2], k.shape[2], mask, causal, q.device)
+    s = torch.where(on, scale * (q @ k.transpose(-1, -2)), -torch.inf)
+    return torch.softmax(s, -1).nan_to_num(0.0) @ v
+
+
+def tiny_decoder():
+    """(with torch's attention, switched), both on the CPU."""
+    from transformers import LlamaConfig, LlamaModel
+    torch.manual_seed(0)
+    ref = LlamaModel(LlamaConfig(vocab_size=300, hidden_size=128, num_hidden_layers=2, num_attention_heads=4,
+                                 num_key_value_heads=2, intermediate_size=256, attn_implementation="eager")).eval()
+    return ref, use_in_backbone(copy.deepcopy(ref))
+
+
+def left_padded(B, S, seed):
+    g = torch.Generator().manual_seed(seed)
+    mask = torch.ones(B, S, dtype=torch.long)
+    for b in range(1, B):
+        mask[b, :b + 1] = 0
+    return torch.randint(0, 300, (B, S), generator=g), mask
+
+
+def test_the_masks_columns_are_the_keys(monkeypatch):
+    """A mask over more columns than there are keys, or fewer: the first ones are the keys', as in torch's attention."""
+    m = torch.tensor([[0, 1, 1, 1, 0, 1], [1, 1, 0, 1, 1, 1]])
+    assert torch.equal(key_mask(2, 4, 4, attention_mask=m), m[:, :4])
+    assert torch.equal(key_mask(2, 2, 3, q_offset=3, kv_offset=2, attention_mask=m), m[:, 2:5])
+    assert torch.equal(key_mask(2, 4, 8, attention_mask=m), nn.functional.pad(m, (0, 2)))
+    assert torch.equal(key_mask(2, 4, 7, attention_mask=m != 0), nn.functional.pad(m != 0, (0, 1)))
+    monkeypatch.setattr("sparton_amd.backbone.attention", plain_attention)
+    ref, ours = tiny_decoder()
+    ids, mask = left_padded(3, 12, seed=1)
+    with torch.no_grad():
+        a, b = (m(ids[:, :6], mask).last_hidden_state for m in (ref, ours))
+    on = mask[:, :6].bool()
+    torch.testing.assert_close(b[on], a[on], rtol=1e-4, atol=1e-5)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("padded", [True, False])
