@@ -52,19 +52,23 @@ def attention_forward(module: nn.Module, query: Tensor, key: Tensor, value: Tens
 def key_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function=None, attention_mask=None, **kwargs):
     """The registry's mask: the tokenizer's values of the keys, [B, kv_length], or None. Its column j is
     position j, and the keys are the positions from kv_offset on; a position past its last column takes no
-    part. What is causal is known to the attention itself."""
+    part. What is causal is known to the attention itself, whose rows are the last ones of the keys: behind
+    several rows there may be no room in a cache allocated ahead; behind one row the room is masked, from the
+    cache's length on the device, if that is where the cache keeps it."""
     from transformers.masking_utils import bidirectional_mask_function, causal_mask_function
     if mask_function not in (None, bidirectional_mask_function, causal_mask_function):
         raise ValueError("sparton attention supports plain bidirectional and causal attention over padded batches; "
                          "this model asks for another pattern (windows, packed sequences)")
-    if (mask_function is causal_mask_function and isinstance(q_offset, int) and isinstance(kv_offset, int)
-            and q_offset + q_length != kv_offset + kv_length):
+    one = mask_function is causal_mask_function and q_length == 1 and isinstance(q_offset, Tensor)
+    if mask_function is causal_mask_function and not one and int(q_offset) + q_length != kv_offset + kv_length:
         raise ValueError("sparton attention's causal rows are the last ones of the keys; this cache has room behind them")
-    if attention_mask is None:
-        return None
-    if kv_offset != 0 or attention_mask.shape[-1] != kv_length:
+    if attention_mask is not None and (kv_offset != 0 or attention_mask.shape[-1] != kv_length):
         attention_mask = attention_mask[:, kv_offset:kv_offset + kv_length]
         attention_mask = nn.functional.pad(attention_mask, (0, kv_length - attention_mask.shape[-1]))
+    if one:
+        device = kwargs.get("device", q_offset.device)
+        seen = (torch.arange(kv_offset, kv_offset + kv_length, device=device) <= q_offset).expand(batch_size, -1)
+        attention_mask = seen if attention_mask is None else seen & (attention_mask != 0)
     return attention_mask
 
 

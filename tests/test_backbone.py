@@ -154,6 +154,49 @@ def test_the_masks_columns_are_the_keys(monkeypatch):
     torch.testing.assert_close(b[on], a[on], rtol=1e-4, atol=1e-5)
 
 
+def test_a_mask_of_a_cache_with_room():
+    """The cache's length as a tensor: one new token sees what is in use; several rows must be the last ones."""
+    from transformers.masking_utils import causal_mask_function
+    at = lambda rows, keys, offset, m=None: key_mask(2, rows, keys, q_offset=torch.tensor(offset),
+                                                     mask_function=causal_mask_function, attention_mask=m)
+    got = at(1, 8, 5)
+    assert got.shape == (2, 8) and got.dtype == torch.bool and torch.equal(got[0], torch.arange(8) <= 5)
+    m = torch.tensor([[0, 1, 1, 1, 1, 1], [1, 1, 1, 0, 1, 1]])
+    want = nn.functional.pad(m, (0, 2)).bool()
+    assert torch.equal(at(1, 8, 5, m), want)
+    assert torch.equal(at(1, 8, 3, m), want & (torch.arange(8) <= 3))
+    with pytest.raises(ValueError, match="room"):
+        at(3, 8, 3)
+    with pytest.raises(ValueError, match="room"):
+        at(8, 16, 0)
+    assert at(3, 8, 5) is None and at(8, 8, 0) is None
+    assert torch.equal(at(3, 6, 3, m), m)
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_a_token_over_a_static_cache(padded, monkeypatch):
+    """Hidden states token by token over a cache allocated ahead, against torch's attention on the same cache."""
+    from transformers import StaticCache
+    monkeypatch.setattr("sparton_amd.backbone.attention", plain_attention)
+    ref, ours = tiny_decoder()
+    ids, mask = left_padded(3, 9, seed=2)
+    out = {}
+    for model in (ref, ours):
+        cache, rows = StaticCache(config=ref.config, max_cache_len=16), []
+        with torch.no_grad():
+            ref(ids[:, :6], mask[:, :6] if padded else None, past_key_values=cache, use_cache=True)
+            for n in range(6, 9):
+                rows.append(model(ids[:, n:n + 1], mask[:, :n + 1] if padded else None, past_key_values=cache,
+                                  use_cache=True).last_hidden_state)
+        out[model] = torch.cat(rows, 1)
+    torch.testing.assert_close(out[ours], out[ref], rtol=1e-4, atol=1e-5)
+    cache = StaticCache(config=ref.config, max_cache_len=16)
+    with torch.no_grad():
+        ref(ids[:, :6], past_key_values=cache, use_cache=True)
+        with pytest.raises(ValueError, match="room"):
+            ours(ids[:, 6:8], past_key_values=cache, use_cache=True)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("padded", [True, False])
@@ -193,6 +236,26 @@ def test_decoder_backbone_is_causal(device):
         first = ours(ids[:1, :25], use_cache=True)
         last = ours(ids[:1, 25:30], past_key_values=first.past_key_values, use_cache=True).last_hidden_state
     torch.testing.assert_close(last, whole[:, 25:], rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("padded", [False, True])
+def test_a_token_over_a_static_cache_on_the_kernels(padded, device):
+    """As above, the cache prefilled by torch's attention."""
+    from transformers import StaticCache
+    say(f"static cache, padded={padded}")
+    ref, ours = (m.to(device) for m in tiny_decoder())
+    ids, mask = (t.to(device) for t in left_padded(3, 9, seed=2))
+    out = {}
+    for model in (ref, ours):
+        cache, rows = StaticCache(config=ref.config, max_cache_len=200), []
+        with torch.no_grad():
+            ref(ids[:, :6], mask[:, :6] if padded else None, past_key_values=cache, use_cache=True)
+            for n in range(6, 9):
+                rows.append(model(ids[:, n:n + 1], mask[:, :n + 1] if padded else None, past_key_values=cache,
+                                  use_cache=True).last_hidden_state)
+        out[model] = torch.cat(rows, 1)
+    torch.testing.assert_close(out[ours], out[ref], rtol=1e-4, atol=1e-5)
 
 
 @pytest.mark.gpu
