@@ -123,6 +123,16 @@ __device__ __forceinline__ frag_t<T> lds_cols(const char* tile, int row0, int db
   }
 }
 
+// Probabilities and ds reach below fp16's normal range (2^-14), where they would lose bits, or all of them
+// while the row's sum still counts them. In fp16 the forward's, which are at most 2^8 (see below), carry a
+// factor 2^7, the dv product's, which are at most 1, 2^10, and ds one of its column (see ColScale).
+template <typename T> constexpr float kLog2UpFwd = 0.0f;
+template <> constexpr float kLog2UpFwd<f16> = 7.0f;
+template <typename T> constexpr float kDownFwd = 1.0f;
+template <> constexpr float kDownFwd<f16> = 0x1p-7f;
+template <typename T> constexpr float kLog2Up = 0.0f;
+template <> constexpr float kLog2Up<f16> = 10.0f;
+
 // Registers [KC/2 c, KC/2 (c + 1)) of a result as the right operand of step c, rounded to T. The
 // rounding of a probability (or of ds) to 16 bits is off by at most half a step of its own value,
 // and independent from key to key: it adds to an output's error what the output's own rounding does.
@@ -496,7 +506,7 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) * DH <= 256 ? 2 : 1) void a
         for (int r = 0; r < 16; ++r) acc[db][r] *= a;
       m = mn;
     }
-    const float mm = m == -INFINITY ? 0.0f : m;
+    const float mm = (m == -INFINITY ? 0.0f : m) - kLog2UpFwd<T>;
     float sum = 0.0f;
 #pragma unroll
     for (int jb = 0; jb < JB; ++jb)
@@ -571,7 +581,7 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) * DH <= 256 ? 2 : 1) void a
   if (!row.in) return;
   const bool none = l == 0.0f;
   const float inv = none ? 0.0f : 1.0f / l;
-  const float lse = none ? -INFINITY : m + __builtin_amdgcn_logf(l);
+  const float lse = none ? -INFINITY : m + __builtin_amdgcn_logf(l * kDownFwd<T>);
   if constexpr (SPLIT) {
     const int64_t to = ((int64_t)bh * p.splits + split) * p.R + r0 + wr * 32 + (lane & 31);
     store_col<float, Gm::DB>(p.part + to * p.D, acc, inv, half, p.D);
@@ -627,10 +637,9 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(Params p) {
 }
 
 // ---- backward ----------------------------------------------------------------------------
-// ds holds products of a probability and a gradient, which may lie below fp16's normal range (2^-14).
-// In fp16 each column of ds (one row's in the dq kernel, one key's in the dk kernel) is therefore
-// multiplied by a power of two that puts its largest value so far near 2^10; when a tile passes 2^14
-// the column's sums are rescaled. Other types need no such factor.
+// In fp16 each column of ds (one row's in the dq kernel, one key's in the dk kernel) is multiplied by a
+// power of two that puts its largest value so far near 2^10; when a tile passes 2^14 the column's sums
+// are rescaled. Other types need no such factor.
 template <typename T> struct ColScale {
   __device__ __forceinline__ float inv() const { return 1.0f; }
   template <int DB> __device__ __forceinline__ void apply(f32x16&, f32x16 (&)[DB]) {}
@@ -658,9 +667,6 @@ template <> struct ColScale<f16> {
     for (int r = 0; r < 16; ++r) ds[r] *= f;
   }
 };
-// In fp16 the probabilities of the dv product carry a factor 2^10 for the same reason.
-template <typename T> constexpr float kLog2Up = 0.0f;
-template <> constexpr float kLog2Up<f16> = 10.0f;
 
 // Sums of the waves of a workgroup that hold the same rows (or keys) added in order, through LDS, into
 // the first's. Wave w's place in it is `mine` of `step` apart, N in all; every wave calls it.

@@ -393,3 +393,30 @@ def test_output_changed_in_place(D, device):
         assert "inplace" in str(e)
     else:
         assert all(torch.equal(g, want[n]) for g, n in zip(grads, ("dq", "dk", "dv")))
+
+
+@pytest.mark.parametrize("B,Sq", [(200, 33), (1, 33), (1, 1)])  # whole rows, and rows split over the keys
+def test_fp16_keys_far_below_the_largest(B, Sq, device):
+    """40000 keys of 2^-26 of the first one's weight hold 0.06% of each row, and here all of its value.
+
+    Probabilities of the second product are fp16 with a factor 2^7, relative to a maximum that is at most the
+    row's: normal ones are off by u = 2^-11 of their value, others by 2^-25 2^-7. The scores are exact."""
+    say(f"fp16, small probabilities {B} {Sq}")
+    Sk, D = 40001, 64
+    q, k = torch.zeros(1, 1, Sq, D), torch.zeros(1, 1, Sk, D)
+    q[..., 0], k[..., 0, 0] = 16.0, 9.0  # scores 18 and 0: exp(-18) = 2^-25.97
+    v = torch.randint(500, 1500, (1, 1, Sk, D), generator=torch.Generator().manual_seed(0)).float()
+    v[:, :, 0] = 0.0
+    q, k, v = (t.half().to(device) for t in (q, k, v))
+    with torch.no_grad():
+        got = attention(*(t.expand(B, -1, -1, -1) for t in (q, k, v)))
+    s = 0.125 * (q.double() @ k.double().transpose(-1, -2).contiguous())
+    p = torch.softmax(s, -1)
+    want = p @ v.double()
+    # as in the reference's tolerances: ep of a probability and its row's sum, the sums over the keys, the output
+    ep = 2.0 ** -22 * (1 + s.abs() + torch.logsumexp(s, -1, keepdim=True)) + (Sk + 4) * 2.0 ** -24
+    ep = ep + (p * ep).sum(-1, keepdim=True)
+    u = 2.0 ** -11
+    tol = u * want + (p * (u + ep + (Sk + 4) * 2.0 ** -24) + 2.0 ** -32) @ v.double()
+    assert bool((tol < 0.03 * want).all())
+    close(got, (want.expand(B, -1, -1, -1), tol.expand(B, -1, -1, -1)), "out")
