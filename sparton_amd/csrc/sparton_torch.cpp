@@ -647,7 +647,7 @@ variable_list once(variable_list grads) {
 // size that is not a multiple of 16 bytes is padded with zero columns, which change no product.
 Tensor attention_rows(const Tensor& t) {
   const int64_t unit = 16 / t.element_size(), pad = (unit - t.size(3) % unit) % unit;
-  if (pad > 0) return at::constant_pad_nd(t, {0, pad});
+  if (pad > 0) return at::constant_pad_nd(t, {0, pad}).contiguous();  // heads innermost would stay so
   bool ok = t.stride(3) == 1 || t.size(3) == 1;
   for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) % unit == 0 && t.stride(i) >= 0));
   Tensor c = ok ? t : t.contiguous();

@@ -420,3 +420,17 @@ def test_fp16_keys_far_below_the_largest(B, Sq, device):
     tol = u * want + (p * (u + ep + (Sk + 4) * 2.0 ** -24) + 2.0 ** -32) @ v.double()
     assert bool((tol < 0.03 * want).all())
     close(got, (want.expand(B, -1, -1, -1), tol.expand(B, -1, -1, -1)), "out")
+
+
+@pytest.mark.parametrize("D", [20, 64])
+def test_heads_innermost_in_memory(D, device):
+    """[B,S,D,H] in memory, inputs and upstream gradient: the same bits as [B,S,H,D], padded head size or not."""
+    say(f"heads innermost, {D}")
+    q, k, v, m, do = make(2, 4, 4, 35, 41, D, "bf16", "int64", device)
+    last = lambda t: t.permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)
+    want, got = run(q, k, v, m, do, False), run(*map(last, (q, k, v)), m, last(do), False)
+    assert last(q).stride(1) == 1 and all(torch.equal(got[n], want[n]) for n in want)
+    out, lse = torch.ops.sparton.attention_fwd(last(q), last(k), last(v), m, False, D ** -0.5)
+    grads = torch.ops.sparton.attention_bwd(last(do), q, k, v, m, last(out), lse, False, D ** -0.5)
+    for n, t in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        assert torch.equal(t, want[n]), n
