@@ -296,8 +296,10 @@ int sparton_loss_bwd_terms(const void* q, const void* d, const float* probs,
  *     s_ij = scale q_i . k_j;  p_ij = softmax over the keys j that row i may look at;  o_i = sum_j p_ij v_j
  * q and o are [B, Hq, Sq, D], k and v [B, Hk, Sk, D]; query head h reads key head h / (Hq / Hk).
  * A key takes part where mask[b, j] is nonzero (mask may be NULL: every key) and, with `causal`,
- * where j <= i + Sk - Sq. A row without keys gives zeros, and zero gradients. Values of keys that
- * take no part reach no output, whatever they are. Sums, maxima and log sums are fp32.
+ * where j <= i + Sk - Sq. A row without keys gives zeros, and zero gradients. Keys that the mask drops
+ * reach no output, whatever they hold. Pairs that `causal` alone hides are multiplied with probability 0:
+ * a v, or in the backward a q, k, v or d_o, that is not finite may reach any row and key of its batch row
+ * and key head as 0 * NaN does. Sums, maxima and log sums are fp32.
  * Strides are in elements; the innermost is 1. Bases are 16-byte aligned, and so are the strides
  * (multiples of 8 elements, 4 for fp32) of dimensions larger than 1. D * element size is a multiple
  * of 16 bytes and D <= 128; 0 < scale < infinity. Sizes whose rows pass 32 bits, or whose workgroups (one

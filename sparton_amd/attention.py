@@ -138,7 +138,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor] = None
     h / (Hq / Hk)), D <= 128, one float dtype; strided views are read as they are where rows start on
     16 bytes. key_mask [B,Sk], bool or integer as a tokenizer gives it: nonzero takes part. causal: row
     i sees the keys j <= i + Sk - Sq. scale defaults to D ** -0.5. Returns [B,Hq,Sq,D], laid out
-    [B,Sq,Hq,D] in memory. A row that sees no key gives zeros, and gives and takes no gradient.
+    [B,Sq,Hq,D] in memory. A row that sees no key gives zeros, and gives and takes no gradient. Keys whose
+    mask is zero may hold anything; what causal alone hides is multiplied by 0, so NaN and infinities
+    there can reach the rows before it, as in torch's products.
     Under autocast the inputs are cast to its dtype, as torch's attention does."""
     dev = q.device.type
     if dev in ("cuda", "cpu") and torch.is_autocast_enabled(dev):

@@ -5,8 +5,9 @@
 //     dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
 // A key takes part where the key mask is nonzero and, with `causal`, where j <= i + Sk - Sq. Query
 // head h reads key head h / (Hq / Hk); dk and dv are summed over the heads that share one. A row with
-// no key gives o = 0 and zero gradients. Keys that take no part are never multiplied: what their
-// memory holds (NaN, infinities) reaches no output.
+// no key gives o = 0 and zero gradients. A key that the mask drops is replaced by zeros: what its memory
+// holds (NaN, infinities) reaches no output. A pair that `causal` hides while another row of the tile sees
+// the key is multiplied, with p = 0: there 0 * NaN is NaN.
 //
 // Every product runs on 32x32 MFMAs with fp32 sums, in transposed form: a wave holds 32 rows as the
 // columns of its results, one column per lane (and per half of the wave half of that column's

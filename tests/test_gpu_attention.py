@@ -434,3 +434,30 @@ def test_heads_innermost_in_memory(D, device):
     grads = torch.ops.sparton.attention_bwd(last(do), q, k, v, m, last(out), lse, False, D ** -0.5)
     for n, t in zip(("out", "dq", "dk", "dv"), (out, *grads)):
         assert torch.equal(t, want[n]), n
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_causal_keys_that_are_not_finite(dt, device):
+    """One value of one key: what it may reach, and what it may not. The mask's keys are another matter."""
+    say(f"causal, not finite, {dt}")
+    j, d = 100, 7
+    q, k, v, m, do = make(2, 4, 2, 150, 150, 64, dt, "none", device)
+    want = run(q, k, v, m, do, True)
+    for bad in (float("nan"), float("inf")):
+        k2, v2 = k.clone(), v.clone()
+        k2[0, 0, j, d], v2[0, 0, j, d] = bad, bad
+        got = run(q, k, v2, m, do, True)
+        # forward: its own column of the rows that share the key head, and there of every row that sees it
+        assert not bool(torch.isfinite(got["out"][0, :2, j:, d]).any())
+        other = [c for c in range(64) if c != d]
+        assert torch.equal(got["out"][0, :2][..., other], want["out"][0, :2][..., other])
+        with torch.no_grad():  # a key's scores are dropped, not multiplied
+            assert torch.equal(attention(q, k2, v, causal=True)[0, :2, :j], want["out"][0, :2, :j])
+        for res in (got, run(q, k2, v, m, do, True)):
+            for n, heads in (("out", 2), ("dq", 2), ("dk", 1), ("dv", 1)):  # the other key head, the other batch row
+                assert torch.equal(res[n][0, heads:], want[n][0, heads:]) and torch.equal(res[n][1], want[n][1]), n
+        m2 = torch.ones(2, 150, dtype=torch.bool, device=device)
+        m2[0, j] = False
+        masked = run(q, k, v, m2, do, True)
+        for n, t in run(q, k2, v2, m2, do, True).items():
+            assert torch.equal(t, masked[n]), n
