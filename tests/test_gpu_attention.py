@@ -461,3 +461,25 @@ def test_causal_keys_that_are_not_finite(dt, device):
         masked = run(q, k, v, m2, do, True)
         for n, t in run(q, k2, v2, m2, do, True).items():
             assert torch.equal(t, masked[n]), n
+
+
+# Every kernel that the launch rules choose from (tests/test_operators_boundary.py counts them): workgroups of 32,
+# 64 and 128 rows, whole and split over the keys, and of 64 and 128 keys, for each type and head block.
+SHAPES = [  # B, Hq, Hk, Sq, Sk, mask, causal; B of the first two times 12 heads is what 128 rows need
+    (None, 12, 12, 101, 97, "int64 holes empty", False),
+    (None, 24, 12, 131, 135, "int64 left", True),
+    (2, 2, 2, 70, 150, "bool holes", True),
+    (1, 2, 1, 41, 1100, "int64", False),
+    (1, 2, 2, 140, 2500, "int64 holes", True),
+    (2, 4, 2, 9, 201, "int64", True),
+    (1, 4, 2, 5, 1501, "int64 holes", False),
+]
+EVERY = [(B or (22 if dt != "fp32" else 43), Hq, Hk, Sq, Sk, D, dt, mask, causal)
+         for dt in DT for D in (24, 64, 104) for B, Hq, Hk, Sq, Sk, mask, causal in SHAPES]
+
+
+@pytest.mark.parametrize("case", EVERY, ids=["-".join(str(x).replace(" ", "_") for x in c) for c in EVERY])
+def test_attention_on_every_kernel(case, device):
+    B, Hq, Hk, Sq, Sk, D, dt, mask, causal = case
+    say(f"attention {case}")
+    check(*make(B, Hq, Hk, Sq, Sk, D, dt, mask, device), causal)

@@ -127,6 +127,41 @@ def test_attention_workspace():
     assert fwd(d, ws=None) == -4 and fwd(d, ws_bytes=few - 1) == -4 and fwd(d, ws=P + 16) == -2
 
 
+def attention_kernels(B, Hq, Hk, Sq, Sk, D, dt, *_):
+    """The kernels that a training step of these sizes launches: (kernel, type, head block, rows or keys of a
+    workgroup, split). The rules of sparton_attention.hip once more."""
+    cdiv, es, pairs, R = lambda a, b: -(-a // b), 4 if dt == "fp32" else 2, B * Hk, Hq // Hk * Sq
+    block = 32 if D <= 32 else 64 if D <= 64 else 128
+    small = lambda n: pairs * cdiv(n, 128) < (512 if es == 4 else 200)
+    rows = 32 if R <= 32 else 64 if small(R) and (es == 4 or Sk <= 2048) else 128
+    groups, tiles = pairs * cdiv(R, rows), cdiv(Sk, 128 if rows == 32 else 64 if rows == 64 or block <= 64 else 32)
+    n = 1 if groups >= 192 else min(cdiv(512, groups), max(tiles // 4, 1), 64)
+    return {("fwd", dt, block, rows, cdiv(tiles, cdiv(tiles, n)) > 1), ("dq", dt, block, 64 if small(R) else 128),
+            ("dkv", dt, block, 64 if small(Sk) else 128)}
+
+
+def test_the_attention_cases_reach_every_kernel():
+    from test_gpu_attention import EVERY
+    every = {(k, dt, block, n) for k in ("dq", "dkv") for dt in ("bf16", "fp16", "fp32") for block in (32, 64, 128)
+             for n in (64, 128)}
+    every |= {("fwd", dt, block, rows, split) for dt in ("bf16", "fp16", "fp32") for block in (32, 64, 128)
+              for rows in (32, 64, 128) for split in (False, True)}
+    # fp32 has 128 rows a workgroup only where workgroups are too many to be split
+    every -= {("fwd", "fp32", block, 128, True) for block in (32, 64, 128)}
+    assert set().union(*(attention_kernels(*c) for c in EVERY)) == every
+
+
+def test_the_rules_above_are_the_librarys():
+    """The workspace tells which forward calls are split, and over how many workgroups."""
+    from test_gpu_attention import CASES, EVERY, FEW
+    for B, Hq, Hk, Sq, Sk, D, dt, *_ in [*CASES, *EVERY, *FEW]:
+        D += -D % (4 if dt == "fp32" else 8)
+        need = _lib.load().sparton_attention_workspace_bytes(
+            desc(B=B, Hq=Hq, Hk=Hk, Sq=Sq, Sk=Sk, D=D, dtype=("fp32", "bf16", "fp16").index(dt)))
+        (split,) = (k[4] for k in attention_kernels(B, Hq, Hk, Sq, Sk, D, dt) if k[0] == "fwd")
+        assert (need > 0) == split, (B, Hq, Hk, Sq, Sk, D, dt)
+
+
 def q4(B=2, H=4, S=8, D=64, **kw):
     return torch.zeros(B, H, S, D, **kw)
 
