@@ -292,3 +292,13 @@ def test_norm_graph_replays(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(outs, want))
+
+
+@pytest.mark.parametrize("D", [5, 301, 907, 1501, 3001, 6007, 12001])
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+def test_norm_with_more_rows_than_workgroups(dt, D, device):
+    """Each width's kernels for each type, where a workgroup takes several rows (the forward's at 4096 rows of one
+    wave, 1024 of four, 512 of eight; the backward's at 2048, 512 and 256)."""
+    M = 4500 if D <= 1024 else 1100
+    say(f"layer_norm {M} x {D} {dt}")
+    check(make((M, D), dt, "fp32" if D % 3 else "same", device))
