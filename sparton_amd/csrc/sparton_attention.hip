@@ -696,12 +696,12 @@ __device__ __forceinline__ void join_sums(f32x16 (&acc)[DB], char* smem, int wav
 // The scores come again from q and k rather than from memory: at 12 heads of 8192 x 8192 they would be
 // 1.6 GB to write and read. There it takes 355 us, 870 TFLOP/s, products and vector work overlapping as
 // in the forward; 32 x 12 heads of 256 x 256, padded, 24 us.
-template <typename T, int DH, int WR, int WK, int JB, int NBUF>
+template <typename T, int DH, int WR, int WK, int JB>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_dq_kernel(Params p) {
   typedef Geo<T, DH> Gm;
   constexpr int BK = 32 * JB * WK, NW = JB * WK, TILE = BK * Gm::ROW, RB = 32 * WR;
-  static_assert(WR * WK * 64 == kThreads && (WK == 1 || NBUF * 2 * TILE >= kThreads / 2 * DH * 4), "joining waves reuse the tiles");
-  __shared__ __attribute__((aligned(16))) char smem[NBUF * 2 * TILE];
+  static_assert(WR * WK * 64 == kThreads && (WK == 1 || 4 * TILE >= kThreads / 2 * DH * 4), "joining waves reuse the tiles");
+  __shared__ __attribute__((aligned(16))) char smem[4 * TILE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wr = wave % WR, wk = wave / WR;
   const int row_tiles = (p.R + RB - 1) / RB;
@@ -809,9 +809,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_
           acc[db] = mma(lds_cols<T, DH>(kt, (wk * JB + jb) * 32 + c * Gm::KC, db, lane), df, acc[db]);
       }
     }
-    if (NBUF == 1) __syncthreads();
     if (tn < t_end) {
-      if (NBUF == 2) buf ^= 1;
+      buf ^= 1;
       ks.template clear<NW>(wn);
       vs.template clear<NW>(wn);
       ks.put(smem + buf * 2 * TILE);
@@ -845,13 +844,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_
 // registers of a whole SIMD for one wave: 16 x 32 heads over 8 key heads, 512 x 512 x 128 causal and
 // padded, 148 us, where the forward takes 82 and dq 106 (tiles of 32 rows in place of 64 were slower by
 // a quarter).
-template <typename T, int DH, int KG, int RG, int IB, int NBUF>
+template <typename T, int DH, int KG, int RG, int IB>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 128 ? 2 : 1) void attn_dkv_kernel(Params p) {
   typedef Geo<T, DH> Gm;
   constexpr int BR = 32 * IB * RG, KB = 32 * KG, TILE = BR * Gm::ROW;
-  static_assert(KG * RG * 64 == kThreads && (RG == 1 || NBUF * 2 * TILE >= kThreads / 2 * DH * 4), "joining waves reuse the tiles");
-  __shared__ __attribute__((aligned(16))) char smem[NBUF * 2 * TILE];
-  __shared__ __attribute__((aligned(16))) float stat[NBUF * 2 * BR];  // lse, -delta of the tile's rows
+  static_assert(KG * RG * 64 == kThreads && (RG == 1 || 4 * TILE >= kThreads / 2 * DH * 4), "joining waves reuse the tiles");
+  __shared__ __attribute__((aligned(16))) char smem[4 * TILE];
+  __shared__ __attribute__((aligned(16))) float stat[4 * BR];  // lse, -delta of the tile's rows
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int kg = wave % KG, rg = wave / KG;
   const int key_tiles = (p.Sk + KB - 1) / KB;
@@ -969,9 +968,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 128 ? 2 : 1) void attn_
           }
         }
       }
-      if (NBUF == 1) __syncthreads();
       if (gn < p.G) {
-        if (NBUF == 2) buf ^= 1;
+        buf ^= 1;
         put(buf, itn);
       }
       __syncthreads();
@@ -1036,8 +1034,14 @@ size_t fwd_bytes(const FwdPlan& f, int64_t B, int64_t Hk, int64_t R, int64_t D) 
 template <typename T, int DH, int WR, int WK, int JB, int NBUF>
 void launch_fwd_rows(const FwdPlan& f, const Params& p, hipStream_t st) {
   const dim3 grid((unsigned)(f.groups * f.splits)), block(kThreads);
-  if (f.splits > 1) hipLaunchKernelGGL((attn_fwd_kernel<T, DH, WR, WK, JB, NBUF, true>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((attn_fwd_kernel<T, DH, WR, WK, JB, NBUF, false>), grid, block, 0, st, p);
+  // fp32 has workgroups of 128 rows only where there are too many for a split.
+  if constexpr (sizeof(T) == 2 || WR < 4) {
+    if (f.splits > 1) {
+      hipLaunchKernelGGL((attn_fwd_kernel<T, DH, WR, WK, JB, NBUF, true>), grid, block, 0, st, p);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((attn_fwd_kernel<T, DH, WR, WK, JB, NBUF, false>), grid, block, 0, st, p);
 }
 
 template <typename T, int DH>
@@ -1058,15 +1062,15 @@ void launch_bwd(const Params& p, hipStream_t st) {
   constexpr int JB = DH == 128 ? 1 : 2;
   if (p.R > 0) {
     if (!small_groups(bh, p.R, sizeof(T)))
-      hipLaunchKernelGGL((attn_dq_kernel<T, DH, 4, 1, JB, 2>), dim3((unsigned)(bh * cdiv(p.R, 128))), block, 0, st, p);
+      hipLaunchKernelGGL((attn_dq_kernel<T, DH, 4, 1, JB>), dim3((unsigned)(bh * cdiv(p.R, 128))), block, 0, st, p);
     else
-      hipLaunchKernelGGL((attn_dq_kernel<T, DH, 2, 2, 1, 2>), dim3((unsigned)(bh * cdiv(p.R, 64))), block, 0, st, p);
+      hipLaunchKernelGGL((attn_dq_kernel<T, DH, 2, 2, 1>), dim3((unsigned)(bh * cdiv(p.R, 64))), block, 0, st, p);
   }
   if (p.Sk > 0) {
     if (!small_groups(bh, p.Sk, sizeof(T)))
-      hipLaunchKernelGGL((attn_dkv_kernel<T, DH, 4, 1, 2, 2>), dim3((unsigned)(bh * cdiv(p.Sk, 128))), block, 0, st, p);
+      hipLaunchKernelGGL((attn_dkv_kernel<T, DH, 4, 1, 2>), dim3((unsigned)(bh * cdiv(p.Sk, 128))), block, 0, st, p);
     else
-      hipLaunchKernelGGL((attn_dkv_kernel<T, DH, 2, 2, 1, 2>), dim3((unsigned)(bh * cdiv(p.Sk, 64))), block, 0, st, p);
+      hipLaunchKernelGGL((attn_dkv_kernel<T, DH, 2, 2, 1>), dim3((unsigned)(bh * cdiv(p.Sk, 64))), block, 0, st, p);
   }
 }
 
