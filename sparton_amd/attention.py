@@ -28,7 +28,7 @@ MAX_HEAD_DIM = 128
 _FLOAT_DTYPES = tuple(_lib.DTYPE_CODE)
 # A float mask is refused: added to the scores (0 keeps a key) and multiplied into them (0 drops it)
 # are both in use, and mean the opposite of each other.
-_KEY_MASK_DTYPES = (torch.bool, torch.uint8, torch.int32, torch.int64)
+KEY_MASK_DTYPES = (torch.bool, torch.uint8, torch.int32, torch.int64)
 
 
 def _check(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor], scale: float, op: str) -> None:
@@ -48,7 +48,7 @@ def _check(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor], scale: f
     if key_mask is not None:
         if tuple(key_mask.shape) != (B, Sk):
             raise ValueError(f"{op}: key_mask must be [B,Sk]=[{B},{Sk}], got {tuple(key_mask.shape)}")
-        if key_mask.dtype not in _KEY_MASK_DTYPES:
+        if key_mask.dtype not in KEY_MASK_DTYPES:
             raise TypeError(f"{op}: key_mask must be bool or integer (nonzero: the key takes part), got "
                             f"{key_mask.dtype}")
     if not (scale > 0.0 and math.isfinite(scale)):

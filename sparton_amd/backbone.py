@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 from torch import Tensor, nn
 
-from .attention import attention
+from .attention import KEY_MASK_DTYPES, attention
 from .norm import SpartonLayerNorm
 
 NAME = "sparton"
@@ -62,6 +62,8 @@ def key_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_func
     one = mask_function is causal_mask_function and q_length == 1 and isinstance(q_offset, Tensor)
     if mask_function is causal_mask_function and not one and int(q_offset) + q_length != kv_offset + kv_length:
         raise ValueError("sparton attention's causal rows are the last ones of the keys; this cache has room behind them")
+    if attention_mask is not None and attention_mask.dtype not in KEY_MASK_DTYPES:
+        attention_mask = attention_mask != 0  # true or false to transformers too, whatever the type
     if attention_mask is not None and (kv_offset != 0 or attention_mask.shape[-1] != kv_length):
         attention_mask = attention_mask[:, kv_offset:kv_offset + kv_length]
         attention_mask = nn.functional.pad(attention_mask, (0, kv_length - attention_mask.shape[-1]))

@@ -154,6 +154,16 @@ def test_the_masks_columns_are_the_keys(monkeypatch):
     torch.testing.assert_close(b[on], a[on], rtol=1e-4, atol=1e-5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.int8, torch.int16])
+def test_a_mask_of_any_type(dtype):
+    """transformers reads a mask's values as true or false; so does a switched model."""
+    m = torch.tensor([[0, 1, 1, 1], [1, 1, 0, 1]])
+    got = key_mask(2, 4, 4, attention_mask=m.to(dtype))
+    assert got.dtype == torch.bool and torch.equal(got, m.bool())
+    for own in (torch.bool, torch.uint8, torch.int32, torch.int64):
+        assert key_mask(2, 4, 4, attention_mask=m.to(own)).dtype == own
+
+
 def test_a_mask_of_a_cache_with_room():
     """The cache's length as a tensor: one new token sees what is in use; several rows must be the last ones."""
     from transformers.masking_utils import causal_mask_function
