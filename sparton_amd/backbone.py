@@ -110,6 +110,6 @@ def use_in_backbone(model: nn.Module) -> nn.Module:
     for module, name, norm in norms:
         setattr(module, name, norm)
     for module in model.modules():
-        if type(module).__name__ in _RESIDUAL_BLOCKS:
+        if type(module).__name__ in _RESIDUAL_BLOCKS and isinstance(module.LayerNorm, SpartonLayerNorm):
             module.forward = _BlockForward(_residual_norm, module)
     return model

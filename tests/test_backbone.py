@@ -82,6 +82,20 @@ def test_a_refused_model_stays_as_it_was():
     assert not any(type(m) is sparton_amd.SpartonLayerNorm or "forward" in m.__dict__ for m in llm.modules())
 
 
+@pytest.mark.parametrize("norm", [lambda: nn.LayerNorm(128, elementwise_affine=False), lambda: nn.Identity()])
+def test_a_block_whose_norm_is_another_stays_as_it_is(norm, monkeypatch):
+    """Its own forward runs, with the norm that it has."""
+    monkeypatch.setattr("sparton_amd.backbone.attention", plain_attention)
+    monkeypatch.setattr("sparton_amd.norm.layer_norm", lambda x, w, b=None, eps=1e-5, residual=None:
+                        nn.functional.layer_norm(x if residual is None else x + residual, x.shape[-1:], w, b, eps))
+    ref = base(tiny("bert"))
+    ref.encoder.layer[1].output.LayerNorm = norm()
+    ours = use_in_backbone(copy.deepcopy(ref))
+    ids = torch.arange(12).reshape(2, 6) + 5
+    with torch.no_grad():
+        torch.testing.assert_close(ours(ids).last_hidden_state, ref(ids).last_hidden_state, rtol=1e-4, atol=1e-5)
+
+
 def test_refusals():
     q = torch.zeros(1, 2, 4, 8)
     with pytest.raises(ValueError, match="dropout"):
