@@ -15,6 +15,7 @@ Device tensors only, like the head.
 """
 from __future__ import annotations
 
+import copy
 import math
 from typing import Optional, Tuple
 
@@ -120,7 +121,7 @@ def layer_norm(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, eps: fl
 class SpartonLayerNorm(nn.LayerNorm):
     """An affine nn.LayerNorm over the last dimension on the kernels above, with an optional residual:
     norm(x, residual) is LayerNorm(x + residual). `SpartonLayerNorm.of(layer_norm)` shares an existing
-    module's parameters (names and state_dict unchanged).
+    module's parameters (names and state_dict unchanged) and keeps its hooks.
 
     Under autocast the inputs are cast to float32 and so is the output, as torch's layer_norm does;
     inputs of two dtypes are summed in the wider one, as torch's sum would be."""
@@ -131,11 +132,8 @@ class SpartonLayerNorm(nn.LayerNorm):
             raise ValueError(f"SpartonLayerNorm needs an affine LayerNorm over one dimension, got {layer_norm}")
         if layer_norm.normalized_shape[0] > MAX_WIDTH:
             raise ValueError(f"SpartonLayerNorm takes rows up to {MAX_WIDTH}, got {layer_norm.normalized_shape[0]}")
-        m = cls.__new__(cls)
-        nn.Module.__init__(m)
-        m.normalized_shape, m.eps, m.elementwise_affine = layer_norm.normalized_shape, layer_norm.eps, True
-        m.weight, m.bias = layer_norm.weight, layer_norm.bias
-        m.training = layer_norm.training
+        m = copy.copy(layer_norm)  # the same parameters, hooks and mode
+        m.__class__ = cls
         return m
 
     def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:

@@ -96,6 +96,21 @@ def test_a_block_whose_norm_is_another_stays_as_it_is(norm, monkeypatch):
         torch.testing.assert_close(ours(ids).last_hidden_state, ref(ids).last_hidden_state, rtol=1e-4, atol=1e-5)
 
 
+def test_norms_keep_their_hooks(monkeypatch):
+    monkeypatch.setattr("sparton_amd.norm.layer_norm", lambda x, w, b=None, eps=1e-5, residual=None:
+                        nn.functional.layer_norm(x if residual is None else x + residual, x.shape[-1:], w, b, eps))
+    model, seen = nn.Module(), []
+    model.norm = ln = nn.LayerNorm(16)
+    first = ln.register_forward_hook(lambda m, args, out: seen.append("out"))
+    ln.register_forward_pre_hook(lambda m, args: seen.append("in"))
+    model.norm = sparton_amd.SpartonLayerNorm.of(ln)
+    x = torch.randn(3, 16)
+    assert torch.equal(model.norm(x), nn.functional.layer_norm(x, (16,), ln.weight, ln.bias)) and seen == ["in", "out"]
+    first.remove()
+    model.norm(x)
+    assert seen == ["in", "out", "in"]
+
+
 def test_refusals():
     q = torch.zeros(1, 2, 4, 8)
     with pytest.raises(ValueError, match="dropout"):
