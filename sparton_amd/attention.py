@@ -146,7 +146,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor] = None
     if dev in ("cuda", "cpu") and torch.is_autocast_enabled(dev):
         dt = torch.get_autocast_dtype(dev)
         q, k, v = q.to(dt), k.to(dt), v.to(dt)
-    scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
+    if scale is None:  # of a shape that is refused below, any
+        scale = float(q.shape[-1]) ** -0.5 if q.dim() > 0 and q.shape[-1] > 0 else 1.0
+    scale = float(scale)
     if torch.compiler.is_compiling() or not q.is_cuda:  # the registered op: fake + autograd
         return torch.ops.sparton.attention_fwd(q, k, v, key_mask, causal, scale)[0]
     _check(q, k, v, key_mask, scale, "attention")

@@ -126,12 +126,20 @@ class SpartonLayerNorm(nn.LayerNorm):
     Under autocast the inputs are cast to float32 and so is the output, as torch's layer_norm does;
     inputs of two dtypes are summed in the wider one, as torch's sum would be."""
 
-    @classmethod
-    def of(cls, layer_norm: nn.LayerNorm) -> "SpartonLayerNorm":
+    def __init__(self, *args, **kwargs):
+        super().__init__(*args, **kwargs)
+        self._check_module(self)
+
+    @staticmethod
+    def _check_module(layer_norm: nn.LayerNorm) -> None:
         if len(layer_norm.normalized_shape) != 1 or layer_norm.weight is None:
             raise ValueError(f"SpartonLayerNorm needs an affine LayerNorm over one dimension, got {layer_norm}")
         if layer_norm.normalized_shape[0] > MAX_WIDTH:
             raise ValueError(f"SpartonLayerNorm takes rows up to {MAX_WIDTH}, got {layer_norm.normalized_shape[0]}")
+
+    @classmethod
+    def of(cls, layer_norm: nn.LayerNorm) -> "SpartonLayerNorm":
+        cls._check_module(layer_norm)
         m = copy.copy(layer_norm)  # the same parameters, hooks and mode
         m.__class__ = cls
         return m

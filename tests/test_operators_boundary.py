@@ -189,6 +189,12 @@ def test_attention_refusals(args, kw, error):
         attention(*args, **kw)
 
 
+@pytest.mark.parametrize("q", [q4(D=0), torch.zeros(()), torch.zeros(3, 0)], ids=["empty heads", "0-d", "2-d"])
+def test_attention_default_scale_of_other_shapes(q):
+    with pytest.raises(ValueError, match="attention"):
+        attention(q, q, q)
+
+
 def nfwd(**kw):
     a = dict(x=P, r=P, w=P, b=P, vec=0, eps=1e-5, y=P, mean=P, rstd=P, M=4, D=64, dtype=1, stream=None)
     a.update(kw)
@@ -258,6 +264,13 @@ def test_layer_norm_module_surface():
         m(torch.zeros(2, 32))
     assert SpartonLayerNorm(16).weight.shape == (16,)
     assert sparton_amd.SpartonLayerNorm is SpartonLayerNorm
+
+
+def test_layer_norm_module_needs_its_weight():
+    for bad in (dict(elementwise_affine=False), dict(normalized_shape=(4, 8)), dict(normalized_shape=16400)):
+        with pytest.raises(ValueError, match="SpartonLayerNorm"):
+            SpartonLayerNorm(**{"normalized_shape": 16, **bad})
+    assert SpartonLayerNorm(16, bias=False).bias is None
 
 
 def pfwd(**kw):
