@@ -140,8 +140,9 @@ class SpartonLayerNorm(nn.LayerNorm):
     @classmethod
     def of(cls, layer_norm: nn.LayerNorm) -> "SpartonLayerNorm":
         cls._check_module(layer_norm)
-        m = copy.copy(layer_norm)  # the same parameters, hooks and mode
+        m = copy.copy(layer_norm)  # the same hooks and mode
         m.__class__ = cls
+        m._parameters = dict(m._parameters)  # and parameters, until either module is given another one
         return m
 
     def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:

@@ -109,6 +109,8 @@ def test_norms_keep_their_hooks(monkeypatch):
     first.remove()
     model.norm(x)
     assert seen == ["in", "out", "in"]
+    ln.weight = nn.Parameter(torch.zeros(16))  # the module that it was made of goes its own way
+    assert bool((model.norm.weight == 1).all())
 
 
 def test_refusals():
