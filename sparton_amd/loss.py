@@ -325,5 +325,7 @@ def preference_loss(query_reps: Tensor, pos_reps: Tensor, neg_reps: Tensor, ref_
 @torch.no_grad()
 def preference_margin(query_reps: Tensor, pos_reps: Tensor, neg_reps: Tensor, temperature: float = 1.0) -> Tensor:
     """The margins [B] (fp32) of a reference model's reps, for preference_loss's ref_margin."""
+    if torch.compiler.is_compiling():  # the registered op, which has a fake
+        return torch.ops.sparton.preference_fwd(query_reps, pos_reps, neg_reps, None, float(temperature), 1.0, 0.0)[1]
     _check_pairs(query_reps, pos_reps, neg_reps, None, float(temperature), 1.0, 0.0, "preference_margin")
     return _eager.load().preference_margin(query_reps, pos_reps, neg_reps, float(temperature))

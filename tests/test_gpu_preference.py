@@ -230,3 +230,11 @@ def test_preference_graph_replays(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_preference_margin_compiles(device):
+    say("margin, compile")
+    q, p, n, _ = make(5, 300, "bf16", device)
+    f = lambda a, b, c: preference_margin(a, b, c, 3.0) * 2
+    got = torch.compile(f, backend="aot_eager", fullgraph=True)(q.requires_grad_(), p, n)
+    assert not got.requires_grad and torch.equal(got, f(q, p, n))
