@@ -250,6 +250,10 @@ struct KeyBits {
     }
     return t;
   }
+  // Whether no tile after t, below t_end, has a key (false where that takes another load of the mask).
+  template <int NW> __device__ __forceinline__ bool last(int t, int t_end) const {
+    return (t_end * NW - 1) >> 6 == chunk && !__any(word != 0 && (int)(threadIdx.x & 63) > ((t * NW + NW - 1) & 63));
+  }
 };
 
 // What a staged chunk is read from past the last row and past D: every load is then unconditional.
@@ -702,6 +706,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_
   constexpr int BK = 32 * JB * WK, NW = JB * WK, TILE = BK * Gm::ROW, RB = 32 * WR;
   static_assert(WR * WK * 64 == kThreads && (WK == 1 || 4 * TILE >= kThreads / 2 * DH * 4), "joining waves reuse the tiles");
   __shared__ __attribute__((aligned(16))) char smem[4 * TILE];
+  __shared__ float wave_sums[WK > 1 ? kThreads : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wr = wave % WR, wk = wave / WR;
   const int row_tiles = (p.R + RB - 1) / RB;
@@ -762,6 +767,50 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_
     ks.put(smem);
     vs.put(smem + TILE);
     __syncthreads();
+  }
+  // In 16 bits do . o has the output's rounding in it. Where a row sees few keys delta takes most of each
+  // do . v away, and that error with it (rows of up to 32 causal keys: dq off by twice its other roundings).
+  // A row whose keys all lie in its first tile gets delta = sum_j p_ij (do_i . v_j) instead, which has none.
+  if constexpr (sizeof(T) == 2) {
+    if (t < t_end) {
+      const bool last = bits.last<NW>(t, t_end);
+      const int seen = (t + 1) * BK - off;  // with `causal`, rows before it see no key behind this tile
+      if (last || (p.causal && i_lo < seen)) {
+        float a = 0.0f;
+#pragma unroll
+        for (int jb = 0; jb < JB; ++jb) {
+          f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+          for (int c = 0; c < Gm::NC; ++c) {
+            const int at = lds_at<T, DH>((wk * JB + jb) * 32 + (lane & 31), 2 * c + half);
+            s = mma(lds_frag<T>(smem + at), qf[c], s);
+            dp = mma(lds_frag<T>(smem + TILE + at), gf[c], dp);
+          }
+          uint32_t word = w[jb];
+#pragma unroll
+          for (int x = 1; x < WK; ++x) word = wk == x ? w[x * JB + jb] : word;
+          word >>= 4 * half;
+          const int lim = p.causal ? row.i + off - (t * BK + (wk * JB + jb) * 32 + 4 * half) : 31;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(s[r], p.c, -lse));
+            a = fmaf((word >> reg_row(r)) & 1 && reg_row(r) <= lim ? e : 0.0f, dp[r], a);
+          }
+        }
+        a = other_half_sum(a);
+        if constexpr (WK > 1) {
+          wave_sums[wave * 64 + lane] = a;
+          __syncthreads();
+          a = 0.0f;
+#pragma unroll
+          for (int x = 0; x < WK; ++x) a += wave_sums[(wr + x * WR) * 64 + lane];
+        }
+        if (last || row.i < seen) {
+          delta = a;
+          if (half == 0 && wk == 0 && row.in) p.delta[((int64_t)b * p.Hq + hk * p.G + row.g) * p.Sq + row.i] = a;
+        }
+      }
+    }
   }
   int buf = 0;
   while (t < t_end) {

@@ -1,8 +1,10 @@
 """GPU parity of the attention kernels against 64 bits (tests/_attention_ref.py derives the tolerances)."""
+import math
+
 import pytest
 import torch
 
-from _attention_ref import close, reference
+from _attention_ref import U32, allowed_pairs, close, reference
 from _parity import say
 from sparton_amd.attention import attention
 
@@ -483,3 +485,53 @@ def test_attention_on_every_kernel(case, device):
     B, Hq, Hk, Sq, Sk, D, dt, mask, causal = case
     say(f"attention {case}")
     check(*make(B, Hq, Hk, Sq, Sk, D, dt, mask, device), causal)
+
+
+@pytest.mark.parametrize("case", [  # at most 32 keys a row: every row's lie in one tile
+    (3, 4, 2, 31, 31, 64, "bf16", "none", True),
+    (40, 12, 6, 32, 32, 64, "bf16", "int64", True),     # groups of 128 rows, four query heads' rows in some
+    (5, 2, 2, 9, 9, 64, "fp16", "none", False),
+    (2, 2, 2, 4, 4, 128, "fp16", "none", True),
+    (30, 12, 12, 19, 23, 104, "bf16", "bool left", True),
+    (3, 4, 4, 45, 26, 32, "fp16", "int64 empty", False),
+    (25, 8, 8, 17, 30, 20, "bf16", "int64 holes", True),
+    (2, 3, 3, 70, 300, 64, "bf16", "few", False),        # only 20 keys of 300 take part
+    (1, 3, 3, 70, 300, 128, "bf16", "few", True),
+], ids=str)
+def test_gradients_of_rows_with_few_keys(case, device):
+    """There do . v and delta nearly cancel (with one key ds is 0), so delta must not carry the output's rounding:
+    as in the reference's tolerances, but for delta, which is then sum_j p_ij (do_i . v_j), each term off by ep and
+    by the product's sums, and n sums in fp32."""
+    say(f"few keys {case}")
+    B, Hq, Hk, Sq, Sk, D, dt, mask, causal = case
+    q, k, v, m, do = make(B, Hq, Hk, Sq, Sk, D, dt, "none" if mask == "few" else mask, device, scale_do=1.0)
+    if mask == "few":
+        m = torch.zeros(B, Sk, dtype=torch.int64, device=device)
+        m[:, 35:55] = 1
+    got = run(q, k, v, m, do, causal)
+    u, tiny = torch.finfo(q.dtype).eps / 2, 2.0 ** -34 if dt == "fp16" else 0.0
+    sub = 2.0 ** -25 if dt == "fp16" else 2.0 ** -126
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    G, scale = Hq // Hk, D ** -0.5
+    k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+    on = allowed_pairs(B, Sq, Sk, m, causal, device)
+    kt, vt = k.transpose(-1, -2).contiguous(), v.transpose(-1, -2).contiguous()
+    s = scale * (q @ kt)
+    L = torch.logsumexp(torch.where(on, s, -math.inf), -1, keepdim=True)
+    some = on.any(-1, keepdim=True)
+    p = torch.where(on, torch.exp(s - torch.where(some, L, 0.0)), 0.0)
+    ep = torch.where(on, (D + 2) * U32 * scale * (q.abs() @ kt.abs())
+                     + 2.0 ** -22 * (1 + s.abs() + torch.where(some, L, 0.0).abs()), 0.0)
+    ep = ep + (p * ep).sum(-1, keepdim=True) + (Sk + 4) * U32
+    dp, e_dp = do @ vt, (D + 2) * U32 * (do.abs() @ vt.abs())
+    delta = (p * dp).sum(-1, keepdim=True)
+    e_delta = (p * ((ep + (Sk + 4) * U32) * dp.abs() + e_dp)).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    e_ds = (u + ep + 4 * U32) * ds.abs() + p * (e_dp + e_delta)
+    e_ds = e_ds + tiny * torch.maximum(ds.abs().amax(-1, keepdim=True), ds.abs().amax(-2, keepdim=True)) * on
+    dq = scale * (ds @ k)
+    close(got["dq"], (dq, u * dq.abs() + scale * ((e_ds + (Sk + 4) * U32 * ds.abs()) @ k.abs()) + sub), "dq")
+    shared = lambda t: t.reshape(B, Hk, G, Sk, D).sum(2)
+    dk = shared(scale * (ds.transpose(-1, -2).contiguous() @ q))
+    tol = shared(scale * ((e_ds + (G * Sq + 4) * U32 * ds.abs()).transpose(-1, -2).contiguous() @ q.abs()))
+    close(got["dk"], (dk, u * dk.abs() + tol + sub), "dk")
