@@ -377,12 +377,15 @@ __device__ __forceinline__ void pos_range(const Params& p, int r0, int r1, int* 
 //
 // What bounds it. Long rows (12 heads of 8192 x 8192 x 64, bf16): 270 us, 760 TFLOP/s, half of what a
 // large library product reaches on the card: 32 x 32 scores take eight MFMAs of 32 cycles, 16
-// exponentials of 8, and some 60 maxima, multiply-adds, sums and conversions of 4 cycles or less, and
-// two waves a SIMD overlap the matrix and the vector unit only in part. Short rows (padded 32 x 12 heads
+// exponentials of 8, and some 60 maxima, multiply-adds, sums and conversions of 4 cycles or less. Three
+// waves a SIMD (149 registers; 768 workgroups) overlap the matrix and the vector unit only in part: the
+// matrix unit is busy 39% of the time, and so is the LDS, of which each fragment feeds one MFMA. Short rows (padded 32 x 12 heads
 // of 256 x 256: 18 us) pay for the way to the first tile, four tiles being all there are. A
 // token against a long cache (4 x 8 key heads of 20001 x 128, 9000 or more in use) is bound by memory:
-// 54 us, 4.4 TB/s. The tile's keys pass from memory through registers to two LDS buffers, so that the
-// next tile's loads run under this one's products and a masked key's memory can be replaced by zeros.
+// 50 us, 4.7 TB/s, though at head size 128 the four waves that share a row block spill 36 to 40 registers a
+// lane in 16 bits, and in fp32 hold one wave a SIMD (all 20001 keys: 190 us, 3.4 TB/s). The tile's keys
+// pass from memory through registers to two LDS buffers, so that the next tile's loads run under this one's
+// products and a masked key's memory can be replaced by zeros.
 template <typename T, int DH, int WR, int WK, int JB, int NBUF, bool SPLIT>
 __global__ __launch_bounds__(64 * WR * WK, sizeof(T) * DH <= 256 ? 2 : 1) void attn_fwd_kernel(Params p) {
   typedef Geo<T, DH> Gm;
@@ -889,10 +892,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 256 ? 2 : 1) void attn_
 // column throughout, which is written as zeros: no element needs the key mask here.
 // A kernel of its own, so that both sums stay in registers and nothing is added by atomics: the price is
 // a second pass over the scores. At 12 heads of 8192 x 8192 x 64 it takes 480 us, 860 TFLOP/s: the
-// matrix unit is busy 42% of the time and the LDS 59%, conflicts among that 11. Head size 128 takes the
-// registers of a whole SIMD for one wave: 16 x 32 heads over 8 key heads, 512 x 512 x 128 causal and
-// padded, 148 us, where the forward takes 82 and dq 106 (tiles of 32 rows in place of 64 were slower by
-// a quarter).
+// matrix unit is busy 43% of the time and the LDS 48%, of which bank conflicts are 11. Head size 128 takes
+// the registers of a whole SIMD for one wave: 16 x 32 heads over 8 key heads, 512 x 512 x 128 causal and
+// padded, 145 us, where the forward takes 80 and dq 104 (tiles of 32 rows in place of 64 were slower by
+// a quarter). In fp32 it spills there besides, 105 to 201 registers a lane: 8 x 16 heads of 512 x 512 x 128
+// take 680 us, 51 TFLOP/s, where dq takes 278 (93) and the forward 200 (86).
 template <typename T, int DH, int KG, int RG, int IB>
 __global__ __launch_bounds__(kThreads, sizeof(T) * DH <= 128 ? 2 : 1) void attn_dkv_kernel(Params p) {
   typedef Geo<T, DH> Gm;
@@ -1055,10 +1059,11 @@ struct FwdPlan {
 };
 
 // Workgroups of 64 rows (or keys), whose waves share the other side and join at the end, where those of
-// 128 do not fill the chip once (in fp32, whose products take longer, twice). 12 heads of 1024 x 1024,
-// bf16, 96 groups of 128 rows: dq 26.5 us with 128, 20.3 with 64; dk and dv 27.8 and 20.4.
-// 4 x 12 heads of 512 x 512, 192 groups: 18.6 and 17.6, 18.6 and 18.8; 8 x 12 heads, 384 groups: dk and
-// dv 27 and 33. fp32, 7 x 12 heads of 181 x 181, 168 groups: dk and dv 34 and 23.
+// 128 are few: below 200 in 16 bits, in fp32, whose products take longer, below 512 (twice the CUs).
+// 12 heads of 1024 x 1024, bf16, 96 groups of 128 rows: dq 26.5 us with 128, 20.3 with 64; dk and dv 27.8
+// and 20.4. 4 x 12 heads of 512 x 512, 192 groups: 18.6 and 17.6, 18.6 and 18.8; 8 x 12 heads, 384 groups:
+// dk and dv 27 and 33, dq and the forward not measured there. fp32, 7 x 12 heads of 181 x 181, 168 groups:
+// dk and dv 34 and 23.
 bool small_groups(int64_t pairs, int64_t n, int es) { return pairs * cdiv(n, 128) < (es == 4 ? kTargetGroups : 200); }
 
 // Keys are split over workgroups where those are few and each has many tiles. In 16 bits long keys are
@@ -1095,7 +1100,7 @@ void launch_fwd_rows(const FwdPlan& f, const Params& p, hipStream_t st) {
 
 template <typename T, int DH>
 void launch_fwd(const FwdPlan& f, const Params& p, hipStream_t st) {
-  constexpr int JB = DH == 128 ? 1 : 2;  // 32 or 64 keys a tile: what leaves a SIMD two waves' registers
+  constexpr int JB = DH == 128 ? 1 : 2;  // 32 or 64 keys a tile: in 16 bits what leaves a SIMD two waves' registers
   if (f.rows == 32) launch_fwd_rows<T, DH, 1, 4, 1, 1>(f, p, st);
   else if (f.rows == 128) launch_fwd_rows<T, DH, 4, 1, JB, 2>(f, p, st);
   else launch_fwd_rows<T, DH, 2, 2, 1, 2>(f, p, st);

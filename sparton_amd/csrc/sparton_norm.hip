@@ -14,8 +14,11 @@
 // Every sum has a fixed order, so results are bitwise reproducible.
 //
 // Rows wider than a wave holds without spilling are shared by several waves, at the price of a barrier
-// a sum. bf16: 8192 x 768 with a residual, forward 10.0 us (3.8 TB/s), backward 12.6 (4.0) and 3.8 to add
-// the column sums; 16385 x 4096, forward 57 us (4.7 TB/s), backward 76 (5.3) and 4.9. A copy reaches 4.9.
+// a sum; past 8192 elements the backward's eight spill all the same (14 registers a lane in bf16, 30 in
+// fp16, 172 in fp32). bf16: 8192 x 768 with a residual, forward 10.0 us (3.8 TB/s), backward 12.6 (4.0) and
+// 3.8 to add the column sums; 16385 x 4096, forward 55 to 62 us from box to box (4.4 to 4.8 TB/s), backward
+// 76 to 80 (5.1 to 5.3) and 4.9. A copy reaches 4.9. 4096 x 16384 with a residual: backward 126 us in bf16
+// (4.2 TB/s), 460 in fp32 (2.3).
 
 #include <math.h>
 
