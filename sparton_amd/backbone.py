@@ -68,8 +68,8 @@ def key_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_func
         attention_mask = attention_mask[:, kv_offset:kv_offset + kv_length]
         attention_mask = nn.functional.pad(attention_mask, (0, kv_length - attention_mask.shape[-1]))
     if one:
-        device = kwargs.get("device", q_offset.device)
-        seen = (torch.arange(kv_offset, kv_offset + kv_length, device=device) <= q_offset).expand(batch_size, -1)
+        at = torch.arange(kv_offset, kv_offset + kv_length, device=kwargs.get("device") or q_offset.device)
+        seen = (at <= q_offset).expand(batch_size, -1)
         attention_mask = seen if attention_mask is None else seen & (attention_mask != 0)
     return attention_mask
 
