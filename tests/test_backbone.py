@@ -205,6 +205,8 @@ def test_a_mask_of_a_cache_with_room():
     m = torch.tensor([[0, 1, 1, 1, 1, 1], [1, 1, 1, 0, 1, 1]])
     want = nn.functional.pad(m, (0, 2)).bool()
     assert torch.equal(at(1, 8, 5, m), want)
+    assert torch.equal(key_mask(2, 1, 8, q_offset=torch.tensor(5), mask_function=causal_mask_function, attention_mask=m,
+                                device=None), want)
     assert torch.equal(at(1, 8, 3, m), want & (torch.arange(8) <= 3))
     with pytest.raises(ValueError, match="room"):
         at(3, 8, 3)
