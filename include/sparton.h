@@ -55,6 +55,14 @@ enum sparton_dtype {
  */
 #define SPARTON_F32_SPLIT 0x100
 
+/* Activation of the gated feed-forward product; gelu is the erf form. */
+enum sparton_activation {
+  SPARTON_SILU = 0,
+  SPARTON_GELU = 1,
+  SPARTON_GELU_TANH = 2,
+  SPARTON_RELU = 3,
+};
+
 /* Element type of the attention mask. Any nonzero value takes part in the
  * multiply; a tokenizer mask is int64 0/1. */
 enum sparton_mask_dtype {
@@ -355,6 +363,80 @@ int sparton_layer_norm_bwd(const void* dy, const void* x, const void* residual, 
                            int vec_dtype, const float* mean, const float* rstd, void* dx, void* d_weight,
                            void* d_bias, void* workspace, size_t workspace_bytes, int64_t M, int64_t D,
                            int dtype, void* stream);
+
+/*
+ * Root-mean-square norm of a backbone's rows with the residual's addition, over rows of D elements
+ * (1 <= D <= 16384; any alignment of whole elements). No counterpart in the reference.
+ *     h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight
+ * `dtype` is the type of x, residual, y, h and their gradients, `vec_dtype` that of weight and its gradient:
+ * SPARTON_F32 or `dtype`. residual may be NULL: h is then x. The norm reads the unrounded sum.
+ */
+size_t sparton_rms_norm_workspace_bytes(int64_t M, int64_t D); /* of the backward: column partial sums */
+
+/* Forward: y, h (may be NULL) and each row's 1/sqrt(mean + eps) (fp32 [M], may be NULL). */
+int sparton_rms_norm_fwd(const void* x, const void* residual, const void* weight, int vec_dtype, float eps,
+                         void* y, void* h, float* rstd, int64_t M, int64_t D, int dtype, void* stream);
+
+/* Forward with y in e4m3 (OCP, one byte) and a scale a row, fp32 [M]: y8 = e4m3(y / scale) with
+ * scale = max(max |y| / 448, 2^-126). A row with NaN or infinities is NaN where they are or all over. */
+int sparton_rms_norm_fwd_quantized(const void* x, const void* residual, const void* weight, int vec_dtype, float eps,
+                              void* y, float* scale, void* h, int64_t M, int64_t D, int dtype, void* stream);
+
+/* Backward: dx, the gradient of x and of residual alike, from dy, dh (the gradient of h; may be NULL), the
+ * forward's h (x where there was no residual) and rstd; and the sum over rows d_weight (may be NULL), added
+ * in fp32 and rounded once. Deterministic. */
+int sparton_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, int vec_dtype,
+                         const float* rstd, void* dx, void* d_weight, void* workspace, size_t workspace_bytes,
+                         int64_t M, int64_t D, int dtype, void* stream);
+
+/*
+ * Embedding: N rows of D elements from a table [V, D], times `scale`. No counterpart in the reference.
+ *     out[i] = scale table[ids[i]];   d_table[v] = scale sum of d_out[i] over ids[i] == v, ascending in i
+ * ids: `ids_dtype` SPARTON_MASK_I64 or SPARTON_MASK_I32. An id outside [0, V) reads nothing, gives a row of
+ * NaN and has no gradient; the id padding_idx (-1: none) has a row and no gradient. Any alignment of whole
+ * elements; N, V < 2^31 - 1024, D <= 2^20.
+ */
+int sparton_embedding_fwd(const void* ids, int ids_dtype, const void* table, float scale, void* out, int64_t N,
+                          int64_t V, int64_t D, int dtype, void* stream);
+
+/* Bytes of device scratch of the backward: the ids sorted, and sums of ids with many entries. */
+size_t sparton_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype);
+
+/* Backward: every row of d_table is written, those without a token with zeros. fp32 sums, rounded once;
+ * deterministic. */
+int sparton_embedding_bwd(const void* ids, int ids_dtype, const void* d_out, float scale, int64_t padding_idx,
+                          void* d_table, void* workspace, size_t workspace_bytes, int64_t N, int64_t V, int64_t D,
+                          int dtype, void* stream);
+
+/*
+ * Gated feed-forward product of M rows: x [M, D], w_gate and w_up [F, D], h [M, F], row-major. No counterpart
+ * in the reference.
+ *     g = x w_gate' + b_gate;  u = x w_up' + b_up;  h = activation(g) u
+ * D * element size is a multiple of 16 bytes; x and the weights have 16-byte aligned bases. b_gate and b_up may
+ * be NULL. Sums and g, u are fp32.
+ */
+
+/* Forward: h, and g and u (fp32 [M, F], for the backward; both or neither may be NULL). */
+int sparton_gated_fwd(const void* x, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
+                      int activation, void* h, float* gate, float* up, int64_t M, int64_t D, int64_t F, int dtype,
+                      void* stream);
+
+/* Forward on e4m3 rows (OCP) with a scale a row, x_scale [M], gate_scale and up_scale [F]; h in out_dtype. D is a
+ * multiple of 16. */
+int sparton_gated_fwd_quantized(const void* x, const float* x_scale, const void* w_gate, const float* gate_scale,
+                           const void* w_up, const float* up_scale, int activation, void* h, int64_t M, int64_t D,
+                           int64_t F, int out_dtype, void* stream);
+
+/* Bytes of device scratch of the backward: the gradients of g and u, and partial sums. */
+size_t sparton_gated_workspace_bytes(int64_t M, int64_t D, int64_t F, int with_bias, int dtype);
+
+/* Backward from dh and the forward's x, weights, g and u: dx, d_w_gate with d_w_up, d_b_gate and d_b_up (each may be
+ * NULL: not computed; the weights' both or neither). The gradients of g and u are rounded to `dtype` for the
+ * products and not for the biases' sums. Deterministic. */
+int sparton_gated_bwd(const void* dh, const void* x, const void* w_gate, const void* w_up, const float* gate,
+                      const float* up, int activation, void* dx, void* d_w_gate, void* d_w_up, void* d_b_gate,
+                      void* d_b_up, void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F,
+                      int dtype, void* stream);
 
 /*
  * Preference loss on pairs: for each of B rows a query's reps q, a preferred document's pos and a

@@ -15,10 +15,11 @@ import torch  # noqa: F401  (must be imported first: see module docstring)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 DEFAULT_LIB = os.path.join(_HERE, "libsparton_hip.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 # enum sparton_dtype / sparton_mask_dtype (include/sparton.h)
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATION_CODE = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}  # enum sparton_activation
 F32_SPLIT = 0x100  # SPARTON_F32_SPLIT
 
 
@@ -68,6 +69,17 @@ EXPORTED_SYMBOLS = (
     "sparton_layer_norm_fwd",
     "sparton_layer_norm_bwd",
     "sparton_layer_norm_workspace_bytes",
+    "sparton_rms_norm_fwd",
+    "sparton_rms_norm_fwd_quantized",
+    "sparton_rms_norm_bwd",
+    "sparton_rms_norm_workspace_bytes",
+    "sparton_embedding_fwd",
+    "sparton_embedding_bwd",
+    "sparton_embedding_workspace_bytes",
+    "sparton_gated_fwd",
+    "sparton_gated_fwd_quantized",
+    "sparton_gated_bwd",
+    "sparton_gated_workspace_bytes",
     "sparton_preference_fwd",
     "sparton_preference_bwd",
     "sparton_preference_workspace_bytes",
@@ -172,6 +184,25 @@ def load() -> ctypes.CDLL:
         L.sparton_layer_norm_bwd.restype = ctypes.c_int
         L.sparton_layer_norm_workspace_bytes.argtypes = [_i64, _i64]
         L.sparton_layer_norm_workspace_bytes.restype = ctypes.c_size_t
+        c_int, c_float, size_t = ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+        L.sparton_rms_norm_fwd.argtypes = [_vp] * 3 + [c_int, c_float] + [_vp] * 3 + [_i64, _i64, c_int, _vp]
+        L.sparton_rms_norm_fwd_quantized.argtypes = L.sparton_rms_norm_fwd.argtypes
+        L.sparton_rms_norm_bwd.argtypes = [_vp] * 4 + [c_int] + [_vp] * 4 + [size_t, _i64, _i64, c_int, _vp]
+        L.sparton_rms_norm_workspace_bytes.argtypes = [_i64, _i64]
+        L.sparton_embedding_fwd.argtypes = [_vp, c_int, _vp, c_float, _vp] + [_i64] * 3 + [c_int, _vp]
+        L.sparton_embedding_bwd.argtypes = ([_vp, c_int, _vp, c_float, _i64, _vp, _vp, size_t] + [_i64] * 3
+                                            + [c_int, _vp])
+        L.sparton_embedding_workspace_bytes.argtypes = [_i64] * 3 + [c_int]
+        L.sparton_gated_fwd.argtypes = [_vp] * 5 + [c_int] + [_vp] * 3 + [_i64] * 3 + [c_int, _vp]
+        L.sparton_gated_fwd_quantized.argtypes = [_vp] * 6 + [c_int, _vp] + [_i64] * 3 + [c_int, _vp]
+        L.sparton_gated_bwd.argtypes = [_vp] * 6 + [c_int] + [_vp] * 6 + [size_t] + [_i64] * 3 + [c_int, _vp]
+        L.sparton_gated_workspace_bytes.argtypes = [_i64] * 3 + [c_int, c_int]
+        for call in (L.sparton_rms_norm_fwd, L.sparton_rms_norm_fwd_quantized, L.sparton_rms_norm_bwd, L.sparton_embedding_fwd,
+                     L.sparton_embedding_bwd, L.sparton_gated_fwd, L.sparton_gated_fwd_quantized, L.sparton_gated_bwd):
+            call.restype = c_int
+        for size in (L.sparton_rms_norm_workspace_bytes, L.sparton_embedding_workspace_bytes,
+                     L.sparton_gated_workspace_bytes):
+            size.restype = size_t
         L.sparton_preference_fwd.argtypes = ([_vp] * 4 + [_i64, _i64] + [ctypes.c_float] * 3 + [_vp] * 4
                                              + [ctypes.c_size_t, ctypes.c_int, _vp])
         L.sparton_preference_fwd.restype = ctypes.c_int

@@ -19,7 +19,8 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 TORCH_LIB_NAME = "libsparton_torch.so"   # the eager torch ops (C++ autograd), on the C ABI above
 TORCH_LIB_PATH = os.path.join(HERE, TORCH_LIB_NAME)
 SOURCES = ["sparton_fwd.hip", "sparton_bwd.hip", "sparton_transform.hip", "sparton_loss.hip",
-           "sparton_attention.hip", "sparton_norm.hip", "sparton_preference.hip", "sparton_probe.hip", "sparton_capi.cpp"]
+           "sparton_attention.hip", "sparton_norm.hip", "sparton_preference.hip", "sparton_embedding.hip",
+           "sparton_rms_norm.hip", "sparton_gated.hip", "sparton_probe.hip", "sparton_capi.cpp"]
 ARCH = os.environ.get("SPARTON_OFFLOAD_ARCH", "gfx950")
 
 # Packed-fp32 VALU ops are disabled on purpose: hipcc would otherwise emit

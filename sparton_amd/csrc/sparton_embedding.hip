@@ -1,0 +1,446 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens, on gfx950:
+//     out[i, :] = scale table[id_i, :]
+//     d table[v, :] = scale sum over i with id_i = v of d out[i, :], in ascending order of i; 0 for other rows
+// An id outside [0, V) reads nothing: its row is NaN and it has no gradient. The padding id has a row and no
+// gradient.
+//
+// Forward: one pass, bound by memory.
+//
+// Backward: the ids are sorted with their places (a place breaks ties, so the order is the same every time),
+// and the sorted list is cut into chunks of kChunk entries. A wave takes a chunk and 64 vectors of 16 bytes of the
+// row width, keeps the sum of the running id in fp32, and writes a table row where an id's entries end. The sum of
+// an id whose entries go on in a neighbouring chunk is left in fp32 in the workspace, and a second launch adds such
+// sums in order: an id that half of the batch has is then summed by as many waves as any other entries. Rows
+// without a token are zeroed by other waves of the first launch, so every row is written once and d table needs no
+// clearing. No atomics: results are bitwise reproducible.
+//
+// The sort ranks each key among its wave's 64, then among 4 x 64, 4 x 256 (LDS) and 16 x 1024, 16 x 16384, ...
+// (memory): a key's rank is its own place in its list and, by binary search, the number of keys before it in each
+// of the others. No counts, no scans, one launch to 1024 keys and another for each factor of 16.
+
+#include <algorithm>
+
+#include "sparton_common.h"
+#include "sparton_rows.h"
+
+namespace sparton {
+namespace emb {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;           // forward: vectors of a thread
+constexpr int kTile = 1024;          // keys that one workgroup sorts
+constexpr int kWays = 16;            // lists that a merge launch joins into one
+constexpr int kChunk = 32;           // sorted entries of a wave
+constexpr int kInFlight = 8;
+constexpr int kJoinWaves = 4;
+constexpr int kZeroBytes = 32 << 10; // about what a wave zeroes
+constexpr uint32_t kNone = 0x7fffffffu;  // key of an entry without a gradient: behind every id
+constexpr int64_t kMaxD = 1 << 20;
+constexpr uint64_t kMaxThreads = 1ull << 32;  // a launch holds fewer (past that, workgroups were left out)
+
+// The id at place i, or kNone.
+__device__ __forceinline__ uint32_t id_at(const void* ids, int ids_dtype, int64_t i, int64_t V) {
+  if (ids_dtype == SPARTON_MASK_I64) {  // uniform
+    const int64_t v = ((const int64_t*)ids)[i];
+    return v >= 0 && v < V ? (uint32_t)v : kNone;
+  }
+  const int32_t v = ((const int32_t*)ids)[i];
+  return v >= 0 && v < V ? (uint32_t)v : kNone;
+}
+
+// ---- forward ------------------------------------------------------------------------------
+// Vector o of the row-major list of all rows' vectors: thread t of a workgroup takes kUnroll of them, kThreads
+// apart. The workgroup's first row comes from one 64-bit division, each vector's from a 32-bit one.
+template <typename T, int VE>
+__global__ __launch_bounds__(kThreads) void embed_fwd_kernel(const void* __restrict__ ids, int ids_dtype,
+                                                             const T* __restrict__ table, float scale,
+                                                             T* __restrict__ out, int64_t N, int64_t V, int D) {
+  const uint32_t nv = (uint32_t)cdiv(D, VE);
+  const int64_t first = (int64_t)blockIdx.x * (kThreads * kUnroll);
+  const int64_t row0 = first / nv;
+  const uint32_t off0 = (uint32_t)(first - row0 * nv);
+  int64_t row[kUnroll];
+  int at[kUnroll];
+  uint32_t id[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t o = off0 + u * kThreads + threadIdx.x, r = o / nv;
+    row[u] = row0 + r;
+    at[u] = min((int)((o - r * nv) * VE), D - VE);
+    id[u] = row[u] < N ? id_at(ids, ids_dtype, row[u], V) : kNone;
+  }
+  vec_t<T, VE> v[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    if (id[u] != kNone) v[u] = load_any<T, VE>(table + (int64_t)id[u] * D + at[u]);
+    else
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[u][e] = from_f32<T>(__builtin_nanf(""));
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    if (row[u] >= N) continue;
+    vec_t<T, VE> w;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) w[e] = from_f32<T>(scale * to_f32(v[u][e]));
+    store_any<T, VE>(out + row[u] * D + at[u], w);
+  }
+}
+
+// ---- sort ---------------------------------------------------------------------------------
+// How many of the ascending keys[0, n) lie before `key`, where keys equal to it do if `ties`; n <= 2^STEPS - 1.
+template <int STEPS> __device__ __forceinline__ int before(const uint32_t* keys, int n, uint32_t key, bool ties) {
+  const uint32_t edge = key + (ties ? 1u : 0u);  // keys are below 2^31
+  int lo = 0;
+#pragma unroll
+  for (int s = STEPS - 1; s >= 0; --s) {
+    const int probe = lo + (1 << s);
+    if (probe <= n && keys[probe - 1] < edge) lo = probe;
+  }
+  return lo;
+}
+
+// One merge step within a workgroup: runs of 2^LOG ascending keys become runs of 4 x 2^LOG.
+template <int LOG>
+__device__ __forceinline__ void merge4(uint32_t& key, uint32_t& place, uint32_t* keys, uint32_t* places) {
+  const int t = threadIdx.x, own = (t >> LOG) & 3, base = t & ~((4 << LOG) - 1);
+  keys[t] = key;
+  __syncthreads();
+  int rank = t & ((1 << LOG) - 1);
+#pragma unroll
+  for (int d = 1; d < 4; ++d) {
+    const int other = (own + d) & 3;
+    rank += before<LOG + 1>(keys + base + (other << LOG), 1 << LOG, key, other < own);
+  }
+  __syncthreads();
+  keys[base + rank] = key;
+  places[base + rank] = place;
+  __syncthreads();
+  key = keys[t];
+  place = places[t];
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(kTile) void embed_sort_kernel(const void* __restrict__ ids, int ids_dtype, int N, int64_t V,
+                                                           int64_t padding, uint32_t* __restrict__ keys_out,
+                                                           uint32_t* __restrict__ places_out) {
+  __shared__ uint32_t keys[kTile], places[kTile];
+  const int t = threadIdx.x, lane = t & 63;
+  const int i = blockIdx.x * kTile + t;
+  uint32_t key = i < N ? id_at(ids, ids_dtype, i, V) : kNone;
+  if (key == (uint64_t)padding) key = kNone;
+  int rank = 0;
+#pragma unroll 16
+  for (int j = 0; j < 64; ++j)
+    rank += (uint32_t)__builtin_amdgcn_readlane((int)key, j) < key + (lane > j ? 1u : 0u) ? 1 : 0;
+  keys[(t & ~63) + rank] = key;
+  places[(t & ~63) + rank] = (uint32_t)i;
+  __syncthreads();
+  key = keys[t];
+  uint32_t place = places[t];
+  __syncthreads();
+  merge4<6>(key, place, keys, places);
+  merge4<8>(key, place, keys, places);
+  // Entries past N have the greatest key and places past every other's: they are last of the last tile.
+  if (i < N) {
+    keys_out[i] = key;
+    places_out[i] = place;
+  }
+}
+
+// Runs of `run` ascending keys, kWays at a time, become runs of kWays `run`.
+__global__ __launch_bounds__(kThreads) void embed_merge_kernel(const uint32_t* __restrict__ keys,
+                                                               const uint32_t* __restrict__ places, int N, int run,
+                                                               uint32_t* __restrict__ keys_out,
+                                                               uint32_t* __restrict__ places_out) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= N) return;
+  const uint32_t key = keys[i];
+  const int64_t base = i / ((int64_t)run * kWays) * ((int64_t)run * kWays);
+  const int own = (int)((i - base) / run);
+  const int lists = (int)min((int64_t)kWays, cdiv(N - base, run));
+  int64_t rank = i - base - (int64_t)own * run;
+  int lo[kWays];
+#pragma unroll
+  for (int w = 0; w < kWays; ++w) lo[w] = 0;
+  // The searches step together, so that their loads are in flight at once.
+  for (int step = run; step > 0; step >>= 1) {
+#pragma unroll
+    for (int w = 0; w < kWays; ++w) {
+      if (w == own || w >= lists) continue;
+      const int64_t at = base + (int64_t)w * run + lo[w] + step - 1;
+      if (lo[w] + step <= run && at < N && keys[at] < key + (w < own ? 1u : 0u)) lo[w] += step;
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < kWays; ++w) rank += lo[w];
+  keys_out[base + rank] = key;
+  places_out[base + rank] = places[i];
+}
+
+// ---- backward -----------------------------------------------------------------------------
+struct Params {
+  const uint32_t *keys, *places;  // [N] ascending
+  const void* dy;
+  void* dw;
+  float* part;  // [chunks][2][D]: what goes on from the chunk before, and into the one behind
+  int N, D, chunks, cols, zero_rows;
+  int64_t V;
+  float scale;
+};
+
+template <typename T, int VE> __device__ __forceinline__ void put_row(T* to, const float* a, float scale) {
+  vec_t<T, VE> o;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) o[e] = from_f32<T>(scale * a[e]);
+  store_any<T, VE>(to, o);
+}
+
+// Waves [0, chunks cols) sum chunks, the others zero the table rows that no entry names.
+template <typename T, int VE> __global__ __launch_bounds__(kThreads) void embed_bwd_kernel(Params p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = (int64_t)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t sums = (int64_t)p.chunks * p.cols;
+  if (wave >= sums) {
+    const int64_t v0 = (wave - sums) * p.zero_rows;
+    if (v0 >= p.V) return;
+    const int64_t v = v0 + lane;
+    bool hit = lane >= p.zero_rows || v >= p.V;
+    if (!hit) {
+      int lo = 0;
+      for (int n = p.N; n > 0;) {  // first entry that is not before v
+        const int half = n >> 1;
+        if (p.keys[lo + half] < (uint32_t)v) {
+          lo += half + 1;
+          n -= half + 1;
+        } else {
+          n = half;
+        }
+      }
+      hit = lo < p.N && p.keys[lo] == (uint32_t)v;
+    }
+    float zeros[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) zeros[e] = 0.0f;
+    for (uint64_t bits = ~__ballot(hit); bits != 0; bits &= bits - 1) {
+      T* row = (T*)p.dw + (v0 + __builtin_ctzll(bits)) * p.D;
+      for (int at = lane * VE; at < p.D; at += 64 * VE) put_row<T, VE>(row + min(at, p.D - VE), zeros, 1.0f);
+    }
+    return;
+  }
+  const int chunk = (int)(wave / p.cols), col = (int)(wave % p.cols);
+  const int want = (col * 64 + lane) * VE;
+  const int at = min(want, p.D - VE);  // past the row's end: its last vector again, kept by nobody
+  const bool mine = want < p.D;
+  const int first = chunk * kChunk, n = min(kChunk, p.N - first);
+  // Lane l holds entry l of the chunk; lane kChunk the entry before it, lane kChunk + 1 the one behind.
+  const int look = lane < kChunk ? first + min(lane, n - 1) : lane == kChunk ? first - 1 : first + n;
+  const bool real = look >= 0 && look < p.N;
+  const uint32_t key = real ? p.keys[look] : kNone;
+  const uint32_t place = real ? p.places[look] : 0u;
+  const uint32_t prev = (uint32_t)__builtin_amdgcn_readlane((int)key, kChunk);
+  const uint32_t next = (uint32_t)__builtin_amdgcn_readlane((int)key, kChunk + 1);
+  float a[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) a[e] = 0.0f;
+  bool from_before = prev == (uint32_t)__builtin_amdgcn_readlane((int)key, 0);
+  for (int i0 = 0; i0 < n; i0 += kInFlight) {
+    vec_t<T, VE> v[kInFlight];
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j) {  // past n: the last entry again
+      const uint32_t row = (uint32_t)__builtin_amdgcn_readlane((int)place, min(i0 + j, n - 1));
+      v[j] = load_any<T, VE>((const T*)p.dy + (int64_t)row * p.D + at);
+    }
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j) {
+      const int i = i0 + j;
+      if (i >= n) break;
+      const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)key, i);
+      if (id == kNone) return;  // it and all behind it have no gradient
+#pragma unroll
+      for (int e = 0; e < VE; ++e) a[e] += to_f32(v[j][e]);
+      const uint32_t after = i + 1 < n ? (uint32_t)__builtin_amdgcn_readlane((int)key, i + 1) : next;
+      const bool goes_on = i + 1 == n && after == id;
+      if (after != id || goes_on) {
+        if (mine) {
+          if (from_before || goes_on) {
+            float* to = p.part + ((int64_t)chunk * 2 + (from_before ? 0 : 1)) * p.D + at;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) to[e] = a[e];
+          } else {
+            put_row<T, VE>((T*)p.dw + (int64_t)id * p.D + at, a, p.scale);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < VE; ++e) a[e] = 0.0f;
+        from_before = false;
+      }
+    }
+  }
+}
+
+// The id whose entries reach from chunk b into chunk b + 1 and began in chunk b: the sums of its chunks in
+// their order, a run of them a wave, and the waves' sums in order. 256 columns a workgroup.
+template <typename T> __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(Params p) {
+  __shared__ float sums[kJoinWaves][256];
+  const int b = blockIdx.x, last = (b + 1) * kChunk - 1;
+  const uint32_t id = p.keys[last];
+  if (id == kNone || p.keys[last + 1] != id) return;
+  const int first = b * kChunk;
+  if (first > 0 && p.keys[first] == id && p.keys[first - 1] == id) return;  // it began before chunk b
+  int lo = last + 1;
+  for (int n = p.N - lo; n > 0;) {  // first entry behind the id's
+    const int half = n >> 1;
+    if (p.keys[lo + half] <= id) {
+      lo += half + 1;
+      n -= half + 1;
+    } else {
+      n = half;
+    }
+  }
+  const int count = (lo - 1) / kChunk - b + 1;  // chunks: b's second sum, then first sums
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, seg = (count + kJoinWaves - 1) / kJoinWaves;
+  const int end = min(count, (wave + 1) * seg);
+  int at[4];
+  float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) at[e] = min((int)blockIdx.y * 256 + e * 64 + lane, p.D - 1);
+#pragma unroll 4
+  for (int c = wave * seg; c < end; ++c) {
+    const float* from = p.part + ((int64_t)(b + c) * 2 + (c == 0 ? 1 : 0)) * p.D;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] += from[at[e]];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sums[wave][e * 64 + lane] = a[e];
+  __syncthreads();
+  const int column = blockIdx.y * 256 + threadIdx.x;
+  if (column >= p.D) return;
+  float s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kJoinWaves; ++w) s += sums[w][threadIdx.x];
+  ((T*)p.dw)[(int64_t)id * p.D + column] = from_f32<T>(p.scale * s);
+}
+
+// ---- launches -----------------------------------------------------------------------------
+int vec_of(int64_t D, int dtype) {
+  const int ve = dtype == SPARTON_F32 ? 4 : 8;
+  return D < ve ? 1 : ve;
+}
+
+int zero_rows(int64_t D, int dtype) {
+  const int64_t row = D * (dtype == SPARTON_F32 ? 4 : 2);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(64, kZeroBytes / row));
+}
+
+// Bytes of the two sets of sorted keys and places, and of the chunks' sums.
+size_t list_bytes(int64_t N) { return (size_t)round_up(N * 4, 256); }
+size_t part_bytes(int64_t N, int64_t D) { return (size_t)(cdiv(N, kChunk) * 2 * D * 4); }
+
+int check(int64_t N, int64_t V, int64_t D, int dtype, int ids_dtype) {
+  if (N < 0 || V < 0 || D <= 0 || dtype < SPARTON_F32 || dtype > SPARTON_F16) return SPARTON_EINVAL;
+  if (ids_dtype != SPARTON_MASK_I64 && ids_dtype != SPARTON_MASK_I32) return SPARTON_EINVAL;
+  if (D > kMaxD || N > INT32_MAX - kTile || V >= (int64_t)kNone) return SPARTON_EUNSUPPORTED;
+  const int64_t nv = cdiv(D, vec_of(D, dtype));
+  if ((uint64_t)cdiv(N * nv, kThreads * kUnroll) * kThreads >= kMaxThreads) return SPARTON_EUNSUPPORTED;
+  const uint64_t waves = (uint64_t)(cdiv(N, kChunk) * cdiv(nv, 64) + cdiv(V, zero_rows(D, dtype)));
+  if (waves * 64 + kThreads >= kMaxThreads || (uint64_t)cdiv(N, kChunk) * cdiv(D, 256) * 64 * kJoinWaves >= kMaxThreads)
+    return SPARTON_EUNSUPPORTED;
+  return SPARTON_OK;
+}
+
+template <typename T, int VE>
+void forward(const void* ids, int ids_dtype, const void* table, float scale, void* out, int64_t N, int64_t V, int64_t D,
+             hipStream_t st) {
+  const int64_t vectors = N * cdiv(D, VE);
+  hipLaunchKernelGGL((embed_fwd_kernel<T, VE>), dim3((unsigned)cdiv(vectors, kThreads * kUnroll)), dim3(kThreads), 0, st,
+                     ids, ids_dtype, (const T*)table, scale, (T*)out, N, V, (int)D);
+}
+
+template <typename T, int VE> void backward(const Params& p, hipStream_t st) {
+  const int64_t waves = (int64_t)p.chunks * p.cols + cdiv(p.V, p.zero_rows);
+  hipLaunchKernelGGL((embed_bwd_kernel<T, VE>), dim3((unsigned)cdiv(waves, kThreads / 64)), dim3(kThreads), 0, st, p);
+  if (p.chunks > 1)
+    hipLaunchKernelGGL((embed_join_kernel<T>), dim3((unsigned)(p.chunks - 1), (unsigned)cdiv(p.D, 256)),
+                       dim3(64 * kJoinWaves), 0, st, p);
+}
+
+}  // namespace emb
+}  // namespace sparton
+
+using namespace sparton;
+
+#define SPARTON_EXPORT extern "C" __attribute__((visibility("default")))
+
+SPARTON_EXPORT int sparton_embedding_fwd(const void* ids, int ids_dtype, const void* table, float scale, void* out,
+                                         int64_t N, int64_t V, int64_t D, int dtype, void* stream) {
+  const int rc = emb::check(N, V, D, dtype, ids_dtype);
+  if (rc != SPARTON_OK) return rc;
+  if (N == 0) return SPARTON_OK;
+  if (ids == nullptr || out == nullptr || (table == nullptr && V > 0)) return SPARTON_EINVAL;
+  const uintptr_t es = dtype == SPARTON_F32 ? 4 : 2;
+  if (!aligned(ids, ids_dtype == SPARTON_MASK_I64 ? 8 : 4) || !aligned(table, es) || !aligned(out, es))
+    return SPARTON_EALIGN;
+  hipStream_t st = (hipStream_t)stream;
+  const bool one = emb::vec_of(D, dtype) == 1;
+  if (dtype == SPARTON_BF16)
+    one ? emb::forward<bf16, 1>(ids, ids_dtype, table, scale, out, N, V, D, st)
+        : emb::forward<bf16, 8>(ids, ids_dtype, table, scale, out, N, V, D, st);
+  else if (dtype == SPARTON_F16)
+    one ? emb::forward<f16, 1>(ids, ids_dtype, table, scale, out, N, V, D, st)
+        : emb::forward<f16, 8>(ids, ids_dtype, table, scale, out, N, V, D, st);
+  else
+    one ? emb::forward<float, 1>(ids, ids_dtype, table, scale, out, N, V, D, st)
+        : emb::forward<float, 4>(ids, ids_dtype, table, scale, out, N, V, D, st);
+  return (int)hipGetLastError();
+}
+
+SPARTON_EXPORT size_t sparton_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype) {
+  if (emb::check(N, V, D, dtype, SPARTON_MASK_I64) != SPARTON_OK || N == 0) return 0;
+  return 4 * emb::list_bytes(N) + emb::part_bytes(N, D);
+}
+
+SPARTON_EXPORT int sparton_embedding_bwd(const void* ids, int ids_dtype, const void* d_out, float scale, int64_t padding_idx,
+                                         void* d_table, void* workspace, size_t workspace_bytes, int64_t N, int64_t V,
+                                         int64_t D, int dtype, void* stream) {
+  const int rc = emb::check(N, V, D, dtype, ids_dtype);
+  if (rc != SPARTON_OK) return rc;
+  if (V == 0) return SPARTON_OK;
+  if (d_table == nullptr || (N > 0 && (ids == nullptr || d_out == nullptr))) return SPARTON_EINVAL;
+  const uintptr_t es = dtype == SPARTON_F32 ? 4 : 2;
+  if (!aligned(ids, ids_dtype == SPARTON_MASK_I64 ? 8 : 4) || !aligned(d_out, es) || !aligned(d_table, es))
+    return SPARTON_EALIGN;
+  hipStream_t st = (hipStream_t)stream;
+  emb::Params p = {};
+  if (N > 0) {
+    if (workspace == nullptr || workspace_bytes < sparton_embedding_workspace_bytes(N, V, D, dtype))
+      return SPARTON_EWORKSPACE;
+    if (!aligned(workspace, 256)) return SPARTON_EALIGN;
+    const size_t list = emb::list_bytes(N);
+    uint32_t* k[2] = {(uint32_t*)workspace, (uint32_t*)((char*)workspace + list)};
+    uint32_t* at[2] = {(uint32_t*)((char*)workspace + 2 * list), (uint32_t*)((char*)workspace + 3 * list)};
+    p.part = (float*)((char*)workspace + 4 * list);
+    hipLaunchKernelGGL(emb::embed_sort_kernel, dim3((unsigned)cdiv(N, emb::kTile)), dim3(emb::kTile), 0, st, ids,
+                       ids_dtype, (int)N, V, padding_idx, k[0], at[0]);
+    int in = 0;
+    for (int64_t run = emb::kTile; run < N; run *= emb::kWays, in ^= 1)
+      hipLaunchKernelGGL(emb::embed_merge_kernel, dim3((unsigned)cdiv(N, emb::kThreads)), dim3(emb::kThreads), 0, st,
+                         k[in], at[in], (int)N, (int)run, k[in ^ 1], at[in ^ 1]);
+    p.keys = k[in];
+    p.places = at[in];
+  }
+  const int ve = emb::vec_of(D, dtype);
+  p.dy = d_out;
+  p.dw = d_table;
+  p.N = (int)N;
+  p.D = (int)D;
+  p.V = V;
+  p.chunks = (int)cdiv(N, emb::kChunk);
+  p.cols = (int)cdiv(cdiv(D, ve), 64);
+  p.zero_rows = emb::zero_rows(D, dtype);
+  p.scale = scale;
+  if (dtype == SPARTON_BF16) ve == 1 ? emb::backward<bf16, 1>(p, st) : emb::backward<bf16, 8>(p, st);
+  else if (dtype == SPARTON_F16) ve == 1 ? emb::backward<f16, 1>(p, st) : emb::backward<f16, 8>(p, st);
+  else ve == 1 ? emb::backward<float, 1>(p, st) : emb::backward<float, 4>(p, st);
+  return (int)hipGetLastError();
+}

@@ -1,0 +1,791 @@
+// Gated feed-forward product, forward and backward, on gfx950:
+//     g = x Wg' + bg,  u = x Wu' + bu,  h = act(g) u             x [M, D], Wg and Wu [F, D], h [M, F]
+//     du = dh act(g),  dg = dh u act'(g)
+//     dx = dg Wg + du Wu,  dWg = dg' x,  dWu = du' x,  db = column sums of dg and du
+// and the forward on e4m3 rows and weights with a scale a row.
+//
+// One kernel runs every product. A workgroup's tile is BQ rows by BP columns of the result, its inner dimension
+// streams through two LDS stages in slabs of 128 bytes, copied there directly from memory. A wave holds its part as
+// 32x32 MFMA results in transposed form: a lane is a row of the result, and its registers hold groups of four
+// consecutive columns, which it stores as one vector. The forward's columns are 32 of the gate, 32 of the up
+// projection and so on, so g and u of one element meet in one lane.
+//
+// An operand whose memory runs along the inner dimension (x and the weights forward, dg and du for dx) is staged as
+// rows of 128 bytes; one that runs across it (the weights for dx, everything for dW) as it lies, 64 rows of BQ or BP
+// columns, and read with the transposing LDS loads (fp32: element by element). Nothing is transposed in memory.
+// Both have their 16-byte chunks XORed so that the reads spread over all banks. What lies past an operand's end is
+// given an address past the buffer's, which reads as zero.
+//
+// The 8-bit matrix instructions add the products of eight neighbours with about 14 bits below the largest one's power
+// of two (what is further below is dropped), and such sums in fp32. The rows' own rounding to e4m3, 2^-4, is far above that.
+//
+// Between forward and backward g and u are kept in fp32: in 16 bits their rounding, on top of that of dg and du to
+// the matrix instructions' operands, would double the gradients' error. In fp16, dg and du have fp16's range, as dh has.
+
+#include <math.h>
+
+#include <algorithm>
+
+#include "sparton_common.h"
+#include "sparton_rows.h"
+
+namespace sparton {
+namespace gated {
+
+constexpr int kSlab = 128;  // bytes of the inner dimension
+constexpr int kGroupQ = 8;  // row tiles that share the weights' tiles while both are in an XCD's L2
+constexpr uint64_t kMaxThreads = 1ull << 32;  // a launch holds fewer (past that, workgroups were left out)
+
+struct e4m3 {
+  uint8_t bits;
+};
+
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+
+// ---- activations --------------------------------------------------------------------------
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// act(g), and its derivative where it is asked for.
+template <bool GRAD> __device__ __forceinline__ float activate(int act, float g, float* d) {
+  switch (act) {  // uniform
+    case SPARTON_SILU: {
+      const float s = sigmoid(g);
+      if (GRAD) *d = s * (1.0f + g * (1.0f - s));
+      return g * s;
+    }
+    case SPARTON_GELU: {
+      const float c = 0.5f * erfcf(-0.70710678118654752f * g);
+      if (GRAD) *d = c + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+      return g * c;
+    }
+    case SPARTON_GELU_TANH: {  // 0.5 (1 + tanh(z)) = sigmoid(2 z)
+      const float s = sigmoid(g * (1.5957691216057308f + 0.071354816272600243f * g * g));
+      if (GRAD) *d = s + g * s * (1.0f - s) * (1.5957691216057308f + 0.21406444881780073f * g * g);
+      return g * s;
+    }
+    default: {  // SPARTON_RELU
+      if (GRAD) *d = g > 0.0f ? 1.0f : 0.0f;
+      return g > 0.0f || g != g ? g : 0.0f;
+    }
+  }
+}
+
+// ---- matrix instructions ------------------------------------------------------------------
+// A step's operand: CH chunks of 16 bytes a lane. Lane l holds row (or column) l % 32, and of each 32 bytes of the
+// inner dimension the half l / 32.
+template <typename T> constexpr int kCh = 1;
+template <> constexpr int kCh<e4m3> = 2;
+template <typename T> struct Frag {
+  u32x4 c[kCh<T>];
+};
+
+__device__ __forceinline__ void mma(f32x16& d, const Frag<bf16>& a, const Frag<bf16>& b) {
+  d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.c[0]), __builtin_bit_cast(bf16x8, b.c[0]), d, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& d, const Frag<f16>& a, const Frag<f16>& b) {
+  d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a.c[0]), __builtin_bit_cast(f16x8, b.c[0]), d, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& d, const Frag<float>& a, const Frag<float>& b) {
+  const f32x4 x = __builtin_bit_cast(f32x4, a.c[0]), y = __builtin_bit_cast(f32x4, b.c[0]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) d = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], d, 0, 0, 0);
+}
+__device__ __forceinline__ i32x8 wide(const Frag<e4m3>& f) {
+  return __builtin_shufflevector(__builtin_bit_cast(i32x4, f.c[0]), __builtin_bit_cast(i32x4, f.c[1]), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ void mma(f32x16& d, const Frag<e4m3>& a, const Frag<e4m3>& b) {
+  d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), d, 0, 0, 0, 0, 0, 0);
+}
+
+// ---- operands -----------------------------------------------------------------------------
+// One operand of a product: n rows (columns, where it lies across the inner dimension) that start `ld` bytes apart.
+// b1: the second half of the inner dimension (dx), or the rows that take turns with b0's (forward).
+struct Side {
+  const char *b0, *b1;
+  int64_t ld, n;
+};
+
+__device__ __forceinline__ int swizzle_rows(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+
+// A wave's share of copying one operand's slabs: R rows of 128 bytes, or 128 / sizeof(T) rows of R elements (KM), by
+// NW waves, 64 chunks of 16 bytes a copy. PAIR: rows 64 k .. + 31 of b0, rows 64 k + 32 .. + 63 of b1.
+template <typename T, bool KM, int R, int NW, bool PAIR> struct Copy {
+  static constexpr int E = sizeof(T), N = R / 8 / NW, CPR = KM ? R * E / 16 : 8;
+  static_assert(R % (8 * NW) == 0, "every wave copies as much");
+  static_assert(!KM || (E == 2 ? 64 / CPR * NW % 4 == 0 : 64 / CPR * NW % 8 == 0 || CPR == 64), "one swizzle a lane");
+  static constexpr uint32_t kNowhere = 0xc0000000u;
+  uint32_t off[N];
+  int at;  // KC: byte of the slab; KM: its row
+  const char *b0, *b1;
+  int64_t step;
+  __device__ __forceinline__ void init(const Side& s, int64_t first) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if constexpr (!KM) {
+      at = ((lane & 7) ^ (lane >> 3) ^ (w & 1)) * 16;
+      step = kSlab;
+      b0 = s.b0 + first * s.ld;
+      b1 = s.b1 + first * s.ld;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = 8 * (w + NW * i) + (lane >> 3), row = PAIR ? (r >> 6) * 32 + (r & 31) : r;
+        off[i] = first + row < s.n ? (uint32_t)(row * s.ld + at) : kNowhere;
+      }
+    } else {
+      const int c = w * 64 + lane, row = c / CPR, phys = c % CPR;
+      const int chunk = phys ^ (E == 2 ? (row & 3) << 2 : ((row >> 2) & 1) << 3);
+      at = row;
+      step = (int64_t)(kSlab / E) * s.ld;
+      b0 = s.b0 + first * E;
+      b1 = s.b1 + first * E;
+      const bool in = first + chunk * (16 / E) < s.n;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        off[i] = in ? (uint32_t)((row + i * (NW * 64 / CPR)) * s.ld + chunk * 16) : kNowhere;
+    }
+  }
+  // Slab k of one half, of whose inner dimension `left` elements are left, into LDS at `to` (this wave's first chunk).
+  __device__ __forceinline__ void issue(int half, int k, int64_t left, uint32_t to) const {
+    const char* base = (!PAIR && half ? b1 : b0) + k * step;
+    const char* other = PAIR ? b1 + k * step : base;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      const char* from = PAIR && (((w + NW * i) >> 2) & 1) ? other : base;
+      const bool in = KM ? at + i * (NW * 64 / CPR) < left : at < left * E;
+      const uint32_t o = in ? off[i] : kNowhere;
+      u32x4 rsrc;
+      rsrc[0] = (uint32_t)(uintptr_t)from;
+      rsrc[1] = (uint32_t)((uintptr_t)from >> 32);
+      rsrc[2] = 0x80000000u;
+      rsrc[3] = 0x00020000u;
+      const uint32_t dst = to + (uint32_t)(i * NW) * 1024u;
+      // The compiler would wait for a copy it knows of before any LDS read; these are waited for at the slab's end.
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(o), "s"(rsrc));
+    }
+  }
+};
+
+// Where a lane's fragments lie in a slab: J blocks of 32 rows (columns) from block `blk` on.
+template <typename T, bool KM, int R, int J> struct Read {
+  static constexpr int E = sizeof(T);
+  const char* p[KM ? J : 4];
+  __device__ __forceinline__ void init(int blk) {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+    if constexpr (!KM) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        p[s] = (const char*)(uintptr_t)((blk * 32 + l32) * kSlab + ((2 * s + h) ^ swizzle_rows(l32)) * 16);
+    } else if constexpr (E == 2) {
+      const int q = lane & 15, kk = q >> 2;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        p[j] = (const char*)(uintptr_t)((8 * h + kk) * (R * 2) + (((blk + j) * 4) ^ (kk << 2)) * 16 + ((lane >> 4) & 1) * 32 +
+                                        (q & 3) * 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        p[j] = (const char*)(uintptr_t)(4 * h * (R * 4) + (((blk + j) * 8) ^ (h << 3)) * 16 + l32 * 4);
+    }
+  }
+  // Block j's operand of step s, of the slab at `slab`.
+  __device__ __forceinline__ Frag<T> get(const char* slab, int j, int s) const {
+    Frag<T> f;
+    if constexpr (!KM) {
+#pragma unroll
+      for (int c = 0; c < kCh<T>; ++c) f.c[c] = *(const u32x4*)(slab + (uintptr_t)p[s * kCh<T> + c] + j * 32 * kSlab);
+    } else if constexpr (E == 2) {
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const char* at = slab + (uintptr_t)p[j] + s * 16 * (R * 2);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * (R * 2)));
+      f.c[0] = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const char* at = slab + (uintptr_t)p[j] + s * 8 * (R * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f.c[0][e] = *(const uint32_t*)(at + e * (R * 4));
+    }
+    return f;
+  }
+};
+
+// ---- the product --------------------------------------------------------------------------
+struct Params {
+  Side q, p;              // rows and columns of the result
+  int64_t K;              // inner dimension of a half, in elements
+  int half_slabs, slabs;  // of one half, and of all halves
+  int tq, tp, splits, per_split;
+  // plain results: rows [0, q.n) of out, or fp32 sums of each split; `turns` problems beside each other
+  void* out[2];
+  const char* q_turn;
+  float* part;
+  int turns;
+  // the gated result
+  void* h;
+  float *g, *u;
+  const void *bg, *bu;
+  const float *sx, *sg, *su;
+  int act;
+};
+
+// Four consecutive columns of a result's row, of which `n` are there.
+template <typename T> __device__ __forceinline__ void store4(T* p, const float* v, int64_t n) {
+  if (n >= 4) {
+    vec_t<T, 4> o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(v[e]);
+    store_any<T, 4>(p, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < n) p[e] = from_f32<T>(v[e]);
+  }
+}
+
+// A workgroup's tile. Consecutive workgroups go to the eight XCDs in turn: each XCD takes a run of the tiles, which
+// walk kGroupQ row tiles before the next column tile, so that what is in flight shares operands in its L2.
+struct Place {
+  int q, p, split, turn;
+};
+__device__ __forceinline__ Place place_of(const Params& a) {
+  const int tiles = a.tq * a.tp * a.splits * a.turns, w = blockIdx.x, x = w & 7, per = tiles >> 3, more = tiles & 7;
+  int i = x * per + min(x, more) + (w >> 3);
+  Place r;
+  r.turn = i / (a.tq * a.tp * a.splits);
+  i -= r.turn * a.tq * a.tp * a.splits;
+  r.split = i / (a.tq * a.tp);
+  i -= r.split * a.tq * a.tp;
+  const int group = i / (kGroupQ * a.tp), first = group * kGroupQ, rows = min(kGroupQ, a.tq - first);
+  i -= first * a.tp;
+  r.p = i / rows;
+  r.q = first + i - r.p * rows;
+  return r;
+}
+
+template <typename T, typename O, bool GATED>
+__device__ __forceinline__ void write(const Params& a, int64_t row, int64_t col, int split, int turn, const f32x16& c0,
+                                      const f32x16& c1, int r) {
+  if (row >= a.q.n || col >= a.p.n) return;
+  const int64_t at = row * a.p.n + col, left = a.p.n - col;
+  float v[4];
+  if constexpr (GATED) {
+    float g[4], u[4], d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t f = min(col + e, a.p.n - 1);
+      g[e] = c0[r + e];
+      u[e] = c1[r + e];
+      if constexpr (sizeof(T) == 1) {
+        const float sx = a.sx[row];
+        g[e] *= sx * a.sg[f];
+        u[e] *= sx * a.su[f];
+      }
+      if (a.bg != nullptr) g[e] += to_f32(((const O*)a.bg)[f]);
+      if (a.bu != nullptr) u[e] += to_f32(((const O*)a.bu)[f]);
+      v[e] = activate<false>(a.act, g[e], &d) * u[e];
+    }
+    store4<O>((O*)a.h + at, v, left);
+    if (a.g != nullptr) {
+      store4<float>(a.g + at, g, left);
+      store4<float>(a.u + at, u, left);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = c0[r + e];
+    if (a.splits > 1) store4<float>(a.part + ((int64_t)split * a.turns + turn) * a.q.n * a.p.n + at, v, left);
+    else store4<O>((O*)a.out[turn] + at, v, left);
+  }
+}
+
+// WQ x WP waves, each JQ x JP blocks of 32 x 32.
+template <typename T, typename O, bool QKM, bool PKM, bool GATED, int WQ, int WP, int JQ, int JP>
+__global__ __launch_bounds__(64 * WQ * WP, 2) void gated_gemm_kernel(Params a) {
+  constexpr int NW = WQ * WP, BQ = WQ * JQ * 32, BP = WP * JP * 32, STAGE = (BQ + BP) * kSlab;
+  constexpr int STEPS = 4 / kCh<T>;
+  static_assert(!GATED || JP == 2, "a wave holds a gate block and the up block beside it");
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  const Place at = place_of(a);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = w % WQ, wp = w / WQ;
+  Copy<T, QKM, BQ, NW, false> cq;
+  Copy<T, PKM, BP, NW, GATED> cp;
+  Side q = a.q;
+  if (at.turn > 0) q.b0 = a.q_turn;
+  cq.init(q, (int64_t)at.q * BQ);
+  cp.init(a.p, (int64_t)at.p * (GATED ? BP / 2 : BP));
+  Read<T, QKM, BQ, JQ> rq;
+  Read<T, PKM, BP, JP> rp;
+  rq.init(wq * JQ);
+  rp.init(wp * JP);
+  f32x16 acc[JQ][JP];
+#pragma unroll
+  for (int i = 0; i < JQ; ++i)
+#pragma unroll
+    for (int j = 0; j < JP; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+  const int k_end = min(a.slabs, (at.split + 1) * a.per_split);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  const auto issue = [&](int k, int stage) {
+    const int half = k >= a.half_slabs ? 1 : 0, kk = k - half * a.half_slabs;
+    const int64_t left = a.K - (int64_t)kk * (kSlab / (int)sizeof(T));
+    const uint32_t to = lds0 + stage * STAGE + w * 1024;
+    cq.issue(half, kk, left, to);
+    cp.issue(half, kk, left, to + BQ * kSlab);
+  };
+  int k = at.split * a.per_split, stage = 0;
+  if (k < k_end) issue(k, 0);
+  for (; k < k_end; ++k, stage ^= 1) {
+    // This slab has landed for every wave, and the stage before it is read out.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (k + 1 < k_end) issue(k + 1, stage ^ 1);
+    const char* sq = lds + stage * STAGE;
+    const char* sp = sq + BQ * kSlab;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      Frag<T> fp[JP], fq[JQ];
+#pragma unroll
+      for (int j = 0; j < JP; ++j) fp[j] = rp.get(sp, j, s);
+#pragma unroll
+      for (int i = 0; i < JQ; ++i) fq[i] = rq.get(sq, i, s);
+#pragma unroll
+      for (int i = 0; i < JQ; ++i)
+#pragma unroll
+        for (int j = 0; j < JP; ++j) mma(acc[i][j], fp[j], fq[i]);
+    }
+  }
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < JQ; ++i) {
+    const int64_t row = (int64_t)at.q * BQ + (wq * JQ + i) * 32 + l32;
+    if constexpr (GATED) {
+      const int64_t col = (int64_t)at.p * (BP / 2) + wp * 32 + 4 * h;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) write<T, O, true>(a, row, col + 8 * r, at.split, at.turn, acc[i][0], acc[i][1], 4 * r);
+    } else {
+#pragma unroll
+      for (int j = 0; j < JP; ++j) {
+        const int64_t col = (int64_t)at.p * BP + (wp * JP + j) * 32 + 4 * h;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) write<T, O, false>(a, row, col + 8 * r, at.split, at.turn, acc[i][j], acc[i][j], 4 * r);
+      }
+    }
+  }
+}
+
+// ---- few rows -----------------------------------------------------------------------------
+// Up to 64 rows: bound by reading the weights. A workgroup has 32 gate and 32 up rows; its waves share the inner
+// dimension, each with its operands straight from memory into registers, kAhead steps ahead, and their sums are
+// added in wave order in LDS.
+constexpr int kFewWaves = 8;
+
+template <typename T, typename O, int JQ>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void gated_few_kernel(Params a) {
+  constexpr int EPC = 16 / sizeof(T), KSTEP = 2 * EPC * kCh<T>;  // elements of a step
+  constexpr int kAhead = 4 / kCh<T>;
+  __shared__ float sums[kFewWaves * JQ * 2 * 16 * 64];  // [wave][block][gate, up][register][lane]
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t f0 = (int64_t)blockIdx.x * 32, f = min(f0 + l32, a.p.n - 1);
+  const char* wg = a.p.b0 + f * a.p.ld;
+  const char* wu = a.p.b1 + f * a.p.ld;
+  const char* x[JQ];
+#pragma unroll
+  for (int i = 0; i < JQ; ++i) x[i] = a.q.b0 + min((int64_t)(i * 32 + l32), a.q.n - 1) * a.q.ld;
+  const int steps = (int)cdiv(a.K, KSTEP), per = (steps + kFewWaves - 1) / kFewWaves;
+  const int s1 = min(steps, (w + 1) * per);
+  f32x16 ag[JQ], au[JQ];
+#pragma unroll
+  for (int i = 0; i < JQ; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ag[i][e] = au[i][e] = 0.0f;
+  Frag<T> fg[kAhead], fu[kAhead], fx[kAhead][JQ];
+  const auto load = [&](int slot, int s) {
+#pragma unroll
+    for (int c = 0; c < kCh<T>; ++c) {
+      const int64_t k = (int64_t)s * KSTEP + (2 * c + h) * EPC;
+      const bool in = s < s1 && k < a.K;
+      const int64_t o = (in ? k : 0) * (int64_t)sizeof(T);
+      const u32x4 zero = {0, 0, 0, 0};
+      const u32x4 vg = *(const u32x4*)(wg + o), vu = *(const u32x4*)(wu + o);
+      fg[slot].c[c] = in ? vg : zero;
+      fu[slot].c[c] = in ? vu : zero;
+#pragma unroll
+      for (int i = 0; i < JQ; ++i) {
+        const u32x4 vx = *(const u32x4*)(x[i] + o);
+        fx[slot][i].c[c] = in ? vx : zero;
+      }
+    }
+  };
+  const int s0 = w * per;
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) load(n, s0 + n);
+  for (int s = s0; s < s1; s += kAhead) {
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      // steps past s1 multiply zeros
+#pragma unroll
+      for (int i = 0; i < JQ; ++i) {
+        mma(ag[i], fg[n], fx[n][i]);
+        mma(au[i], fu[n], fx[n][i]);
+      }
+      load(n, s + kAhead + n);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < JQ; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      sums[(((w * JQ + i) * 2 + 0) * 16 + e) * 64 + lane] = ag[i][e];
+      sums[(((w * JQ + i) * 2 + 1) * 16 + e) * 64 + lane] = au[i][e];
+    }
+  __syncthreads();
+  // Wave w takes registers 4 (w % 4) .. + 3 of block w / 4.
+  for (int o = w; o < JQ * 4; o += kFewWaves) {
+    const int i = o >> 2, r = o & 3;
+    f32x16 g, u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float sg = 0.0f, su = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kFewWaves; ++v) {
+        sg += sums[(((v * JQ + i) * 2 + 0) * 16 + 4 * r + e) * 64 + lane];
+        su += sums[(((v * JQ + i) * 2 + 1) * 16 + 4 * r + e) * 64 + lane];
+      }
+      g[e] = sg;
+      u[e] = su;
+    }
+    write<T, O, true>(a, i * 32 + l32, f0 + 8 * r + 4 * h, 0, 0, g, u, 0);
+  }
+}
+
+// ---- dg and du ----------------------------------------------------------------------------
+constexpr int kActThreads = 256;
+constexpr int kActCols = 4;  // columns of a thread
+
+// dg and du [M, ld], zeros past F, and with `part` the column sums of a workgroup's rows, before their rounding.
+template <typename T>
+__global__ __launch_bounds__(kActThreads) void gated_act_bwd_kernel(const T* __restrict__ dh, const float* __restrict__ g,
+                                                                    const float* __restrict__ u, T* __restrict__ dg,
+                                                                    T* __restrict__ du, float* __restrict__ part,
+                                                                    int64_t M, int64_t F, int64_t ld, int act, int rows,
+                                                                    int strips) {
+  const int strip = blockIdx.x % strips;
+  const int64_t blk = blockIdx.x / strips, col = ((int64_t)strip * kActThreads + threadIdx.x) * kActCols;
+  const int64_t r0 = blk * rows, r1 = min(M, r0 + rows);
+  if (col >= ld) return;
+  const int n = (int)max((int64_t)0, min((int64_t)kActCols, F - col));
+  float sg[kActCols] = {}, su[kActCols] = {};
+  for (int64_t r = r0; r < r1; ++r) {
+    float vd[kActCols], vg[kActCols], vu[kActCols], og[kActCols], ou[kActCols];
+    const int64_t at = r * F + col;
+    if (n == kActCols) {
+      const vec_t<T, 4> d = load_any<T, 4>(dh + at);
+      const vec_t<float, 4> a = load_any<float, 4>(g + at), b = load_any<float, 4>(u + at);
+#pragma unroll
+      for (int e = 0; e < kActCols; ++e) vd[e] = to_f32(d[e]), vg[e] = a[e], vu[e] = b[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < kActCols; ++e) {
+        vd[e] = e < n ? to_f32(dh[at + e]) : 0.0f;
+        vg[e] = e < n ? g[at + e] : 0.0f;
+        vu[e] = e < n ? u[at + e] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kActCols; ++e) {
+      float d;
+      const float a = activate<true>(act, vg[e], &d);
+      og[e] = vd[e] * vu[e] * d;
+      ou[e] = vd[e] * a;
+      if (part != nullptr) {
+        sg[e] += og[e];
+        su[e] += ou[e];
+      }
+    }
+    store4<T>(dg + r * ld + col, og, ld - col);
+    store4<T>(du + r * ld + col, ou, ld - col);
+  }
+  if (part == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < kActCols; ++e) {
+    if (e >= n) break;
+    part[blk * 2 * F + col + e] = sg[e];
+    part[blk * 2 * F + F + col + e] = su[e];
+  }
+}
+
+// The splits' sums added in order.
+template <typename O>
+__global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ part, int splits, int64_t n, int turns,
+                                                         O* out0, O* out1) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n * turns) return;
+  const int64_t total = n * turns;
+  float v[4];
+  const int64_t left = min((int64_t)4, total - i);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float s = 0.0f;
+    const int64_t at = min(i + e, total - 1);
+    for (int k = 0; k < splits; ++k) s += part[k * total + at];
+    v[e] = s;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t at = i + e;
+    if (e < left) (at < n ? out0 + at : out1 + (at - n))[0] = from_f32<O>(v[e]);
+  }
+}
+
+// ---- launches -----------------------------------------------------------------------------
+constexpr int kCus = 256;
+constexpr int64_t kFewRows = 64;
+constexpr int kBiasBlocks = 256;
+
+struct Split {
+  bool small;
+  int tq, tp, splits, per_split, slabs;
+};
+
+// 256 x 256 tiles where there is one for most CUs, else 128 x 128; and where those are few too, the inner dimension
+// is split over workgroups, in runs of eight slabs or more.
+Split split_of(int64_t rows, int64_t cols, int64_t turns, int64_t slabs, bool may_split) {
+  Split s;
+  s.small = cdiv(rows, 256) * cdiv(cols, 256) * turns < 192;
+  const int64_t b = s.small ? 128 : 256;
+  s.tq = (int)cdiv(rows, b);
+  s.tp = (int)cdiv(cols, b);
+  s.slabs = (int)slabs;
+  const int64_t tiles = std::max<int64_t>(1, (int64_t)s.tq * s.tp * turns);
+  int64_t n = 1;
+  if (may_split && tiles < 2 * kCus) n = std::max<int64_t>(1, std::min<int64_t>(cdiv(2 * kCus, tiles), slabs / 8));
+  n = std::min<int64_t>(n, 16);
+  s.per_split = (int)std::max<int64_t>(1, cdiv(slabs, n));
+  s.splits = (int)std::max<int64_t>(1, cdiv(slabs, s.per_split));
+  return s;
+}
+
+template <typename T, typename O, bool QKM, bool PKM, bool GATED> int gemm(Params p, const Split& s, hipStream_t st) {
+  p.tq = s.tq;
+  p.tp = s.tp;
+  p.splits = s.splits;
+  p.per_split = s.per_split;
+  p.slabs = s.slabs;
+  const unsigned grid = (unsigned)((int64_t)s.tq * s.tp * s.splits * p.turns);
+  if (grid == 0) return SPARTON_OK;
+  if (s.small)
+    hipLaunchKernelGGL((gated_gemm_kernel<T, O, QKM, PKM, GATED, 2, 2, 2, 2>), dim3(grid), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((gated_gemm_kernel<T, O, QKM, PKM, GATED, 2, 4, 4, 2>), dim3(grid), dim3(512), 0, st, p);
+  return (int)hipGetLastError();
+}
+
+int64_t es_of(int dtype) { return dtype == SPARTON_F32 ? 4 : 2; }
+int64_t pad_of(int64_t F, int dtype) { return round_up(F, 16 / es_of(dtype)); }
+
+int check(int64_t M, int64_t D, int64_t F, int dtype, int64_t es, int act) {
+  if (M < 0 || D <= 0 || F < 0 || dtype < SPARTON_F32 || dtype > SPARTON_F16) return SPARTON_EINVAL;
+  if (act < SPARTON_SILU || act > SPARTON_RELU || D * es % 16 != 0) return SPARTON_EINVAL;
+  // 256 rows of an operand lie within 2^31 bytes
+  if (D > (1 << 20) || F > (1 << 20) || M > INT32_MAX) return SPARTON_EUNSUPPORTED;
+  const uint64_t tiles = std::max((uint64_t)cdiv(std::max<int64_t>(M, 1), 128) * cdiv(std::max(F, D), 64),
+                                  (uint64_t)cdiv(F, 128) * cdiv(D, 128) * 2);
+  return tiles * 256 >= kMaxThreads ? SPARTON_EUNSUPPORTED : SPARTON_OK;
+}
+
+template <typename T, typename O> int forward(Params& p, hipStream_t st) {
+  p.turns = 1;
+  if (p.q.n <= kFewRows) {
+    const dim3 grid((unsigned)cdiv(p.p.n, 32)), block(64 * kFewWaves);
+    if (p.q.n <= 32) hipLaunchKernelGGL((gated_few_kernel<T, O, 1>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((gated_few_kernel<T, O, 2>), grid, block, 0, st, p);
+    return (int)hipGetLastError();
+  }
+  const int64_t slabs = cdiv(p.K * (int64_t)sizeof(T), kSlab);
+  p.half_slabs = (int)slabs;
+  return gemm<T, O, false, false, true>(p, split_of(p.q.n, 2 * p.p.n, 1, slabs, false), st);
+}
+
+struct Plan {
+  Split dx, dw;
+  size_t act, part, bias;  // bytes
+  int rows, strips, blocks;
+};
+
+Plan plan_of(int64_t M, int64_t D, int64_t F, int dtype, bool with_bias) {
+  const int64_t es = es_of(dtype), ld = pad_of(F, dtype);
+  Plan p;
+  p.dx = split_of(M, D, 1, 2 * cdiv(F * es, kSlab), true);
+  p.dw = split_of(F, D, 2, cdiv(M * es, kSlab), true);
+  p.act = (size_t)round_up(2 * M * ld * es, 256);
+  p.part = 0;
+  if (p.dx.splits > 1) p.part = (size_t)round_up((int64_t)p.dx.splits * M * D * 4, 256);
+  if (p.dw.splits > 1) p.part = std::max(p.part, (size_t)round_up((int64_t)p.dw.splits * 2 * F * D * 4, 256));
+  p.strips = (int)cdiv(ld, kActThreads * kActCols);
+  const int64_t want = with_bias ? kBiasBlocks : 4096;
+  p.rows = (int)std::max<int64_t>(1, cdiv(M * (with_bias ? 1 : p.strips), want));
+  p.blocks = (int)cdiv(M, p.rows);
+  p.bias = with_bias ? (size_t)round_up((int64_t)p.blocks * 2 * F * 4, 256) : 0;
+  return p;
+}
+
+template <typename T>
+int backward(const T* dh, const char* x, const char* wg, const char* wu, const float* g, const float* u, T* dx, T* dwg, T* dwu,
+             T* dbg, T* dbu, char* ws, int64_t M, int64_t D, int64_t F, int act, int dtype, hipStream_t st) {
+  constexpr int64_t E = sizeof(T);
+  const bool with_bias = dbg != nullptr || dbu != nullptr;
+  const Plan pl = plan_of(M, D, F, dtype, with_bias);
+  const int64_t ld = pad_of(F, dtype);
+  T* dg = (T*)ws;
+  T* du = dg + M * ld;
+  float* part = (float*)(ws + pl.act);
+  float* bias = with_bias ? (float*)(ws + pl.act + pl.part) : nullptr;
+  if (M > 0) {
+    hipLaunchKernelGGL(gated_act_bwd_kernel<T>, dim3((unsigned)(pl.blocks * (int64_t)pl.strips)), dim3(kActThreads), 0, st, dh, g,
+                       u, dg, du, bias, M, F, ld, act, pl.rows, pl.strips);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  if (with_bias) {
+    hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)cdiv(2 * F, 64)), dim3(64 * kSumWaves), 0, st, (const float*)bias,
+                       M > 0 ? pl.blocks : 0, (int)F, (int)(2 * F), dbg, dbu, dtype);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  const auto join = [&](const Split& s, int64_t n, int turns, T* a, T* b) {
+    if (s.splits <= 1) return (int)hipGetLastError();
+    hipLaunchKernelGGL(gated_join_kernel<T>, dim3((unsigned)cdiv(n * turns, 1024)), dim3(256), 0, st, (const float*)part, s.splits,
+                       n, turns, a, b);
+    return (int)hipGetLastError();
+  };
+  if (dx != nullptr && M > 0) {
+    Params p = {};
+    p.q = Side{(const char*)dg, (const char*)du, ld * E, M};
+    p.p = Side{wg, wu, D * E, D};
+    p.K = F;
+    p.half_slabs = (int)cdiv(F * E, kSlab);
+    p.turns = 1;
+    p.out[0] = dx;
+    p.part = part;
+    int rc = gemm<T, T, false, true, false>(p, pl.dx, st);
+    if (rc == 0) rc = join(pl.dx, M * D, 1, dx, nullptr);
+    if (rc != 0) return rc;
+  }
+  if (dwg != nullptr) {
+    Params p = {};
+    p.q = Side{(const char*)dg, (const char*)dg, ld * E, F};
+    p.q_turn = (const char*)du;
+    p.p = Side{x, x, D * E, D};
+    p.K = M;
+    p.half_slabs = (int)cdiv(M * E, kSlab);
+    p.turns = 2;
+    p.out[0] = dwg;
+    p.out[1] = dwu;
+    p.part = part;
+    int rc = gemm<T, T, true, true, false>(p, pl.dw, st);
+    if (rc == 0) rc = join(pl.dw, F * D, 2, dwg, dwu);
+    if (rc != 0) return rc;
+  }
+  return SPARTON_OK;
+}
+
+}  // namespace gated
+}  // namespace sparton
+
+using namespace sparton;
+
+#define SPARTON_EXPORT extern "C" __attribute__((visibility("default")))
+
+SPARTON_EXPORT int sparton_gated_fwd(const void* x, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
+                                     int activation, void* h, float* gate, float* up, int64_t M, int64_t D, int64_t F, int dtype,
+                                     void* stream) {
+  const int rc = gated::check(M, D, F, dtype, dtype == SPARTON_F32 ? 4 : 2, activation);
+  if (rc != SPARTON_OK) return rc;
+  if (M == 0 || F == 0) return SPARTON_OK;
+  if (x == nullptr || w_gate == nullptr || w_up == nullptr || h == nullptr || (gate == nullptr) != (up == nullptr))
+    return SPARTON_EINVAL;
+  const uintptr_t es = (uintptr_t)gated::es_of(dtype);
+  if (!aligned(x, 16) || !aligned(w_gate, 16) || !aligned(w_up, 16) || !aligned(h, es) || !aligned(b_gate, es) ||
+      !aligned(b_up, es) || !aligned(gate, 4) || !aligned(up, 4))
+    return SPARTON_EALIGN;
+  gated::Params p = {};
+  p.q = gated::Side{(const char*)x, (const char*)x, D * (int64_t)es, M};
+  p.p = gated::Side{(const char*)w_gate, (const char*)w_up, D * (int64_t)es, F};
+  p.K = D;
+  p.h = h;
+  p.g = gate;
+  p.u = up;
+  p.bg = b_gate;
+  p.bu = b_up;
+  p.act = activation;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == SPARTON_BF16) return gated::forward<bf16, bf16>(p, st);
+  if (dtype == SPARTON_F16) return gated::forward<f16, f16>(p, st);
+  return gated::forward<float, float>(p, st);
+}
+
+SPARTON_EXPORT int sparton_gated_fwd_quantized(const void* x, const float* x_scale, const void* w_gate, const float* gate_scale,
+                                          const void* w_up, const float* up_scale, int activation, void* h, int64_t M,
+                                          int64_t D, int64_t F, int out_dtype, void* stream) {
+  const int rc = gated::check(M, D, F, out_dtype, 1, activation);
+  if (rc != SPARTON_OK) return rc;
+  if (M == 0 || F == 0) return SPARTON_OK;
+  if (x == nullptr || w_gate == nullptr || w_up == nullptr || h == nullptr || x_scale == nullptr || gate_scale == nullptr ||
+      up_scale == nullptr)
+    return SPARTON_EINVAL;
+  if (!aligned(x, 16) || !aligned(w_gate, 16) || !aligned(w_up, 16) || !aligned(h, (uintptr_t)gated::es_of(out_dtype)) ||
+      !aligned(x_scale, 4) || !aligned(gate_scale, 4) || !aligned(up_scale, 4))
+    return SPARTON_EALIGN;
+  gated::Params p = {};
+  p.q = gated::Side{(const char*)x, (const char*)x, D, M};
+  p.p = gated::Side{(const char*)w_gate, (const char*)w_up, D, F};
+  p.K = D;
+  p.h = h;
+  p.sx = x_scale;
+  p.sg = gate_scale;
+  p.su = up_scale;
+  p.act = activation;
+  hipStream_t st = (hipStream_t)stream;
+  if (out_dtype == SPARTON_BF16) return gated::forward<gated::e4m3, bf16>(p, st);
+  if (out_dtype == SPARTON_F16) return gated::forward<gated::e4m3, f16>(p, st);
+  return gated::forward<gated::e4m3, float>(p, st);
+}
+
+SPARTON_EXPORT size_t sparton_gated_workspace_bytes(int64_t M, int64_t D, int64_t F, int with_bias, int dtype) {
+  if (gated::check(M, D, F, dtype, dtype == SPARTON_F32 ? 4 : 2, SPARTON_SILU) != SPARTON_OK || M == 0 || F == 0) return 0;
+  const gated::Plan p = gated::plan_of(M, D, F, dtype, with_bias != 0);
+  return p.act + p.part + p.bias;
+}
+
+SPARTON_EXPORT int sparton_gated_bwd(const void* dh, const void* x, const void* w_gate, const void* w_up, const float* gate,
+                                     const float* up, int activation, void* dx, void* d_w_gate, void* d_w_up, void* d_b_gate,
+                                     void* d_b_up, void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F,
+                                     int dtype, void* stream) {
+  const int rc = gated::check(M, D, F, dtype, dtype == SPARTON_F32 ? 4 : 2, activation);
+  if (rc != SPARTON_OK) return rc;
+  if ((d_w_gate == nullptr) != (d_w_up == nullptr)) return SPARTON_EINVAL;
+  if (F == 0 && (dx != nullptr || d_w_gate != nullptr)) return SPARTON_EUNSUPPORTED;
+  if (F == 0) return SPARTON_OK;
+  if (M > 0 && (dh == nullptr || x == nullptr || w_gate == nullptr || w_up == nullptr || gate == nullptr || up == nullptr))
+    return SPARTON_EINVAL;
+  const uintptr_t es = (uintptr_t)gated::es_of(dtype);
+  if (!aligned(x, 16) || !aligned(w_gate, 16) || !aligned(w_up, 16) || !aligned(dh, es) || !aligned(dx, es) ||
+      !aligned(d_w_gate, es) || !aligned(d_w_up, es) || !aligned(d_b_gate, es) || !aligned(d_b_up, es) || !aligned(gate, 4) ||
+      !aligned(up, 4))
+    return SPARTON_EALIGN;
+  const bool with_bias = d_b_gate != nullptr || d_b_up != nullptr;
+  const size_t need = sparton_gated_workspace_bytes(M, D, F, with_bias, dtype);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return SPARTON_EWORKSPACE;
+  if (need > 0 && !aligned(workspace, 256)) return SPARTON_EALIGN;
+  hipStream_t st = (hipStream_t)stream;
+  const char *cx = (const char*)x, *cg = (const char*)w_gate, *cu = (const char*)w_up;
+  char* ws = (char*)workspace;
+  if (dtype == SPARTON_BF16)
+    return gated::backward<bf16>((const bf16*)dh, cx, cg, cu, gate, up, (bf16*)dx, (bf16*)d_w_gate, (bf16*)d_w_up, (bf16*)d_b_gate,
+                                 (bf16*)d_b_up, ws, M, D, F, activation, dtype, st);
+  if (dtype == SPARTON_F16)
+    return gated::backward<f16>((const f16*)dh, cx, cg, cu, gate, up, (f16*)dx, (f16*)d_w_gate, (f16*)d_w_up, (f16*)d_b_gate,
+                                (f16*)d_b_up, ws, M, D, F, activation, dtype, st);
+  return gated::backward<float>((const float*)dh, cx, cg, cu, gate, up, (float*)dx, (float*)d_w_gate, (float*)d_w_up,
+                                (float*)d_b_gate, (float*)d_b_up, ws, M, D, F, activation, dtype, st);
+}

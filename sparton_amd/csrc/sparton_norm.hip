@@ -25,6 +25,7 @@
 #include <algorithm>
 
 #include "sparton_common.h"
+#include "sparton_rows.h"
 
 namespace sparton {
 namespace norm {
@@ -32,7 +33,6 @@ namespace norm {
 constexpr int kFwdWaves = 4;    // forward workgroups of 4 waves, or of the 8 waves of one row
 constexpr int kBwdWaves = 8;
 constexpr int kBwdBlocks = 256; // backward: one workgroup per CU, so that few partial sums are written
-constexpr int kSumWaves = 16;
 constexpr int64_t kMaxD = 16384;
 
 struct Params {
@@ -44,67 +44,6 @@ struct Params {
   int D, vec_dtype;
   float eps, inv_d;
 };
-
-// A 16-byte vector (or one element) at any address.
-template <typename T, int VE> struct Vec {
-  typedef __attribute__((ext_vector_type(VE))) T type;
-  typedef type loose __attribute__((aligned(sizeof(T))));
-};
-template <typename T> struct Vec<T, 1> {
-  struct type {
-    T v;
-    __device__ __forceinline__ T operator[](int) const { return v; }
-    __device__ __forceinline__ T& operator[](int) { return v; }
-  };
-  typedef type loose;
-};
-template <typename T, int VE> using vec_t = typename Vec<T, VE>::type;
-template <typename T, int VE> __device__ __forceinline__ vec_t<T, VE> load_any(const T* p) {
-  return *(const typename Vec<T, VE>::loose*)p;
-}
-template <typename T, int VE> __device__ __forceinline__ void store_any(T* p, vec_t<T, VE> v) {
-  *(typename Vec<T, VE>::loose*)p = v;
-}
-
-// Where a lane's vector lies in the row, and which of its elements are its own: from `own` on. Past
-// the row end none are (own = VE), and the loads repeat the row's last vector.
-template <int VE> struct Place {
-  int at, own;
-  __device__ __forceinline__ Place(int want, int D) {
-    at = min(want, D - VE);
-    own = want >= D ? VE : want - at;
-  }
-};
-
-// A lane's elements of weight or bias, in fp32 or in the rows' type.
-template <typename T, int VE> __device__ __forceinline__ void vec_param(float* out, const void* p, int dt, int at) {
-  if (dt == SPARTON_F32) {  // uniform
-    constexpr int N = VE < 4 ? VE : 4;
-#pragma unroll
-    for (int i = 0; i < VE; i += N) {
-      const vec_t<float, N> v = load_any<float, N>((const float*)p + at + i);
-#pragma unroll
-      for (int e = 0; e < N; ++e) out[i + e] = v[e];
-    }
-  } else {
-    const vec_t<T, VE> v = load_any<T, VE>((const T*)p + at);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) out[e] = to_f32(v[e]);
-  }
-}
-
-// Sum over the WPR waves of a row, in wave order; result in every lane. `slot` is the row group's
-// [WPR] floats of LDS; consecutive sums alternate between two of them, so one barrier each will do.
-template <int WPR> __device__ __forceinline__ float row_sum(float x, float* slot, int wave_in_row) {
-  x = wave_sum(x);
-  if constexpr (WPR == 1) return x;
-  if ((threadIdx.x & 63) == 0) slot[wave_in_row] = x;
-  __syncthreads();
-  float s = 0.0f;
-#pragma unroll
-  for (int w = 0; w < WPR; ++w) s += slot[w];
-  return s;
-}
 
 // ---- forward ------------------------------------------------------------------------------
 template <typename T, int VE, int NP, int WPR>
@@ -299,37 +238,6 @@ __global__ __launch_bounds__(64 * kBwdWaves) void norm_bwd_kernel(Params p) {
     }
 }
 
-// part[blocks][2][D] summed in block order: 64 columns a workgroup, one per lane; wave w adds blocks
-// [w seg, (w + 1) seg), and wave 0 the waves' sums in wave order. 1.5 MB in 3.8 us at D = 768, most of it
-// the launch.
-__global__ __launch_bounds__(64 * kSumWaves) void norm_colsum_kernel(const float* __restrict__ part, int blocks, int D,
-                                                                     void* dgamma, void* dbeta, int vec_dtype) {
-  __shared__ float wsum[kSumWaves][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int col = blockIdx.x * 64 + lane, ncol = 2 * D;
-  const int seg = (blocks + kSumWaves - 1) / kSumWaves;
-  float a = 0.0f;
-  if (col < ncol) {
-    const int b1 = min(blocks, (wave + 1) * seg);
-#pragma unroll 8
-    for (int b = wave * seg; b < b1; ++b) a += part[(int64_t)b * ncol + col];
-  }
-  wsum[wave][lane] = a;
-  __syncthreads();
-  if (wave > 0 || col >= ncol) return;
-  a = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kSumWaves; ++w) a += wsum[w][lane];
-  void* to = col < D ? dgamma : dbeta;
-  if (to == nullptr) return;
-  const int c = col < D ? col : col - D;
-  switch (vec_dtype) {
-    case SPARTON_BF16: ((bf16*)to)[c] = from_f32<bf16>(a); break;
-    case SPARTON_F16: ((f16*)to)[c] = from_f32<f16>(a); break;
-    default: ((float*)to)[c] = a;
-  }
-}
-
 // ---- launches -----------------------------------------------------------------------------
 int waves_per_row(int64_t D) { return D <= 1024 ? 1 : D <= 2048 ? 4 : 8; }
 
@@ -368,8 +276,6 @@ void run(const Params& p, int dtype, bool bwd, hipStream_t st) {
   else launch_t<float>(p, bwd, st);
 }
 
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
 int check(int64_t M, int64_t D, int dtype, int vec_dtype) {
   if (M < 0 || D <= 0 || dtype < SPARTON_F32 || dtype > SPARTON_F16) return SPARTON_EINVAL;
   if (vec_dtype != SPARTON_F32 && vec_dtype != dtype) return SPARTON_EINVAL;
@@ -392,8 +298,8 @@ SPARTON_EXPORT int sparton_layer_norm_fwd(const void* x, const void* residual, c
   if (M == 0) return SPARTON_OK;
   if (x == nullptr || weight == nullptr || y == nullptr || (mean == nullptr) != (rstd == nullptr)) return SPARTON_EINVAL;
   const uintptr_t es = dtype == SPARTON_F32 ? 4 : 2, vs = vec_dtype == SPARTON_F32 ? 4 : 2;
-  if (!norm::aligned(x, es) || !norm::aligned(residual, es) || !norm::aligned(y, es) || !norm::aligned(weight, vs) ||
-      !norm::aligned(bias, vs) || !norm::aligned(mean, 4) || !norm::aligned(rstd, 4))
+  if (!aligned(x, es) || !aligned(residual, es) || !aligned(y, es) || !aligned(weight, vs) ||
+      !aligned(bias, vs) || !aligned(mean, 4) || !aligned(rstd, 4))
     return SPARTON_EALIGN;
   norm::Params p = {};
   p.x = x;
@@ -426,16 +332,16 @@ SPARTON_EXPORT int sparton_layer_norm_bwd(const void* dy, const void* x, const v
   if (M > 0 && (dy == nullptr || x == nullptr || weight == nullptr || mean == nullptr || rstd == nullptr || dx == nullptr))
     return SPARTON_EINVAL;
   const uintptr_t es = dtype == SPARTON_F32 ? 4 : 2, vs = vec_dtype == SPARTON_F32 ? 4 : 2;
-  if (!norm::aligned(dy, es) || !norm::aligned(x, es) || !norm::aligned(residual, es) || !norm::aligned(dx, es) ||
-      !norm::aligned(weight, vs) || !norm::aligned(d_weight, vs) || !norm::aligned(d_bias, vs) ||
-      !norm::aligned(mean, 4) || !norm::aligned(rstd, 4))
+  if (!aligned(dy, es) || !aligned(x, es) || !aligned(residual, es) || !aligned(dx, es) ||
+      !aligned(weight, vs) || !aligned(d_weight, vs) || !aligned(d_bias, vs) ||
+      !aligned(mean, 4) || !aligned(rstd, 4))
     return SPARTON_EALIGN;
   hipStream_t st = (hipStream_t)stream;
   int blocks = 0;
   if (M > 0) {
     const size_t need = sparton_layer_norm_workspace_bytes(M, D);
     if (workspace == nullptr || workspace_bytes < need) return SPARTON_EWORKSPACE;
-    if (!norm::aligned(workspace, 256)) return SPARTON_EALIGN;
+    if (!aligned(workspace, 256)) return SPARTON_EALIGN;
     norm::Params p = {};
     p.dy = dy;
     p.x = x;
@@ -455,7 +361,7 @@ SPARTON_EXPORT int sparton_layer_norm_bwd(const void* dy, const void* x, const v
     if (e != hipSuccess) return (int)e;
   }
   if (d_weight == nullptr && d_bias == nullptr) return SPARTON_OK;
-  hipLaunchKernelGGL(norm::norm_colsum_kernel, dim3((unsigned)cdiv(2 * D, 64)), dim3(64 * norm::kSumWaves), 0, st,
-                     (const float*)workspace, blocks, (int)D, d_weight, d_bias, vec_dtype);
+  hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)cdiv(2 * D, 64)), dim3(64 * kSumWaves), 0, st,
+                     (const float*)workspace, blocks, (int)D, 2 * (int)D, d_weight, d_bias, vec_dtype);
   return (int)hipGetLastError();
 }

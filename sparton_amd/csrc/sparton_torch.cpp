@@ -951,6 +951,308 @@ std::tuple<Tensor, Tensor> preference_cuda(const Tensor& q, const Tensor& p, con
   return {loss, margin};
 }
 
+// Whether a graph is to be kept: the dispatcher calls the autograd kernels without one too.
+template <typename... T> bool wants_grad(const T&... t) {
+  return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
+}
+
+// ---- the RMS norm --------------------------------------------------------------------------
+
+struct RmsOut {
+  Tensor y, h, rstd;
+};
+
+RmsOut rms_run(const Tensor& x, const Tensor& r, const Tensor& w, double eps, bool with_stats) {
+  const int64_t D = x.size(-1), M = D == 0 ? 0 : x.numel() / D;
+  RmsOut o;
+  o.y = at::empty(x.sizes(), x.options());
+  if (r.defined()) o.h = at::empty(x.sizes(), x.options());
+  if (with_stats) o.rstd = at::empty({M}, x.options().dtype(at::kFloat));
+  check(sparton_rms_norm_fwd(x.data_ptr(), ptr(r), w.data_ptr(), dtype_code(w.scalar_type()), (float)eps, o.y.data_ptr(),
+                             mptr(o.h), with_stats ? o.rstd.data_ptr<float>() : nullptr, M, D, dtype_code(x.scalar_type()),
+                             stream_of(x)),
+        "sparton_rms_norm_fwd");
+  return o;
+}
+
+std::tuple<Tensor, Tensor> rms_grads(const Tensor& dy_in, const Tensor& dh_in, const Tensor& h, const Tensor& w,
+                                     const Tensor& rstd, bool with_dw) {
+  const int64_t D = h.size(-1), M = rstd.size(0);
+  Tensor dy = dy_in.to(h.scalar_type()).contiguous();
+  Tensor dh = dh_in.defined() ? dh_in.to(h.scalar_type()).contiguous() : Tensor();
+  Tensor dx = at::empty(h.sizes(), h.options());
+  Tensor dw = with_dw ? at::empty({D}, w.options()) : Tensor();
+  const size_t ws_bytes = sparton_rms_norm_workspace_bytes(M, D);
+  Tensor ws = workspace(ws_bytes, h);
+  check(sparton_rms_norm_bwd(dy.data_ptr(), ptr(dh), h.data_ptr(), w.data_ptr(), dtype_code(w.scalar_type()),
+                             rstd.data_ptr<float>(), dx.data_ptr(), mptr(dw), ws.data_ptr(), ws_bytes, M, D,
+                             dtype_code(h.scalar_type()), stream_of(h)),
+        "sparton_rms_norm_bwd");
+  return {dx, dw};
+}
+
+std::tuple<Tensor, Tensor, Tensor> rms_fwd_cuda(const Tensor& x, const c10::optional<Tensor>& r, const Tensor& w, double eps) {
+  c10::OptionalDeviceGuard guard(x.device());
+  RmsOut o = rms_run(x.contiguous(), whole(r), w.contiguous(), eps, true);
+  return {o.y, o.h.defined() ? o.h : at::empty({0}, x.options()), o.rstd};
+}
+std::tuple<Tensor, Tensor> rms_bwd_cuda(const Tensor& dy, const c10::optional<Tensor>& dh, const Tensor& h, const Tensor& w,
+                                        const Tensor& rstd) {
+  c10::OptionalDeviceGuard guard(h.device());
+  return rms_grads(dy, whole(dh), h.contiguous(), w.contiguous(), rstd, true);
+}
+
+struct RmsFn : public torch::autograd::Function<RmsFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& r_in, const Tensor& w_in, bool has_r,
+                               double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::OptionalDeviceGuard guard(x_in.device());
+    Tensor x = x_in.contiguous(), w = w_in.contiguous();
+    RmsOut o = rms_run(x, has_r ? r_in.contiguous() : Tensor(), w, eps, true);
+    ctx->save_for_backward({has_r ? o.h : x, w, o.rstd});
+    ctx->saved_data["has_r"] = has_r;
+    ctx->set_materialize_grads(false);
+    return has_r ? variable_list{o.y, o.h} : variable_list{o.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool has_r = ctx->saved_data["has_r"].toBool();
+    const Tensor dh = has_r ? grads[1] : Tensor();
+    if (!grads[0].defined()) return once({dh, dh, Tensor(), Tensor(), Tensor()});
+    auto s = ctx->get_saved_variables();
+    c10::OptionalDeviceGuard guard(s[0].device());
+    auto [dx, dw] = rms_grads(grads[0], dh, s[0], s[1], s[2], ctx->needs_input_grad(2));
+    return once({dx, has_r ? dx : Tensor(), dw, Tensor(), Tensor()});
+  }
+};
+
+Tensor rms_cuda(const Tensor& x, const Tensor& w, double eps) {
+  c10::OptionalDeviceGuard guard(x.device());
+  return rms_run(x.contiguous(), Tensor(), w.contiguous(), eps, false).y;
+}
+std::tuple<Tensor, Tensor> rms_add_cuda(const Tensor& x, const Tensor& r, const Tensor& w, double eps) {
+  c10::OptionalDeviceGuard guard(x.device());
+  RmsOut o = rms_run(x.contiguous(), r.contiguous(), w.contiguous(), eps, false);
+  return {o.y, o.h};
+}
+Tensor rms_autograd(const Tensor& x, const Tensor& w, double eps) {
+  if (wants_grad(x, w)) return RmsFn::apply(x, x, w, false, eps)[0];
+  at::AutoDispatchBelowADInplaceOrView below;
+  return rms_cuda(x, w, eps);
+}
+std::tuple<Tensor, Tensor> rms_add_autograd(const Tensor& x, const Tensor& r, const Tensor& w, double eps) {
+  if (wants_grad(x, r, w)) {
+    auto o = RmsFn::apply(x, r, w, true, eps);
+    return {o[0], o[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return rms_add_cuda(x, r, w, eps);
+}
+std::tuple<Tensor, Tensor, Tensor> rms_8bit_cuda(const Tensor& x_in, const c10::optional<Tensor>& r_in, const Tensor& w_in,
+                                                 double eps) {
+  c10::OptionalDeviceGuard guard(x_in.device());
+  Tensor x = x_in.contiguous(), r = whole(r_in), w = w_in.contiguous();
+  const int64_t D = x.size(-1), M = D == 0 ? 0 : x.numel() / D;
+  Tensor y = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  Tensor h = r.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  check(sparton_rms_norm_fwd_quantized(x.data_ptr(), ptr(r), w.data_ptr(), dtype_code(w.scalar_type()), (float)eps, y.data_ptr(),
+                                  scale.data_ptr<float>(), r.defined() ? h.data_ptr() : nullptr, M, D,
+                                  dtype_code(x.scalar_type()), stream_of(x)),
+        "sparton_rms_norm_fwd_quantized");
+  return {y, scale, h};
+}
+
+// ---- the embedding -------------------------------------------------------------------------
+
+Tensor embedding_run(const Tensor& ids, const Tensor& w, double scale) {
+  auto shape = ids.sizes().vec();
+  shape.push_back(w.size(1));
+  Tensor out = at::empty(shape, w.options());
+  check(sparton_embedding_fwd(ids.data_ptr(), mask_code(ids.scalar_type()), w.data_ptr(), (float)scale, out.data_ptr(),
+                              ids.numel(), w.size(0), w.size(1), dtype_code(w.scalar_type()), stream_of(w)),
+        "sparton_embedding_fwd");
+  return out;
+}
+
+Tensor embedding_grad(const Tensor& d_out, const Tensor& ids, int64_t rows, double scale, int64_t padding) {
+  Tensor g = d_out.contiguous();
+  const int64_t N = ids.numel(), D = g.size(-1);
+  Tensor dw = at::empty({rows, D}, g.options());
+  const int dt = dtype_code(g.scalar_type());
+  const size_t ws_bytes = sparton_embedding_workspace_bytes(N, rows, D, dt);
+  Tensor ws = workspace(ws_bytes, g);
+  check(sparton_embedding_bwd(ids.data_ptr(), mask_code(ids.scalar_type()), g.data_ptr(), (float)scale, padding, dw.data_ptr(),
+                              ws.data_ptr(), ws_bytes, N, rows, D, dt, stream_of(g)),
+        "sparton_embedding_bwd");
+  return dw;
+}
+
+Tensor embedding_cuda(const Tensor& ids, const Tensor& w, double scale, int64_t) {
+  c10::OptionalDeviceGuard guard(w.device());
+  return embedding_run(ids.contiguous(), w.contiguous(), scale);
+}
+Tensor embedding_bwd_cuda(const Tensor& d_out, const Tensor& ids, int64_t rows, double scale, int64_t padding) {
+  c10::OptionalDeviceGuard guard(d_out.device());
+  return embedding_grad(d_out, ids.contiguous(), rows, scale, padding);
+}
+
+struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& ids_in, const Tensor& w, double scale, int64_t padding) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::OptionalDeviceGuard guard(w.device());
+    Tensor ids = ids_in.contiguous();
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = w.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["dtype"] = (int64_t)w.scalar_type();
+    return embedding_run(ids, w.contiguous(), scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return variable_list(4);
+    auto s = ctx->get_saved_variables();
+    c10::OptionalDeviceGuard guard(s[0].device());
+    Tensor g = grads[0].to((at::ScalarType)ctx->saved_data["dtype"].toInt());
+    return once({Tensor(), embedding_grad(g, s[0], ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(),
+                                          ctx->saved_data["padding"].toInt()),
+                 Tensor(), Tensor()});
+  }
+};
+
+Tensor embedding_autograd(const Tensor& ids, const Tensor& w, double scale, int64_t padding) {
+  if (wants_grad(w)) return EmbeddingFn::apply(ids, w, scale, padding);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return embedding_cuda(ids, w, scale, padding);
+}
+
+// ---- the gated feed-forward product --------------------------------------------------------
+
+// Rows of whole 16 bytes, as the C ABI reads them: a width that is not is padded with zero columns, which change
+// no product.
+Tensor gated_rows(const Tensor& t) {
+  const int64_t unit = 16 / t.element_size(), pad = (unit - t.size(-1) % unit) % unit;
+  return pad > 0 ? at::constant_pad_nd(t.element_size() == 1 ? t.view(at::kByte) : t, {0, pad}).contiguous() : dense(t);
+}
+
+struct GatedOut {
+  Tensor h, g, u;
+};
+
+// x [..., D] and the weights [F, D] as gated_rows gives them.
+GatedOut gated_run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& bg, const Tensor& bu, int64_t act,
+                   bool with_saved) {
+  const int64_t D = x.size(-1), F = wg.size(0), M = x.numel() / D;
+  auto shape = x.sizes().vec();
+  shape.back() = F;
+  GatedOut o;
+  o.h = at::empty(shape, x.options());
+  if (with_saved) {
+    o.g = at::empty({M, F}, x.options().dtype(at::kFloat));
+    o.u = at::empty_like(o.g);
+  }
+  check(sparton_gated_fwd(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), ptr(bg), ptr(bu), (int)act, o.h.data_ptr(),
+                          with_saved ? o.g.data_ptr<float>() : nullptr, with_saved ? o.u.data_ptr<float>() : nullptr, M, D, F,
+                          dtype_code(x.scalar_type()), stream_of(x)),
+        "sparton_gated_fwd");
+  return o;
+}
+
+// (dx, dw_gate, dw_up, db_gate, db_up) of width D; what is not asked for stays undefined.
+variable_list gated_grads(const Tensor& dh_in, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& g,
+                          const Tensor& u, int64_t act, int64_t D, bool need_x, bool need_w, bool need_bg, bool need_bu) {
+  const int64_t P = x.size(-1), F = wg.size(0), M = g.size(0);
+  Tensor dh = dh_in.to(x.scalar_type()).contiguous();
+  variable_list d(5);
+  if (need_x) d[0] = at::empty(x.sizes(), x.options());
+  if (need_w) d[1] = at::empty(wg.sizes(), x.options()), d[2] = at::empty_like(d[1]);
+  if (need_bg) d[3] = at::empty({F}, x.options());
+  if (need_bu) d[4] = at::empty({F}, x.options());
+  const int dt = dtype_code(x.scalar_type());
+  if (F == 0) {
+    for (Tensor& t : d)
+      if (t.defined()) t.zero_();
+  } else {
+    const size_t ws_bytes = sparton_gated_workspace_bytes(M, P, F, need_bg || need_bu, dt);
+    Tensor ws = workspace(ws_bytes, x);
+    check(sparton_gated_bwd(dh.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), g.data_ptr<float>(), u.data_ptr<float>(),
+                            (int)act, mptr(d[0]), mptr(d[1]), mptr(d[2]), mptr(d[3]), mptr(d[4]), ws.data_ptr(), ws_bytes, M, P, F,
+                            dt, stream_of(x)),
+          "sparton_gated_bwd");
+  }
+  for (int i = 0; i < 3; ++i)
+    if (d[i].defined() && P != D) d[i] = d[i].narrow(-1, 0, D).contiguous();
+  return d;
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_fwd_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu,
+                                                  const c10::optional<Tensor>& bg, const c10::optional<Tensor>& bu, int64_t act) {
+  c10::OptionalDeviceGuard guard(x.device());
+  GatedOut o = gated_run(gated_rows(x), gated_rows(wg), gated_rows(wu), whole(bg), whole(bu), act, true);
+  return {o.h, o.g, o.u};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_bwd_cuda(const Tensor& dh, const Tensor& x, const Tensor& wg,
+                                                                  const Tensor& wu, const Tensor& g, const Tensor& u,
+                                                                  int64_t act, bool has_bg, bool has_bu) {
+  c10::OptionalDeviceGuard guard(x.device());
+  auto d = gated_grads(dh, gated_rows(x), gated_rows(wg), gated_rows(wu), g, u, act, x.size(-1), true, true, has_bg, has_bu);
+  for (int i = 3; i < 5; ++i)
+    if (!d[i].defined()) d[i] = at::empty({0}, x.options());
+  return {d[0], d[1], d[2], d[3], d[4]};
+}
+
+struct GatedFn : public torch::autograd::Function<GatedFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& wg_in, const Tensor& wu_in, const Tensor& bg,
+                        const Tensor& bu, bool has_bg, bool has_bu, int64_t act) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::OptionalDeviceGuard guard(x_in.device());
+    Tensor x = gated_rows(x_in), wg = gated_rows(wg_in), wu = gated_rows(wu_in);
+    GatedOut o = gated_run(x, wg, wu, has_bg ? bg.contiguous() : Tensor(), has_bu ? bu.contiguous() : Tensor(), act, true);
+    ctx->save_for_backward({x, wg, wu, o.g, o.u});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["D"] = x_in.size(-1);
+    ctx->saved_data["has_bg"] = has_bg;
+    ctx->saved_data["has_bu"] = has_bu;
+    return o.h;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return variable_list(8);
+    auto s = ctx->get_saved_variables();
+    c10::OptionalDeviceGuard guard(s[0].device());
+    const auto need = [&](size_t i) { return ctx->needs_input_grad(i); };
+    auto d = gated_grads(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["act"].toInt(), ctx->saved_data["D"].toInt(),
+                         need(0), need(1) || need(2), ctx->saved_data["has_bg"].toBool() && need(3),
+                         ctx->saved_data["has_bu"].toBool() && need(4));
+    return once({d[0], d[1], d[2], d[3], d[4], Tensor(), Tensor(), Tensor()});
+  }
+};
+
+Tensor gated_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu, const c10::optional<Tensor>& bg,
+                  const c10::optional<Tensor>& bu, int64_t act) {
+  c10::OptionalDeviceGuard guard(x.device());
+  return gated_run(gated_rows(x), gated_rows(wg), gated_rows(wu), whole(bg), whole(bu), act, false).h;
+}
+Tensor gated_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu, const c10::optional<Tensor>& bg,
+                      const c10::optional<Tensor>& bu, int64_t act) {
+  if (wants_grad(x, wg, wu, bg.value_or(Tensor()), bu.value_or(Tensor())))
+    return GatedFn::apply(x, wg, wu, bg.has_value() ? *bg : x, bu.has_value() ? *bu : x, bg.has_value(), bu.has_value(), act);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return gated_cuda(x, wg, wu, bg, bu, act);
+}
+Tensor gated_8bit_cuda(const Tensor& x_in, const Tensor& sx, const Tensor& wg_in, const Tensor& sg, const Tensor& wu_in,
+                       const Tensor& su, int64_t act, at::ScalarType out_dtype) {
+  c10::OptionalDeviceGuard guard(x_in.device());
+  Tensor x = gated_rows(x_in), wg = gated_rows(wg_in), wu = gated_rows(wu_in);
+  const int64_t D = x.size(-1), F = wg.size(0), M = x.numel() / D;
+  auto shape = x.sizes().vec();
+  shape.back() = F;
+  Tensor h = at::empty(shape, x.options().dtype(out_dtype));
+  Tensor a = sx.contiguous(), b = sg.contiguous(), c = su.contiguous();
+  check(sparton_gated_fwd_quantized(x.data_ptr(), a.data_ptr<float>(), wg.data_ptr(), b.data_ptr<float>(), wu.data_ptr(),
+                               c.data_ptr<float>(), (int)act, h.data_ptr(), M, D, F, dtype_code(out_dtype), stream_of(x)),
+        "sparton_gated_fwd_quantized");
+  return h;
+}
+
 // CPU tensors: the same refusal as the reference's `assert hidden.is_cuda`
 // (sparton_kernel.py:650), as a RuntimeError.
 [[noreturn]] void cpu_refused(const char* op) {
@@ -985,6 +1287,20 @@ TORCH_LIBRARY(sparton_eager, m) {
         "float smoothing) -> (Tensor, Tensor, Tensor)");
   m.def("preference_bwd(Tensor grad, Tensor q, Tensor pos, Tensor neg, Tensor coef) -> (Tensor, Tensor, Tensor)");
   m.def("preference_margin(Tensor q, Tensor pos, Tensor neg, float temperature) -> Tensor");
+  m.def("rms_norm(Tensor x, Tensor weight, float eps) -> Tensor");
+  m.def("rms_norm_add(Tensor x, Tensor residual, Tensor weight, float eps) -> (Tensor, Tensor)");
+  m.def("rms_norm_fwd(Tensor x, Tensor? residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("rms_norm_bwd(Tensor dy, Tensor? dh, Tensor h, Tensor weight, Tensor rstd) -> (Tensor, Tensor)");
+  m.def("rms_norm_8bit(Tensor x, Tensor? residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("embedding(Tensor ids, Tensor weight, float scale, int padding) -> Tensor");
+  m.def("embedding_bwd(Tensor d_out, Tensor ids, int rows, float scale, int padding) -> Tensor");
+  m.def("gated(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int activation) -> Tensor");
+  m.def("gated_fwd(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int activation) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("gated_bwd(Tensor dh, Tensor x, Tensor w_gate, Tensor w_up, Tensor gate, Tensor up, int activation, "
+        "bool has_b_gate, bool has_b_up) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("gated_8bit(Tensor x, Tensor x_scale, Tensor w_gate, Tensor gate_scale, Tensor w_up, Tensor up_scale, "
+        "int activation, ScalarType out_dtype) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(sparton_eager, CUDA, m) {
@@ -1004,6 +1320,17 @@ TORCH_LIBRARY_IMPL(sparton_eager, CUDA, m) {
   m.impl("preference_fwd", &preference_fwd_cuda);
   m.impl("preference_bwd", &preference_bwd_cuda);
   m.impl("preference_margin", &preference_margin_cuda);
+  m.impl("rms_norm", &rms_cuda);
+  m.impl("rms_norm_add", &rms_add_cuda);
+  m.impl("rms_norm_fwd", &rms_fwd_cuda);
+  m.impl("rms_norm_bwd", &rms_bwd_cuda);
+  m.impl("rms_norm_8bit", &rms_8bit_cuda);
+  m.impl("embedding", &embedding_cuda);
+  m.impl("embedding_bwd", &embedding_bwd_cuda);
+  m.impl("gated", &gated_cuda);
+  m.impl("gated_fwd", &gated_fwd_cuda);
+  m.impl("gated_bwd", &gated_bwd_cuda);
+  m.impl("gated_8bit", &gated_8bit_cuda);
 }
 
 TORCH_LIBRARY_IMPL(sparton_eager, AutogradCUDA, m) {
@@ -1015,6 +1342,10 @@ TORCH_LIBRARY_IMPL(sparton_eager, AutogradCUDA, m) {
   m.impl("attention", &attention_autograd);
   m.impl("layer_norm", &norm_autograd);
   m.impl("preference_loss", &preference_autograd);
+  m.impl("rms_norm", &rms_autograd);
+  m.impl("rms_norm_add", &rms_add_autograd);
+  m.impl("embedding", &embedding_autograd);
+  m.impl("gated", &gated_autograd);
 }
 
 TORCH_LIBRARY_IMPL(sparton_eager, CPU, m) {

@@ -1,0 +1,231 @@
+"""Gated feed-forward product of a backbone layer, forward and backward, on hand-written HIP kernels.
+
+    g = x Wg' + bg;   u = x Wu' + bu;   h = act(g) u
+
+the first half of a gated block, whose second is a plain product. (The reference's backbones run
+torch's, training/model.py:88-139.) Both projections, the activation and the product are one kernel:
+g and u meet in registers. The backward has one product for x and one for both weights, and keeps g and u
+in fp32 in between. A few rows (new tokens) take a kernel that streams the weights once; rows and weights
+in e4m3 with a scale a row take the matrix cores' 8-bit rate.
+
+    sparton::gated_fwd(x, w_gate, w_up, b_gate?, b_up?, activation) -> (h, gate, up)
+    sparton::gated_bwd(dh, x, w_gate, w_up, gate, up, activation, has_b_gate, has_b_up)
+        -> (dx, d_w_gate, d_w_up, d_b_gate, d_b_up)
+    sparton::gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation, out_dtype) -> h
+
+Device tensors only, like the head.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+import torch.nn.functional as F
+from torch import Tensor, nn
+
+from . import _eager, _lib
+
+ACTIVATIONS = tuple(_lib.ACTIVATION_CODE)
+MAX_WIDTH = 1 << 20
+E4M3_MAX = 448.0
+_FLOAT_DTYPES = tuple(_lib.DTYPE_CODE)
+_E4M3 = torch.float8_e4m3fn
+
+
+def _code(activation: str, op: str) -> int:
+    if activation not in _lib.ACTIVATION_CODE:
+        raise ValueError(f"{op}: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    return _lib.ACTIVATION_CODE[activation]
+
+
+def _check_shapes(x: Tensor, w_gate: Tensor, w_up: Tensor, op: str) -> Tuple[int, int]:
+    D = x.shape[-1] if x.dim() > 0 else 0
+    if not 1 <= D <= MAX_WIDTH:
+        raise ValueError(f"{op}: x must be [..., D] with D between 1 and {MAX_WIDTH}, got {tuple(x.shape)}")
+    for w in (w_gate, w_up):
+        if w.dim() != 2 or w.shape[1] != D or w.shape != w_gate.shape or w.shape[0] > MAX_WIDTH:
+            raise ValueError(f"{op}: w_gate and w_up must both be [F, {D}] with F up to {MAX_WIDTH}, got "
+                             f"{tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    if x.numel() // D >= 2 ** 31:
+        raise ValueError(f"{op}: {x.numel() // D} rows are too many")
+    return D, w_gate.shape[0]
+
+
+def _require_device(x: Tensor, others, op: str) -> None:
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{op}: all tensors must be on {x.device}, got {t.device}")
+    if not x.is_cuda:
+        raise RuntimeError(f"{op} only supports ROCm/HIP device tensors (got device {x.device})")
+
+
+def _check(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tensor], b_up: Optional[Tensor], op: str) -> None:
+    _D, width = _check_shapes(x, w_gate, w_up, op)
+    for t in (w_gate, w_up, b_gate, b_up):
+        if t is not None and (x.dtype not in _FLOAT_DTYPES or t.dtype != x.dtype):
+            raise TypeError(f"{op}: x, weights and biases must share one float dtype, got {x.dtype} and {t.dtype}")
+    for b in (b_gate, b_up):
+        if b is not None and tuple(b.shape) != (width,):
+            raise ValueError(f"{op}: biases must be [{width}], got {tuple(b.shape)}")
+    _require_device(x, (w_gate, w_up, b_gate, b_up), op)
+
+
+@torch.library.custom_op("sparton::gated_fwd", mutates_args=())
+def gated_fwd(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tensor], b_up: Optional[Tensor],
+              activation: str) -> Tuple[Tensor, Tensor, Tensor]:
+    """(h in x's dtype; g and u, fp32 [rows, F], for the backward)."""
+    op = "sparton::gated_fwd"
+    code = _code(activation, op)
+    _check(x, w_gate, w_up, b_gate, b_up, op)
+    return _eager.load().gated_fwd(x, w_gate, w_up, b_gate, b_up, code)
+
+
+@gated_fwd.register_fake
+def _(x, w_gate, w_up, b_gate, b_up, activation):
+    width = w_gate.shape[0]
+    saved = x.new_empty((x.numel() // x.shape[-1], width), dtype=torch.float32)
+    return x.new_empty((*x.shape[:-1], width)), saved, torch.empty_like(saved)
+
+
+@torch.library.custom_op("sparton::gated_bwd", mutates_args=())
+def gated_bwd(dh: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, gate: Tensor, up: Tensor, activation: str,
+              has_b_gate: bool, has_b_up: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(dx, d_w_gate, d_w_up, d_b_gate, d_b_up) in x's dtype; the biases' are empty where there are none."""
+    op = "sparton::gated_bwd"
+    code = _code(activation, op)
+    _check(x, w_gate, w_up, None, None, op)
+    D, width = x.shape[-1], w_gate.shape[0]
+    if tuple(dh.shape) != (*x.shape[:-1], width):
+        raise ValueError(f"{op}: dh must be {(*x.shape[:-1], width)}, got {tuple(dh.shape)}")
+    for t in (gate, up):
+        if tuple(t.shape) != (x.numel() // D, width) or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{op}: gate and up must be contiguous float32 [{x.numel() // D}, {width}]")
+    _require_device(x, (dh, gate, up), op)
+    return _eager.load().gated_bwd(dh, x, w_gate, w_up, gate, up, code, has_b_gate, has_b_up)
+
+
+@gated_bwd.register_fake
+def _(dh, x, w_gate, w_up, gate, up, activation, has_b_gate, has_b_up):
+    width = w_gate.shape[0]
+    return (x.new_empty(x.shape), w_gate.new_empty(w_gate.shape), w_up.new_empty(w_up.shape),
+            x.new_empty((width if has_b_gate else 0,)), x.new_empty((width if has_b_up else 0,)))
+
+
+def _setup_context(ctx, inputs, output):
+    x, w_gate, w_up, b_gate, b_up, activation = inputs
+    _h, gate, up = output
+    ctx.mark_non_differentiable(gate, up)  # kept for the backward only
+    ctx.set_materialize_grads(False)
+    ctx.activation, ctx.has_b_gate, ctx.has_b_up = activation, b_gate is not None, b_up is not None
+    ctx.save_for_backward(x, w_gate, w_up, gate, up)
+
+
+def _backward(ctx, dh, _d_gate, _d_up):
+    if dh is None:  # h did not reach the loss
+        return (None,) * 6
+    dx, dwg, dwu, dbg, dbu = torch.ops.sparton.gated_bwd(dh, *ctx.saved_tensors, ctx.activation, ctx.has_b_gate,
+                                                         ctx.has_b_up)
+    return dx, dwg, dwu, dbg if ctx.has_b_gate else None, dbu if ctx.has_b_up else None, None
+
+
+gated_fwd.register_autograd(_backward, setup_context=_setup_context)
+
+
+def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tensor] = None, b_up: Optional[Tensor] = None,
+                 activation: str = "silu") -> Tensor:
+    """act(x w_gate' + b_gate) * (x w_up' + b_up): [..., F] from x [..., D] and weights [F, D] (as nn.Linear has
+    them), one float dtype. activation: "silu", "gelu" (erf), "gelu_tanh" or "relu". A width that is not a multiple
+    of 16 bytes costs padded copies of x and the weights. Under autocast the inputs are cast to its dtype, as
+    torch's linear does."""
+    code = _code(activation, "gated_linear")
+    dev = x.device.type
+    if dev in ("cuda", "cpu") and torch.is_autocast_enabled(dev):
+        dt = torch.get_autocast_dtype(dev)
+        x, w_gate, w_up = x.to(dt), w_gate.to(dt), w_up.to(dt)
+        b_gate, b_up = (b.to(dt) if b is not None else None for b in (b_gate, b_up))
+    if torch.compiler.is_compiling() or not x.is_cuda:  # the registered op: fake + autograd
+        _check_shapes(x, w_gate, w_up, "gated_linear")
+        return torch.ops.sparton.gated_fwd(x, w_gate, w_up, b_gate, b_up, activation)[0]
+    _check(x, w_gate, w_up, b_gate, b_up, "gated_linear")
+    return _eager.load().gated(x, w_gate, w_up, b_gate, b_up, code)
+
+
+@torch.library.custom_op("sparton::gated_8bit", mutates_args=())
+def gated_8bit(x: Tensor, x_scale: Tensor, w_gate: Tensor, gate_scale: Tensor, w_up: Tensor, up_scale: Tensor,
+               activation: str, out_dtype: torch.dtype) -> Tensor:
+    """gated_linear_8bit, without a gradient."""
+    op = "sparton::gated_8bit"
+    code = _code(activation, op)
+    _D, width = _check_shapes(x, w_gate, w_up, op)
+    for t in (x, w_gate, w_up):
+        if t.dtype != _E4M3:
+            raise TypeError(f"{op}: x and weights must be float8_e4m3fn, got {t.dtype}")
+    if out_dtype not in _FLOAT_DTYPES:
+        raise TypeError(f"{op}: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    for t, shape in ((x_scale, tuple(x.shape[:-1])), (gate_scale, (width,)), (up_scale, (width,))):
+        if tuple(t.shape) != shape or t.dtype != torch.float32:
+            raise ValueError(f"{op}: a scale a row is float32 {shape}, got {t.dtype} {tuple(t.shape)}")
+    _require_device(x, (x_scale, w_gate, gate_scale, w_up, up_scale), op)
+    return _eager.load().gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, code, out_dtype)
+
+
+@gated_8bit.register_fake
+def _(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation, out_dtype):
+    return x.new_empty((*x.shape[:-1], w_gate.shape[0]), dtype=out_dtype)
+
+
+def gated_linear_8bit(x: Tensor, x_scale: Tensor, w_gate: Tensor, gate_scale: Tensor, w_up: Tensor, up_scale: Tensor,
+                      activation: str = "silu", out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """act(g) * u of e4m3 rows: g = (x w_gate') x_scale gate_scale, u likewise, summed in fp32. x [..., D] and x_scale
+    [...] as rms_norm_8bit gives them, weights [F, D] and scales [F] as quantize_rows does. For inference: there is no
+    gradient."""
+    return torch.ops.sparton.gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation, out_dtype)
+
+
+def quantize_rows(t: Tensor) -> Tuple[Tensor, Tensor]:
+    """(e4m3 rows, fp32 scale of each): t ~ rows * scale[..., None], the largest magnitude of a row at 448. To lay out
+    a model's weights once; plain torch operations."""
+    t = t.detach().float()
+    scale = (t.abs().amax(-1) / E4M3_MAX).clamp_min(2.0 ** -126)
+    return (t / scale[..., None]).clamp(-E4M3_MAX, E4M3_MAX).to(_E4M3), scale
+
+
+def activation_name(fn) -> Optional[str]:
+    """The kernels' name of a module's activation, or None if they do not compute it."""
+    if isinstance(fn, nn.SiLU) or fn is F.silu or type(fn).__name__ == "SiLUActivation":
+        return "silu"
+    if isinstance(fn, nn.GELU):
+        return "gelu_tanh" if fn.approximate == "tanh" else "gelu"
+    if fn is F.gelu or type(fn).__name__ == "GELUActivation":
+        return "gelu"
+    if type(fn).__name__ == "GELUTanh":
+        return "gelu_tanh"
+    if isinstance(fn, nn.ReLU) or fn is F.relu:
+        return "relu"
+    return None
+
+
+class SpartonGatedMLP(nn.Module):
+    """A gated block, down_proj(act(gate_proj(x)) * up_proj(x)), its first half on the kernels above.
+    `SpartonGatedMLP.of(block)` shares the three nn.Linear of an existing block (names and state_dict unchanged)."""
+
+    def __init__(self, gate_proj: nn.Linear, up_proj: nn.Linear, down_proj: nn.Linear, activation: str = "silu"):
+        super().__init__()
+        _code(activation, "SpartonGatedMLP")
+        if gate_proj.weight.shape != up_proj.weight.shape or down_proj.in_features != gate_proj.out_features:
+            raise ValueError("SpartonGatedMLP needs gate_proj and up_proj of one shape and down_proj behind them, got "
+                             f"{gate_proj}, {up_proj} and {down_proj}")
+        self.gate_proj, self.up_proj, self.down_proj, self.activation = gate_proj, up_proj, down_proj, activation
+
+    @classmethod
+    def of(cls, block: nn.Module) -> "SpartonGatedMLP":
+        name = activation_name(getattr(block, "act_fn", None))
+        if name is None:
+            raise ValueError(f"SpartonGatedMLP computes {', '.join(ACTIVATIONS)}; this block's activation is "
+                             f"{getattr(block, 'act_fn', None)!r}")
+        m = cls(block.gate_proj, block.up_proj, block.down_proj, name)
+        return m.train(block.training)
+
+    def forward(self, x: Tensor) -> Tensor:
+        gate, up = self.gate_proj, self.up_proj
+        return self.down_proj(gated_linear(x, gate.weight, up.weight, gate.bias, up.bias, self.activation))

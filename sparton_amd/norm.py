@@ -1,4 +1,5 @@
-"""LayerNorm of a backbone's rows, with the residual sum in front of it, on hand-written HIP kernels.
+"""LayerNorm and root-mean-square norm of a backbone's rows, with the residual sum in front, on hand-written HIP
+kernels.
 
     y = LayerNorm(x + residual) * weight + bias        per row over the last dimension D
 
@@ -11,13 +12,22 @@ The residual sum is formed in fp32 and not rounded, so nothing of it is stored.
     sparton::layer_norm_fwd(x, residual?, weight, bias?, eps) -> (y, mean, rstd)
     sparton::layer_norm_bwd(dy, x, residual?, weight, has_bias, mean, rstd) -> (dx, d_weight, d_bias)
 
+The root-mean-square norm of decoder backbones has the sum as an output too (the next layer's residual), and
+its rows in e4m3 with a scale each where a product in 8 bits reads them:
+
+    h = x + residual;   y = h / sqrt(mean(h^2) + eps) * weight
+
+    sparton::rms_norm_fwd(x, residual?, weight, eps) -> (y, h, rstd)      h is empty without a residual
+    sparton::rms_norm_bwd(dy, dh?, h, weight, rstd) -> (dx, d_weight)
+    sparton::rms_norm_8bit(x, residual?, weight, eps) -> (y in e4m3, scale, h)
+
 Device tensors only, like the head.
 """
 from __future__ import annotations
 
 import copy
 import math
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor, nn
@@ -157,3 +167,139 @@ class SpartonLayerNorm(nn.LayerNorm):
         if weight.dtype not in (torch.float32, x.dtype):
             weight, bias = weight.to(x.dtype), bias.to(x.dtype) if bias is not None else None
         return layer_norm(x, weight, bias, self.eps, residual)
+
+
+# ---- the root-mean-square norm ----------------------------------------------------------------
+
+@torch.library.custom_op("sparton::rms_norm_fwd", mutates_args=())
+def rms_norm_fwd(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """(y and the rounded sum h in x's dtype, rstd per row in fp32 for the backward); h is empty without a residual."""
+    _check(x, residual, weight, None, eps, "sparton::rms_norm_fwd")
+    return _eager.load().rms_norm_fwd(x, residual, weight, eps)
+
+
+@rms_norm_fwd.register_fake
+def _(x, residual, weight, eps):
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    return x.new_empty(x.shape), x.new_empty(x.shape if residual is not None else (0,)), x.new_empty(
+        (rows,), dtype=torch.float32)
+
+
+@torch.library.custom_op("sparton::rms_norm_bwd", mutates_args=())
+def rms_norm_bwd(dy: Tensor, dh: Optional[Tensor], h: Tensor, weight: Tensor, rstd: Tensor) -> Tuple[Tensor, Tensor]:
+    """(the gradient of x and of the residual alike, in h's dtype; d_weight in the weight's). h: the forward's, or x
+    where there was no residual; dh: its gradient."""
+    op = "sparton::rms_norm_bwd"
+    D = _check(h, None, weight, None, 0.0, op)
+    for t in (dy, dh):
+        if t is not None and (t.shape != h.shape or t.device != h.device):
+            raise ValueError(f"{op}: dy and dh must be {tuple(h.shape)} on {h.device}, got {tuple(t.shape)} on {t.device}")
+    if tuple(rstd.shape) != (h.numel() // D,) or rstd.dtype != torch.float32 or rstd.device != h.device \
+            or not rstd.is_contiguous():
+        raise ValueError(f"{op}: rstd must be contiguous float32 [{h.numel() // D}] on {h.device}")
+    return _eager.load().rms_norm_bwd(dy, dh.to(h.dtype) if dh is not None else None, h, weight, rstd)
+
+
+@rms_norm_bwd.register_fake
+def _(dy, dh, h, weight, rstd):
+    return h.new_empty(h.shape), weight.new_empty(weight.shape)
+
+
+def _rms_setup_context(ctx, inputs, output):
+    x, residual, weight, _eps = inputs
+    _y, h, rstd = output
+    ctx.mark_non_differentiable(rstd)
+    ctx.set_materialize_grads(False)
+    ctx.has_residual = residual is not None
+    ctx.save_for_backward(h if residual is not None else x, weight, rstd)
+
+
+def _rms_backward(ctx, dy, dh, _drstd):
+    h, weight, rstd = ctx.saved_tensors
+    dh = dh if ctx.has_residual else None
+    if dy is None:  # y did not reach the loss
+        return dh, dh, None, None
+    dx, dw = torch.ops.sparton.rms_norm_bwd(dy, dh, h, weight, rstd)
+    return dx, (dx if ctx.has_residual else None), dw, None
+
+
+rms_norm_fwd.register_autograd(_rms_backward, setup_context=_rms_setup_context)
+
+
+def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6,
+             residual: Optional[Tensor] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+    """x / sqrt(mean(x^2) + eps) * weight over the last dimension (up to 16384), in x's dtype; weight is float32 (a
+    master) or of x's dtype, and gets its gradient in it. With a residual: (the norm of h = x + residual, h); the norm
+    reads the sum before it is rounded."""
+    eps = float(eps)
+    if torch.compiler.is_compiling() or not x.is_cuda:  # the registered op: fake + autograd
+        y, h, _ = torch.ops.sparton.rms_norm_fwd(x, residual, weight, eps)
+        return y if residual is None else (y, h)
+    _check(x, residual, weight, None, eps, "rms_norm")
+    if residual is None:
+        return _eager.load().rms_norm(x, weight, eps)
+    return _eager.load().rms_norm_add(x, residual, weight, eps)
+
+
+@torch.library.custom_op("sparton::rms_norm_8bit", mutates_args=())
+def _rms_norm_8bit(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """(y in e4m3, a scale a row, h), without a gradient; h is empty without a residual."""
+    _check(x, residual, weight, None, eps, "sparton::rms_norm_8bit")
+    return _eager.load().rms_norm_8bit(x, residual, weight, eps)
+
+
+@_rms_norm_8bit.register_fake
+def _(x, residual, weight, eps):
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32),
+            x.new_empty(x.shape if residual is not None else (0,)))
+
+
+def rms_norm_8bit(x: Tensor, weight: Tensor, eps: float = 1e-6, residual: Optional[Tensor] = None):
+    """(y8, scale), with a residual (y8, scale, h): the rows of rms_norm in e4m3, y ~ y8 * scale[..., None], as
+    feed_forward.gated_linear_8bit reads them. scale (fp32) puts a row's largest magnitude at 448. For inference:
+    inputs that ask for a gradient are refused."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+        raise ValueError("rms_norm_8bit has no gradient: call it under torch.no_grad()")
+    y, scale, h = torch.ops.sparton.rms_norm_8bit(x, residual, weight, float(eps))
+    return (y, scale) if residual is None else (y, scale, h)
+
+
+class SpartonRMSNorm(nn.Module):
+    """A root-mean-square norm over the last dimension on the kernels above: norm(x), or norm(x, residual) for
+    (norm of the sum, sum). `SpartonRMSNorm.of(module)` shares an existing module's weight (name and state_dict
+    unchanged) and keeps its hooks.
+
+    A weight wider than x (float32 masters) stays as it is and the result is x's dtype; under autocast too, as the
+    inputs are rows of the autocast dtype there."""
+
+    def __init__(self, width: int, eps: float = 1e-6, device=None, dtype=None):
+        super().__init__()
+        if not 1 <= width <= MAX_WIDTH:
+            raise ValueError(f"SpartonRMSNorm takes rows up to {MAX_WIDTH}, got {width}")
+        self.weight = nn.Parameter(torch.ones(width, device=device, dtype=dtype))
+        self.eps = float(eps)
+
+    @classmethod
+    def of(cls, module: nn.Module) -> "SpartonRMSNorm":
+        weight, eps = getattr(module, "weight", None), getattr(module, "variance_epsilon", getattr(module, "eps", None))
+        if not isinstance(weight, Tensor) or weight.dim() != 1 or not isinstance(eps, float):
+            raise ValueError(f"SpartonRMSNorm needs a weight over one dimension and an epsilon, got {module}")
+        if not 1 <= weight.shape[0] <= MAX_WIDTH:
+            raise ValueError(f"SpartonRMSNorm takes rows up to {MAX_WIDTH}, got {weight.shape[0]}")
+        m = copy.copy(module)  # the same hooks and mode
+        m.__class__ = cls
+        m._parameters = dict(m._parameters)  # and parameters, until either module is given another one
+        m.eps = float(eps)
+        return m
+
+    def extra_repr(self) -> str:
+        return f"{self.weight.shape[0]}, eps={self.eps}"
+
+    def forward(self, x: Tensor, residual: Optional[Tensor] = None):
+        weight = self.weight
+        if residual is not None and residual.dtype != x.dtype:
+            dt = torch.promote_types(x.dtype, residual.dtype)
+            x, residual = x.to(dt), residual.to(dt)
+        if weight.dtype not in (torch.float32, x.dtype):
+            weight = weight.to(x.dtype)
+        return rms_norm(x, weight, self.eps, residual)
