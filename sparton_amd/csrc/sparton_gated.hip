@@ -25,6 +25,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "sparton_common.h"
 #include "sparton_rows.h"
@@ -44,30 +45,57 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 
 // ---- activations --------------------------------------------------------------------------
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+// On the hardware's base-2 exponential and reciprocal (1 ulp each); the exponents' own rounding makes exp(-x) off by
+// x 2^-24.
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * -1.44269504088896341f); }
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_neg(x)); }
+
+// The normal distribution's integral up to g: with x = |g| / sqrt(2) and t = 1 / (1 + 0.4 x),
+//     erfc(x) / 2 = exp(-x^2) t Q(t),   Q(t) = erfc(x) exp(x^2) / (2 t), a smooth function on (0, 1],
+// here its polynomial of degree 10, fitted for the least relative error (6e-9, below fp32's). e: exp(-g^2 / 2).
+__device__ __forceinline__ float normal_below(float g, float e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.28284271247461901f, fabsf(g), 1.0f));
+  float q = -0.014607510529458523f;
+  q = fmaf(q, t, 0.07022310048341751f);
+  q = fmaf(q, t, -0.11776304990053177f);
+  q = fmaf(q, t, 0.06877996772527695f);
+  q = fmaf(q, t, -0.023447012528777122f);
+  q = fmaf(q, t, 0.04195791855454445f);
+  q = fmaf(q, t, 0.05950424075126648f);
+  q = fmaf(q, t, 0.08586962521076202f);
+  q = fmaf(q, t, 0.10380686819553375f);
+  q = fmaf(q, t, 0.11283793300390244f);
+  q = fmaf(q, t, 0.11283791810274124f);
+  const float w = t * q * e;
+  return g < 0.0f ? w : 1.0f - w;
+}
 
 // act(g), and its derivative where it is asked for.
-template <bool GRAD> __device__ __forceinline__ float activate(int act, float g, float* d) {
+template <int ACT, bool GRAD> __device__ __forceinline__ float activate(float g, float* d) {
+  if constexpr (ACT == SPARTON_SILU) {
+    const float s = sigmoid(g);
+    if (GRAD) *d = s * fmaf(g, 1.0f - s, 1.0f);
+    return g * s;
+  } else if constexpr (ACT == SPARTON_GELU) {
+    const float e = exp_neg(0.5f * g * g), c = normal_below(g, e);
+    if (GRAD) *d = fmaf(g * e, 0.39894228040143268f, c);
+    return g * c;
+  } else if constexpr (ACT == SPARTON_GELU_TANH) {  // (1 + tanh(z)) / 2 = sigmoid(2 z)
+    const float s = sigmoid(g * fmaf(0.071354816272600243f, g * g, 1.5957691216057308f));
+    if (GRAD) *d = fmaf(g * s * (1.0f - s), fmaf(0.21406444881780073f, g * g, 1.5957691216057308f), s);
+    return g * s;
+  } else {
+    if (GRAD) *d = g > 0.0f ? 1.0f : 0.0f;
+    return g > 0.0f || g != g ? g : 0.0f;
+  }
+}
+// f(std::integral_constant<int, act>)
+template <typename F> __device__ __forceinline__ void with_activation(int act, const F& f) {
   switch (act) {  // uniform
-    case SPARTON_SILU: {
-      const float s = sigmoid(g);
-      if (GRAD) *d = s * (1.0f + g * (1.0f - s));
-      return g * s;
-    }
-    case SPARTON_GELU: {
-      const float c = 0.5f * erfcf(-0.70710678118654752f * g);
-      if (GRAD) *d = c + g * expf(-0.5f * g * g) * 0.39894228040143268f;
-      return g * c;
-    }
-    case SPARTON_GELU_TANH: {  // 0.5 (1 + tanh(z)) = sigmoid(2 z)
-      const float s = sigmoid(g * (1.5957691216057308f + 0.071354816272600243f * g * g));
-      if (GRAD) *d = s + g * s * (1.0f - s) * (1.5957691216057308f + 0.21406444881780073f * g * g);
-      return g * s;
-    }
-    default: {  // SPARTON_RELU
-      if (GRAD) *d = g > 0.0f ? 1.0f : 0.0f;
-      return g > 0.0f || g != g ? g : 0.0f;
-    }
+    case SPARTON_SILU: return f(std::integral_constant<int, SPARTON_SILU>());
+    case SPARTON_GELU: return f(std::integral_constant<int, SPARTON_GELU>());
+    case SPARTON_GELU_TANH: return f(std::integral_constant<int, SPARTON_GELU_TANH>());
+    default: return f(std::integral_constant<int, SPARTON_RELU>());
   }
 }
 
@@ -144,25 +172,29 @@ template <typename T, bool KM, int R, int NW, bool PAIR> struct Copy {
         off[i] = in ? (uint32_t)((row + i * (NW * 64 / CPR)) * s.ld + chunk * 16) : kNowhere;
     }
   }
-  // Slab k of one half, of whose inner dimension `left` elements are left, into LDS at `to` (this wave's first chunk).
-  __device__ __forceinline__ void issue(int half, int k, int64_t left, uint32_t to) const {
-    const char* base = (!PAIR && half ? b1 : b0) + k * step;
-    const char* other = PAIR ? b1 + k * step : base;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-      const char* from = PAIR && (((w + NW * i) >> 2) & 1) ? other : base;
-      const bool in = KM ? at + i * (NW * 64 / CPR) < left : at < left * E;
-      const uint32_t o = in ? off[i] : kNowhere;
-      u32x4 rsrc;
-      rsrc[0] = (uint32_t)(uintptr_t)from;
-      rsrc[1] = (uint32_t)((uintptr_t)from >> 32);
-      rsrc[2] = 0x80000000u;
-      rsrc[3] = 0x00020000u;
-      const uint32_t dst = to + (uint32_t)(i * NW) * 1024u;
-      // The compiler would wait for a copy it knows of before any LDS read; these are waited for at the slab's end.
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(o), "s"(rsrc));
-    }
+  // What the copies of one slab share.
+  struct Slab {
+    const char *p0, *p1;
+    int64_t left;
+  };
+  // Slab k of one half, of whose inner dimension `left` elements (none or fewer: zeros) are left.
+  __device__ __forceinline__ Slab slab(int half, int k, int64_t left) const {
+    const char* p0 = (!PAIR && half ? b1 : b0) + k * step;
+    return Slab{p0, PAIR ? b1 + k * step : p0, left};
+  }
+  // Copy i of this wave, into LDS from `to` (the wave's first chunk) on.
+  __device__ __forceinline__ void issue(const Slab& s, int i, uint32_t to) const {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool in = KM ? at + i * (NW * 64 / CPR) < s.left : at < s.left * E;
+    const uint32_t o = in ? off[i] : kNowhere, dst = to + (uint32_t)(i * NW) * 1024u;
+    const uintptr_t from = (uintptr_t)(PAIR && (((w + NW * i) >> 2) & 1) ? s.p1 : s.p0);
+    u32x4 r;  // the compiler does not see that these are the same in every lane
+    r[0] = __builtin_amdgcn_readfirstlane((uint32_t)from);
+    r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(from >> 32));
+    r[2] = 0x80000000u;
+    r[3] = 0x00020000u;
+    // The compiler would wait for a copy it knows of before any LDS read; these are waited for at the slab's end.
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(o), "s"(r));
   }
 };
 
@@ -228,20 +260,6 @@ struct Params {
   int act;
 };
 
-// Four consecutive columns of a result's row, of which `n` are there.
-template <typename T> __device__ __forceinline__ void store4(T* p, const float* v, int64_t n) {
-  if (n >= 4) {
-    vec_t<T, 4> o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(v[e]);
-    store_any<T, 4>(p, o);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (e < n) p[e] = from_f32<T>(v[e]);
-  }
-}
-
 // A workgroup's tile. Consecutive workgroups go to the eight XCDs in turn: each XCD takes a run of the tiles, which
 // walk kGroupQ row tiles before the next column tile, so that what is in flight shares operands in its L2.
 struct Place {
@@ -262,52 +280,82 @@ __device__ __forceinline__ Place place_of(const Params& a) {
   return r;
 }
 
-template <typename T, typename O, bool GATED>
-__device__ __forceinline__ void write(const Params& a, int64_t row, int64_t col, int split, int turn, const f32x16& c0,
-                                      const f32x16& c1, int r) {
-  if (row >= a.q.n || col >= a.p.n) return;
-  const int64_t at = row * a.p.n + col, left = a.p.n - col;
-  float v[4];
-  if constexpr (GATED) {
-    float g[4], u[4], d;
+// N consecutive columns of a result's row, of which `n` are there.
+template <typename T, int N> __device__ __forceinline__ void store_n(T* p, const float* v, int64_t n) {
+  constexpr int V = N * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t f = min(col + e, a.p.n - 1);
-      g[e] = c0[r + e];
-      u[e] = c1[r + e];
-      if constexpr (sizeof(T) == 1) {
-        const float sx = a.sx[row];
-        g[e] *= sx * a.sg[f];
-        u[e] *= sx * a.su[f];
-      }
-      if (a.bg != nullptr) g[e] += to_f32(((const O*)a.bg)[f]);
-      if (a.bu != nullptr) u[e] += to_f32(((const O*)a.bu)[f]);
-      v[e] = activate<false>(a.act, g[e], &d) * u[e];
-    }
-    store4<O>((O*)a.h + at, v, left);
-    if (a.g != nullptr) {
-      store4<float>(a.g + at, g, left);
-      store4<float>(a.u + at, u, left);
-    }
-  } else {
+  for (int k = 0; k < N; k += V) {
+    if (n >= k + V) {
+      vec_t<T, V> o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = c0[r + e];
-    if (a.splits > 1) store4<float>(a.part + ((int64_t)split * a.turns + turn) * a.q.n * a.p.n + at, v, left);
-    else store4<O>((O*)a.out[turn] + at, v, left);
+      for (int e = 0; e < V; ++e) o[e] = from_f32<T>(v[k + e]);
+      store_any<T, V>(p + k, o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V - 1; ++e)
+        if (k + e < n) p[k + e] = from_f32<T>(v[k + e]);
+    }
   }
 }
 
+// A lane's four columns of the gated result: what is the same in every row, read once.
+template <typename T, typename O> struct Columns {
+  int64_t col, left;  // columns from col on that are there: none for 0 or fewer
+  float bg[4], bu[4], sg[4], su[4];
+  __device__ __forceinline__ void init(const Params& a, int64_t col_) {
+    col = col_;
+    left = a.p.n - col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t f = min(col + e, a.p.n - 1);
+      bg[e] = a.bg != nullptr ? to_f32(((const O*)a.bg)[f]) : 0.0f;
+      bu[e] = a.bu != nullptr ? to_f32(((const O*)a.bu)[f]) : 0.0f;
+      if constexpr (sizeof(T) == 1) {
+        sg[e] = a.sg[f];
+        su[e] = a.su[f];
+      }
+    }
+  }
+  // One row of them from the products' sums (8 bits: before the scales): h, and g and u where they are kept.
+  template <int ACT> __device__ __forceinline__ void write(const Params& a, int64_t row, f32x4 gs, f32x4 us) const {
+    if (row >= a.q.n || left <= 0) return;
+    float v[4], g[4], u[4], d;
+    float sx = 1.0f;
+    if constexpr (sizeof(T) == 1) sx = a.sx[row];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      g[e] = sizeof(T) == 1 ? gs[e] * (sx * sg[e]) : gs[e] + bg[e];
+      u[e] = sizeof(T) == 1 ? us[e] * (sx * su[e]) : us[e] + bu[e];
+      v[e] = activate<ACT, false>(g[e], &d) * u[e];
+    }
+    const int64_t at = row * a.p.n + col;
+    store_n<O, 4>((O*)a.h + at, v, left);
+    if (sizeof(T) > 1 && a.g != nullptr) {
+      store_n<float, 4>(a.g + at, g, left);
+      store_n<float, 4>(a.u + at, u, left);
+    }
+  }
+};
+
 // WQ x WP waves, each JQ x JP blocks of 32 x 32.
-template <typename T, typename O, bool QKM, bool PKM, bool GATED, int WQ, int WP, int JQ, int JP>
-__global__ __launch_bounds__(64 * WQ * WP, 2) void gated_gemm_kernel(Params a) {
+//
+// A step's operands are read while the step before it multiplies, across the slabs' ends too: the barrier that ends
+// slab k (its last operands are in registers, slab k + 1 has landed) comes before k's last step, beside which k + 1's
+// first operands are read and the copies of slab k + 2 begin, into the stage that k leaves.
+template <typename T, typename O, bool QKM, bool PKM, bool GATED, int WQ, int WP, int JQ, int JP, int OCC>
+__global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a) {
   constexpr int NW = WQ * WP, BQ = WQ * JQ * 32, BP = WP * JP * 32, STAGE = (BQ + BP) * kSlab;
-  constexpr int STEPS = 4 / kCh<T>;
-  static_assert(!GATED || JP == 2, "a wave holds a gate block and the up block beside it");
+  constexpr int STEPS = 4 / kCh<T>, MMAS = JQ * JP, READS = JQ + JP;
+  static_assert(!GATED || JP % 2 == 0, "a wave holds gate blocks and the up blocks beside them");
   __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
   const Place at = place_of(a);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = w % WQ, wp = w / WQ;
   Copy<T, QKM, BQ, NW, false> cq;
   Copy<T, PKM, BP, NW, GATED> cp;
+  constexpr int NQ = decltype(cq)::N, NC = NQ + decltype(cp)::N;
+  // Copies beside a slab's last step, and the rest beside the next one's first: what is left of that slab is their
+  // time to land.
+  constexpr int EARLY = STEPS == 4 ? NC / 2 : NC;
   Side q = a.q;
   if (at.turn > 0) q.b0 = a.q_turn;
   cq.init(q, (int64_t)at.q * BQ);
@@ -323,50 +371,101 @@ __global__ __launch_bounds__(64 * WQ * WP, 2) void gated_gemm_kernel(Params a) {
     for (int j = 0; j < JP; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-  const int k_end = min(a.slabs, (at.split + 1) * a.per_split);
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-  const auto issue = [&](int k, int stage) {
+  const int k0 = at.split * a.per_split, k_end = min(a.slabs, k0 + a.per_split);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + w * 1024;
+  typename Copy<T, QKM, BQ, NW, false>::Slab sq;
+  typename Copy<T, PKM, BP, NW, GATED>::Slab sp;
+  const auto prepare = [&](int k) {
     const int half = k >= a.half_slabs ? 1 : 0, kk = k - half * a.half_slabs;
-    const int64_t left = a.K - (int64_t)kk * (kSlab / (int)sizeof(T));
-    const uint32_t to = lds0 + stage * STAGE + w * 1024;
-    cq.issue(half, kk, left, to);
-    cp.issue(half, kk, left, to + BQ * kSlab);
+    const int64_t left = k < k_end ? a.K - (int64_t)kk * (kSlab / (int)sizeof(T)) : 0;
+    sq = cq.slab(half, kk, left);
+    sp = cp.slab(half, kk, left);
   };
-  int k = at.split * a.per_split, stage = 0;
-  if (k < k_end) issue(k, 0);
-  for (; k < k_end; ++k, stage ^= 1) {
-    // This slab has landed for every wave, and the stage before it is read out.
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (k + 1 < k_end) issue(k + 1, stage ^ 1);
-    const char* sq = lds + stage * STAGE;
-    const char* sp = sq + BQ * kSlab;
+  const auto copy = [&](int n, int stage) {
+    const uint32_t to = lds0 + stage * STAGE;
+    if (n < NQ) cq.issue(sq, n, to);
+    else cp.issue(sp, n - NQ, to + BQ * kSlab);
+  };
+  Frag<T> fq[2][JQ], fp[2][JP];
+  const auto read = [&](int set, int n, int s, int stage) {
+    const char* from = lds + stage * STAGE;
+    if (n < JP) fp[set][n] = rp.get(from + BQ * kSlab, n, s);
+    else fq[set][n - JP] = rq.get(from, n - JP, s);
+  };
+  prepare(k0);
+#pragma unroll
+  for (int n = 0; n < NC; ++n) copy(n, 0);
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  prepare(k0 + 1);
+#pragma unroll
+  for (int n = 0; n < READS; ++n) read(0, n, 0, 0);
+#pragma unroll
+  for (int n = 0; n < EARLY; ++n) copy(n, 1);
+  int stage = 0;
+  for (int k = k0; k < k_end; ++k, stage ^= 1) {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      Frag<T> fp[JP], fq[JQ];
+      const bool last = s == STEPS - 1;
+      if (last) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        prepare(k + 2);
+      }
 #pragma unroll
-      for (int j = 0; j < JP; ++j) fp[j] = rp.get(sp, j, s);
+      for (int n = 0; n < MMAS; ++n) {
+        // next step's operands, evenly between the products, and copies likewise
 #pragma unroll
-      for (int i = 0; i < JQ; ++i) fq[i] = rq.get(sq, i, s);
+        for (int i = 0; i < (READS + MMAS - 1) / MMAS; ++i)
+          if (n * READS / MMAS + i < (n + 1) * READS / MMAS)
+            read((s + 1) & 1, n * READS / MMAS + i, last ? 0 : s + 1, last ? stage ^ 1 : stage);
 #pragma unroll
-      for (int i = 0; i < JQ; ++i)
-#pragma unroll
-        for (int j = 0; j < JP; ++j) mma(acc[i][j], fp[j], fq[i]);
+        for (int i = 0; i < (NC + MMAS - 1) / MMAS; ++i) {
+          if (last && n * EARLY / MMAS + i < (n + 1) * EARLY / MMAS) copy(n * EARLY / MMAS + i, stage);
+          if (s == 0 && n * (NC - EARLY) / MMAS + i < (n + 1) * (NC - EARLY) / MMAS)
+            copy(EARLY + n * (NC - EARLY) / MMAS + i, stage ^ 1);
+        }
+        mma(acc[n / JP][n % JP], fp[s & 1][n % JP], fq[s & 1][n / JP]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // zeros of slabs past the end: LDS is this workgroup's until then
+  __syncthreads();
+  // A wave's 32 rows at a time pass through LDS of its own, so that its lanes store whole runs of a row.
+  constexpr int COLS = JP * 32, LD = COLS + 4, CPL = GATED ? 4 : 16 / (int)sizeof(O);
+  constexpr int LPR = (GATED ? COLS / 2 : COLS) / CPL, ROWS = 64 / LPR;
+  static_assert(NW * 32 * LD * 4 <= 2 * STAGE, "fits the stages");
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  float* mine = (float*)lds + w * 32 * LD;
+  const int c = lane % LPR * CPL, r0 = lane / LPR;
+  Columns<T, O> cols;
+  if constexpr (GATED) cols.init(a, (int64_t)at.p * (BP / 2) + wp * (COLS / 2) + c);
 #pragma unroll
   for (int i = 0; i < JQ; ++i) {
-    const int64_t row = (int64_t)at.q * BQ + (wq * JQ + i) * 32 + l32;
+#pragma unroll
+    for (int j = 0; j < JP; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *(f32x4*)(mine + l32 * LD + j * 32 + 8 * r + 4 * h) =
+            f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+    const int64_t row0 = (int64_t)at.q * BQ + (wq * JQ + i) * 32;
     if constexpr (GATED) {
-      const int64_t col = (int64_t)at.p * (BP / 2) + wp * 32 + 4 * h;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) write<T, O, true>(a, row, col + 8 * r, at.split, at.turn, acc[i][0], acc[i][1], 4 * r);
+      const float* from = mine + (c >> 5) * 64 + (c & 31);
+      with_activation(a.act, [&](auto act) {
+#pragma unroll 4
+        for (int r = r0; r < 32; r += ROWS)
+          cols.template write<decltype(act)::value>(a, row0 + r, *(const f32x4*)(from + r * LD), *(const f32x4*)(from + r * LD + 32));
+      });
     } else {
+      const int64_t col = (int64_t)at.p * BP + wp * COLS + c, left = a.p.n - col;
+#pragma unroll 4
+      for (int r = r0; r < 32; r += ROWS) {
+        float v[CPL];
 #pragma unroll
-      for (int j = 0; j < JP; ++j) {
-        const int64_t col = (int64_t)at.p * BP + (wp * JP + j) * 32 + 4 * h;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) write<T, O, false>(a, row, col + 8 * r, at.split, at.turn, acc[i][j], acc[i][j], 4 * r);
+        for (int e = 0; e < CPL; e += 4) *(f32x4*)(v + e) = *(const f32x4*)(mine + r * LD + c + e);
+        if (row0 + r >= a.q.n || left <= 0) continue;
+        const int64_t to = (row0 + r) * a.p.n + col;
+        if (a.splits > 1) store_n<float, CPL>(a.part + ((int64_t)at.split * a.turns + at.turn) * a.q.n * a.p.n + to, v, left);
+        else store_n<O, CPL>((O*)a.out[at.turn] + to, v, left);
       }
     }
   }
@@ -442,7 +541,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void gated_few_kernel(Params a) 
   // Wave w takes registers 4 (w % 4) .. + 3 of block w / 4.
   for (int o = w; o < JQ * 4; o += kFewWaves) {
     const int i = o >> 2, r = o & 3;
-    f32x16 g, u;
+    f32x4 g, u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float sg = 0.0f, su = 0.0f;
@@ -454,7 +553,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void gated_few_kernel(Params a) 
       g[e] = sg;
       u[e] = su;
     }
-    write<T, O, true>(a, i * 32 + l32, f0 + 8 * r + 4 * h, 0, 0, g, u, 0);
+    Columns<T, O> cols;
+    cols.init(a, f0 + 8 * r + 4 * h);
+    with_activation(a.act, [&](auto act) { cols.template write<decltype(act)::value>(a, i * 32 + l32, g, u); });
   }
 }
 
@@ -463,18 +564,18 @@ constexpr int kActThreads = 256;
 constexpr int kActCols = 4;  // columns of a thread
 
 // dg and du [M, ld], zeros past F, and with `part` the column sums of a workgroup's rows, before their rounding.
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(kActThreads) void gated_act_bwd_kernel(const T* __restrict__ dh, const float* __restrict__ g,
                                                                     const float* __restrict__ u, T* __restrict__ dg,
-                                                                    T* __restrict__ du, float* __restrict__ part,
-                                                                    int64_t M, int64_t F, int64_t ld, int act, int rows,
-                                                                    int strips) {
+                                                                    T* __restrict__ du, float* __restrict__ part, int64_t M,
+                                                                    int64_t F, int64_t ld, int rows, int strips) {
   const int strip = blockIdx.x % strips;
   const int64_t blk = blockIdx.x / strips, col = ((int64_t)strip * kActThreads + threadIdx.x) * kActCols;
   const int64_t r0 = blk * rows, r1 = min(M, r0 + rows);
   if (col >= ld) return;
   const int n = (int)max((int64_t)0, min((int64_t)kActCols, F - col));
   float sg[kActCols] = {}, su[kActCols] = {};
+#pragma unroll 2
   for (int64_t r = r0; r < r1; ++r) {
     float vd[kActCols], vg[kActCols], vu[kActCols], og[kActCols], ou[kActCols];
     const int64_t at = r * F + col;
@@ -494,7 +595,7 @@ __global__ __launch_bounds__(kActThreads) void gated_act_bwd_kernel(const T* __r
 #pragma unroll
     for (int e = 0; e < kActCols; ++e) {
       float d;
-      const float a = activate<true>(act, vg[e], &d);
+      const float a = activate<ACT, true>(vg[e], &d);
       og[e] = vd[e] * vu[e] * d;
       ou[e] = vd[e] * a;
       if (part != nullptr) {
@@ -502,8 +603,8 @@ __global__ __launch_bounds__(kActThreads) void gated_act_bwd_kernel(const T* __r
         su[e] += ou[e];
       }
     }
-    store4<T>(dg + r * ld + col, og, ld - col);
-    store4<T>(du + r * ld + col, ou, ld - col);
+    store_n<T, 4>(dg + r * ld + col, og, ld - col);
+    store_n<T, 4>(du + r * ld + col, ou, ld - col);
   }
   if (part == nullptr) return;
 #pragma unroll
@@ -574,9 +675,9 @@ template <typename T, typename O, bool QKM, bool PKM, bool GATED> int gemm(Param
   const unsigned grid = (unsigned)((int64_t)s.tq * s.tp * s.splits * p.turns);
   if (grid == 0) return SPARTON_OK;
   if (s.small)
-    hipLaunchKernelGGL((gated_gemm_kernel<T, O, QKM, PKM, GATED, 2, 2, 2, 2>), dim3(grid), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((gated_gemm_kernel<T, O, QKM, PKM, GATED, 2, 2, 2, 2, 2>), dim3(grid), dim3(256), 0, st, p);
   else
-    hipLaunchKernelGGL((gated_gemm_kernel<T, O, QKM, PKM, GATED, 2, 4, 4, 2>), dim3(grid), dim3(512), 0, st, p);
+    hipLaunchKernelGGL((gated_gemm_kernel<T, O, QKM, PKM, GATED, 2, 2, 4, 4, 1>), dim3(grid), dim3(256), 0, st, p);
   return (int)hipGetLastError();
 }
 
@@ -641,8 +742,14 @@ int backward(const T* dh, const char* x, const char* wg, const char* wu, const f
   float* part = (float*)(ws + pl.act);
   float* bias = with_bias ? (float*)(ws + pl.act + pl.part) : nullptr;
   if (M > 0) {
-    hipLaunchKernelGGL(gated_act_bwd_kernel<T>, dim3((unsigned)(pl.blocks * (int64_t)pl.strips)), dim3(kActThreads), 0, st, dh, g,
-                       u, dg, du, bias, M, F, ld, act, pl.rows, pl.strips);
+    const auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(pl.blocks * (int64_t)pl.strips)), dim3(kActThreads), 0, st, dh, g, u, dg, du, bias,
+                         M, F, ld, pl.rows, pl.strips);
+    };
+    if (act == SPARTON_SILU) launch(gated_act_bwd_kernel<T, SPARTON_SILU>);
+    else if (act == SPARTON_GELU) launch(gated_act_bwd_kernel<T, SPARTON_GELU>);
+    else if (act == SPARTON_GELU_TANH) launch(gated_act_bwd_kernel<T, SPARTON_GELU_TANH>);
+    else launch(gated_act_bwd_kernel<T, SPARTON_RELU>);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
