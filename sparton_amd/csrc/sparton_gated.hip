@@ -316,23 +316,21 @@ template <typename T, typename O> struct Columns {
       }
     }
   }
-  // One row of them from the products' sums (8 bits: before the scales): h, and g and u where they are kept.
-  template <int ACT> __device__ __forceinline__ void write(const Params& a, int64_t row, f32x4 gs, f32x4 us) const {
-    if (row >= a.q.n || left <= 0) return;
+  // One row of them from the products' sums (8 bits: before the scales): h, and g and u where they are kept, at `at`
+  // elements from the pointers. WHOLE: all four columns are there.
+  template <int ACT, bool WHOLE>
+  __device__ __forceinline__ void write(O* h, float* gk, float* uk, uint32_t at, float sx, f32x4 gs, f32x4 us) const {
     float v[4], g[4], u[4], d;
-    float sx = 1.0f;
-    if constexpr (sizeof(T) == 1) sx = a.sx[row];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       g[e] = sizeof(T) == 1 ? gs[e] * (sx * sg[e]) : gs[e] + bg[e];
       u[e] = sizeof(T) == 1 ? us[e] * (sx * su[e]) : us[e] + bu[e];
       v[e] = activate<ACT, false>(g[e], &d) * u[e];
     }
-    const int64_t at = row * a.p.n + col;
-    store_n<O, 4>((O*)a.h + at, v, left);
-    if (sizeof(T) > 1 && a.g != nullptr) {
-      store_n<float, 4>(a.g + at, g, left);
-      store_n<float, 4>(a.u + at, u, left);
+    store_n<O, 4>(h + at, v, WHOLE ? 4 : left);
+    if (sizeof(T) > 1 && gk != nullptr) {
+      store_n<float, 4>(gk + at, g, WHOLE ? 4 : left);
+      store_n<float, 4>(uk + at, u, WHOLE ? 4 : left);
     }
   }
 };
@@ -439,6 +437,10 @@ __global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a)
   const int c = lane % LPR * CPL, r0 = lane / LPR;
   Columns<T, O> cols;
   if constexpr (GATED) cols.init(a, (int64_t)at.p * (BP / 2) + wp * (COLS / 2) + c);
+  // Offsets within 32 rows fit 32 bits. A tile that lies inside the result needs no bounds.
+  const int64_t rows0 = (int64_t)at.q * BQ + wq * JQ * 32, width = a.p.n;
+  const bool inside = ((int64_t)at.q + 1) * BQ <= a.q.n && ((int64_t)at.p + 1) * (GATED ? BP / 2 : BP) <= width;
+  const uint32_t step = ROWS * (uint32_t)width, first = r0 * (uint32_t)width + c;
 #pragma unroll
   for (int i = 0; i < JQ; ++i) {
 #pragma unroll
@@ -447,26 +449,42 @@ __global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a)
       for (int r = 0; r < 4; ++r)
         *(f32x4*)(mine + l32 * LD + j * 32 + 8 * r + 4 * h) =
             f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
-    const int64_t row0 = (int64_t)at.q * BQ + (wq * JQ + i) * 32;
+    const int64_t row0 = rows0 + i * 32;
     if constexpr (GATED) {
+      const int64_t to = row0 * width + (int64_t)at.p * (BP / 2) + wp * (COLS / 2);
+      O* ph = (O*)a.h + to;
+      float* pg = a.g != nullptr ? a.g + to : nullptr;
+      float* pu = a.g != nullptr ? a.u + to : nullptr;
       const float* from = mine + (c >> 5) * 64 + (c & 31);
-      with_activation(a.act, [&](auto act) {
+      const auto rows = [&](auto act, auto whole) {
 #pragma unroll 4
-        for (int r = r0; r < 32; r += ROWS)
-          cols.template write<decltype(act)::value>(a, row0 + r, *(const f32x4*)(from + r * LD), *(const f32x4*)(from + r * LD + 32));
-      });
+        for (int r = 0; r < 32 / ROWS; ++r) {
+          const int64_t row = row0 + r0 + r * ROWS;
+          if (!decltype(whole)::value && (row >= a.q.n || cols.left <= 0)) continue;
+          const float* v = from + (r0 + r * ROWS) * LD;
+          cols.template write<decltype(act)::value, decltype(whole)::value>(ph, pg, pu, first + r * step,
+                                                                            sizeof(T) == 1 ? a.sx[row] : 1.0f, *(const f32x4*)v,
+                                                                            *(const f32x4*)(v + 32));
+        }
+      };
+      with_activation(a.act, [&](auto act) { inside ? rows(act, std::true_type()) : rows(act, std::false_type()); });
     } else {
-      const int64_t col = (int64_t)at.p * BP + wp * COLS + c, left = a.p.n - col;
+      const int64_t left = width - ((int64_t)at.p * BP + wp * COLS + c);
+      const int64_t to = row0 * width + (int64_t)at.p * BP + wp * COLS;
+      const auto rows = [&](auto* out, auto whole) {
+        typedef std::remove_pointer_t<decltype(out)> R;
 #pragma unroll 4
-      for (int r = r0; r < 32; r += ROWS) {
-        float v[CPL];
+        for (int r = 0; r < 32 / ROWS; ++r) {
+          if (!decltype(whole)::value && (row0 + r0 + r * ROWS >= a.q.n || left <= 0)) continue;
+          float v[CPL];
 #pragma unroll
-        for (int e = 0; e < CPL; e += 4) *(f32x4*)(v + e) = *(const f32x4*)(mine + r * LD + c + e);
-        if (row0 + r >= a.q.n || left <= 0) continue;
-        const int64_t to = (row0 + r) * a.p.n + col;
-        if (a.splits > 1) store_n<float, CPL>(a.part + ((int64_t)at.split * a.turns + at.turn) * a.q.n * a.p.n + to, v, left);
-        else store_n<O, CPL>((O*)a.out[at.turn] + to, v, left);
-      }
+          for (int e = 0; e < CPL; e += 4) *(f32x4*)(v + e) = *(const f32x4*)(mine + (r0 + r * ROWS) * LD + c + e);
+          store_n<R, CPL>(out + first + r * step, v, decltype(whole)::value ? CPL : left);
+        }
+      };
+      const auto either = [&](auto* out) { inside ? rows(out, std::true_type()) : rows(out, std::false_type()); };
+      if (a.splits > 1) either(a.part + ((int64_t)at.split * a.turns + at.turn) * a.q.n * width + to);
+      else either((O*)a.out[at.turn] + to);
     }
   }
 }
@@ -555,7 +573,13 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void gated_few_kernel(Params a) 
     }
     Columns<T, O> cols;
     cols.init(a, f0 + 8 * r + 4 * h);
-    with_activation(a.act, [&](auto act) { cols.template write<decltype(act)::value>(a, i * 32 + l32, g, u); });
+    const int64_t row = i * 32 + l32;
+    if (row >= a.q.n || cols.left <= 0) continue;
+    const uint32_t to = (uint32_t)(row * a.p.n + cols.col);  // 64 rows of up to 2^20
+    const float sx = sizeof(T) == 1 ? a.sx[row] : 1.0f;
+    with_activation(a.act, [&](auto act) {
+      cols.template write<decltype(act)::value, false>((O*)a.h, a.g, a.u, to, sx, g, u);
+    });
   }
 }
 
