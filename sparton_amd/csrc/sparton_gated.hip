@@ -141,6 +141,7 @@ __device__ __forceinline__ int swizzle_rows(int row) { return (row & 7) ^ ((row 
 template <typename T, bool KM, int R, int NW, bool PAIR> struct Copy {
   static constexpr int E = sizeof(T), N = R / 8 / NW, CPR = KM ? R * E / 16 : 8;
   static_assert(R % (8 * NW) == 0, "every wave copies as much");
+  static_assert(!PAIR || NW == 4, "the waves' copies i are rows 32 i .. + 31");
   static_assert(!KM || (E == 2 ? 64 / CPR * NW % 4 == 0 : 64 / CPR * NW % 8 == 0 || CPR == 64), "one swizzle a lane");
   static constexpr uint32_t kNowhere = 0xc0000000u;
   uint32_t off[N];
@@ -184,10 +185,9 @@ template <typename T, bool KM, int R, int NW, bool PAIR> struct Copy {
   }
   // Copy i of this wave, into LDS from `to` (the wave's first chunk) on.
   __device__ __forceinline__ void issue(const Slab& s, int i, uint32_t to) const {
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool in = KM ? at + i * (NW * 64 / CPR) < s.left : at < s.left * E;
     const uint32_t o = in ? off[i] : kNowhere, dst = to + (uint32_t)(i * NW) * 1024u;
-    const uintptr_t from = (uintptr_t)(PAIR && (((w + NW * i) >> 2) & 1) ? s.p1 : s.p0);
+    const uintptr_t from = (uintptr_t)(PAIR && (i & 1) ? s.p1 : s.p0);  // 32 rows a copy of all four waves
     u32x4 r;  // the compiler does not see that these are the same in every lane
     r[0] = __builtin_amdgcn_readfirstlane((uint32_t)from);
     r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(from >> 32));
@@ -339,21 +339,19 @@ template <typename T, typename O> struct Columns {
 //
 // A step's operands are read while the step before it multiplies, across the slabs' ends too: the barrier that ends
 // slab k (its last operands are in registers, slab k + 1 has landed) comes before k's last step, beside which k + 1's
-// first operands are read and the copies of slab k + 2 begin, into the stage that k leaves.
+// first operands are read and the rows of slab k + 2 are copied into the stage that k leaves. Columns have three
+// stages: those of slab k + 2 are copied beside k's other steps and have a whole slab more to land.
 template <typename T, typename O, bool QKM, bool PKM, bool GATED, int WQ, int WP, int JQ, int JP, int OCC>
 __global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a) {
-  constexpr int NW = WQ * WP, BQ = WQ * JQ * 32, BP = WP * JP * 32, STAGE = (BQ + BP) * kSlab;
+  constexpr int NW = WQ * WP, BQ = WQ * JQ * 32, BP = WP * JP * 32, QS = BQ * kSlab, PS = BP * kSlab;
   constexpr int STEPS = 4 / kCh<T>, MMAS = JQ * JP, READS = JQ + JP;
   static_assert(!GATED || JP % 2 == 0, "a wave holds gate blocks and the up blocks beside them");
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds[2 * QS + 3 * PS];
   const Place at = place_of(a);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = w % WQ, wp = w / WQ;
   Copy<T, QKM, BQ, NW, false> cq;
   Copy<T, PKM, BP, NW, GATED> cp;
-  constexpr int NQ = decltype(cq)::N, NC = NQ + decltype(cp)::N;
-  // Copies beside a slab's last step, and the rest beside the next one's first: what is left of that slab is their
-  // time to land.
-  constexpr int EARLY = STEPS == 4 ? NC / 2 : NC;
+  constexpr int NQ = decltype(cq)::N, NP = decltype(cp)::N;
   Side q = a.q;
   if (at.turn > 0) q.b0 = a.q_turn;
   cq.init(q, (int64_t)at.q * BQ);
@@ -379,59 +377,64 @@ __global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a)
     sq = cq.slab(half, kk, left);
     sp = cp.slab(half, kk, left);
   };
-  const auto copy = [&](int n, int stage) {
-    const uint32_t to = lds0 + stage * STAGE;
-    if (n < NQ) cq.issue(sq, n, to);
-    else cp.issue(sp, n - NQ, to + BQ * kSlab);
-  };
   Frag<T> fq[2][JQ], fp[2][JP];
-  const auto read = [&](int set, int n, int s, int stage) {
-    const char* from = lds + stage * STAGE;
-    if (n < JP) fp[set][n] = rp.get(from + BQ * kSlab, n, s);
-    else fq[set][n - JP] = rq.get(from, n - JP, s);
+  const auto read = [&](int set, int n, int s, int oq, int op) {
+    if (n < JP) fp[set][n] = rp.get(lds + op, n, s);
+    else fq[set][n - JP] = rq.get(lds + oq, n - JP, s);
   };
-  prepare(k0);
+  // where the rows of slabs k and k + 1 lie, and the columns of k, k + 1 and k + 2
+  int q0 = 0, q1 = QS, p0 = 2 * QS, p1 = p0 + PS, p2 = p1 + PS;
+  const auto whole = [&](int k, int oq, int op) {
+    prepare(k);
 #pragma unroll
-  for (int n = 0; n < NC; ++n) copy(n, 0);
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-  prepare(k0 + 1);
+    for (int n = 0; n < NP; ++n) cp.issue(sp, n, lds0 + op);
 #pragma unroll
-  for (int n = 0; n < READS; ++n) read(0, n, 0, 0);
+    for (int n = 0; n < NQ; ++n) cq.issue(sq, n, lds0 + oq);
+  };
+  whole(k0, q0, p0);
+  whole(k0 + 1, q1, p1);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(NP + NQ) : "memory");
 #pragma unroll
-  for (int n = 0; n < EARLY; ++n) copy(n, 1);
-  int stage = 0;
-  for (int k = k0; k < k_end; ++k, stage ^= 1) {
+  for (int n = 0; n < READS; ++n) read(0, n, 0, q0, p0);
+  for (int k = k0; k < k_end; ++k) {
+    prepare(k + 2);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       const bool last = s == STEPS - 1;
-      if (last) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        prepare(k + 2);
-      }
+      // all but this slab's copies of columns have landed
+      if (last) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NP) : "memory");
 #pragma unroll
       for (int n = 0; n < MMAS; ++n) {
         // next step's operands, evenly between the products, and copies likewise
 #pragma unroll
         for (int i = 0; i < (READS + MMAS - 1) / MMAS; ++i)
           if (n * READS / MMAS + i < (n + 1) * READS / MMAS)
-            read((s + 1) & 1, n * READS / MMAS + i, last ? 0 : s + 1, last ? stage ^ 1 : stage);
+            read((s + 1) & 1, n * READS / MMAS + i, last ? 0 : s + 1, last ? q1 : q0, last ? p1 : p0);
+        constexpr int EARLY = (STEPS - 1) * MMAS;
+        const int m = s * MMAS + n;
 #pragma unroll
-        for (int i = 0; i < (NC + MMAS - 1) / MMAS; ++i) {
-          if (last && n * EARLY / MMAS + i < (n + 1) * EARLY / MMAS) copy(n * EARLY / MMAS + i, stage);
-          if (s == 0 && n * (NC - EARLY) / MMAS + i < (n + 1) * (NC - EARLY) / MMAS)
-            copy(EARLY + n * (NC - EARLY) / MMAS + i, stage ^ 1);
-        }
+        for (int i = 0; i < (NQ + MMAS - 1) / MMAS; ++i)
+          if (last && n * NQ / MMAS + i < (n + 1) * NQ / MMAS) cq.issue(sq, n * NQ / MMAS + i, lds0 + q0);
+#pragma unroll
+        for (int i = 0; i < (NP + EARLY - 1) / EARLY; ++i)
+          if (!last && m * NP / EARLY + i < (m + 1) * NP / EARLY) cp.issue(sp, m * NP / EARLY + i, lds0 + p2);
         mma(acc[n / JP][n % JP], fp[s & 1][n % JP], fq[s & 1][n / JP]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    const int t = p0;
+    p0 = p1;
+    p1 = p2;
+    p2 = t;
+    q1 = q0;
+    q0 = QS - q0;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // zeros of slabs past the end: LDS is this workgroup's until then
   __syncthreads();
   // A wave's 32 rows at a time pass through LDS of its own, so that its lanes store whole runs of a row.
   constexpr int COLS = JP * 32, LD = COLS + 4, CPL = GATED ? 4 : 16 / (int)sizeof(O);
   constexpr int LPR = (GATED ? COLS / 2 : COLS) / CPL, ROWS = 64 / LPR;
-  static_assert(NW * 32 * LD * 4 <= 2 * STAGE, "fits the stages");
+  static_assert(NW * 32 * LD * 4 <= 2 * QS + 3 * PS, "fits the stages");
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   float* mine = (float*)lds + w * 32 * LD;
   const int c = lane % LPR * CPL, r0 = lane / LPR;
