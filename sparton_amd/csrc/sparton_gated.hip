@@ -142,7 +142,6 @@ template <typename T, bool KM, int R, int NW, bool PAIR> struct Copy {
   static constexpr int E = sizeof(T), N = R / 8 / NW, CPR = KM ? R * E / 16 : 8;
   static_assert(R % (8 * NW) == 0, "every wave copies as much");
   static_assert(!PAIR || NW == 4, "the waves' copies i are rows 32 i .. + 31");
-  static_assert(!KM || (E == 2 ? 64 / CPR * NW % 4 == 0 : 64 / CPR * NW % 8 == 0 || CPR == 64), "one swizzle a lane");
   static constexpr uint32_t kNowhere = 0xc0000000u;
   uint32_t off[N];
   int at;  // KC: byte of the slab; KM: its row
@@ -161,16 +160,17 @@ template <typename T, bool KM, int R, int NW, bool PAIR> struct Copy {
         off[i] = first + row < s.n ? (uint32_t)(row * s.ld + at) : kNowhere;
       }
     } else {
-      const int c = w * 64 + lane, row = c / CPR, phys = c % CPR;
-      const int chunk = phys ^ (E == 2 ? (row & 3) << 2 : ((row >> 2) & 1) << 3);
-      at = row;
+      const int c = w * 64 + lane;
+      at = c / CPR;
       step = (int64_t)(kSlab / E) * s.ld;
       b0 = s.b0 + first * E;
       b1 = s.b1 + first * E;
-      const bool in = first + chunk * (16 / E) < s.n;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        off[i] = in ? (uint32_t)((row + i * (NW * 64 / CPR)) * s.ld + chunk * 16) : kNowhere;
+      for (int i = 0; i < N; ++i) {
+        const int row = at + i * (NW * 64 / CPR);
+        const int chunk = c % CPR ^ (E == 2 ? (row & 3) << 2 : ((row >> 2) & 1) << 3);
+        off[i] = first + chunk * (16 / E) < s.n ? (uint32_t)(row * s.ld + chunk * 16) : kNowhere;
+      }
     }
   }
   // What the copies of one slab share.
@@ -642,27 +642,28 @@ __global__ __launch_bounds__(kActThreads) void gated_act_bwd_kernel(const T* __r
   }
 }
 
-// The splits' sums added in order.
+// The splits' sums [split][turn][n] added in order, a turn a row of the grid: four elements a thread, four splits' loads
+// in flight.
 template <typename O>
-__global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ part, int splits, int64_t n, int turns,
-                                                         O* out0, O* out1) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n * turns) return;
-  const int64_t total = n * turns;
-  float v[4];
-  const int64_t left = min((int64_t)4, total - i);
+__global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ part, int splits, int64_t n, O* out0, O* out1) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, stride = n * gridDim.y;
+  if (i >= n) return;
+  const float* from = part + blockIdx.y * n + i;
+  O* out = (blockIdx.y == 0 ? out0 : out1) + i;
+  float v[4] = {};
+  if (i + 4 <= n) {
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const vec_t<float, 4> p = load_any<float, 4>(from + k * stride);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float s = 0.0f;
-    const int64_t at = min(i + e, total - 1);
-    for (int k = 0; k < splits; ++k) s += part[k * total + at];
-    v[e] = s;
+      for (int e = 0; e < 4; ++e) v[e] += p[e];
+    }
+  } else {
+    for (int k = 0; k < splits; ++k)
+      for (int e = 0; e < 3; ++e)
+        if (i + e < n) v[e] += from[k * stride + e];
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t at = i + e;
-    if (e < left) (at < n ? out0 + at : out1 + (at - n))[0] = from_f32<O>(v[e]);
-  }
+  store_n<O, 4>(out, v, n - i);
 }
 
 // ---- launches -----------------------------------------------------------------------------
@@ -675,22 +676,35 @@ struct Split {
   int tq, tp, splits, per_split, slabs;
 };
 
-// 256 x 256 tiles where there is one for most CUs, else 128 x 128; and where those are few too, the inner dimension
-// is split over workgroups, in runs of eight slabs or more.
-Split split_of(int64_t rows, int64_t cols, int64_t turns, int64_t slabs, bool may_split) {
-  Split s;
-  s.small = cdiv(rows, 256) * cdiv(cols, 256) * turns < 192;
-  const int64_t b = s.small ? 128 : 256;
-  s.tq = (int)cdiv(rows, b);
-  s.tp = (int)cdiv(cols, b);
-  s.slabs = (int)slabs;
-  const int64_t tiles = std::max<int64_t>(1, (int64_t)s.tq * s.tp * turns);
-  int64_t n = 1;
-  if (may_split && tiles < 2 * kCus) n = std::max<int64_t>(1, std::min<int64_t>(cdiv(2 * kCus, tiles), slabs / 8));
-  n = std::min<int64_t>(n, 16);
-  s.per_split = (int)std::max<int64_t>(1, cdiv(slabs, n));
-  s.splits = (int)std::max<int64_t>(1, cdiv(slabs, s.per_split));
-  return s;
+// The tile and the number of workgroups that share a tile's inner dimension: what an estimate of the time says. A CU
+// holds one workgroup of 256 x 256 or two of 128 x 128. Microseconds a slab and a tile's start and end, as measured:
+//               256 x 256       128 x 128, one on its CU       two
+//     16 bits   1.45            0.47                           0.9
+//     fp32      7.3             1.95                           3.6
+//     around    10              6                              6
+// and a join of splits reads 4.5 MB a microsecond. bf16, dx of 8192 x 768 x 2048 (96 tiles of 256, 384 of 128): 256 82 us,
+// 128 57, and split in two 82 and 85. dx of 8192 x 4096 x 11264: 1098 and 1485. dx of 300 x 768 x 2048: 128 32, split in
+// four 16. dW of 8192 x 2048 x 2048: 178 and 145.
+Split split_of(int64_t rows, int64_t cols, int64_t turns, int64_t slabs, int64_t es, bool may_split) {
+  Split best = {};
+  double least = -1.0;
+  for (int small = 0; small < 2; ++small) {
+    const int64_t b = small ? 128 : 256, tq = cdiv(rows, b), tp = cdiv(cols, b), tiles = std::max<int64_t>(1, tq * tp * turns);
+    const int64_t most = may_split && tiles < 2 * kCus ? std::min<int64_t>(16, std::max<int64_t>(1, slabs / 4)) : 1;
+    for (int64_t n = 1; n <= most; ++n) {
+      const int64_t per = std::max<int64_t>(1, cdiv(slabs, n)), splits = std::max<int64_t>(1, cdiv(slabs, per)), groups = tiles * splits;
+      if (splits != n && n > 1) continue;
+      const bool alone = groups <= kCus;
+      const double slab = es == 4 ? (small ? (alone ? 1.95 : 3.6) : 7.3) : (small ? (alone ? 0.47 : 0.9) : 1.45);
+      double time = (double)cdiv(groups, small ? 2 * kCus : kCus) * ((double)per * slab + (small ? 6.0 : 10.0));
+      if (splits > 1) time += 4.0 + (double)(rows * cols * turns) * (8.0 * (double)splits + 2.0) / 4.5e6;
+      if (least < 0.0 || time < least) {
+        least = time;
+        best = Split{small != 0, (int)tq, (int)tp, (int)splits, (int)per, (int)slabs};
+      }
+    }
+  }
+  return best;
 }
 
 template <typename T, typename O, bool QKM, bool PKM, bool GATED> int gemm(Params p, const Split& s, hipStream_t st) {
@@ -731,7 +745,7 @@ template <typename T, typename O> int forward(Params& p, hipStream_t st) {
   }
   const int64_t slabs = cdiv(p.K * (int64_t)sizeof(T), kSlab);
   p.half_slabs = (int)slabs;
-  return gemm<T, O, false, false, true>(p, split_of(p.q.n, 2 * p.p.n, 1, slabs, false), st);
+  return gemm<T, O, false, false, true>(p, split_of(p.q.n, 2 * p.p.n, 1, slabs, sizeof(T), false), st);
 }
 
 struct Plan {
@@ -743,8 +757,8 @@ struct Plan {
 Plan plan_of(int64_t M, int64_t D, int64_t F, int dtype, bool with_bias) {
   const int64_t es = es_of(dtype), ld = pad_of(F, dtype);
   Plan p;
-  p.dx = split_of(M, D, 1, 2 * cdiv(F * es, kSlab), true);
-  p.dw = split_of(F, D, 2, cdiv(M * es, kSlab), true);
+  p.dx = split_of(M, D, 1, 2 * cdiv(F * es, kSlab), es, true);
+  p.dw = split_of(F, D, 2, cdiv(M * es, kSlab), es, true);
   p.act = (size_t)round_up(2 * M * ld * es, 256);
   p.part = 0;
   if (p.dx.splits > 1) p.part = (size_t)round_up((int64_t)p.dx.splits * M * D * 4, 256);
@@ -788,8 +802,8 @@ int backward(const T* dh, const char* x, const char* wg, const char* wu, const f
   }
   const auto join = [&](const Split& s, int64_t n, int turns, T* a, T* b) {
     if (s.splits <= 1) return (int)hipGetLastError();
-    hipLaunchKernelGGL(gated_join_kernel<T>, dim3((unsigned)cdiv(n * turns, 1024)), dim3(256), 0, st, (const float*)part, s.splits,
-                       n, turns, a, b);
+    hipLaunchKernelGGL(gated_join_kernel<T>, dim3((unsigned)cdiv(n, 1024), (unsigned)turns), dim3(256), 0, st, (const float*)part,
+                       s.splits, n, a, b);
     return (int)hipGetLastError();
   };
   if (dx != nullptr && M > 0) {

@@ -127,7 +127,8 @@ def check(args, name):
 SIZES = [  # M, D, F: few rows, both tile sizes, every edge within and at a tile, split inner dimensions
     (1, 8, 1), (1, 64, 32), (3, 72, 33), (16, 768, 100), (32, 8, 64), (33, 200, 65), (64, 1000, 31), (65, 64, 64), (65, 8, 1),
     (100, 136, 127), (128, 128, 128), (129, 72, 129), (200, 1024, 257), (257, 768, 300), (300, 520, 1000), (1000, 64, 2048),
-    (512, 256, 4000), (2049, 264, 1500), (4096, 128, 3000), (1500, 2048, 1100),
+    (512, 256, 4000), (2049, 264, 1500), (4096, 128, 3000), (1500, 2048, 1100), (66, 272, 11450), (3437, 136, 8663),
+    (659, 136, 9167), (5226, 1560, 65), (8990, 136, 4532), (8301, 416, 360), (264, 64, 11198),
 ]
 
 
@@ -159,7 +160,7 @@ def test_gated_matches_64_bits(M, D, F, dt, name, bias, device):
 
 
 E4M3_SIZES = [(1, 16, 1), (5, 64, 33), (32, 768, 100), (33, 144, 65), (64, 1000, 96), (65, 128, 64), (100, 272, 127),
-              (129, 4096, 129), (300, 768, 1000), (3000, 256, 2100), (200, 33, 70)]
+              (129, 4096, 129), (300, 768, 1000), (3000, 256, 2100), (200, 33, 70), (679, 72, 5466)]
 
 
 @pytest.mark.parametrize("M,D,F", E4M3_SIZES, ids=["-".join(map(str, s)) for s in E4M3_SIZES])

@@ -229,7 +229,66 @@ def test_gated_workspace():
     assert size(8192, 4096, 11264, 0, 1) == 2 * 8192 * 11264 * 2     # dg and du; enough tiles: no partial sums
     assert size(4, 64, 33, 0, 1) == 2 * 4 * 40 * 2 + -(2 * 4 * 40 * 2) % 256  # rows padded to 16 bytes
     assert size(4, 64, 33, 1, 1) > size(4, 64, 33, 0, 1)
-    assert size(8192, 768, 2048, 0, 1) > 2 * 8192 * 2048 * 2         # few tiles: the inner dimension is split
+    assert size(8192, 768, 2048, 0, 1) == 2 * 8192 * 2048 * 2
+    assert size(300, 768, 2048, 0, 1) > 2 * 300 * 2048 * 2           # few tiles: dx splits its inner dimension
+
+
+def split_of(rows, cols, turns, slabs, es, may_split):
+    """(128 x 128 tiles, splits): the rule of sparton_gated.hip once more."""
+    cdiv, best = lambda a, b: -(-a // b), None
+    for small in (0, 1):
+        b = 128 if small else 256
+        tiles = max(1, cdiv(rows, b) * cdiv(cols, b) * turns)
+        for n in range(1, (min(16, max(1, slabs // 4)) if may_split and tiles < 512 else 1) + 1):
+            per = max(1, cdiv(slabs, n))
+            splits = max(1, cdiv(slabs, per))
+            groups = tiles * splits
+            if splits != n and n > 1:
+                continue
+            alone = groups <= 256
+            slab = (1.95 if alone else 3.6) if es == 4 else (0.47 if alone else 0.9)
+            slab = slab if small else 7.3 if es == 4 else 1.45
+            time = cdiv(groups, 512 if small else 256) * (per * slab + (6.0 if small else 10.0))
+            if splits > 1:
+                time += 4.0 + rows * cols * turns * (8.0 * splits + 2.0) / 4.5e6
+            if best is None or time < best[0]:
+                best = (time, small == 1, splits)
+    return best[1:]
+
+
+def gated_kernels(M, D, F, dt):
+    """The kernels that a training step of these sizes launches: (product, type, 128 x 128 tiles, split)."""
+    cdiv, es = lambda a, b: -(-a // b), 4 if dt == "fp32" else 2
+    D += -D % (16 // es)
+    fwd = ("few", dt, M <= 32, False) if M <= 64 else ("fwd", dt, split_of(M, 2 * F, 1, cdiv(D * es, 128), es, False)[0], False)
+    dx, dw = split_of(M, D, 1, 2 * cdiv(F * es, 128), es, True), split_of(F, D, 2, cdiv(M * es, 128), es, True)
+    return {fwd, ("dx", dt, dx[0], dx[1] > 1), ("dw", dt, dw[0], dw[1] > 1)}
+
+
+def test_the_gated_cases_reach_every_kernel():
+    from test_gpu_gated import E4M3_SIZES, SIZES
+    every = {(p, dt, small, split) for p in ("dx", "dw") for dt in ("fp32", "bf16", "fp16") for small in (True, False)
+             for split in (True, False)}
+    every |= {(p, dt, small, False) for p in ("few", "fwd") for dt in ("fp32", "bf16", "fp16") for small in (True, False)}
+    got = set().union(*(gated_kernels(*s, dt) for s in SIZES for dt in ("fp32", "bf16", "fp16")))
+    assert got == every, every ^ got
+    bits8 = {("few", M <= 32) if M <= 64 else ("fwd", split_of(M, 2 * F, 1, -(-(D + -D % 16) // 128), 1, False)[0])
+             for M, D, F in E4M3_SIZES}
+    assert bits8 == {(p, small) for p in ("few", "fwd") for small in (True, False)}
+
+
+def test_the_rule_above_is_the_librarys():
+    """The workspace tells how the inner dimensions are split."""
+    from test_gpu_gated import CASES, SIZES
+    cdiv, up = lambda a, b: -(-a // b), lambda n: n + -n % 256
+    for M, D, F, dt in [*((*s, dt) for s in SIZES for dt in ("fp32", "bf16")), *(c[:4] for c in CASES),
+                        (8192, 768, 2048, "bf16"), (512, 4096, 11264, "bf16"), (2048, 768, 1152, "fp16")]:
+        es = 4 if dt == "fp32" else 2
+        D, Fp = D + -D % (16 // es), F + -F % (16 // es)
+        dx, dw = split_of(M, D, 1, 2 * cdiv(F * es, 128), es, True)[1], split_of(F, D, 2, cdiv(M * es, 128), es, True)[1]
+        part = max(up(dx * M * D * 4) if dx > 1 else 0, up(dw * 2 * F * D * 4) if dw > 1 else 0)
+        got = _lib.load().sparton_gated_workspace_bytes(M, D, F, 0, ("fp32", "bf16", "fp16").index(dt))
+        assert got == up(2 * M * Fp * es) + part, (M, D, F, dt)
 
 
 X, W = torch.zeros(3, 8), torch.zeros(6, 8)
