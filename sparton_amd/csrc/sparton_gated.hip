@@ -493,97 +493,115 @@ __global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a)
 }
 
 // ---- few rows -----------------------------------------------------------------------------
-// Up to 64 rows: bound by reading the weights. A workgroup has 32 gate and 32 up rows; its waves share the inner
-// dimension, each with its operands straight from memory into registers, kAhead steps ahead, and their sums are
-// added in wave order in LDS.
-constexpr int kFewWaves = 8;
+// Up to 64 rows: bound by reading the weights. A workgroup has 16 gate and 16 up rows; its four waves share the inner
+// dimension, each with its operands straight from memory into registers, a slab of 128 bytes ahead, and their
+// sums are added in wave order in LDS. A slab's loads are issued together: each takes 16 rows' lines in part, and
+// those that follow find them on their way. What is in flight has to fit the L1, or lines are fetched again. Four rows,
+// D = 4096, F = 11264, bf16, one, two and three slabs ahead: 36.1, 38.6 and 61.4 us (5.1 TB/s, as a copy); eight waves and
+// one slab 38.4; 32 columns a workgroup by 32-wide products with four steps of 32 bytes ahead 70.
+constexpr int kFewWaves = 4;
+constexpr int kFewCols = 16;
+
+// 16 x 16 results: lane l holds row (column) l % 16 and, of each 64 bytes of the inner dimension, quarter l / 16 (8 bits:
+// of each 128).
+__device__ __forceinline__ void mma16(f32x4& d, const Frag<bf16>& a, const Frag<bf16>& b) {
+  d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.c[0]), __builtin_bit_cast(bf16x8, b.c[0]), d, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(f32x4& d, const Frag<f16>& a, const Frag<f16>& b) {
+  d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.c[0]), __builtin_bit_cast(f16x8, b.c[0]), d, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(f32x4& d, const Frag<float>& a, const Frag<float>& b) {
+  const f32x4 x = __builtin_bit_cast(f32x4, a.c[0]), y = __builtin_bit_cast(f32x4, b.c[0]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) d = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], d, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(f32x4& d, const Frag<e4m3>& a, const Frag<e4m3>& b) {
+  d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a), wide(b), d, 0, 0, 0, 0, 0, 0);
+}
 
 template <typename T, typename O, int JQ>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void gated_few_kernel(Params a) {
-  constexpr int EPC = 16 / sizeof(T), KSTEP = 2 * EPC * kCh<T>;  // elements of a step
-  constexpr int kAhead = 4 / kCh<T>;
-  __shared__ float sums[kFewWaves * JQ * 2 * 16 * 64];  // [wave][block][gate, up][register][lane]
-  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  constexpr int STEPS = 2 / kCh<T>, E = sizeof(T);  // of a slab
+  __shared__ float sums[kFewWaves][JQ][2][4][64];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, quarter = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t f0 = (int64_t)blockIdx.x * 32, f = min(f0 + l32, a.p.n - 1);
+  const int64_t f0 = (int64_t)blockIdx.x * kFewCols, f = min(f0 + l16, a.p.n - 1);
   const char* wg = a.p.b0 + f * a.p.ld;
   const char* wu = a.p.b1 + f * a.p.ld;
   const char* x[JQ];
 #pragma unroll
-  for (int i = 0; i < JQ; ++i) x[i] = a.q.b0 + min((int64_t)(i * 32 + l32), a.q.n - 1) * a.q.ld;
-  const int steps = (int)cdiv(a.K, KSTEP), per = (steps + kFewWaves - 1) / kFewWaves;
-  const int s1 = min(steps, (w + 1) * per);
-  f32x16 ag[JQ], au[JQ];
+  for (int i = 0; i < JQ; ++i) x[i] = a.q.b0 + min((int64_t)(i * 16 + l16), a.q.n - 1) * a.q.ld;
+  const int64_t row = a.K * E;  // bytes
+  const int slabs = (int)cdiv(row, kSlab), per = (slabs + kFewWaves - 1) / kFewWaves, s0 = w * per, s1 = min(slabs, s0 + per);
+  f32x4 ag[JQ], au[JQ];
 #pragma unroll
-  for (int i = 0; i < JQ; ++i)
+  for (int i = 0; i < JQ; ++i) ag[i] = au[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  Frag<T> fg[STEPS], fu[STEPS], fx[STEPS][JQ];
+  const auto load = [&](int s) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) ag[i][e] = au[i][e] = 0.0f;
-  Frag<T> fg[kAhead], fu[kAhead], fx[kAhead][JQ];
-  const auto load = [&](int slot, int s) {
+    for (int t = 0; t < STEPS; ++t)
 #pragma unroll
-    for (int c = 0; c < kCh<T>; ++c) {
-      const int64_t k = (int64_t)s * KSTEP + (2 * c + h) * EPC;
-      const bool in = s < s1 && k < a.K;
-      const int64_t o = (in ? k : 0) * (int64_t)sizeof(T);
-      const u32x4 zero = {0, 0, 0, 0};
-      const u32x4 vg = *(const u32x4*)(wg + o), vu = *(const u32x4*)(wu + o);
-      fg[slot].c[c] = in ? vg : zero;
-      fu[slot].c[c] = in ? vu : zero;
+      for (int c = 0; c < kCh<T>; ++c) {
+        const int64_t at = (int64_t)s * kSlab + (kCh<T> == 1 ? t * 64 + quarter * 16 : quarter * 32 + c * 16);
+        const bool in = s < s1 && at < row;
+        const int64_t o = in ? at : 0;
+        const u32x4 zero = {0, 0, 0, 0}, vg = *(const u32x4*)(wg + o), vu = *(const u32x4*)(wu + o);
+        fg[t].c[c] = in ? vg : zero;
+        fu[t].c[c] = in ? vu : zero;
 #pragma unroll
-      for (int i = 0; i < JQ; ++i) {
-        const u32x4 vx = *(const u32x4*)(x[i] + o);
-        fx[slot][i].c[c] = in ? vx : zero;
+        for (int i = 0; i < JQ; ++i) {
+          const u32x4 vx = *(const u32x4*)(x[i] + o);
+          fx[t][i].c[c] = in ? vx : zero;
+        }
       }
-    }
   };
-  const int s0 = w * per;
+  load(s0);
+  for (int s = s0; s < s1; ++s) {
+    Frag<T> g[STEPS], u[STEPS], v[STEPS][JQ];
 #pragma unroll
-  for (int n = 0; n < kAhead; ++n) load(n, s0 + n);
-  for (int s = s0; s < s1; s += kAhead) {
+    for (int t = 0; t < STEPS; ++t) {
+      g[t] = fg[t];
+      u[t] = fu[t];
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) {
-      // steps past s1 multiply zeros
+      for (int i = 0; i < JQ; ++i) v[t][i] = fx[t][i];
+    }
+    load(s + 1);
+#pragma unroll
+    for (int t = 0; t < STEPS; ++t)
 #pragma unroll
       for (int i = 0; i < JQ; ++i) {
-        mma(ag[i], fg[n], fx[n][i]);
-        mma(au[i], fu[n], fx[n][i]);
+        mma16(ag[i], g[t], v[t][i]);
+        mma16(au[i], u[t], v[t][i]);
       }
-      load(n, s + kAhead + n);
-    }
   }
 #pragma unroll
   for (int i = 0; i < JQ; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      sums[(((w * JQ + i) * 2 + 0) * 16 + e) * 64 + lane] = ag[i][e];
-      sums[(((w * JQ + i) * 2 + 1) * 16 + e) * 64 + lane] = au[i][e];
-    }
-  __syncthreads();
-  // Wave w takes registers 4 (w % 4) .. + 3 of block w / 4.
-  for (int o = w; o < JQ * 4; o += kFewWaves) {
-    const int i = o >> 2, r = o & 3;
-    f32x4 g, u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      float sg = 0.0f, su = 0.0f;
-#pragma unroll
-      for (int v = 0; v < kFewWaves; ++v) {
-        sg += sums[(((v * JQ + i) * 2 + 0) * 16 + 4 * r + e) * 64 + lane];
-        su += sums[(((v * JQ + i) * 2 + 1) * 16 + 4 * r + e) * 64 + lane];
-      }
-      g[e] = sg;
-      u[e] = su;
+      sums[w][i][0][e][lane] = ag[i][e];
+      sums[w][i][1][e][lane] = au[i][e];
     }
-    Columns<T, O> cols;
-    cols.init(a, f0 + 8 * r + 4 * h);
-    const int64_t row = i * 32 + l32;
-    if (row >= a.q.n || cols.left <= 0) continue;
-    const uint32_t to = (uint32_t)(row * a.p.n + cols.col);  // 64 rows of up to 2^20
-    const float sx = sizeof(T) == 1 ? a.sx[row] : 1.0f;
-    with_activation(a.act, [&](auto act) {
-      cols.template write<decltype(act)::value, false>((O*)a.h, a.g, a.u, to, sx, g, u);
-    });
+  __syncthreads();
+  if (w >= JQ) return;  // wave w ends block w
+  f32x4 g, u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    g[e] = u[e] = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) {
+      g[e] += sums[v][w][0][e][lane];
+      u[e] += sums[v][w][1][e][lane];
+    }
   }
+  Columns<T, O> cols;
+  cols.init(a, f0 + 4 * quarter);
+  const int64_t m = w * 16 + l16;
+  if (m >= a.q.n || cols.left <= 0) return;
+  const uint32_t to = (uint32_t)(m * a.p.n + cols.col);  // 64 rows of up to 2^20
+  const float sx = sizeof(T) == 1 ? a.sx[m] : 1.0f;
+  with_activation(a.act, [&](auto act) {
+    cols.template write<decltype(act)::value, false>((O*)a.h, a.g, a.u, to, sx, g, u);
+  });
 }
 
 // ---- dg and du ----------------------------------------------------------------------------
@@ -668,7 +686,9 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict
 
 // ---- launches -----------------------------------------------------------------------------
 constexpr int kCus = 256;
-constexpr int64_t kFewRows = 64;
+// Rows that the kernel for few of them takes: 64, or 32 where the weights are large. bf16, its times and the tiles':
+// D = 4096, F = 11264: 32 rows 55 and 54 us, 64 rows 76 and 54; D = 1024, F = 4096: 64 rows 9.7 and 12.2.
+constexpr int64_t kFewRows = 64, kFewRowsLarge = 32, kLargeWeight = 1 << 23;
 constexpr int kBiasBlocks = 256;
 
 struct Split {
@@ -737,10 +757,11 @@ int check(int64_t M, int64_t D, int64_t F, int dtype, int64_t es, int act) {
 
 template <typename T, typename O> int forward(Params& p, hipStream_t st) {
   p.turns = 1;
-  if (p.q.n <= kFewRows) {
-    const dim3 grid((unsigned)cdiv(p.p.n, 32)), block(64 * kFewWaves);
-    if (p.q.n <= 32) hipLaunchKernelGGL((gated_few_kernel<T, O, 1>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((gated_few_kernel<T, O, 2>), grid, block, 0, st, p);
+  if (p.q.n <= (p.p.n * p.K > kLargeWeight ? kFewRowsLarge : kFewRows)) {
+    const dim3 grid((unsigned)cdiv(p.p.n, kFewCols)), block(64 * kFewWaves);
+    if (p.q.n <= 16) hipLaunchKernelGGL((gated_few_kernel<T, O, 1>), grid, block, 0, st, p);
+    else if (p.q.n <= 32) hipLaunchKernelGGL((gated_few_kernel<T, O, 2>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((gated_few_kernel<T, O, 4>), grid, block, 0, st, p);
     return (int)hipGetLastError();
   }
   const int64_t slabs = cdiv(p.K * (int64_t)sizeof(T), kSlab);

@@ -256,11 +256,16 @@ def split_of(rows, cols, turns, slabs, es, may_split):
     return best[1:]
 
 
+def few(M):
+    """Blocks of 16 rows of the kernel for few of them."""
+    return 1 if M <= 16 else 2 if M <= 32 else 4
+
+
 def gated_kernels(M, D, F, dt):
     """The kernels that a training step of these sizes launches: (product, type, 128 x 128 tiles, split)."""
     cdiv, es = lambda a, b: -(-a // b), 4 if dt == "fp32" else 2
     D += -D % (16 // es)
-    fwd = ("few", dt, M <= 32, False) if M <= 64 else ("fwd", dt, split_of(M, 2 * F, 1, cdiv(D * es, 128), es, False)[0], False)
+    fwd = ("few", dt, few(M), False) if M <= (32 if F * D > 1 << 23 else 64) else ("fwd", dt, split_of(M, 2 * F, 1, cdiv(D * es, 128), es, False)[0], False)
     dx, dw = split_of(M, D, 1, 2 * cdiv(F * es, 128), es, True), split_of(F, D, 2, cdiv(M * es, 128), es, True)
     return {fwd, ("dx", dt, dx[0], dx[1] > 1), ("dw", dt, dw[0], dw[1] > 1)}
 
@@ -269,12 +274,13 @@ def test_the_gated_cases_reach_every_kernel():
     from test_gpu_gated import E4M3_SIZES, SIZES
     every = {(p, dt, small, split) for p in ("dx", "dw") for dt in ("fp32", "bf16", "fp16") for small in (True, False)
              for split in (True, False)}
-    every |= {(p, dt, small, False) for p in ("few", "fwd") for dt in ("fp32", "bf16", "fp16") for small in (True, False)}
+    every |= {("fwd", dt, small, False) for dt in ("fp32", "bf16", "fp16") for small in (True, False)}
+    every |= {("few", dt, blocks, False) for dt in ("fp32", "bf16", "fp16") for blocks in (1, 2, 4)}
     got = set().union(*(gated_kernels(*s, dt) for s in SIZES for dt in ("fp32", "bf16", "fp16")))
     assert got == every, every ^ got
-    bits8 = {("few", M <= 32) if M <= 64 else ("fwd", split_of(M, 2 * F, 1, -(-(D + -D % 16) // 128), 1, False)[0])
+    bits8 = {("few", few(M)) if M <= 64 else ("fwd", split_of(M, 2 * F, 1, -(-(D + -D % 16) // 128), 1, False)[0])
              for M, D, F in E4M3_SIZES}
-    assert bits8 == {(p, small) for p in ("few", "fwd") for small in (True, False)}
+    assert bits8 == {("fwd", True), ("fwd", False), ("few", 1), ("few", 2), ("few", 4)}
 
 
 def test_the_rule_above_is_the_librarys():
