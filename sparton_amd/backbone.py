@@ -1,27 +1,34 @@
 """A transformers backbone's attention and norms on the framework's kernels.
 
-    use_in_backbone(model)
+    use_in_backbone(model, rms_norm=False, feed_forward=False, embedding=False)
 
 switches a transformers model in place: its attention to `sparton_amd.attention` (through the
 library's own registry of attention implementations, under the name "sparton"), its LayerNorms to
 `SpartonLayerNorm`, and the output blocks of BERT, RoBERTa and XLM-RoBERTa layers to the norm with
 the residual sum inside. Parameters, their names and the state_dict stay as they are. The families are
 the reference's (training/model.py:14-40): bert, distilbert, roberta, xlm-roberta; decoder-only
-backbones whose attention goes through the same registry run causal.
+backbones whose attention goes through the same registry run causal. Asked for, the rest of such a backbone's
+layer is switched too: root-mean-square norms to `SpartonRMSNorm` (and layers that add their attention's output
+and norm the sum to the norm that does both), gated feed-forward blocks to `gated_linear`, embeddings to
+`SpartonEmbedding`. Whether a module computes what the kernels do is found by running a small copy of it on
+the CPU; one that does not keeps its own forward.
 
 What the kernels do not compute is refused when it is asked for, never approximated: dropout on the
 attention probabilities, sliding windows, position biases, masks that are not one value per key.
 """
 from __future__ import annotations
 
+import copy
 import functools
-from typing import Optional
+from typing import Callable, Dict, Optional
 
 import torch
 from torch import Tensor, nn
 
+from . import feed_forward as _ff
 from .attention import KEY_MASK_DTYPES, attention
-from .norm import SpartonLayerNorm
+from .embedding import SpartonEmbedding
+from .norm import SpartonLayerNorm, SpartonRMSNorm
 
 NAME = "sparton"
 # dense -> dropout -> LayerNorm(. + input): the output blocks of an encoder layer.
@@ -95,20 +102,132 @@ class _BlockForward(functools.partial):
         return self.args[0]
 
 
-def use_in_backbone(model: nn.Module) -> nn.Module:
+def _gated_block(self, x: Tensor) -> Tensor:
+    gate, up = self.gate_proj, self.up_proj
+    h = _ff.gated_linear(x, gate.weight, up.weight, gate.bias, up.bias, _ff.activation_name(self.act_fn))
+    return self.down_proj(h)
+
+
+def _pre_norm_layer(self, hidden_states: Tensor, **kwargs) -> Tensor:
+    attended = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **kwargs)[0]
+    hidden_states, residual = self.post_attention_layernorm(attended, hidden_states)
+    return residual + self.mlp(hidden_states)
+
+
+# ---- what a module computes: a small copy of it, on the CPU, against the formula -------------
+
+class _Times(nn.Module):
+    """Stands for a submodule: what goes through it is seen in the result."""
+
+    def __init__(self, factor: float):
+        super().__init__()
+        self.factor = factor
+
+    def forward(self, x):
+        return x * self.factor
+
+
+class _Attended(nn.Module):
+    def forward(self, hidden_states, **kwargs):
+        return hidden_states * 3.0, None
+
+
+def _computes(module: nn.Module, children: Dict[str, nn.Module], x: Tensor, want: Callable[[], Tensor]) -> bool:
+    """Whether the class's forward, on a copy with these submodules instead, gives `want` for x."""
+    probe = copy.copy(module)
+    probe._modules, probe.training = dict(children), False
+    try:
+        with torch.no_grad():
+            got = type(module).forward(probe, x)
+            return isinstance(got, Tensor) and bool(torch.allclose(got, want(), rtol=1e-4, atol=1e-5))
+    except Exception:  # whatever it is, it is not what the kernels compute
+        return False
+
+
+def _is_rms_norm(m: nn.Module) -> bool:
+    if isinstance(m, SpartonRMSNorm) or not type(m).__name__.endswith("RMSNorm") or list(m._parameters) != ["weight"]:
+        return False
+    weight, eps = m.weight, getattr(m, "variance_epsilon", getattr(m, "eps", None))
+    if weight is None or weight.dim() != 1 or not isinstance(eps, float):
+        return False
+    g = torch.Generator().manual_seed(0)
+    n = weight.shape[0]
+    x, w = torch.randn(3, n, generator=g), torch.rand(n, generator=g) + 0.5
+    probe = copy.copy(m)
+    probe._parameters = {"weight": nn.Parameter(w)}
+    return _computes(probe, {}, x, lambda: w * x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps))
+
+
+def _is_gated_block(m: nn.Module) -> bool:
+    """down_proj(act_fn(gate_proj(x)) * up_proj(x)) of plain linears, and nothing else in it."""
+    if set(m._modules) != {"gate_proj", "up_proj", "down_proj", "act_fn"} or m._parameters or m._buffers:
+        return False
+    name, linears = _ff.activation_name(m.act_fn), (m.gate_proj, m.up_proj, m.down_proj)
+    if name is None or any(type(t) is not nn.Linear for t in linears) or linears[0].weight.shape != linears[1].weight.shape:
+        return False
+    small = [nn.Linear(4, 6), nn.Linear(4, 6), nn.Linear(6, 4)]
+    x = torch.linspace(-2, 2, 12).view(3, 4)
+    act = {"silu": nn.functional.silu, "gelu": nn.functional.gelu, "relu": torch.relu,
+           "gelu_tanh": lambda t: nn.functional.gelu(t, approximate="tanh")}[name]
+    return _computes(m, dict(zip(("gate_proj", "up_proj", "down_proj"), small), act_fn=m.act_fn), x,
+                     lambda: small[2](act(small[0](x)) * small[1](x)))
+
+
+def _is_pre_norm_layer(m: nn.Module) -> bool:
+    """h = x + self_attn(input_layernorm(x)); h + mlp(post_attention_layernorm(h))."""
+    names = ("input_layernorm", "self_attn", "post_attention_layernorm", "mlp")
+    if set(m._modules) != set(names) or m._parameters or m._buffers:
+        return False
+    x = torch.linspace(-1, 1, 12).view(1, 3, 4)
+    children = dict(zip(names, (_Times(2.0), _Attended(), _Times(5.0), _Times(7.0))))
+    return _computes(m, children, x, lambda: 36.0 * (x * 7.0))  # x + 3 * 2 x, and 1 + 5 * 7 times that
+
+
+def use_in_backbone(model: nn.Module, *, rms_norm: bool = False, feed_forward: bool = False,
+                    embedding: bool = False) -> nn.Module:
     """Switch a transformers model (or a masked LM with its head) in place; returns it. A model that
-    cannot be switched raises and stays as it was."""
+    cannot be switched, or that has nothing of a kind that is asked for, raises and stays as it was."""
     norms = [(module, name, SpartonLayerNorm.of(child)) for module in model.modules()
              for name, child in module.named_children()
              if type(child) is nn.LayerNorm and len(child.normalized_shape) == 1 and child.weight is not None]
+    modules = list(model.modules())
+    children = [(module, name, child) for module in modules for name, child in module.named_children()]
+    made: Dict[int, nn.Module] = {}  # a module in several places becomes one
+
+    def replaced(child: nn.Module, make) -> nn.Module:
+        if id(child) not in made:
+            made[id(child)] = make(child)
+        return made[id(child)]
+
+    forwards = []
+    if rms_norm:
+        found = [(m, n, replaced(c, SpartonRMSNorm.of)) for m, n, c in children if _is_rms_norm(c)]
+        if not found and not any(isinstance(m, SpartonRMSNorm) for m in modules):
+            raise ValueError(f"{type(model).__name__} has no root-mean-square norm that the kernels compute")
+        norms += found
+        ours = {id(c) for _, _, c in children if isinstance(c, SpartonRMSNorm) or id(c) in made}
+        forwards += [(m, _pre_norm_layer) for m in modules if "forward" not in m.__dict__ and _is_pre_norm_layer(m)
+                     and id(m.post_attention_layernorm) in ours]
+    if feed_forward:
+        blocks = [m for m in modules if _is_gated_block(m)]
+        if not blocks:
+            raise ValueError(f"{type(model).__name__} has no gated feed-forward block that the kernels compute")
+        forwards += [(m, _gated_block) for m in blocks if "forward" not in m.__dict__]
+    if embedding:
+        found = [(m, n, replaced(c, SpartonEmbedding.of)) for m, n, c in children if type(c) is nn.Embedding]
+        if not found and not any(isinstance(m, SpartonEmbedding) for m in modules):
+            raise ValueError(f"{type(model).__name__} has no nn.Embedding")
+        norms += found
     register()
     before = model.config._attn_implementation
     model.set_attn_implementation(NAME)
     if model.config._attn_implementation != NAME:
         model.set_attn_implementation(before)
         raise ValueError(f"{type(model).__name__} does not take its attention from transformers' registry")
-    for module, name, norm in norms:
-        setattr(module, name, norm)
+    for module, name, child in norms:
+        setattr(module, name, child)
+    for module, forward in forwards:
+        module.forward = _BlockForward(forward, module)
     for module in model.modules():
         if type(module).__name__ in _RESIDUAL_BLOCKS and isinstance(module.LayerNorm, SpartonLayerNorm):
             module.forward = _BlockForward(_residual_norm, module)
