@@ -14,9 +14,9 @@
 // without a token are zeroed by other waves of the first launch, so every row is written once and d table needs no
 // clearing. No atomics: results are bitwise reproducible.
 //
-// The sort ranks each key among its wave's 64, then among 4 x 64, 4 x 256 (LDS) and 16 x 1024, 16 x 16384, ...
-// (memory): a key's rank is its own place in its list and, by binary search, the number of keys before it in each
-// of the others. No counts, no scans, one launch to 1024 keys and another for each factor of 16.
+// The sort ranks each key among its wave's 64, then among 4 x 64 and 4 x 256, in a second launch among 32 x 1024 (all in
+// LDS), and in further ones among 16 x 32768, ... (memory): a key's rank is its own place in its list and, by binary
+// search, the number of keys before it in each of the others. No counts and no scans.
 
 #include <algorithm>
 
@@ -29,7 +29,8 @@ namespace emb {
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;           // forward: vectors of a thread
 constexpr int kTile = 1024;          // keys that one workgroup sorts
-constexpr int kWays = 16;            // lists that a merge launch joins into one
+constexpr int kTileWays = 32;        // tiles that the first merge launch joins into one run, in LDS
+constexpr int kWays = 16;            // runs that a later one joins
 constexpr int kChunk = 32;           // sorted entries of a wave
 constexpr int kInFlight = 8;
 constexpr int kJoinWaves = 4;
@@ -145,18 +146,19 @@ __global__ __launch_bounds__(kTile) void embed_sort_kernel(const void* __restric
   }
 }
 
-// The place, in its group of up to kWays runs of `run` ascending keys each, that key i of the group goes to when the
+// The place, in its group of up to WAYS runs of `run` ascending keys each, that key i of the group goes to when the
 // group becomes one run; `keys` are the group's `count`. The searches step together and read without a branch, so that
 // their reads are in flight at once; what a search reads past the group's end, it reads from its last key and drops.
-template <typename P, typename I> __device__ __forceinline__ I merged_place(P keys, uint32_t key, I i, I count, I run) {
+template <int WAYS, typename P, typename I>
+__device__ __forceinline__ I merged_place(P keys, uint32_t key, I i, I count, I run) {
   const I own = i / run;
   const int lists = __builtin_amdgcn_readfirstlane((int)cdiv(count, run));  // the same for the whole workgroup
-  I lo[kWays];
+  I lo[WAYS];
 #pragma unroll
-  for (int w = 0; w < kWays; ++w) lo[w] = 0;
+  for (int w = 0; w < WAYS; ++w) lo[w] = 0;
   for (I step = run; step > 0; step >>= 1) {
 #pragma unroll
-    for (int w0 = 0; w0 < kWays; w0 += 4) {
+    for (int w0 = 0; w0 < WAYS; w0 += 4) {
       if (w0 >= lists) continue;
 #pragma unroll
       for (int w = w0; w < w0 + 4; ++w) {
@@ -168,7 +170,7 @@ template <typename P, typename I> __device__ __forceinline__ I merged_place(P ke
   }
   I rank = i - own * run;
 #pragma unroll
-  for (int w = 0; w < kWays; ++w) rank += w == own ? 0 : lo[w];
+  for (int w = 0; w < WAYS; ++w) rank += w == own ? 0 : lo[w];
   return rank;
 }
 
@@ -177,22 +179,29 @@ __global__ __launch_bounds__(kThreads) void embed_merge_tiles_kernel(const uint3
                                                                      const uint32_t* __restrict__ places, int N,
                                                                      uint32_t* __restrict__ keys_out,
                                                                      uint32_t* __restrict__ places_out) {
-  __shared__ uint32_t all[kTile * kWays];
+  __shared__ uint32_t all[kTile * kTileWays];
   const int64_t first = (int64_t)blockIdx.x * kThreads, i = first + threadIdx.x;
-  const int64_t base = first / (kTile * kWays) * (kTile * kWays);
-  const int count = (int)min((int64_t)kTile * kWays, N - base);
-  // Sixteen vectors a thread, all on their way before the first is stored; past the last key, the last vector again.
-  constexpr int VECS = kTile * kWays / 4 / kThreads;
-  u32x4 v[VECS];
+  const int64_t base = first / (kTile * kTileWays) * (kTile * kTileWays);
+  const int count = (int)min((int64_t)kTile * kTileWays, N - base);
+  // A tile is one vector a thread. All are on their way before the first is stored; past the last key, the last vector
+  // again, and from the first whole four tiles past it, none.
+  static_assert(kTile == 4 * kThreads, "a vector a thread");
+  u32x4 v[kTileWays];
 #pragma unroll
-  for (int n = 0; n < VECS; ++n) v[n] = *(const u32x4*)(keys + base + min((n * kThreads + (int)threadIdx.x) * 4, (count - 1) & ~3));
+  for (int n0 = 0; n0 < kTileWays; n0 += 4)
+    if (n0 * kTile < count)
 #pragma unroll
-  for (int n = 0; n < VECS; ++n) *(u32x4*)(all + (n * kThreads + threadIdx.x) * 4) = v[n];
+      for (int n = n0; n < n0 + 4; ++n) v[n] = *(const u32x4*)(keys + base + min((n * kThreads + (int)threadIdx.x) * 4, (count - 1) & ~3));
   const uint32_t place = i < N ? places[i] : 0u;
+#pragma unroll
+  for (int n0 = 0; n0 < kTileWays; n0 += 4)
+    if (n0 * kTile < count)
+#pragma unroll
+      for (int n = n0; n < n0 + 4; ++n) *(u32x4*)(all + (n * kThreads + threadIdx.x) * 4) = v[n];
   __syncthreads();
   if (i >= N) return;
   const uint32_t key = all[i - base];
-  const int64_t to = base + merged_place<const uint32_t*, int>(all, key, (int)(i - base), count, kTile);
+  const int64_t to = base + merged_place<kTileWays, const uint32_t*, int>(all, key, (int)(i - base), count, kTile);
   keys_out[to] = key;
   places_out[to] = place;
 }
@@ -205,7 +214,7 @@ __global__ __launch_bounds__(kThreads) void embed_merge_kernel(const uint32_t* _
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (i >= N) return;
   const int64_t group = (int64_t)run * kWays, base = i / group * group;
-  const int64_t to = base + merged_place<const uint32_t*, int64_t>(keys + base, keys[i], i - base, min(group, N - base), run);
+  const int64_t to = base + merged_place<kWays, const uint32_t*, int64_t>(keys + base, keys[i], i - base, min(group, N - base), run);
   keys_out[to] = keys[i];
   places_out[to] = places[i];
 }
@@ -456,7 +465,7 @@ SPARTON_EXPORT int sparton_embedding_bwd(const void* ids, int ids_dtype, const v
                        ids_dtype, (int)N, V, padding_idx, k[0], at[0]);
     int in = 0;
     const dim3 grid((unsigned)cdiv(N, emb::kThreads)), block(emb::kThreads);
-    for (int64_t run = emb::kTile; run < N; run *= emb::kWays, in ^= 1) {
+    for (int64_t run = emb::kTile; run < N; run *= run == emb::kTile ? emb::kTileWays : emb::kWays, in ^= 1) {
       if (run == emb::kTile)
         hipLaunchKernelGGL(emb::embed_merge_tiles_kernel, grid, block, 0, st, k[in], at[in], (int)N, k[in ^ 1], at[in ^ 1]);
       else

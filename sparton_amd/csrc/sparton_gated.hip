@@ -405,11 +405,12 @@ __global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a)
       if (last) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NP) : "memory");
 #pragma unroll
       for (int n = 0; n < MMAS; ++n) {
-        // next step's operands, evenly between the products, and copies likewise
+        // next step's operands beside the first half of the products, and copies evenly
+        constexpr int AT_ONCE = (2 * READS + MMAS - 1) / MMAS;
 #pragma unroll
-        for (int i = 0; i < (READS + MMAS - 1) / MMAS; ++i)
-          if (n * READS / MMAS + i < (n + 1) * READS / MMAS)
-            read((s + 1) & 1, n * READS / MMAS + i, last ? 0 : s + 1, last ? q1 : q0, last ? p1 : p0);
+        for (int i = 0; i < AT_ONCE; ++i)
+          if (n * AT_ONCE + i < READS)
+            read((s + 1) & 1, n * AT_ONCE + i, last ? 0 : s + 1, last ? q1 : q0, last ? p1 : p0);
         constexpr int EARLY = (STEPS - 1) * MMAS;
         const int m = s * MMAS + n;
 #pragma unroll

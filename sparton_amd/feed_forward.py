@@ -150,12 +150,8 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tenso
     return _eager.load().gated(x, w_gate, w_up, b_gate, b_up, code)
 
 
-@torch.library.custom_op("sparton::gated_8bit", mutates_args=())
-def gated_8bit(x: Tensor, x_scale: Tensor, w_gate: Tensor, gate_scale: Tensor, w_up: Tensor, up_scale: Tensor,
-               activation: str, out_dtype: torch.dtype) -> Tensor:
-    """gated_linear_8bit, without a gradient."""
-    op = "sparton::gated_8bit"
-    code = _code(activation, op)
+def _check_8bit(x: Tensor, x_scale: Tensor, w_gate: Tensor, gate_scale: Tensor, w_up: Tensor, up_scale: Tensor,
+                out_dtype: torch.dtype, op: str) -> None:
     _D, width = _check_shapes(x, w_gate, w_up, op)
     for t in (x, w_gate, w_up):
         if t.dtype != _E4M3:
@@ -166,6 +162,15 @@ def gated_8bit(x: Tensor, x_scale: Tensor, w_gate: Tensor, gate_scale: Tensor, w
         if tuple(t.shape) != shape or t.dtype != torch.float32:
             raise ValueError(f"{op}: a scale a row is float32 {shape}, got {t.dtype} {tuple(t.shape)}")
     _require_device(x, (x_scale, w_gate, gate_scale, w_up, up_scale), op)
+
+
+@torch.library.custom_op("sparton::gated_8bit", mutates_args=())
+def gated_8bit(x: Tensor, x_scale: Tensor, w_gate: Tensor, gate_scale: Tensor, w_up: Tensor, up_scale: Tensor,
+               activation: str, out_dtype: torch.dtype) -> Tensor:
+    """gated_linear_8bit, without a gradient."""
+    op = "sparton::gated_8bit"
+    code = _code(activation, op)
+    _check_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, out_dtype, op)
     return _eager.load().gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, code, out_dtype)
 
 
@@ -179,7 +184,11 @@ def gated_linear_8bit(x: Tensor, x_scale: Tensor, w_gate: Tensor, gate_scale: Te
     """act(g) * u of e4m3 rows: g = (x w_gate') x_scale gate_scale, u likewise, summed in fp32. x [..., D] and x_scale
     [...] as rms_norm_8bit gives them, weights [F, D] and scales [F] as quantize_rows does. For inference: there is no
     gradient."""
-    return torch.ops.sparton.gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation, out_dtype)
+    if torch.compiler.is_compiling() or not x.is_cuda:
+        return torch.ops.sparton.gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation, out_dtype)
+    code = _code(activation, "gated_linear_8bit")
+    _check_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, out_dtype, "gated_linear_8bit")
+    return _eager.load().gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, code, out_dtype)
 
 
 def quantize_rows(t: Tensor) -> Tuple[Tensor, Tensor]:

@@ -260,7 +260,12 @@ def rms_norm_8bit(x: Tensor, weight: Tensor, eps: float = 1e-6, residual: Option
     inputs that ask for a gradient are refused."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise ValueError("rms_norm_8bit has no gradient: call it under torch.no_grad()")
-    y, scale, h = torch.ops.sparton.rms_norm_8bit(x, residual, weight, float(eps))
+    eps = float(eps)
+    if torch.compiler.is_compiling() or not x.is_cuda:
+        y, scale, h = torch.ops.sparton.rms_norm_8bit(x, residual, weight, eps)
+    else:
+        _check(x, residual, weight, None, eps, "rms_norm_8bit")
+        y, scale, h = _eager.load().rms_norm_8bit(x, residual, weight, eps)
     return (y, scale) if residual is None else (y, scale, h)
 
 

@@ -80,7 +80,7 @@ CASES = [  # N, V, D, dtype, ids
     (1025, 2000, 768, "fp16", "down"), (2048, 30522, 384, "fp32", "tokens"), (5000, 30522, 768, "bf16", "tokens"),
     (4097, 512, 1023, "bf16", "up"), (3000, 10, 257, "fp32", "tokens"), (3001, 4000, 512, "fp16", "one"),
     (16384, 40, 72, "bf16", "halves"), (16385, 30522, 64, "bf16", "tokens"), (40000, 250002, 16, "fp16", "tokens"),
-    (70001, 33, 5, "fp32", "tokens"), (262145, 1000, 8, "bf16", "tokens"), (40, 300, 20000, "bf16", "tokens"),
+    (32768, 500, 16, "fp32", "down"), (32769, 500, 16, "bf16", "tokens"), (70001, 33, 5, "fp32", "tokens"), (262145, 1000, 8, "bf16", "tokens"), (40, 300, 20000, "bf16", "tokens"),
 ]
 
 
