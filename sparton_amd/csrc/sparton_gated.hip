@@ -246,8 +246,10 @@ struct Params {
   Side q, p;              // rows and columns of the result
   int64_t K;              // inner dimension of a half, in elements
   int half_slabs, slabs;  // of one half, and of all halves
-  int tq, tp, splits, per_split;
-  // plain results: rows [0, q.n) of out, or fp32 sums of each split; `turns` problems beside each other
+  int tq, tp;             // tiles of rows and columns
+  int whole;              // tiles that one workgroup makes; of the others, `splits` share the inner dimension
+  int splits, per_split;
+  // plain results: rows [0, q.n) of out; `turns` problems beside each other. part: [tile - whole][split][BQ][BP]
   void* out[2];
   const char* q_turn;
   float* part;
@@ -260,23 +262,38 @@ struct Params {
   int act;
 };
 
-// A workgroup's tile. Consecutive workgroups go to the eight XCDs in turn: each XCD takes a run of the tiles, which
-// walk kGroupQ row tiles before the next column tile, so that what is in flight shares operands in its L2.
+// A workgroup's tile. Tiles walk kGroupQ row tiles before the next column tile. Consecutive workgroups go to the eight
+// XCDs in turn: each XCD takes a run of the whole tiles, so that what it has in flight shares operands in its L2. The
+// workgroups that share tiles come last.
 struct Place {
-  int q, p, split, turn;
+  int q, p, split, turn, shared;  // shared: the tile's place among those that are, or -1
 };
-__device__ __forceinline__ Place place_of(const Params& a) {
-  const int tiles = a.tq * a.tp * a.splits * a.turns, w = blockIdx.x, x = w & 7, per = tiles >> 3, more = tiles & 7;
-  int i = x * per + min(x, more) + (w >> 3);
-  Place r;
-  r.turn = i / (a.tq * a.tp * a.splits);
-  i -= r.turn * a.tq * a.tp * a.splits;
-  r.split = i / (a.tq * a.tp);
-  i -= r.split * a.tq * a.tp;
+__device__ __forceinline__ Place tile_of(const Params& a, int i) {
+  Place r = {};
+  r.turn = i / (a.tq * a.tp);
+  i -= r.turn * a.tq * a.tp;
   const int group = i / (kGroupQ * a.tp), first = group * kGroupQ, rows = min(kGroupQ, a.tq - first);
   i -= first * a.tp;
   r.p = i / rows;
   r.q = first + i - r.p * rows;
+  return r;
+}
+// Workgroup w's place in n, an XCD's ones in a run.
+__device__ __forceinline__ int in_runs(int w, int n) {
+  const int x = w & 7, per = n >> 3, more = n & 7;
+  return x * per + min(x, more) + (w >> 3);
+}
+__device__ __forceinline__ Place place_of(const Params& a) {
+  const int w = blockIdx.x;
+  if (w < a.whole) {
+    Place r = tile_of(a, in_runs(w, a.whole));
+    r.shared = -1;
+    return r;
+  }
+  const int rest = a.tq * a.tp * a.turns - a.whole, j = in_runs(w - a.whole, rest * a.splits);  // `whole`: rounds of CUs
+  Place r = tile_of(a, a.whole + j % rest);
+  r.shared = j % rest;
+  r.split = j / rest;
   return r;
 }
 
@@ -367,7 +384,7 @@ __global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a)
     for (int j = 0; j < JP; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-  const int k0 = at.split * a.per_split, k_end = min(a.slabs, k0 + a.per_split);
+  const int k0 = at.shared < 0 ? 0 : at.split * a.per_split, k_end = at.shared < 0 ? a.slabs : min(a.slabs, k0 + a.per_split);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + w * 1024;
   typename Copy<T, QKM, BQ, NW, false>::Slab sq;
   typename Copy<T, PKM, BP, NW, GATED>::Slab sp;
@@ -475,7 +492,9 @@ __global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a)
     } else {
       const int64_t left = width - ((int64_t)at.p * BP + wp * COLS + c);
       const int64_t to = row0 * width + (int64_t)at.p * BP + wp * COLS;
-      const auto rows = [&](auto* out, auto whole) {
+      O* out = (O*)a.out[at.turn] + to;
+      float* part = a.part + (((int64_t)at.shared * a.splits + at.split) * BQ + (wq * JQ + i) * 32) * BP + wp * COLS;
+      const auto rows = [&](auto* out, uint32_t first, uint32_t step, auto whole) {
         typedef std::remove_pointer_t<decltype(out)> R;
 #pragma unroll 4
         for (int r = 0; r < 32 / ROWS; ++r) {
@@ -486,9 +505,9 @@ __global__ __launch_bounds__(64 * WQ * WP, OCC) void gated_gemm_kernel(Params a)
           store_n<R, CPL>(out + first + r * step, v, decltype(whole)::value ? CPL : left);
         }
       };
-      const auto either = [&](auto* out) { inside ? rows(out, std::true_type()) : rows(out, std::false_type()); };
-      if (a.splits > 1) either(a.part + ((int64_t)at.split * a.turns + at.turn) * a.q.n * width + to);
-      else either((O*)a.out[at.turn] + to);
+      if (at.shared >= 0) rows(part, r0 * BP + c, ROWS * BP, std::true_type());
+      else if (inside) rows(out, first, step, std::true_type());
+      else rows(out, first, step, std::false_type());
     }
   }
 }
@@ -661,28 +680,21 @@ __global__ __launch_bounds__(kActThreads) void gated_act_bwd_kernel(const T* __r
   }
 }
 
-// The splits' sums [split][turn][n] added in order, a turn a row of the grid: four elements a thread, four splits' loads
-// in flight.
-template <typename O>
-__global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict__ part, int splits, int64_t n, O* out0, O* out1) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, stride = n * gridDim.y;
-  if (i >= n) return;
-  const float* from = part + blockIdx.y * n + i;
-  O* out = (blockIdx.y == 0 ? out0 : out1) + i;
+// The shared tiles' sums added in the splits' order: 1024 elements of a tile a workgroup, four splits' loads in flight.
+template <typename O> __global__ __launch_bounds__(256) void gated_join_kernel(Params a, int B) {
+  const int per = B * B / 1024, tile = blockIdx.x / per, at = (blockIdx.x % per) * 1024 + threadIdx.x * 4;
+  const Place t = tile_of(a, a.whole + tile);
+  const int64_t row = (int64_t)t.q * B + at / B, col = (int64_t)t.p * B + at % B;
+  if (row >= a.q.n || col >= a.p.n) return;
+  const float* from = a.part + (int64_t)tile * a.splits * B * B + at;
   float v[4] = {};
-  if (i + 4 <= n) {
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
-      const vec_t<float, 4> p = load_any<float, 4>(from + k * stride);
+  for (int k = 0; k < a.splits; ++k) {
+    const f32x4 p = *(const f32x4*)(from + (int64_t)k * B * B);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += p[e];
-    }
-  } else {
-    for (int k = 0; k < splits; ++k)
-      for (int e = 0; e < 3; ++e)
-        if (i + e < n) v[e] += from[k * stride + e];
+    for (int e = 0; e < 4; ++e) v[e] += p[e];
   }
-  store_n<O, 4>(out, v, n - i);
+  store_n<O, 4>((O*)a.out[t.turn] + row * a.p.n + col, v, a.p.n - col);
 }
 
 // ---- launches -----------------------------------------------------------------------------
@@ -694,34 +706,41 @@ constexpr int kBiasBlocks = 256;
 
 struct Split {
   bool small;
-  int tq, tp, splits, per_split, slabs;
+  int tq, tp, whole, splits, per_split, slabs;
+  int64_t shared;  // tiles that are cut
+  size_t part_bytes() const { return (size_t)(shared * splits) * (small ? 128 * 128 : 256 * 256) * 4; }
 };
 
-// The tile and the number of workgroups that share a tile's inner dimension: what an estimate of the time says. A CU
-// holds one workgroup of 256 x 256 or two of 128 x 128. Microseconds a slab and a tile's start and end, as measured:
-//               256 x 256       128 x 128, one on its CU       two
-//     16 bits   1.45            0.47                           0.9
-//     fp32      7.3             1.95                           3.6
-//     around    10              6                              6
-// and a join of splits reads 4.5 MB a microsecond. bf16, dx of 8192 x 768 x 2048 (96 tiles of 256, 384 of 128): 256 82 us,
-// 128 57, and split in two 82 and 85. dx of 8192 x 4096 x 11264: 1098 and 1485. dx of 300 x 768 x 2048: 128 32, split in
-// four 16. dW of 8192 x 2048 x 2048: 178 and 145.
+// The tile, and into how many parts the inner dimension of the tiles is cut that do not fill the CUs a last time (for
+// few tiles, all of them): what an estimate of the time says. A CU holds one workgroup of 256 x 256 or two of 128 x 128.
+// Microseconds a slab and a tile's start and end, as measured:
+//               256 x 256, on every CU   on some   128 x 128, two on a CU   one
+//     16 bits   1.45                     1.3       0.9                      0.5
+//     fp32      7.3                      7.3       3.6                      1.95
+//     around    10                                 6
+// and a join writes and reads 6 MB a microsecond; what is split has to promise 3% more than that. bf16, dx of
+// 8192 x 768 x 2048: tiles of 256 80 us, in two parts 72; of 128 59, in two parts 80. dx of 5000 x 1024 x 3000: 113 and in
+// three parts 80; 94 and 93. dx of 300 x 768 x 2048: of 128 31, in four parts 14. dx of 8192 x 4096 x 11264: 1098 and 1485;
+// its dW, 1408 tiles of 256, 1218, the last 128 in two parts 1183.
 Split split_of(int64_t rows, int64_t cols, int64_t turns, int64_t slabs, int64_t es, bool may_split) {
   Split best = {};
   double least = -1.0;
   for (int small = 0; small < 2; ++small) {
-    const int64_t b = small ? 128 : 256, tq = cdiv(rows, b), tp = cdiv(cols, b), tiles = std::max<int64_t>(1, tq * tp * turns);
-    const int64_t most = may_split && tiles < 2 * kCus ? std::min<int64_t>(16, std::max<int64_t>(1, slabs / 4)) : 1;
-    for (int64_t n = 1; n <= most; ++n) {
-      const int64_t per = std::max<int64_t>(1, cdiv(slabs, n)), splits = std::max<int64_t>(1, cdiv(slabs, per)), groups = tiles * splits;
-      if (splits != n && n > 1) continue;
-      const bool alone = groups <= kCus;
-      const double slab = es == 4 ? (small ? (alone ? 1.95 : 3.6) : 7.3) : (small ? (alone ? 0.47 : 0.9) : 1.45);
-      double time = (double)cdiv(groups, small ? 2 * kCus : kCus) * ((double)per * slab + (small ? 6.0 : 10.0));
-      if (splits > 1) time += 4.0 + (double)(rows * cols * turns) * (8.0 * (double)splits + 2.0) / 4.5e6;
+    const int64_t b = small ? 128 : 256, slots = small ? 2 * kCus : kCus, tq = cdiv(rows, b), tp = cdiv(cols, b);
+    const int64_t tiles = tq * tp * turns, rest = tiles % slots;
+    const double around = small ? 6.0 : 10.0, all = es == 4 ? (small ? 3.6 : 7.3) : (small ? 0.9 : 1.45);
+    const double some = es == 4 ? (small ? 1.95 : 7.3) : (small ? 0.5 : 1.3);
+    const double full = (double)(tiles / slots) * ((double)slabs * all + around);
+    for (int64_t n = 1; n <= 16; ++n) {
+      const int64_t per = cdiv(slabs, n), groups = rest * n;
+      if (n > 1 && (!may_split || rest == 0 || slabs < 4 * n || cdiv(slabs, per) != n || groups > 2 * slots)) continue;
+      double time = full;
+      if (rest > 0)
+        time += (double)cdiv(groups, slots) * ((double)per * (groups < kCus || (small && groups == kCus) ? some : all) + around);
+      if (n > 1) time += 3.0 + 0.03 * time + (double)(rest * b * b) * (8.0 * (double)n + 2.0) / 6e6;
       if (least < 0.0 || time < least) {
         least = time;
-        best = Split{small != 0, (int)tq, (int)tp, (int)splits, (int)per, (int)slabs};
+        best = Split{small != 0, (int)tq, (int)tp, (int)(n > 1 ? tiles - rest : tiles), (int)n, (int)per, (int)slabs, n > 1 ? rest : 0};
       }
     }
   }
@@ -731,15 +750,20 @@ Split split_of(int64_t rows, int64_t cols, int64_t turns, int64_t slabs, int64_t
 template <typename T, typename O, bool QKM, bool PKM, bool GATED> int gemm(Params p, const Split& s, hipStream_t st) {
   p.tq = s.tq;
   p.tp = s.tp;
+  p.whole = s.whole;
   p.splits = s.splits;
   p.per_split = s.per_split;
   p.slabs = s.slabs;
-  const unsigned grid = (unsigned)((int64_t)s.tq * s.tp * s.splits * p.turns);
+  const unsigned grid = (unsigned)(s.whole + s.shared * s.splits);
   if (grid == 0) return SPARTON_OK;
   if (s.small)
     hipLaunchKernelGGL((gated_gemm_kernel<T, O, QKM, PKM, GATED, 2, 2, 2, 2, 2>), dim3(grid), dim3(256), 0, st, p);
   else
     hipLaunchKernelGGL((gated_gemm_kernel<T, O, QKM, PKM, GATED, 2, 2, 4, 4, 1>), dim3(grid), dim3(256), 0, st, p);
+  if (s.shared > 0) {
+    const int B = s.small ? 128 : 256;
+    hipLaunchKernelGGL(gated_join_kernel<O>, dim3((unsigned)(s.shared * (B * B / 1024))), dim3(256), 0, st, p, B);
+  }
   return (int)hipGetLastError();
 }
 
@@ -782,9 +806,7 @@ Plan plan_of(int64_t M, int64_t D, int64_t F, int dtype, bool with_bias) {
   p.dx = split_of(M, D, 1, 2 * cdiv(F * es, kSlab), es, true);
   p.dw = split_of(F, D, 2, cdiv(M * es, kSlab), es, true);
   p.act = (size_t)round_up(2 * M * ld * es, 256);
-  p.part = 0;
-  if (p.dx.splits > 1) p.part = (size_t)round_up((int64_t)p.dx.splits * M * D * 4, 256);
-  if (p.dw.splits > 1) p.part = std::max(p.part, (size_t)round_up((int64_t)p.dw.splits * 2 * F * D * 4, 256));
+  p.part = std::max(p.dx.part_bytes(), p.dw.part_bytes());  // of whole 256 bytes
   p.strips = (int)cdiv(ld, kActThreads * kActCols);
   const int64_t want = with_bias ? kBiasBlocks : 4096;
   p.rows = (int)std::max<int64_t>(1, cdiv(M * (with_bias ? 1 : p.strips), want));
@@ -822,12 +844,6 @@ int backward(const T* dh, const char* x, const char* wg, const char* wu, const f
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
-  const auto join = [&](const Split& s, int64_t n, int turns, T* a, T* b) {
-    if (s.splits <= 1) return (int)hipGetLastError();
-    hipLaunchKernelGGL(gated_join_kernel<T>, dim3((unsigned)cdiv(n, 1024), (unsigned)turns), dim3(256), 0, st, (const float*)part,
-                       s.splits, n, a, b);
-    return (int)hipGetLastError();
-  };
   if (dx != nullptr && M > 0) {
     Params p = {};
     p.q = Side{(const char*)dg, (const char*)du, ld * E, M};
@@ -837,8 +853,7 @@ int backward(const T* dh, const char* x, const char* wg, const char* wu, const f
     p.turns = 1;
     p.out[0] = dx;
     p.part = part;
-    int rc = gemm<T, T, false, true, false>(p, pl.dx, st);
-    if (rc == 0) rc = join(pl.dx, M * D, 1, dx, nullptr);
+    const int rc = gemm<T, T, false, true, false>(p, pl.dx, st);
     if (rc != 0) return rc;
   }
   if (dwg != nullptr) {
@@ -852,8 +867,7 @@ int backward(const T* dh, const char* x, const char* wg, const char* wu, const f
     p.out[0] = dwg;
     p.out[1] = dwu;
     p.part = part;
-    int rc = gemm<T, T, true, true, false>(p, pl.dw, st);
-    if (rc == 0) rc = join(pl.dw, F * D, 2, dwg, dwu);
+    const int rc = gemm<T, T, true, true, false>(p, pl.dw, st);
     if (rc != 0) return rc;
   }
   return SPARTON_OK;

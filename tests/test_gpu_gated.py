@@ -127,8 +127,9 @@ def check(args, name):
 SIZES = [  # M, D, F: few rows, both tile sizes, every edge within and at a tile, split inner dimensions
     (1, 8, 1), (1, 64, 32), (3, 72, 33), (16, 768, 100), (32, 8, 64), (33, 200, 65), (64, 1000, 31), (65, 64, 64), (65, 8, 1),
     (100, 136, 127), (128, 128, 128), (129, 72, 129), (200, 1024, 257), (257, 768, 300), (300, 520, 1000), (1000, 64, 2048),
-    (512, 256, 4000), (2049, 264, 1500), (4096, 128, 3000), (1500, 2048, 1100), (66, 272, 11450), (3437, 136, 8663),
-    (659, 136, 9167), (5226, 1560, 65), (8990, 136, 4532), (8301, 416, 360), (264, 64, 11198),
+    (512, 256, 4000), (2049, 264, 1500), (4096, 128, 3000), (1500, 2048, 1100), (405, 280, 13097), (11459, 672, 97),
+    (68, 536, 9814), (2984, 1424, 920), (6642, 1864, 65), (2505, 1544, 2664), (5442, 1616, 1175),
+    (6181, 1760, 5774), (11978, 1728, 3322), (8373, 136, 9767), (13143, 520, 745),
 ]
 
 

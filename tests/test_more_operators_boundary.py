@@ -226,7 +226,9 @@ def test_gated_checks_of_one():
 def test_gated_workspace():
     size = _lib.load().sparton_gated_workspace_bytes
     assert size(0, 64, 32, 0, 1) == 0 and size(4, 60, 32, 0, 1) == 0 and size(4, 64, 0, 0, 1) == 0
-    assert size(8192, 4096, 11264, 0, 1) == 2 * 8192 * 11264 * 2     # dg and du; enough tiles: no partial sums
+    # dg and du; of dW's 1408 tiles the 128 that do not fill the CUs once more are split in two
+    assert size(8192, 4096, 11264, 0, 1) == 2 * 8192 * 11264 * 2 + 128 * 2 * 256 * 256 * 4
+    assert size(8192, 4096, 8192, 0, 1) == 2 * 8192 * 8192 * 2       # whole rounds: no partial sums
     assert size(4, 64, 33, 0, 1) == 2 * 4 * 40 * 2 + -(2 * 4 * 40 * 2) % 256  # rows padded to 16 bytes
     assert size(4, 64, 33, 1, 1) > size(4, 64, 33, 0, 1)
     assert size(8192, 768, 2048, 0, 1) == 2 * 8192 * 2048 * 2
@@ -234,25 +236,25 @@ def test_gated_workspace():
 
 
 def split_of(rows, cols, turns, slabs, es, may_split):
-    """(128 x 128 tiles, splits): the rule of sparton_gated.hip once more."""
+    """(128 x 128 tiles, splits, tiles that are split): the rule of sparton_gated.hip once more."""
     cdiv, best = lambda a, b: -(-a // b), None
     for small in (0, 1):
-        b = 128 if small else 256
-        tiles = max(1, cdiv(rows, b) * cdiv(cols, b) * turns)
-        for n in range(1, (min(16, max(1, slabs // 4)) if may_split and tiles < 512 else 1) + 1):
-            per = max(1, cdiv(slabs, n))
-            splits = max(1, cdiv(slabs, per))
-            groups = tiles * splits
-            if splits != n and n > 1:
+        b, slots = (128, 512) if small else (256, 256)
+        tiles = cdiv(rows, b) * cdiv(cols, b) * turns
+        rest, around = tiles % slots, 6.0 if small else 10.0
+        every = (3.6 if small else 7.3) if es == 4 else (0.9 if small else 1.45)
+        some = (1.95 if small else 7.3) if es == 4 else (0.5 if small else 1.3)
+        for n in range(1, 17):
+            per, groups = cdiv(slabs, n), rest * n
+            if n > 1 and (not may_split or rest == 0 or slabs < 4 * n or cdiv(slabs, per) != n or groups > 2 * slots):
                 continue
-            alone = groups <= 256
-            slab = (1.95 if alone else 3.6) if es == 4 else (0.47 if alone else 0.9)
-            slab = slab if small else 7.3 if es == 4 else 1.45
-            time = cdiv(groups, 512 if small else 256) * (per * slab + (6.0 if small else 10.0))
-            if splits > 1:
-                time += 4.0 + rows * cols * turns * (8.0 * splits + 2.0) / 4.5e6
+            time = tiles // slots * (slabs * every + around)
+            if rest:
+                time += cdiv(groups, slots) * (per * (some if groups < 256 or (small and groups == 256) else every) + around)
+            if n > 1:
+                time += 3.0 + 0.03 * time + rest * b * b * (8.0 * n + 2.0) / 6e6
             if best is None or time < best[0]:
-                best = (time, small == 1, splits)
+                best = (time, small == 1, n, rest if n > 1 else 0)
     return best[1:]
 
 
@@ -262,20 +264,23 @@ def few(M):
 
 
 def gated_kernels(M, D, F, dt):
-    """The kernels that a training step of these sizes launches: (product, type, 128 x 128 tiles, split)."""
+    """The kernels that a training step of these sizes launches: (product, type, 128 x 128 tiles, which of them are
+    split: none, all or the last)."""
     cdiv, es = lambda a, b: -(-a // b), 4 if dt == "fp32" else 2
     D += -D % (16 // es)
-    fwd = ("few", dt, few(M), False) if M <= (32 if F * D > 1 << 23 else 64) else ("fwd", dt, split_of(M, 2 * F, 1, cdiv(D * es, 128), es, False)[0], False)
+    fwd = ("few", dt, few(M), None) if M <= (32 if F * D > 1 << 23 else 64) else ("fwd", dt, split_of(M, 2 * F, 1, cdiv(D * es, 128), es, False)[0], None)
     dx, dw = split_of(M, D, 1, 2 * cdiv(F * es, 128), es, True), split_of(F, D, 2, cdiv(M * es, 128), es, True)
-    return {fwd, ("dx", dt, dx[0], dx[1] > 1), ("dw", dt, dw[0], dw[1] > 1)}
+    b = {True: 128, False: 256}
+    which = lambda s, rows, turns: None if s[1] == 1 else "all" if s[2] == cdiv(rows, b[s[0]]) * cdiv(D, b[s[0]]) * turns else "last"
+    return {fwd, ("dx", dt, dx[0], which(dx, M, 1)), ("dw", dt, dw[0], which(dw, F, 2))}
 
 
 def test_the_gated_cases_reach_every_kernel():
     from test_gpu_gated import E4M3_SIZES, SIZES
     every = {(p, dt, small, split) for p in ("dx", "dw") for dt in ("fp32", "bf16", "fp16") for small in (True, False)
-             for split in (True, False)}
-    every |= {("fwd", dt, small, False) for dt in ("fp32", "bf16", "fp16") for small in (True, False)}
-    every |= {("few", dt, blocks, False) for dt in ("fp32", "bf16", "fp16") for blocks in (1, 2, 4)}
+             for split in (None, "all", "last")}
+    every |= {("fwd", dt, small, None) for dt in ("fp32", "bf16", "fp16") for small in (True, False)}
+    every |= {("few", dt, blocks, None) for dt in ("fp32", "bf16", "fp16") for blocks in (1, 2, 4)}
     got = set().union(*(gated_kernels(*s, dt) for s in SIZES for dt in ("fp32", "bf16", "fp16")))
     assert got == every, every ^ got
     bits8 = {("few", few(M)) if M <= 64 else ("fwd", split_of(M, 2 * F, 1, -(-(D + -D % 16) // 128), 1, False)[0])
@@ -291,8 +296,8 @@ def test_the_rule_above_is_the_librarys():
                         (8192, 768, 2048, "bf16"), (512, 4096, 11264, "bf16"), (2048, 768, 1152, "fp16")]:
         es = 4 if dt == "fp32" else 2
         D, Fp = D + -D % (16 // es), F + -F % (16 // es)
-        dx, dw = split_of(M, D, 1, 2 * cdiv(F * es, 128), es, True)[1], split_of(F, D, 2, cdiv(M * es, 128), es, True)[1]
-        part = max(up(dx * M * D * 4) if dx > 1 else 0, up(dw * 2 * F * D * 4) if dw > 1 else 0)
+        both = split_of(M, D, 1, 2 * cdiv(F * es, 128), es, True), split_of(F, D, 2, cdiv(M * es, 128), es, True)
+        part = max(shared * n * (128 if small else 256) ** 2 * 4 for small, n, shared in both)
         got = _lib.load().sparton_gated_workspace_bytes(M, D, F, 0, ("fp32", "bf16", "fp16").index(dt))
         assert got == up(2 * M * Fp * es) + part, (M, D, F, dt)
 
