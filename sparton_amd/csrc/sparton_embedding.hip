@@ -4,7 +4,7 @@
 // An id outside [0, V) reads nothing: its row is NaN and it has no gradient. The padding id has a row and no
 // gradient.
 //
-// Forward: one pass, bound by memory.
+// Forward: one pass, bound by memory. 32 x 256 tokens of 768, bf16: 6.6 us; 16391 of 768, fp16: 13.1.
 //
 // Backward: the ids are sorted with their places (a place breaks ties, so the order is the same every time),
 // and the sorted list is cut into chunks of kChunk entries. A wave takes a chunk and 64 vectors of 16 bytes of the
@@ -16,7 +16,9 @@
 //
 // The sort ranks each key among its wave's 64, then among 4 x 64 and 4 x 256, in a second launch among 32 x 1024 (all in
 // LDS), and in further ones among 16 x 32768, ... (memory): a key's rank is its own place in its list and, by binary
-// search, the number of keys before it in each of the others. No counts and no scans.
+// search, the number of keys before it in each of the others. No counts and no scans. These launches are bound by
+// their chains of dependent reads, the sums by memory. Measured, sort + merge + sums + join: 8192 tokens of 30522 x 768
+// bf16 7.6 + 8.0 + 14.9 + 4.8 us, 16391 of 250002 x 768 fp16 7.3 + 14.4 + 75.6 + 6.4 (the sums: 409 MB, 5.4 TB/s).
 
 #include <algorithm>
 
@@ -174,7 +176,7 @@ __device__ __forceinline__ I merged_place(P keys, uint32_t key, I i, I count, I 
   return rank;
 }
 
-// Tiles: the group's keys are searched in LDS. 8192 keys: 17.5 us from memory.
+// Tiles: the group's keys are searched in LDS. 8192 keys: 8.0 us, searched in memory 17.5; 16391 keys: 14.4.
 __global__ __launch_bounds__(kThreads) void embed_merge_tiles_kernel(const uint32_t* __restrict__ keys,
                                                                      const uint32_t* __restrict__ places, int N,
                                                                      uint32_t* __restrict__ keys_out,

@@ -5,7 +5,7 @@
 // and the forward on e4m3 rows and weights with a scale a row.
 //
 // One kernel runs every product. A workgroup's tile is BQ rows by BP columns of the result, its inner dimension
-// streams through two LDS stages in slabs of 128 bytes, copied there directly from memory. A wave holds its part as
+// streams through LDS in slabs of 128 bytes (rows in two stages, columns in three), copied there directly from memory. A wave holds its part as
 // 32x32 MFMA results in transposed form: a lane is a row of the result, and its registers hold groups of four
 // consecutive columns, which it stores as one vector. The forward's columns are 32 of the gate, 32 of the up
 // projection and so on, so g and u of one element meet in one lane.
@@ -20,7 +20,13 @@
 // of two (what is further below is dropped), and such sums in fp32. The rows' own rounding to e4m3, 2^-4, is far above that.
 //
 // Between forward and backward g and u are kept in fp32: in 16 bits their rounding, on top of that of dg and du to
-// the matrix instructions' operands, would double the gradients' error. In fp16, dg and du have fp16's range, as dh has.
+// the matrix instructions' operands, would add to the gradients' error. In fp16, dg and du have fp16's range, as dh has.
+//
+// Measured, 8192 x 4096 x 11264 bf16 (M, D, F): forward 1217 us with g and u stored (1242 TFLOP/s), dg and du 254 to 275
+// (5.1 TB/s), dx 1104 (1370), dW 1183 with its join (1278): a library's large products reach 1386 to 1581. The matrix
+// unit is busy for 71, 83 and 75% of the CUs' cycles, at about 1.7 GHz. The forward in e4m3 589 to 690. What is lost is
+// at a tile's ends: about 10 us of each round of tiles beside 1.5 a slab. 8192 x 768 x 2048 bf16, gelu: 73, 34, 55 and
+// 66. 1000 x 768 x 2051 fp32: forward 97 to 104, dx 65, dW 75.
 
 #include <math.h>
 

@@ -10,6 +10,11 @@
 //
 // WPR waves work on one row (1 up to 1024 elements, then 4, then 8), each lane on NP vectors of 16 bytes, as in
 // the LayerNorm (sparton_norm.hip). Every sum has a fixed order, so results are bitwise reproducible.
+//
+// Measured: 8192 x 4096 bf16 with a residual, forward 42 us (268 MB, 6.4 TB/s: more than a large copy's 5.1, as
+// repeated runs probably find part of it cached), backward 45 and 4 for the columns' sums (201 MB, 4.1 TB/s), forward in e4m3
+// 38. A few rows take 2.6, a launch. The backward of rows past 8192 spills 10 registers a lane in fp16 and 200 in
+// fp32.
 
 #include <math.h>
 

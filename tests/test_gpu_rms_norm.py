@@ -6,7 +6,7 @@ mean of squares an fp32 sum of D positive terms, so with s2 = mean(h^2) + eps
     y:  |y| (er + 4 E + u);   h: |h| (E + u)
     xhat = h rstd, of the stored h (rounded to u where there is a residual): |xhat| ex, ex = er + 2 E (+ u)
     g = dy w, c = mean(g xhat): ec = mean|g xhat| (ex + (D + 4) E)
-    dx: rstd (|xhat| ec + |xhat c| (ex + ec0) ...) spelt out below; dw: sum |dy xhat| (ex + (M + 4) E) + u |dw|
+    dx: rstd (|xhat| ec + |xhat c| ex + ...), in full in the test; dw: sum |dy xhat| (ex + (M + 4) E) + u |dw|
     8 bits: a value is off by half a step, 2^-4 of it, or 2^-10 scale below e4m3's normal range (2^-6 scale);
             scale: (er + 6 E) of it"""
 import pytest
