@@ -104,6 +104,8 @@ class _BlockForward(functools.partial):
 
 def _gated_block(self, x: Tensor) -> Tensor:
     gate, up = self.gate_proj, self.up_proj
+    if not _ff.plain_linears(gate, up):  # an adapter or a hook came since
+        return type(self).forward(self, x)
     h = _ff.gated_linear(x, gate.weight, up.weight, gate.bias, up.bias, _ff.activation_name(self.act_fn))
     return self.down_proj(h)
 

@@ -214,9 +214,23 @@ def activation_name(fn) -> Optional[str]:
     return None
 
 
+def hooked(m: nn.Module) -> bool:
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
+def plain_linears(*modules: nn.Module) -> bool:
+    """Whether these do no more than their weights and biases say, which is all that the kernel reads of them: not so
+    for an adapter around one, another forward, or hooks."""
+    return all(type(m) is nn.Linear and "forward" not in m.__dict__ and not hooked(m) for m in modules)
+
+
+_ACTIVATE = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"), "relu": F.relu}
+
+
 class SpartonGatedMLP(nn.Module):
     """A gated block, down_proj(act(gate_proj(x)) * up_proj(x)), its first half on the kernels above.
-    `SpartonGatedMLP.of(block)` shares the three nn.Linear of an existing block (names and state_dict unchanged)."""
+    `SpartonGatedMLP.of(block)` shares the three nn.Linear of an existing block (names and state_dict unchanged).
+    Projections that are more than plain nn.Linear (adapters, hooks) run as they are, then the activation."""
 
     def __init__(self, gate_proj: nn.Linear, up_proj: nn.Linear, down_proj: nn.Linear, activation: str = "silu"):
         super().__init__()
@@ -237,4 +251,6 @@ class SpartonGatedMLP(nn.Module):
 
     def forward(self, x: Tensor) -> Tensor:
         gate, up = self.gate_proj, self.up_proj
+        if not plain_linears(gate, up):
+            return self.down_proj(_ACTIVATE[self.activation](gate(x)) * up(x))
         return self.down_proj(gated_linear(x, gate.weight, up.weight, gate.bias, up.bias, self.activation))

@@ -1,0 +1,77 @@
+"""What a switched backbone does when its modules are changed afterwards, or hide something that a look at their
+submodules does not show: adapters and hooks keep their effect, dropout is not lost. On the CPU, with the operators'
+plain forms where a kernel would run.
+
+Both sides compute the same fp32 formula, so rtol 1e-4 and atol 1e-5 as in test_backbone_gated.py."""
+import copy
+
+import pytest
+import torch
+from torch import nn
+from torch.nn import functional as F
+
+from sparton_amd.backbone import use_in_backbone
+from sparton_amd.feed_forward import SpartonGatedMLP
+from test_backbone_gated import ALL, decoder, plain  # noqa: F401 (a fixture)
+
+IDS = torch.arange(12).reshape(2, 6) + 5
+
+
+class Adapter(nn.Module):
+    """A projection with a low-rank addition, under the name of the one it wraps; `weight` is the base's."""
+
+    def __init__(self, base: nn.Linear):
+        super().__init__()
+        self.base = base
+        self.add = nn.Linear(base.in_features, base.out_features, bias=False)
+
+    weight = property(lambda self: self.base.weight)
+    bias = property(lambda self: self.base.bias)
+
+    def forward(self, x):
+        return self.base(x) + self.add(x)
+
+
+def same(a, b):
+    torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("name", ["gate_proj", "up_proj", "down_proj"])
+def test_an_adapter_put_on_afterwards_counts(name, plain):  # noqa: F811
+    ref = decoder()
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    torch.manual_seed(1)
+    adapter = Adapter(getattr(ref.layers[0].mlp, name))
+    for m in (ref, ours):
+        setattr(m.layers[0].mlp, name, copy.deepcopy(adapter))
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+    assert plain["gated"] == (2 if name == "down_proj" else 1)
+
+
+@pytest.mark.parametrize("name", ["gate_proj", "up_proj"])
+@pytest.mark.parametrize("kind", ["register_forward_hook", "register_forward_pre_hook"])
+def test_hooks_of_a_projection_count(name, kind, plain):  # noqa: F811
+    ref = decoder()
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    hook = (lambda m, args, out: out * 1.5) if kind == "register_forward_hook" else (lambda m, args: (args[0] * 1.5,))
+    for m in (ref, ours):
+        getattr(getattr(m.layers[1].mlp, name), kind)(hook)
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
+def test_the_module_of_a_gated_block_too(act, plain):  # noqa: F811
+    torch.manual_seed(2)
+    gate, up, down = nn.Linear(8, 12), nn.Linear(8, 12), nn.Linear(12, 8)
+    fn = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"), "relu": F.relu}[act]
+    x = torch.randn(3, 8)
+    block = SpartonGatedMLP(gate, up, down, act)
+    block.gate_proj = Adapter(gate)
+    with torch.no_grad():
+        same(block(x), down(fn(block.gate_proj(x)) * up(x)))
+        block.gate_proj = gate
+        gate.register_forward_hook(lambda m, args, out: out + 1)
+        same(block(x), down(fn(gate(x)) * up(x)))
+    assert plain["gated"] == 0
