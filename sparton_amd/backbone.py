@@ -112,7 +112,12 @@ def _gated_block(self, x: Tensor) -> Tensor:
 
 def _pre_norm_layer(self, hidden_states: Tensor, **kwargs) -> Tensor:
     attended = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **kwargs)[0]
-    hidden_states, residual = self.post_attention_layernorm(attended, hidden_states)
+    norm = self.post_attention_layernorm
+    if isinstance(norm, SpartonRMSNorm) and not _ff.hooked(norm):
+        hidden_states, residual = norm(attended, hidden_states)
+    else:  # a hook sees a norm's one input and output, and another module takes no residual
+        residual = hidden_states + attended
+        hidden_states = norm(residual)
     return residual + self.mlp(hidden_states)
 
 

@@ -75,3 +75,28 @@ def test_the_module_of_a_gated_block_too(act, plain):  # noqa: F811
         gate.register_forward_hook(lambda m, args, out: out + 1)
         same(block(x), down(fn(gate(x)) * up(x)))
     assert plain["gated"] == 0
+
+
+def test_a_hook_of_the_fused_norm_sees_the_norm(plain):  # noqa: F811
+    ref = decoder()
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    seen = []
+
+    def hook(m, args, out):
+        seen.append((len(args), out.shape))
+        return out * 1.5
+
+    for m in (ref, ours):
+        m.layers[0].post_attention_layernorm.register_forward_hook(hook)
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+    assert seen[0] == seen[1] == (1, (2, 6, 128))
+
+
+def test_a_norm_put_in_afterwards_runs(plain):  # noqa: F811
+    ref = decoder()
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    for m in (ref, ours):
+        m.layers[0].post_attention_layernorm = nn.LayerNorm(128)
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
