@@ -140,13 +140,17 @@ class _Attended(nn.Module):
 
 
 def _computes(module: nn.Module, children: Dict[str, nn.Module], x: Tensor, want: Callable[[], Tensor]) -> bool:
-    """Whether the class's forward, on a copy with these submodules instead, gives `want` for x."""
+    """Whether the class's forward, on a copy with these submodules instead, gives `want` for x, in evaluation and in
+    training (dropout scales what it keeps)."""
     probe = copy.copy(module)
-    probe._modules, probe.training = dict(children), False
+    probe._modules = dict(children)
     try:
-        with torch.no_grad():
-            got = type(module).forward(probe, x)
-            return isinstance(got, Tensor) and bool(torch.allclose(got, want(), rtol=1e-4, atol=1e-5))
+        with torch.no_grad(), torch.random.fork_rng(devices=[]):
+            for probe.training in (False, True):
+                got = type(module).forward(probe, x)
+                if not isinstance(got, Tensor) or not torch.allclose(got, want(), rtol=1e-4, atol=1e-5):
+                    return False
+            return True
     except Exception:  # whatever it is, it is not what the kernels compute
         return False
 
@@ -172,7 +176,8 @@ def _is_gated_block(m: nn.Module) -> bool:
     name, linears = _ff.activation_name(m.act_fn), (m.gate_proj, m.up_proj, m.down_proj)
     if name is None or any(type(t) is not nn.Linear for t in linears) or linears[0].weight.shape != linears[1].weight.shape:
         return False
-    small = [nn.Linear(4, 6), nn.Linear(4, 6), nn.Linear(6, 4)]
+    with torch.random.fork_rng(devices=[]):  # their first weights are not the caller's random numbers
+        small = [nn.Linear(4, 6), nn.Linear(4, 6), nn.Linear(6, 4)]
     x = torch.linspace(-2, 2, 12).view(3, 4)
     act = {"silu": nn.functional.silu, "gelu": nn.functional.gelu, "relu": torch.relu,
            "gelu_tanh": lambda t: nn.functional.gelu(t, approximate="tanh")}[name]

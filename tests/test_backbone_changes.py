@@ -10,7 +10,7 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
-from sparton_amd.backbone import use_in_backbone
+from sparton_amd.backbone import _is_gated_block, _is_pre_norm_layer, use_in_backbone
 from sparton_amd.feed_forward import SpartonGatedMLP
 from test_backbone_gated import ALL, decoder, plain  # noqa: F401 (a fixture)
 
@@ -100,3 +100,41 @@ def test_a_norm_put_in_afterwards_runs(plain):  # noqa: F811
         m.layers[0].post_attention_layernorm = nn.LayerNorm(128)
     with torch.no_grad():
         same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+
+
+class DropoutBlock(nn.Module):
+    def __init__(self, p):
+        super().__init__()
+        self.gate_proj, self.up_proj, self.down_proj, self.act_fn = nn.Linear(8, 12), nn.Linear(8, 12), nn.Linear(12, 8), nn.SiLU()
+        self.p = p
+
+    def forward(self, x):
+        h = self.act_fn(self.gate_proj(x)) * self.up_proj(x)
+        return self.down_proj(F.dropout(h, self.p, self.training))
+
+
+class DropoutLayer(nn.Module):
+    def __init__(self, p):
+        super().__init__()
+        self.input_layernorm, self.self_attn = nn.Identity(), nn.Identity()
+        self.post_attention_layernorm, self.mlp = nn.Identity(), nn.Identity()
+        self.p = p
+
+    def forward(self, hidden_states, **kwargs):
+        h = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **kwargs)[0]
+        h = hidden_states + F.dropout(h, self.p, self.training)
+        return h + self.mlp(self.post_attention_layernorm(h))
+
+
+@pytest.mark.parametrize("training", [False, True])
+def test_dropout_that_is_no_module_is_not_lost(training):
+    state = torch.random.get_rng_state()
+    for p, ours in ((0.0, True), (0.1, False), (0.01, False)):
+        block, layer = DropoutBlock(p).train(training), DropoutLayer(p).train(training)
+        assert _is_gated_block(block) == ours and _is_pre_norm_layer(layer) == ours
+        assert block.training == training and layer.training == training
+    torch.random.set_rng_state(state)
+    block = DropoutBlock(0.1)
+    state = torch.random.get_rng_state()
+    _is_gated_block(block)
+    assert torch.equal(state, torch.random.get_rng_state())  # looking leaves the caller's random numbers alone
