@@ -182,8 +182,10 @@ def _(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation, out_dtype):
 def gated_linear_8bit(x: Tensor, x_scale: Tensor, w_gate: Tensor, gate_scale: Tensor, w_up: Tensor, up_scale: Tensor,
                       activation: str = "silu", out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """act(g) * u of e4m3 rows: g = (x w_gate') x_scale gate_scale, u likewise, summed in fp32. x [..., D] and x_scale
-    [...] as rms_norm_8bit gives them, weights [F, D] and scales [F] as quantize_rows does. For inference: there is no
-    gradient."""
+    [...] as rms_norm_8bit gives them, weights [F, D] and scales [F] as quantize_rows does. For inference: inputs that
+    ask for a gradient are refused."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, x_scale, w_gate, gate_scale, w_up, up_scale)):
+        raise ValueError("gated_linear_8bit has no gradient: call it under torch.no_grad()")
     if torch.compiler.is_compiling() or not x.is_cuda:
         return torch.ops.sparton.gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation, out_dtype)
     code = _code(activation, "gated_linear_8bit")

@@ -11,7 +11,7 @@ from torch import nn
 from torch.nn import functional as F
 
 from sparton_amd.backbone import _is_gated_block, _is_pre_norm_layer, use_in_backbone
-from sparton_amd.feed_forward import SpartonGatedMLP
+from sparton_amd.feed_forward import SpartonGatedMLP, gated_linear_8bit, quantize_rows
 from test_backbone_gated import ALL, decoder, plain  # noqa: F401 (a fixture)
 
 IDS = torch.arange(12).reshape(2, 6) + 5
@@ -138,3 +138,15 @@ def test_dropout_that_is_no_module_is_not_lost(training):
     state = torch.random.get_rng_state()
     _is_gated_block(block)
     assert torch.equal(state, torch.random.get_rng_state())  # looking leaves the caller's random numbers alone
+
+
+@pytest.mark.parametrize("which", [1, 3, 5])
+def test_a_scale_that_asks_for_a_gradient_is_refused(which):
+    x, sx = quantize_rows(torch.randn(3, 16))
+    w, sw = quantize_rows(torch.randn(6, 16))
+    args = [x, sx, w, sw.clone(), w, sw.clone()]
+    args[which] = args[which].clone().requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        gated_linear_8bit(*args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="ROCm/HIP device"):
+        gated_linear_8bit(*args)
