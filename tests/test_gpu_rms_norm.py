@@ -291,3 +291,17 @@ def test_rms_norm_opcheck_and_compile(device):
     cf = torch.compile(f, backend="aot_eager", fullgraph=True)
     for p, q in zip(torch.autograd.grad(cf(xl, wl), (xl, wl), dy), torch.autograd.grad(f(xl, wl), (xl, wl), dy)):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("through", ["y", "h", "both"])
+def test_rms_norm_leaves_do_not_share_a_gradient(through, device):
+    """x and the residual have equal gradients, in memory of their own: scaling one (clipping) leaves the other."""
+    say(f"two leaves {through}")
+    x, r = (torch.randn(40, 96, device=device, requires_grad=True) for _ in range(2))
+    w = torch.ones(96, device=device, requires_grad=True)
+    y, h = rms_norm(x, w, 1e-6, r)
+    ((y.square().sum() if through != "h" else 0) + (h.square().sum() if through != "y" else 0)).backward()
+    assert torch.equal(x.grad, r.grad) and x.grad.data_ptr() != r.grad.data_ptr()
+    before = r.grad.clone()
+    x.grad.mul_(2.0)
+    assert torch.equal(r.grad, before)
