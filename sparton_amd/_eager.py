@@ -12,6 +12,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -41,3 +42,9 @@ def load():
             torch.ops.load_library(path)
             _ops = torch.ops.sparton_eager
     return _ops
+
+
+def refuse_forward_mode(op: str, *tensors) -> None:
+    """For the torch.library ops, whose autograd knows the backward alone: a tangent would be lost in them."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{op} has no forward-mode derivative")

@@ -956,6 +956,13 @@ template <typename... T> bool wants_grad(const T&... t) {
   return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
 }
 
+// A forward-mode derivative rides on a tensor that asks for no gradient; without a graph node to refuse it, it would
+// be lost.
+template <typename... T> void refuse_forward_mode(const char* what, const T&... t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!((t.defined() && t._fw_grad(0).defined()) || ...), "sparton: ", what,
+                              " has no forward-mode derivative");
+}
+
 // ---- the RMS norm --------------------------------------------------------------------------
 
 struct RmsOut {
@@ -1035,11 +1042,13 @@ std::tuple<Tensor, Tensor> rms_add_cuda(const Tensor& x, const Tensor& r, const 
   return {o.y, o.h};
 }
 Tensor rms_autograd(const Tensor& x, const Tensor& w, double eps) {
+  refuse_forward_mode("rms_norm", x, w);
   if (wants_grad(x, w)) return RmsFn::apply(x, x, w, false, eps)[0];
   at::AutoDispatchBelowADInplaceOrView below;
   return rms_cuda(x, w, eps);
 }
 std::tuple<Tensor, Tensor> rms_add_autograd(const Tensor& x, const Tensor& r, const Tensor& w, double eps) {
+  refuse_forward_mode("rms_norm", x, r, w);
   if (wants_grad(x, r, w)) {
     auto o = RmsFn::apply(x, r, w, true, eps);
     return {o[0], o[1]};
@@ -1060,6 +1069,11 @@ std::tuple<Tensor, Tensor, Tensor> rms_8bit_cuda(const Tensor& x_in, const c10::
                                   dtype_code(x.scalar_type()), stream_of(x)),
         "sparton_rms_norm_fwd_quantized");
   return {y, scale, h};
+}
+std::tuple<Tensor, Tensor, Tensor> rms_8bit_autograd(const Tensor& x, const c10::optional<Tensor>& r, const Tensor& w, double eps) {
+  refuse_forward_mode("rms_norm_8bit", x, opt(r), w);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return rms_8bit_cuda(x, r, w, eps);
 }
 
 // ---- the embedding -------------------------------------------------------------------------
@@ -1120,6 +1134,7 @@ struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
 };
 
 Tensor embedding_autograd(const Tensor& ids, const Tensor& w, double scale, int64_t padding) {
+  refuse_forward_mode("embedding", w);
   if (wants_grad(w)) return EmbeddingFn::apply(ids, w, scale, padding);
   at::AutoDispatchBelowADInplaceOrView below;
   return embedding_cuda(ids, w, scale, padding);
@@ -1233,6 +1248,7 @@ Tensor gated_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu, const c10
 }
 Tensor gated_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu, const c10::optional<Tensor>& bg,
                       const c10::optional<Tensor>& bu, int64_t act) {
+  refuse_forward_mode("gated_linear", x, wg, wu, opt(bg), opt(bu));
   if (wants_grad(x, wg, wu, bg.value_or(Tensor()), bu.value_or(Tensor())))
     return GatedFn::apply(x, wg, wu, bg.has_value() ? *bg : x, bu.has_value() ? *bu : x, bg.has_value(), bu.has_value(), act);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -1251,6 +1267,12 @@ Tensor gated_8bit_cuda(const Tensor& x_in, const Tensor& sx, const Tensor& wg_in
                                c.data_ptr<float>(), (int)act, h.data_ptr(), M, D, F, dtype_code(out_dtype), stream_of(x)),
         "sparton_gated_fwd_quantized");
   return h;
+}
+Tensor gated_8bit_autograd(const Tensor& x, const Tensor& sx, const Tensor& wg, const Tensor& sg, const Tensor& wu,
+                           const Tensor& su, int64_t act, at::ScalarType out_dtype) {
+  refuse_forward_mode("gated_linear_8bit", x, sx, wg, sg, wu, su);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return gated_8bit_cuda(x, sx, wg, sg, wu, su, act, out_dtype);
 }
 
 // CPU tensors: the same refusal as the reference's `assert hidden.is_cuda`
@@ -1344,8 +1366,10 @@ TORCH_LIBRARY_IMPL(sparton_eager, AutogradCUDA, m) {
   m.impl("preference_loss", &preference_autograd);
   m.impl("rms_norm", &rms_autograd);
   m.impl("rms_norm_add", &rms_add_autograd);
+  m.impl("rms_norm_8bit", &rms_8bit_autograd);
   m.impl("embedding", &embedding_autograd);
   m.impl("gated", &gated_autograd);
+  m.impl("gated_8bit", &gated_8bit_autograd);
 }
 
 TORCH_LIBRARY_IMPL(sparton_eager, CPU, m) {

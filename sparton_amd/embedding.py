@@ -56,6 +56,7 @@ def _check_table(ids: Tensor, weight: Tensor, scale: float, op: str) -> None:
 @torch.library.custom_op("sparton::embedding_fwd", mutates_args=())
 def embedding_fwd(ids: Tensor, weight: Tensor, scale: float, padding: int) -> Tensor:
     """scale * weight[ids]; `padding` (-1: none) is the row that gets no gradient."""
+    _eager.refuse_forward_mode("sparton::embedding_fwd", weight)
     _check_table(ids, weight, scale, "sparton::embedding_fwd")
     return _eager.load().embedding(ids, weight, scale, padding)
 

@@ -76,6 +76,7 @@ def gated_fwd(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tensor],
     """(h in x's dtype; g and u, fp32 [rows, F], for the backward)."""
     op = "sparton::gated_fwd"
     code = _code(activation, op)
+    _eager.refuse_forward_mode(op, x, w_gate, w_up, b_gate, b_up)
     _check(x, w_gate, w_up, b_gate, b_up, op)
     return _eager.load().gated_fwd(x, w_gate, w_up, b_gate, b_up, code)
 
@@ -170,6 +171,7 @@ def gated_8bit(x: Tensor, x_scale: Tensor, w_gate: Tensor, gate_scale: Tensor, w
     """gated_linear_8bit, without a gradient."""
     op = "sparton::gated_8bit"
     code = _code(activation, op)
+    _eager.refuse_forward_mode(op, x, x_scale, w_gate, gate_scale, w_up, up_scale)
     _check_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, out_dtype, op)
     return _eager.load().gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, code, out_dtype)
 

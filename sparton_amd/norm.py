@@ -174,6 +174,7 @@ class SpartonLayerNorm(nn.LayerNorm):
 @torch.library.custom_op("sparton::rms_norm_fwd", mutates_args=())
 def rms_norm_fwd(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float) -> Tuple[Tensor, Tensor, Tensor]:
     """(y and the rounded sum h in x's dtype, rstd per row in fp32 for the backward); h is empty without a residual."""
+    _eager.refuse_forward_mode("sparton::rms_norm_fwd", x, residual, weight)
     _check(x, residual, weight, None, eps, "sparton::rms_norm_fwd")
     return _eager.load().rms_norm_fwd(x, residual, weight, eps)
 
@@ -244,6 +245,7 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6,
 @torch.library.custom_op("sparton::rms_norm_8bit", mutates_args=())
 def _rms_norm_8bit(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float) -> Tuple[Tensor, Tensor, Tensor]:
     """(y in e4m3, a scale a row, h), without a gradient; h is empty without a residual."""
+    _eager.refuse_forward_mode("sparton::rms_norm_8bit", x, residual, weight)
     _check(x, residual, weight, None, eps, "sparton::rms_norm_8bit")
     return _eager.load().rms_norm_8bit(x, residual, weight, eps)
 
