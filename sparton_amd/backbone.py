@@ -104,9 +104,10 @@ class _BlockForward(functools.partial):
 
 def _gated_block(self, x: Tensor) -> Tensor:
     gate, up = self.gate_proj, self.up_proj
-    if not _ff.plain_linears(gate, up):  # an adapter or a hook came since
+    activation = _ff.plain_activation(self.act_fn)
+    if activation is None or not _ff.plain_linears(gate, up):  # an adapter or a hook came since
         return type(self).forward(self, x)
-    h = _ff.gated_linear(x, gate.weight, up.weight, gate.bias, up.bias, _ff.activation_name(self.act_fn))
+    h = _ff.gated_linear(x, gate.weight, up.weight, gate.bias, up.bias, activation)
     return self.down_proj(h)
 
 
@@ -132,6 +133,18 @@ class _Times(nn.Module):
 
     def forward(self, x):
         return x * self.factor
+
+
+class _Bare(nn.Module):
+    """What an activation's class computes: its hooks are not called for a look at the block."""
+
+    def __init__(self, fn):
+        super().__init__()
+        self.fn = [fn]  # not a submodule
+
+    def forward(self, x):
+        fn = self.fn[0]
+        return type(fn).forward(fn, x) if isinstance(fn, nn.Module) else fn(x)
 
 
 class _Attended(nn.Module):
@@ -181,7 +194,7 @@ def _is_gated_block(m: nn.Module) -> bool:
     x = torch.linspace(-2, 2, 12).view(3, 4)
     act = {"silu": nn.functional.silu, "gelu": nn.functional.gelu, "relu": torch.relu,
            "gelu_tanh": lambda t: nn.functional.gelu(t, approximate="tanh")}[name]
-    return _computes(m, dict(zip(("gate_proj", "up_proj", "down_proj"), small), act_fn=m.act_fn), x,
+    return _computes(m, dict(zip(("gate_proj", "up_proj", "down_proj"), small), act_fn=_Bare(m.act_fn)), x,
                      lambda: small[2](act(small[0](x)) * small[1](x)))
 
 

@@ -222,10 +222,21 @@ def hooked(m: nn.Module) -> bool:
     return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
 
 
+def untouched(m: nn.Module) -> bool:
+    """Whether a call of m is its class's forward and nothing else."""
+    return "forward" not in m.__dict__ and not hooked(m)
+
+
 def plain_linears(*modules: nn.Module) -> bool:
     """Whether these do no more than their weights and biases say, which is all that the kernel reads of them: not so
     for an adapter around one, another forward, or hooks."""
-    return all(type(m) is nn.Linear and "forward" not in m.__dict__ and not hooked(m) for m in modules)
+    return all(type(m) is nn.Linear and untouched(m) for m in modules)
+
+
+def plain_activation(fn) -> Optional[str]:
+    """activation_name of what the kernel may compute in fn's place: None for a module with hooks or a forward of its
+    own, which it would pass by."""
+    return activation_name(fn) if not isinstance(fn, nn.Module) or untouched(fn) else None
 
 
 _ACTIVATE = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"), "relu": F.relu}
@@ -246,10 +257,10 @@ class SpartonGatedMLP(nn.Module):
 
     @classmethod
     def of(cls, block: nn.Module) -> "SpartonGatedMLP":
-        name = activation_name(getattr(block, "act_fn", None))
+        name = plain_activation(getattr(block, "act_fn", None))
         if name is None:
-            raise ValueError(f"SpartonGatedMLP computes {', '.join(ACTIVATIONS)}; this block's activation is "
-                             f"{getattr(block, 'act_fn', None)!r}")
+            raise ValueError(f"SpartonGatedMLP computes {', '.join(ACTIVATIONS)}, without hooks; this block's activation "
+                             f"is {getattr(block, 'act_fn', None)!r}")
         m = cls(block.gate_proj, block.up_proj, block.down_proj, name)
         return m.train(block.training)
 

@@ -61,6 +61,39 @@ def test_hooks_of_a_projection_count(name, kind, plain):  # noqa: F811
         same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
 
 
+@pytest.mark.parametrize("before", [False, True])
+@pytest.mark.parametrize("kind", ["register_forward_hook", "register_forward_pre_hook", "forward"])
+def test_hooks_of_the_activation_count(kind, before, plain):  # noqa: F811
+    """Put there before or after the switch; looking at the block does not call them."""
+    ref = decoder()
+    calls = []
+
+    def scaled(m, args, out=None):
+        calls.append(m)
+        return (args[0] * 1.5,) if out is None else out * 1.5
+
+    def put(m):
+        act = m.layers[0].mlp.act_fn
+        if kind == "forward":
+            act.forward = lambda x: scaled(act, None, F.silu(x))
+        else:
+            getattr(act, kind)(scaled)
+
+    ours = copy.deepcopy(ref)
+    if before:
+        put(ours)
+    use_in_backbone(ours, **ALL)
+    assert not calls
+    if not before:
+        put(ours)
+    put(ref)
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+    assert len(calls) == 2 and plain["gated"] == 1
+    with pytest.raises(ValueError, match="activation"):
+        SpartonGatedMLP.of(ref.layers[0].mlp)
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
 def test_the_module_of_a_gated_block_too(act, plain):  # noqa: F811
     torch.manual_seed(2)
