@@ -204,16 +204,18 @@ def quantize_rows(t: Tensor) -> Tuple[Tensor, Tensor]:
 
 
 def activation_name(fn) -> Optional[str]:
-    """The kernels' name of a module's activation, or None if they do not compute it."""
-    if isinstance(fn, nn.SiLU) or fn is F.silu or type(fn).__name__ == "SiLUActivation":
+    """The kernels' name of a module's activation, or None if they do not compute it. A subclass may compute anything."""
+    cls = type(fn)
+    theirs = cls.__name__ if cls.__module__ == "transformers.activations" else None
+    if cls is nn.SiLU or fn is F.silu or theirs == "SiLUActivation":
         return "silu"
-    if isinstance(fn, nn.GELU):
+    if cls is nn.GELU:
         return "gelu_tanh" if fn.approximate == "tanh" else "gelu"
-    if fn is F.gelu or type(fn).__name__ == "GELUActivation":
+    if fn is F.gelu or theirs == "GELUActivation":
         return "gelu"
-    if type(fn).__name__ == "GELUTanh":
+    if theirs == "GELUTanh":
         return "gelu_tanh"
-    if isinstance(fn, nn.ReLU) or fn is F.relu:
+    if cls is nn.ReLU or fn is F.relu:
         return "relu"
     return None
 

@@ -94,6 +94,48 @@ def test_hooks_of_the_activation_count(kind, before, plain):  # noqa: F811
         SpartonGatedMLP.of(ref.layers[0].mlp)
 
 
+class ShiftedSiLU(nn.SiLU):
+    def forward(self, x):
+        return super().forward(x - 1)
+
+
+class SiLUActivation(nn.Module):  # named as one of transformers'
+    def forward(self, x):
+        return x.tanh()
+
+
+OTHERS = dict(subclass=ShiftedSiLU, named=SiLUActivation, tanh=nn.Tanh,
+              sequential=lambda: nn.Sequential(nn.SiLU(), nn.Dropout(0.5)).eval(), function=lambda: torch.sin)
+
+
+@pytest.mark.parametrize("other", OTHERS)
+def test_an_activation_put_in_afterwards_runs(other, plain):  # noqa: F811
+    """Also where its class derives from one that the kernels compute, or has its name."""
+    ref = decoder()
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    for m in (ref, ours):
+        if other == "function":  # a registered module's name takes modules alone
+            del m.layers[0].mlp.act_fn
+        m.layers[0].mlp.act_fn = OTHERS[other]()
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+    assert plain["gated"] == 1
+    if other != "function":
+        assert not _is_gated_block(ref.layers[0].mlp)
+        with pytest.raises(ValueError, match="activation"):
+            SpartonGatedMLP.of(ref.layers[0].mlp)
+
+
+def test_an_activation_of_another_name_put_in_afterwards_runs(plain):  # noqa: F811
+    ref = decoder()
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    for m in (ref, ours):
+        m.layers[0].mlp.act_fn = nn.GELU(approximate="tanh")
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+    assert plain["gated"] == 2
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
 def test_the_module_of_a_gated_block_too(act, plain):  # noqa: F811
     torch.manual_seed(2)
