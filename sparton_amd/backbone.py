@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import copy
 import functools
+import inspect
 from typing import Callable, Dict, Optional
 
 import torch
@@ -34,6 +35,7 @@ NAME = "sparton"
 # dense -> dropout -> LayerNorm(. + input): the output blocks of an encoder layer.
 _RESIDUAL_BLOCKS = ("BertSelfOutput", "BertOutput", "RobertaSelfOutput", "RobertaOutput", "XLMRobertaSelfOutput",
                     "XLMRobertaOutput")
+_REQUIRED = inspect.Parameter.empty  # the default of a parameter that has none
 _UNSUPPORTED = ("sliding_window", "softcap", "s_aux", "position_bias", "head_mask")
 
 
@@ -102,17 +104,26 @@ class _BlockForward(functools.partial):
         return self.args[0]
 
 
-def _gated_block(self, x: Tensor) -> Tensor:
+def _gated_block(self, *args, **kwargs) -> Tensor:
     gate, up = self.gate_proj, self.up_proj
     activation = _ff.plain_activation(self.act_fn)
-    if activation is None or not _ff.plain_linears(gate, up):  # an adapter or a hook came since
-        return type(self).forward(self, x)
+    # an adapter or a hook came since, or the input goes by its name
+    if activation is None or not _ff.plain_linears(gate, up) or kwargs or len(args) != 1:
+        return type(self).forward(self, *args, **kwargs)
+    (x,) = args
     h = _ff.gated_linear(x, gate.weight, up.weight, gate.bias, up.bias, activation)
     return self.down_proj(h)
 
 
-def _pre_norm_layer(self, hidden_states: Tensor, **kwargs) -> Tensor:
-    attended = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **kwargs)[0]
+def _pre_norm_layer(self, params, *args, **kwargs) -> Tensor:
+    """params: the names and defaults of what the layer's own forward takes. All but the hidden states go to the
+    attention by their names, as they do there."""
+    given = dict(zip((name for name, _ in params), args))
+    call = {**dict(params), **given, **kwargs}
+    if len(args) > len(params) or given.keys() & kwargs.keys() or any(v is _REQUIRED for v in call.values()):
+        return type(self).forward(self, *args, **kwargs)  # which refuses the call
+    hidden_states = call.pop(params[0][0])
+    attended = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **call)[0]
     norm = self.post_attention_layernorm
     if isinstance(norm, SpartonRMSNorm) and not _ff.hooked(norm):
         hidden_states, residual = norm(attended, hidden_states)
@@ -148,19 +159,27 @@ class _Bare(nn.Module):
 
 
 class _Attended(nn.Module):
-    def forward(self, hidden_states, **kwargs):
+    """Stands for the attention; takes the hidden states by their name, and beside them what `others` says alone."""
+
+    def __init__(self, others):
+        super().__init__()
+        self.others = others
+
+    def forward(self, *, hidden_states, **kwargs):
+        if kwargs.keys() != self.others.keys() or any(kwargs[n] is not v for n, v in self.others.items()):
+            raise ValueError("another call of the attention")
         return hidden_states * 3.0, None
 
 
-def _computes(module: nn.Module, children: Dict[str, nn.Module], x: Tensor, want: Callable[[], Tensor]) -> bool:
-    """Whether the class's forward, on a copy with these submodules instead, gives `want` for x, in evaluation and in
-    training (dropout scales what it keeps)."""
+def _computes(module: nn.Module, children: Dict[str, nn.Module], x: Tensor, want: Callable[[], Tensor], **kwargs) -> bool:
+    """Whether the class's forward, on a copy with these submodules instead, gives `want` for x (and kwargs), in
+    evaluation and in training (dropout scales what it keeps)."""
     probe = copy.copy(module)
     probe._modules = dict(children)
     try:
         with torch.no_grad(), torch.random.fork_rng(devices=[]):
             for probe.training in (False, True):
-                got = type(module).forward(probe, x)
+                got = type(module).forward(probe, x, **kwargs)
                 if not isinstance(got, Tensor) or not torch.allclose(got, want(), rtol=1e-4, atol=1e-5):
                     return False
             return True
@@ -198,14 +217,30 @@ def _is_gated_block(m: nn.Module) -> bool:
                      lambda: small[2](act(small[0](x)) * small[1](x)))
 
 
+def _params(m: nn.Module) -> Optional[tuple]:
+    """((name, default or _REQUIRED), ...) of what m's class's forward takes, or None if names alone do not say it."""
+    ps = list(inspect.signature(type(m).forward).parameters.values())[1:]
+    if ps and ps[-1].kind is ps[-1].VAR_KEYWORD:
+        ps.pop()
+    if not ps or any(p.kind is not p.POSITIONAL_OR_KEYWORD for p in ps):
+        return None
+    return tuple((p.name, p.default) for p in ps)
+
+
 def _is_pre_norm_layer(m: nn.Module) -> bool:
-    """h = x + self_attn(input_layernorm(x)); h + mlp(post_attention_layernorm(h))."""
+    """h = x + self_attn(input_layernorm(x)); h + mlp(post_attention_layernorm(h)), what it takes besides x going to
+    the attention."""
     names = ("input_layernorm", "self_attn", "post_attention_layernorm", "mlp")
     if set(m._modules) != set(names) or m._parameters or m._buffers:
         return False
+    params = _params(m)
+    if params is None:
+        return False
+    # flags keep their defaults; what may be None is something here, to be seen again in the attention
+    others = {n: object() if default is None or default is _REQUIRED else default for n, default in params[1:]}
     x = torch.linspace(-1, 1, 12).view(1, 3, 4)
-    children = dict(zip(names, (_Times(2.0), _Attended(), _Times(5.0), _Times(7.0))))
-    return _computes(m, children, x, lambda: 36.0 * (x * 7.0))  # x + 3 * 2 x, and 1 + 5 * 7 times that
+    children = dict(zip(names, (_Times(2.0), _Attended(others), _Times(5.0), _Times(7.0))))
+    return _computes(m, children, x, lambda: 36.0 * (x * 7.0), **others)  # x + 3 * 2 x, and 1 + 5 * 7 times that
 
 
 def use_in_backbone(model: nn.Module, *, rms_norm: bool = False, feed_forward: bool = False,
@@ -231,7 +266,7 @@ def use_in_backbone(model: nn.Module, *, rms_norm: bool = False, feed_forward: b
             raise ValueError(f"{type(model).__name__} has no root-mean-square norm that the kernels compute")
         norms += found
         ours = {id(c) for _, _, c in children if isinstance(c, SpartonRMSNorm) or id(c) in made}
-        forwards += [(m, _pre_norm_layer) for m in modules if "forward" not in m.__dict__ and _is_pre_norm_layer(m)
+        forwards += [(m, _pre_norm_layer, _params(m)) for m in modules if "forward" not in m.__dict__ and _is_pre_norm_layer(m)
                      and id(m.post_attention_layernorm) in ours]
     if feed_forward:
         blocks = [m for m in modules if _is_gated_block(m)]
@@ -251,8 +286,8 @@ def use_in_backbone(model: nn.Module, *, rms_norm: bool = False, feed_forward: b
         raise ValueError(f"{type(model).__name__} does not take its attention from transformers' registry")
     for module, name, child in norms:
         setattr(module, name, child)
-    for module, forward in forwards:
-        module.forward = _BlockForward(forward, module)
+    for module, forward, *more in forwards:
+        module.forward = _BlockForward(forward, module, *more)
     for module in model.modules():
         if type(module).__name__ in _RESIDUAL_BLOCKS and isinstance(module.LayerNorm, SpartonLayerNorm):
             module.forward = _BlockForward(_residual_norm, module)

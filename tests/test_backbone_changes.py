@@ -4,6 +4,7 @@ plain forms where a kernel would run.
 
 Both sides compute the same fp32 formula, so rtol 1e-4 and atol 1e-5 as in test_backbone_gated.py."""
 import copy
+import pickle
 
 import pytest
 import torch
@@ -225,3 +226,72 @@ def test_a_scale_that_asks_for_a_gradient_is_refused(which):
         gated_linear_8bit(*args)
     with torch.no_grad(), pytest.raises(RuntimeError, match="ROCm/HIP device"):
         gated_linear_8bit(*args)
+
+
+CALLS = {
+    "by position": lambda layer, x, mask, rope: layer(x, mask, None, None, False, rope),
+    "mask by position": lambda layer, x, mask, rope: layer(x, mask, position_embeddings=rope),
+    "by name": lambda layer, x, mask, rope: layer(hidden_states=x, attention_mask=mask, position_embeddings=rope),
+    "no mask": lambda layer, x, mask, rope: layer(x, position_embeddings=rope),
+    "as the model": lambda layer, x, mask, rope: layer(x, attention_mask=mask, position_ids=None, past_key_values=None,
+                                                       use_cache=False, position_embeddings=rope),
+}
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_a_switched_layer_takes_every_call_of_its_own(call, plain):  # noqa: F811
+    ref = decoder()
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    x = torch.randn(1, 6, 128)
+    rope = ref.rotary_emb(x, torch.arange(6)[None])
+    with torch.no_grad():
+        # causal: what the model gives its layers as a mask, each in its attention's form
+        want = CALLS["by name"](ref.layers[0], x, torch.full((6, 6), -1e30).triu(1)[None, None], rope)
+        for m in (ours, pickle.loads(pickle.dumps(ours)), copy.deepcopy(ours)):
+            before = plain["added"]
+            same(CALLS[call](m.layers[0], x, torch.ones(1, 6), rope), want)
+            assert plain["added"] == before + 1
+
+
+def test_a_call_that_the_layer_refuses_is_refused(plain):  # noqa: F811
+    ref = decoder()
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    x = torch.randn(1, 6, 128)
+    for m in (ref, ours):
+        for args, kw in (((), {}), ((x, None), dict(attention_mask=None)), ((x, None, None, None, False, None, 7), {})):
+            with pytest.raises(TypeError):
+                m.layers[0](*args, **kw)
+
+
+def test_a_switched_block_takes_its_input_by_name(plain):  # noqa: F811
+    ref = decoder()
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    x = torch.randn(2, 128)
+    with torch.no_grad():
+        same(ours.layers[0].mlp(x=x), ref.layers[0].mlp(x))
+    for args, kw in (((), {}), ((x, x), {}), ((x,), dict(x=x))):
+        with pytest.raises(TypeError):
+            ours.layers[0].mlp(*args, **kw)
+
+
+class OtherCall(DropoutLayer):
+    """Gives its attention something else than it was given."""
+
+    def __init__(self, kind):
+        super().__init__(0.0)
+        self.kind = kind
+
+    def forward(self, hidden_states, mask=None, flag=False, **kwargs):
+        x = self.input_layernorm(hidden_states)
+        calls = dict(same=lambda: self.self_attn(hidden_states=x, mask=mask, flag=flag, **kwargs),
+                     position=lambda: self.self_attn(x, mask=mask, flag=flag, **kwargs),
+                     dropped=lambda: self.self_attn(hidden_states=x, mask=mask, **kwargs),
+                     other=lambda: self.self_attn(hidden_states=x, mask=1, flag=flag, **kwargs),
+                     more=lambda: self.self_attn(hidden_states=x, mask=mask, flag=flag, more=1, **kwargs))
+        h = hidden_states + calls[self.kind]()[0]
+        return h + self.mlp(self.post_attention_layernorm(h))
+
+
+@pytest.mark.parametrize("kind", ["same", "position", "dropped", "other", "more"])
+def test_a_layer_that_calls_its_attention_in_another_way_keeps_its_forward(kind):
+    assert _is_pre_norm_layer(OtherCall(kind)) == (kind == "same")
