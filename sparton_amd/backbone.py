@@ -125,9 +125,9 @@ def _pre_norm_layer(self, params, *args, **kwargs) -> Tensor:
     hidden_states = call.pop(params[0][0])
     attended = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **call)[0]
     norm = self.post_attention_layernorm
-    if isinstance(norm, SpartonRMSNorm) and not _ff.hooked(norm):
+    if isinstance(norm, SpartonRMSNorm) and _ff.untouched(norm):
         hidden_states, residual = norm(attended, hidden_states)
-    else:  # a hook sees a norm's one input and output, and another module takes no residual
+    else:  # a hook sees a norm's one input and output, and another module or forward takes no residual
         residual = hidden_states + attended
         hidden_states = norm(residual)
     return residual + self.mlp(hidden_states)
@@ -189,6 +189,8 @@ def _computes(module: nn.Module, children: Dict[str, nn.Module], x: Tensor, want
 
 def _is_rms_norm(m: nn.Module) -> bool:
     if isinstance(m, SpartonRMSNorm) or not type(m).__name__.endswith("RMSNorm") or list(m._parameters) != ["weight"]:
+        return False
+    if "forward" in m.__dict__:
         return False
     weight, eps = m.weight, getattr(m, "variance_epsilon", getattr(m, "eps", None))
     if weight is None or weight.dim() != 1 or not isinstance(eps, float):

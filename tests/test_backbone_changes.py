@@ -295,3 +295,26 @@ class OtherCall(DropoutLayer):
 @pytest.mark.parametrize("kind", ["same", "position", "dropped", "other", "more"])
 def test_a_layer_that_calls_its_attention_in_another_way_keeps_its_forward(kind):
     assert _is_pre_norm_layer(OtherCall(kind)) == (kind == "same")
+
+
+@pytest.mark.parametrize("before", [False, True])
+@pytest.mark.parametrize("name", ["input_layernorm", "post_attention_layernorm"])
+def test_a_norms_own_forward_runs(name, before, plain):  # noqa: F811
+    """Put on the module, as a wrapper for moved weights does, before or after the switch."""
+    ref = decoder()
+
+    def put(m):
+        norm = getattr(m.layers[0], name)
+        own = norm.forward
+        norm.forward = lambda x: own(x) * 1.5
+
+    ours = copy.deepcopy(ref)
+    if before:
+        put(ours)
+    use_in_backbone(ours, **ALL)
+    if not before:
+        put(ours)
+    put(ref)
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+    assert plain["added"] == (1 if name == "post_attention_layernorm" else 2)
