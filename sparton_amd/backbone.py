@@ -93,7 +93,10 @@ def register() -> None:
 
 
 def _residual_norm(self, hidden_states: Tensor, input_tensor: Tensor) -> Tensor:
-    return self.LayerNorm(self.dropout(self.dense(hidden_states)), input_tensor)
+    norm, hidden_states = self.LayerNorm, self.dropout(self.dense(hidden_states))
+    if isinstance(norm, SpartonLayerNorm) and _ff.untouched(norm):
+        return norm(hidden_states, input_tensor)
+    return norm(hidden_states + input_tensor)  # a hook sees the norm's one input; another forward takes no residual
 
 
 class _BlockForward(functools.partial):
@@ -251,7 +254,8 @@ def use_in_backbone(model: nn.Module, *, rms_norm: bool = False, feed_forward: b
     cannot be switched, or that has nothing of a kind that is asked for, raises and stays as it was."""
     norms = [(module, name, SpartonLayerNorm.of(child)) for module in model.modules()
              for name, child in module.named_children()
-             if type(child) is nn.LayerNorm and len(child.normalized_shape) == 1 and child.weight is not None]
+             if type(child) is nn.LayerNorm and len(child.normalized_shape) == 1 and child.weight is not None
+             and "forward" not in child.__dict__]
     modules = list(model.modules())
     children = [(module, name, child) for module in modules for name, child in module.named_children()]
     made: Dict[int, nn.Module] = {}  # a module in several places becomes one

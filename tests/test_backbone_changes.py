@@ -13,6 +13,7 @@ from torch.nn import functional as F
 
 from sparton_amd.backbone import _is_gated_block, _is_pre_norm_layer, use_in_backbone
 from sparton_amd.feed_forward import SpartonGatedMLP, gated_linear_8bit, quantize_rows
+from test_backbone import plain_attention, tiny
 from test_backbone_gated import ALL, decoder, plain  # noqa: F401 (a fixture)
 
 IDS = torch.arange(12).reshape(2, 6) + 5
@@ -318,3 +319,32 @@ def test_a_norms_own_forward_runs(name, before, plain):  # noqa: F811
     with torch.no_grad():
         same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
     assert plain["added"] == (1 if name == "post_attention_layernorm" else 2)
+
+
+@pytest.mark.parametrize("change", ["own forward before", "own forward after", "another module after", "hook before",
+                                    "hook after"])
+def test_an_encoders_layer_norm_changed(change, monkeypatch):
+    monkeypatch.setattr("sparton_amd.backbone.attention", plain_attention)
+    monkeypatch.setattr("sparton_amd.norm.layer_norm", lambda x, w, b=None, eps=1e-5, residual=None:
+                        F.layer_norm(x if residual is None else x + residual, w.shape, w, b, eps))
+    ref = tiny("bert").eval()
+
+    def put(m):
+        block = m.bert.encoder.layer[0].output
+        if change == "another module after":
+            block.LayerNorm = nn.LayerNorm(block.LayerNorm.weight.shape[0])
+        elif change.startswith("hook"):
+            block.LayerNorm.register_forward_pre_hook(lambda m, args: (args[0] + 1.5 * args[0].square(),))
+        else:
+            own = block.LayerNorm.forward
+            block.LayerNorm.forward = lambda x: own(x) * 1.5
+
+    ours = copy.deepcopy(ref)
+    if change.endswith("before"):
+        put(ours)
+    use_in_backbone(ours)
+    if change.endswith("after"):
+        put(ours)
+    put(ref)
+    with torch.no_grad():
+        same(ours(IDS).logits, ref(IDS).logits)
