@@ -21,15 +21,16 @@ from __future__ import annotations
 import copy
 import functools
 import inspect
-from typing import Callable, Dict, Optional
+from typing import Dict, Optional
 
 import torch
 from torch import Tensor, nn
 
 from . import feed_forward as _ff
+from ._look import computes
 from .attention import KEY_MASK_DTYPES, attention
 from .embedding import SpartonEmbedding
-from .norm import SpartonLayerNorm, SpartonRMSNorm
+from .norm import SpartonLayerNorm, SpartonRMSNorm, computes_rms_norm
 
 NAME = "sparton"
 # dense -> dropout -> LayerNorm(. + input): the output blocks of an encoder layer.
@@ -149,18 +150,6 @@ class _Times(nn.Module):
         return x * self.factor
 
 
-class _Bare(nn.Module):
-    """What an activation's class computes: its hooks are not called for a look at the block."""
-
-    def __init__(self, fn):
-        super().__init__()
-        self.fn = [fn]  # not a submodule
-
-    def forward(self, x):
-        fn = self.fn[0]
-        return type(fn).forward(fn, x) if isinstance(fn, nn.Module) else fn(x)
-
-
 class _Attended(nn.Module):
     """Stands for the attention; takes the hidden states by their name, and beside them what `others` says alone."""
 
@@ -174,52 +163,15 @@ class _Attended(nn.Module):
         return hidden_states * 3.0, None
 
 
-def _computes(module: nn.Module, children: Dict[str, nn.Module], x: Tensor, want: Callable[[], Tensor], **kwargs) -> bool:
-    """Whether the class's forward, on a copy with these submodules instead, gives `want` for x (and kwargs), in
-    evaluation and in training (dropout scales what it keeps)."""
-    probe = copy.copy(module)
-    probe._modules = dict(children)
-    try:
-        with torch.no_grad(), torch.random.fork_rng(devices=[]):
-            for probe.training in (False, True):
-                got = type(module).forward(probe, x, **kwargs)
-                if not isinstance(got, Tensor) or not torch.allclose(got, want(), rtol=1e-4, atol=1e-5):
-                    return False
-            return True
-    except Exception:  # whatever it is, it is not what the kernels compute
-        return False
-
-
 def _is_rms_norm(m: nn.Module) -> bool:
-    if isinstance(m, SpartonRMSNorm) or not type(m).__name__.endswith("RMSNorm") or list(m._parameters) != ["weight"]:
-        return False
-    if "forward" in m.__dict__:
-        return False
-    weight, eps = m.weight, getattr(m, "variance_epsilon", getattr(m, "eps", None))
-    if weight is None or weight.dim() != 1 or not isinstance(eps, float):
-        return False
-    g = torch.Generator().manual_seed(0)
-    n = weight.shape[0]
-    x, w = torch.randn(3, n, generator=g), torch.rand(n, generator=g) + 0.5
-    probe = copy.copy(m)
-    probe._parameters = {"weight": nn.Parameter(w)}
-    return _computes(probe, {}, x, lambda: w * x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps))
+    return (not isinstance(m, SpartonRMSNorm) and type(m).__name__.endswith("RMSNorm")
+            and list(m._parameters) == ["weight"] and computes_rms_norm(m))
 
 
 def _is_gated_block(m: nn.Module) -> bool:
     """down_proj(act_fn(gate_proj(x)) * up_proj(x)) of plain linears, and nothing else in it."""
-    if set(m._modules) != {"gate_proj", "up_proj", "down_proj", "act_fn"} or m._parameters or m._buffers:
-        return False
-    name, linears = _ff.activation_name(m.act_fn), (m.gate_proj, m.up_proj, m.down_proj)
-    if name is None or any(type(t) is not nn.Linear for t in linears) or linears[0].weight.shape != linears[1].weight.shape:
-        return False
-    with torch.random.fork_rng(devices=[]):  # their first weights are not the caller's random numbers
-        small = [nn.Linear(4, 6), nn.Linear(4, 6), nn.Linear(6, 4)]
-    x = torch.linspace(-2, 2, 12).view(3, 4)
-    act = {"silu": nn.functional.silu, "gelu": nn.functional.gelu, "relu": torch.relu,
-           "gelu_tanh": lambda t: nn.functional.gelu(t, approximate="tanh")}[name]
-    return _computes(m, dict(zip(("gate_proj", "up_proj", "down_proj"), small), act_fn=_Bare(m.act_fn)), x,
-                     lambda: small[2](act(small[0](x)) * small[1](x)))
+    return (_ff.computes_gated_block(m) and all(type(t) is nn.Linear for t in (m.gate_proj, m.up_proj, m.down_proj))
+            and m.gate_proj.weight.shape == m.up_proj.weight.shape)
 
 
 def _params(m: nn.Module) -> Optional[tuple]:
@@ -245,7 +197,7 @@ def _is_pre_norm_layer(m: nn.Module) -> bool:
     others = {n: object() if default is None or default is _REQUIRED else default for n, default in params[1:]}
     x = torch.linspace(-1, 1, 12).view(1, 3, 4)
     children = dict(zip(names, (_Times(2.0), _Attended(others), _Times(5.0), _Times(7.0))))
-    return _computes(m, children, x, lambda: 36.0 * (x * 7.0), **others)  # x + 3 * 2 x, and 1 + 5 * 7 times that
+    return computes(m, children, x, lambda: 36.0 * (x * 7.0), **others)  # x + 3 * 2 x, and 1 + 5 * 7 times that
 
 
 def use_in_backbone(model: nn.Module, *, rms_norm: bool = False, feed_forward: bool = False,
@@ -280,7 +232,8 @@ def use_in_backbone(model: nn.Module, *, rms_norm: bool = False, feed_forward: b
             raise ValueError(f"{type(model).__name__} has no gated feed-forward block that the kernels compute")
         forwards += [(m, _gated_block) for m in blocks if "forward" not in m.__dict__]
     if embedding:
-        found = [(m, n, replaced(c, SpartonEmbedding.of)) for m, n, c in children if type(c) is nn.Embedding]
+        found = [(m, n, replaced(c, SpartonEmbedding.of)) for m, n, c in children
+                 if type(c) is nn.Embedding and "forward" not in c.__dict__]
         if not found and not any(isinstance(m, SpartonEmbedding) for m in modules):
             raise ValueError(f"{type(model).__name__} has no nn.Embedding")
         norms += found

@@ -117,7 +117,8 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Opti
 class SpartonEmbedding(nn.Embedding):
     """An nn.Embedding on the kernels above, with an optional factor: module.scale * weight[ids].
     `SpartonEmbedding.of(embedding)` shares an existing module's parameter (name and state_dict unchanged)
-    and keeps its hooks. Renormed, sparse and frequency-scaled embeddings are refused."""
+    and keeps its hooks; of a SpartonEmbedding, its factor too, times this one. Renormed, sparse and frequency-scaled
+    embeddings are refused, and modules with another forward than nn.Embedding's."""
 
     scale: float = 1.0
 
@@ -136,10 +137,12 @@ class SpartonEmbedding(nn.Embedding):
     @classmethod
     def of(cls, module: nn.Embedding, scale: float = 1.0) -> "SpartonEmbedding":
         cls._check_module(module)
+        if type(module).forward not in (nn.Embedding.forward, cls.forward) or "forward" in module.__dict__:
+            raise ValueError(f"SpartonEmbedding computes nn.Embedding's rows times a factor; {module} has another forward")
         m = copy.copy(module)  # the same hooks and mode
         m.__class__ = cls
         m._parameters = dict(m._parameters)  # and parameters, until either module is given another one
-        m.scale = float(scale)
+        m.scale = float(scale) * (module.scale if isinstance(module, SpartonEmbedding) else 1.0)
         return m
 
     def forward(self, input: Tensor) -> Tensor:

@@ -24,6 +24,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import _eager, _lib
+from ._look import computes, holds_only
 
 ACTIVATIONS = tuple(_lib.ACTIVATION_CODE)
 MAX_WIDTH = 1 << 20
@@ -244,9 +245,37 @@ def plain_activation(fn) -> Optional[str]:
 _ACTIVATE = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"), "relu": F.relu}
 
 
+class _Bare(nn.Module):
+    """What an activation's class computes: its hooks are not called for a look at the block."""
+
+    def __init__(self, fn):
+        super().__init__()
+        self.fn = [fn]  # not a submodule
+
+    def forward(self, x):
+        fn = self.fn[0]
+        return type(fn).forward(fn, x) if isinstance(fn, nn.Module) else fn(x)
+
+
+def computes_gated_block(m: nn.Module) -> bool:
+    """down_proj(act_fn(gate_proj(x)) * up_proj(x)) with an activation of the kernels, and nothing else in it; the
+    projections may be anything."""
+    if set(m._modules) != {"gate_proj", "up_proj", "down_proj", "act_fn"} or m._parameters or m._buffers:
+        return False
+    name = activation_name(m.act_fn)
+    if name is None:
+        return False
+    with torch.random.fork_rng(devices=[]):  # their first weights are not the caller's random numbers
+        small = [nn.Linear(4, 6), nn.Linear(4, 6), nn.Linear(6, 4)]
+    x = torch.linspace(-2, 2, 12).view(3, 4)
+    return computes(m, dict(zip(("gate_proj", "up_proj", "down_proj"), small), act_fn=_Bare(m.act_fn)), x,
+                    lambda: small[2](_ACTIVATE[name](small[0](x)) * small[1](x)))
+
+
 class SpartonGatedMLP(nn.Module):
     """A gated block, down_proj(act(gate_proj(x)) * up_proj(x)), its first half on the kernels above.
-    `SpartonGatedMLP.of(block)` shares the three nn.Linear of an existing block (names and state_dict unchanged).
+    `SpartonGatedMLP.of(block)` shares the three nn.Linear of an existing block (names and state_dict unchanged); a block
+    that computes something else (seen on a small copy, on the CPU) is refused.
     Projections that are more than plain nn.Linear (adapters, hooks) run as they are, then the activation."""
 
     def __init__(self, gate_proj: nn.Linear, up_proj: nn.Linear, down_proj: nn.Linear, activation: str = "silu"):
@@ -263,6 +292,9 @@ class SpartonGatedMLP(nn.Module):
         if name is None:
             raise ValueError(f"SpartonGatedMLP computes {', '.join(ACTIVATIONS)}, without hooks; this block's activation "
                              f"is {getattr(block, 'act_fn', None)!r}")
+        if "forward" in block.__dict__ or not (holds_only(block) or computes_gated_block(block)):
+            raise ValueError("SpartonGatedMLP computes down_proj(act_fn(gate_proj(x)) * up_proj(x)), which "
+                             f"{block} does not")
         m = cls(block.gate_proj, block.up_proj, block.down_proj, name)
         return m.train(block.training)
 

@@ -33,6 +33,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _eager, _lib
+from ._look import computes, holds_only
 
 MAX_WIDTH = 16384
 _FLOAT_DTYPES = tuple(_lib.DTYPE_CODE)
@@ -271,10 +272,28 @@ def rms_norm_8bit(x: Tensor, weight: Tensor, eps: float = 1e-6, residual: Option
     return (y, scale) if residual is None else (y, scale, h)
 
 
+def _weight_and_eps(m: nn.Module) -> Optional[Tuple[Tensor, float]]:
+    weight, eps = getattr(m, "weight", None), getattr(m, "variance_epsilon", getattr(m, "eps", None))
+    return (weight, eps) if isinstance(weight, Tensor) and weight.dim() == 1 and isinstance(eps, float) else None
+
+
+def computes_rms_norm(m: nn.Module) -> bool:
+    """weight * x / sqrt(mean(x^2) + eps), seen on a copy with another weight."""
+    found = _weight_and_eps(m)
+    if found is None or "forward" in m.__dict__:
+        return False
+    (weight, eps), g = found, torch.Generator().manual_seed(0)
+    n = weight.shape[0]
+    x, w = torch.randn(3, n, generator=g), torch.rand(n, generator=g) + 0.5
+    probe = copy.copy(m)
+    probe._parameters = {"weight": nn.Parameter(w)}
+    return computes(probe, {}, x, lambda: w * x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps))
+
+
 class SpartonRMSNorm(nn.Module):
     """A root-mean-square norm over the last dimension on the kernels above: norm(x), or norm(x, residual) for
     (norm of the sum, sum). `SpartonRMSNorm.of(module)` shares an existing module's weight (name and state_dict
-    unchanged) and keeps its hooks.
+    unchanged) and keeps its hooks; a module that computes something else (seen on a small copy, on the CPU) is refused.
 
     A weight wider than x (float32 masters) stays as it is and the result is x's dtype; under autocast too, as the
     inputs are rows of the autocast dtype there."""
@@ -288,9 +307,13 @@ class SpartonRMSNorm(nn.Module):
 
     @classmethod
     def of(cls, module: nn.Module) -> "SpartonRMSNorm":
-        weight, eps = getattr(module, "weight", None), getattr(module, "variance_epsilon", getattr(module, "eps", None))
-        if not isinstance(weight, Tensor) or weight.dim() != 1 or not isinstance(eps, float):
+        found = _weight_and_eps(module)
+        if found is None:
             raise ValueError(f"SpartonRMSNorm needs a weight over one dimension and an epsilon, got {module}")
+        weight, eps = found
+        ours = type(module).forward is cls.forward and "forward" not in module.__dict__
+        if not ours and not holds_only(module) and not computes_rms_norm(module):
+            raise ValueError(f"SpartonRMSNorm computes weight * x / sqrt(mean(x^2) + eps), which {module} does not")
         if not 1 <= weight.shape[0] <= MAX_WIDTH:
             raise ValueError(f"SpartonRMSNorm takes rows up to {MAX_WIDTH}, got {weight.shape[0]}")
         m = copy.copy(module)  # the same hooks and mode

@@ -12,7 +12,9 @@ from torch import nn
 from torch.nn import functional as F
 
 from sparton_amd.backbone import _is_gated_block, _is_pre_norm_layer, use_in_backbone
+from sparton_amd.embedding import SpartonEmbedding
 from sparton_amd.feed_forward import SpartonGatedMLP, gated_linear_8bit, quantize_rows
+from sparton_amd.norm import SpartonRMSNorm
 from test_backbone import plain_attention, tiny
 from test_backbone_gated import ALL, decoder, plain  # noqa: F401 (a fixture)
 
@@ -348,3 +350,90 @@ def test_an_encoders_layer_norm_changed(change, monkeypatch):
     put(ref)
     with torch.no_grad():
         same(ours(IDS).logits, ref(IDS).logits)
+
+
+# ---- a module made of another computes what that one does, or is refused -----------------------
+
+def own_forward(m, f):
+    m.forward = f
+    return m
+
+
+class MultipliedBlock(DropoutBlock):
+    def forward(self, x):
+        return self.down_proj(0.5 * self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+class DropoutNorm(nn.RMSNorm):
+    def forward(self, x):
+        return F.dropout(super().forward(x), 0.1, self.training)
+
+
+class BiasedNorm(nn.RMSNorm):
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.bias = nn.Parameter(torch.zeros(16))
+
+    def forward(self, x):
+        return super().forward(x) + self.bias
+
+
+class ShiftedEmbedding(nn.Embedding):
+    def forward(self, input):
+        return super().forward(input + 1)
+
+
+def other_modules():
+    from transformers.models.gemma.modeling_gemma import GemmaRMSNorm
+    from transformers.models.gemma3.modeling_gemma3 import Gemma3TextScaledWordEmbedding
+    block, dropped = DropoutBlock(0.0), DropoutBlock(0.0)
+    dropped.dropout = nn.Dropout(0.5)
+    return {
+        "norm of 1 + weight": (SpartonRMSNorm, GemmaRMSNorm(16)),
+        "norm with dropout": (SpartonRMSNorm, DropoutNorm(16, eps=1e-5).eval()),
+        "norm with a bias": (SpartonRMSNorm, BiasedNorm(16, eps=1e-5)),
+        "layer norm": (SpartonRMSNorm, nn.LayerNorm(16)),
+        "norm with its own forward": (SpartonRMSNorm, own_forward(nn.RMSNorm(16, eps=1e-5), lambda x: x)),
+        "scaled embedding": (SpartonEmbedding, Gemma3TextScaledWordEmbedding(10, 16, 0, embed_scale=4.0)),
+        "shifted embedding": (SpartonEmbedding, ShiftedEmbedding(10, 16)),
+        "embedding with its own forward": (SpartonEmbedding, own_forward(nn.Embedding(10, 16), lambda x: x)),
+        "multiplied block": (SpartonGatedMLP, MultipliedBlock(0.0)),
+        "block with dropout": (SpartonGatedMLP, DropoutBlock(0.1)),
+        "block with a module more": (SpartonGatedMLP, dropped),
+        "block with its own forward": (SpartonGatedMLP, own_forward(block, lambda x: x)),
+    }
+
+
+@pytest.mark.parametrize("name", other_modules())
+def test_a_module_that_computes_something_else_is_refused(name):
+    cls, module = other_modules()[name]
+    with pytest.raises(ValueError, match=cls.__name__):
+        cls.of(module)
+
+
+def test_what_the_kernels_compute_is_taken(plain):  # noqa: F811
+    from transformers.models.llama.modeling_llama import LlamaRMSNorm
+    x, ids = torch.randn(5, 16), torch.tensor([1, 4, 1])
+    for norm in (LlamaRMSNorm(16), nn.RMSNorm(16, eps=1e-5), SpartonRMSNorm(16)):
+        with torch.no_grad():
+            norm.weight.uniform_(0.5, 1.5)
+        ours = SpartonRMSNorm.of(norm)
+        same(ours(x), norm(x))
+        assert ours.weight is norm.weight
+    block = DropoutBlock(0.0)
+    same(SpartonGatedMLP.of(block)(x[:, :8]), block(x[:, :8]))
+    table = nn.Embedding(10, 16)
+    once = SpartonEmbedding.of(table, scale=3.0)
+    for ours, factor in ((once, 3), (SpartonEmbedding.of(once), 3), (SpartonEmbedding.of(once, scale=2.0), 6)):
+        same(ours(ids), factor * table(ids))
+
+
+def test_an_embeddings_own_forward_runs(plain):  # noqa: F811
+    ref = decoder()
+    own = ref.embed_tokens.forward
+    ref.embed_tokens.forward = lambda ids: own(ids) * 1.5
+    ref.other = nn.Embedding(4, 4)
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    assert type(ours.embed_tokens) is nn.Embedding and isinstance(ours.other, SpartonEmbedding)
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
