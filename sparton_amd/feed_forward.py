@@ -17,6 +17,7 @@ Device tensors only, like the head.
 """
 from __future__ import annotations
 
+import copy
 from typing import Optional, Tuple
 
 import torch
@@ -274,17 +275,21 @@ def computes_gated_block(m: nn.Module) -> bool:
 
 class SpartonGatedMLP(nn.Module):
     """A gated block, down_proj(act(gate_proj(x)) * up_proj(x)), its first half on the kernels above.
-    `SpartonGatedMLP.of(block)` shares the three nn.Linear of an existing block (names and state_dict unchanged); a block
-    that computes something else (seen on a small copy, on the CPU) is refused.
+    `SpartonGatedMLP.of(block)` shares the three nn.Linear of an existing block (names and state_dict unchanged) and
+    keeps its hooks; a block that computes something else (seen on a small copy, on the CPU) is refused.
     Projections that are more than plain nn.Linear (adapters, hooks) run as they are, then the activation."""
 
     def __init__(self, gate_proj: nn.Linear, up_proj: nn.Linear, down_proj: nn.Linear, activation: str = "silu"):
         super().__init__()
         _code(activation, "SpartonGatedMLP")
+        self._check_shapes(gate_proj, up_proj, down_proj)
+        self.gate_proj, self.up_proj, self.down_proj, self.activation = gate_proj, up_proj, down_proj, activation
+
+    @staticmethod
+    def _check_shapes(gate_proj: nn.Module, up_proj: nn.Module, down_proj: nn.Module) -> None:
         if gate_proj.weight.shape != up_proj.weight.shape or down_proj.in_features != gate_proj.out_features:
             raise ValueError("SpartonGatedMLP needs gate_proj and up_proj of one shape and down_proj behind them, got "
                              f"{gate_proj}, {up_proj} and {down_proj}")
-        self.gate_proj, self.up_proj, self.down_proj, self.activation = gate_proj, up_proj, down_proj, activation
 
     @classmethod
     def of(cls, block: nn.Module) -> "SpartonGatedMLP":
@@ -295,8 +300,12 @@ class SpartonGatedMLP(nn.Module):
         if "forward" in block.__dict__ or not (holds_only(block) or computes_gated_block(block)):
             raise ValueError("SpartonGatedMLP computes down_proj(act_fn(gate_proj(x)) * up_proj(x)), which "
                              f"{block} does not")
-        m = cls(block.gate_proj, block.up_proj, block.down_proj, name)
-        return m.train(block.training)
+        cls._check_shapes(block.gate_proj, block.up_proj, block.down_proj)
+        m = copy.copy(block)  # the same hooks and mode
+        m.__class__ = cls
+        m._modules = {n: c for n, c in block._modules.items() if n in ("gate_proj", "up_proj", "down_proj")}
+        m.activation = name
+        return m
 
     def forward(self, x: Tensor) -> Tensor:
         gate, up = self.gate_proj, self.up_proj

@@ -437,3 +437,20 @@ def test_an_embeddings_own_forward_runs(plain):  # noqa: F811
     assert type(ours.embed_tokens) is nn.Embedding and isinstance(ours.other, SpartonEmbedding)
     with torch.no_grad():
         same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+
+
+@pytest.mark.parametrize("training", [False, True])
+def test_a_module_made_of_a_gated_block_keeps_its_hooks_and_mode(training, plain):  # noqa: F811
+    block, seen = DropoutBlock(0.0).train(training), []
+    block.up_proj.train(not training)  # a mode of its own
+    block.register_forward_hook(lambda m, args, out: out * 1.5)
+    block.register_forward_pre_hook(lambda m, args: seen.append(type(m).__name__))
+    ours = SpartonGatedMLP.of(block)
+    x = torch.randn(3, 8)
+    same(ours(x), block(x))
+    assert seen == ["SpartonGatedMLP", "DropoutBlock"] and plain["gated"] == 1
+    assert ours.training == training and ours.up_proj.training == block.up_proj.training == (not training)
+    assert list(ours.state_dict()) == list(block.state_dict()) and set(dict(ours.named_children())) == {
+        "gate_proj", "up_proj", "down_proj"} and block.act_fn is not None
+    ours.up_proj = nn.Linear(8, 12)  # the block keeps its own
+    assert block.up_proj is not ours.up_proj
