@@ -7,6 +7,8 @@ from typing import Callable, Dict
 import torch
 from torch import Tensor, nn
 
+PLAIN = dict(device="cpu", dtype=torch.float32)  # of what is looked with, whatever torch's defaults are
+
 
 def computes(module: nn.Module, children: Dict[str, nn.Module], x: Tensor, want: Callable[[], Tensor], **kwargs) -> bool:
     """Whether the class's forward, on a copy with these submodules instead, gives `want` for x (and kwargs), in

@@ -27,7 +27,7 @@ import torch
 from torch import Tensor, nn
 
 from . import feed_forward as _ff
-from ._look import computes
+from ._look import PLAIN, computes
 from .attention import KEY_MASK_DTYPES, attention
 from .embedding import SpartonEmbedding
 from .norm import SpartonLayerNorm, SpartonRMSNorm, computes_rms_norm
@@ -195,7 +195,7 @@ def _is_pre_norm_layer(m: nn.Module) -> bool:
         return False
     # flags keep their defaults; what may be None is something here, to be seen again in the attention
     others = {n: object() if default is None or default is _REQUIRED else default for n, default in params[1:]}
-    x = torch.linspace(-1, 1, 12).view(1, 3, 4)
+    x = torch.linspace(-1, 1, 12, **PLAIN).view(1, 3, 4)
     children = dict(zip(names, (_Times(2.0), _Attended(others), _Times(5.0), _Times(7.0))))
     return computes(m, children, x, lambda: 36.0 * (x * 7.0), **others)  # x + 3 * 2 x, and 1 + 5 * 7 times that
 

@@ -25,7 +25,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import _eager, _lib
-from ._look import computes, holds_only
+from ._look import PLAIN, computes, holds_only
 
 ACTIVATIONS = tuple(_lib.ACTIVATION_CODE)
 MAX_WIDTH = 1 << 20
@@ -267,8 +267,8 @@ def computes_gated_block(m: nn.Module) -> bool:
     if name is None:
         return False
     with torch.random.fork_rng(devices=[]):  # their first weights are not the caller's random numbers
-        small = [nn.Linear(4, 6), nn.Linear(4, 6), nn.Linear(6, 4)]
-    x = torch.linspace(-2, 2, 12).view(3, 4)
+        small = [nn.Linear(*n, **PLAIN) for n in ((4, 6), (4, 6), (6, 4))]
+    x = torch.linspace(-2, 2, 12, **PLAIN).view(3, 4)
     return computes(m, dict(zip(("gate_proj", "up_proj", "down_proj"), small), act_fn=_Bare(m.act_fn)), x,
                     lambda: small[2](_ACTIVATE[name](small[0](x)) * small[1](x)))
 

@@ -33,7 +33,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _eager, _lib
-from ._look import computes, holds_only
+from ._look import PLAIN, computes, holds_only
 
 MAX_WIDTH = 16384
 _FLOAT_DTYPES = tuple(_lib.DTYPE_CODE)
@@ -282,9 +282,9 @@ def computes_rms_norm(m: nn.Module) -> bool:
     found = _weight_and_eps(m)
     if found is None or "forward" in m.__dict__:
         return False
-    (weight, eps), g = found, torch.Generator().manual_seed(0)
+    (weight, eps), g = found, torch.Generator("cpu").manual_seed(0)
     n = weight.shape[0]
-    x, w = torch.randn(3, n, generator=g), torch.rand(n, generator=g) + 0.5
+    x, w = torch.randn(3, n, generator=g, **PLAIN), torch.rand(n, generator=g, **PLAIN) + 0.5
     probe = copy.copy(m)
     probe._parameters = {"weight": nn.Parameter(w)}
     return computes(probe, {}, x, lambda: w * x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps))

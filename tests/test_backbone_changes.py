@@ -454,3 +454,25 @@ def test_a_module_made_of_a_gated_block_keeps_its_hooks_and_mode(training, plain
         "gate_proj", "up_proj", "down_proj"} and block.act_fn is not None
     ours.up_proj = nn.Linear(8, 12)  # the block keeps its own
     assert block.up_proj is not ours.up_proj
+
+
+@pytest.mark.parametrize("where", ["float64", "bfloat16", "meta"])
+def test_modules_are_known_whatever_torchs_defaults_are(where, plain):  # noqa: F811
+    ref, norm, block = decoder(), SpartonRMSNorm(16), DropoutBlock(0.0)
+    theirs, layer = nn.RMSNorm(16, eps=1e-5), DropoutLayer(0.0)
+    ours = copy.deepcopy(ref)
+    before = torch.get_default_dtype()
+    try:
+        if where == "meta":
+            torch.set_default_device("meta")
+        else:
+            torch.set_default_dtype(getattr(torch, where))
+        use_in_backbone(ours, **ALL)
+        SpartonRMSNorm.of(norm), SpartonRMSNorm.of(theirs), SpartonGatedMLP.of(block)
+        assert _is_pre_norm_layer(layer)
+    finally:
+        torch.set_default_device(None)
+        torch.set_default_dtype(before)
+    with torch.no_grad():
+        same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
+    assert plain == dict(rms=5, added=2, gated=2, embedding=1)
