@@ -12,7 +12,7 @@ Around them, a backbone layer's own work: `sparton_amd.attention` (padded, causa
 `sparton::preference_fwd/_bwd`).
 `SpartonRMSNorm` (with the residual's addition, and rows in e4m3; ops `sparton::rms_norm_fwd/_bwd/_8bit`),
 `SpartonEmbedding` (gradient by sorted tokens; ops `sparton::embedding_fwd/_bwd`) and `SpartonGatedMLP` (ops
-`sparton::gated_fwd/_bwd/_8bit`) are the rest of a gated backbone's layer.
+`sparton::gated_fwd/_bwd/_infer/_8bit`) are the rest of a gated backbone's layer.
 Importing the package registers the ops; the library itself is loaded on first use
 and raises if it has not been built (`python -m sparton_amd.build`).
 """

@@ -8,6 +8,7 @@ g and u meet in registers. The backward has one product for x and one for both w
 in fp32 in between. A few rows (new tokens) take a kernel that streams the weights once; rows and weights
 in e4m3 with a scale a row take the matrix cores' 8-bit rate.
 
+    sparton::gated_infer(x, w_gate, w_up, b_gate?, b_up?, activation) -> h
     sparton::gated_fwd(x, w_gate, w_up, b_gate?, b_up?, activation) -> (h, gate, up)
     sparton::gated_bwd(dh, x, w_gate, w_up, gate, up, activation, has_b_gate, has_b_up)
         -> (dx, d_w_gate, d_w_up, d_b_gate, d_b_up)
@@ -90,6 +91,22 @@ def _(x, w_gate, w_up, b_gate, b_up, activation):
     return x.new_empty((*x.shape[:-1], width)), saved, torch.empty_like(saved)
 
 
+@torch.library.custom_op("sparton::gated_infer", mutates_args=())
+def gated_infer(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tensor], b_up: Optional[Tensor],
+                activation: str) -> Tensor:
+    """h alone, without a gradient: g and u are not written."""
+    op = "sparton::gated_infer"
+    code = _code(activation, op)
+    _eager.refuse_forward_mode(op, x, w_gate, w_up, b_gate, b_up)
+    _check(x, w_gate, w_up, b_gate, b_up, op)
+    return _eager.load().gated(x, w_gate, w_up, b_gate, b_up, code)
+
+
+@gated_infer.register_fake
+def _(x, w_gate, w_up, b_gate, b_up, activation):
+    return x.new_empty((*x.shape[:-1], w_gate.shape[0]))
+
+
 @torch.library.custom_op("sparton::gated_bwd", mutates_args=())
 def gated_bwd(dh: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, gate: Tensor, up: Tensor, activation: str,
               has_b_gate: bool, has_b_up: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
@@ -148,6 +165,8 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Optional[Tenso
         b_gate, b_up = (b.to(dt) if b is not None else None for b in (b_gate, b_up))
     if torch.compiler.is_compiling() or not x.is_cuda:  # the registered op: fake + autograd
         _check_shapes(x, w_gate, w_up, "gated_linear")
+        if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_gate, w_up, b_gate, b_up))):
+            return torch.ops.sparton.gated_infer(x, w_gate, w_up, b_gate, b_up, activation)
         return torch.ops.sparton.gated_fwd(x, w_gate, w_up, b_gate, b_up, activation)[0]
     _check(x, w_gate, w_up, b_gate, b_up, "gated_linear")
     return _eager.load().gated(x, w_gate, w_up, b_gate, b_up, code)

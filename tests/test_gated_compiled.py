@@ -1,0 +1,52 @@
+"""What a compiled program runs of the gated product: without gradients no g and u are written, and a backward computes
+the gradients that are asked for. On the CPU with tensors without data, which take the compiler's path; on the GPU
+through torch.compile, against the eager calls."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from _parity import say
+from sparton_amd.feed_forward import gated_linear
+
+NAMES = ["x", "w_gate", "w_up", "b_gate", "b_up"]
+
+
+class Calls(TorchDispatchMode):
+    """The framework's operators that are called, with their arguments."""
+
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        if func.namespace == "sparton":
+            self.seen.append((func.name().split("::")[1], args))
+        return func(*args, **(kwargs or {}))
+
+
+def inputs(asked, device="cpu", make=torch.empty):
+    shapes = dict(x=(20, 64), w_gate=(48, 64), w_up=(48, 64), b_gate=(48,), b_up=(48,))
+    return [make(s, device=device).requires_grad_(n in asked) for n, s in shapes.items()]
+
+
+def test_without_gradients_g_and_u_are_not_written():
+    for asked, enabled, op in (([], True, "gated_infer"), (NAMES, False, "gated_infer"), (["b_up"], True, "gated_fwd")):
+        with FakeTensorMode(), Calls() as calls, torch.set_grad_enabled(enabled):
+            h = gated_linear(*inputs(asked))
+            gated_linear(*inputs(asked)[:3])
+        assert h.shape == (20, 48) and h.requires_grad == (op == "gated_fwd")
+        assert [n for n, _ in calls.seen] == [op, op if "b_up" not in asked else "gated_infer"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("asked", [[], NAMES])
+def test_a_compiled_forward(asked, device):
+    say(f"compiled forward, {asked}")
+    args = inputs(asked, device, torch.randn)
+    f = lambda *t: gated_linear(*t) * 2
+    with torch.no_grad():
+        want = f(*args)
+        assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(*args), want)
+    got = torch.compile(f, backend="aot_eager", fullgraph=True)(*args)
+    assert torch.equal(got.detach(), want) and got.requires_grad == bool(asked)
