@@ -1207,11 +1207,12 @@ std::tuple<Tensor, Tensor, Tensor> gated_fwd_cuda(const Tensor& x, const Tensor&
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> gated_bwd_cuda(const Tensor& dh, const Tensor& x, const Tensor& wg,
                                                                   const Tensor& wu, const Tensor& g, const Tensor& u,
-                                                                  int64_t act, bool has_bg, bool has_bu) {
+                                                                  int64_t act, bool has_bg, bool has_bu, bool need_x,
+                                                                  bool need_w) {
   c10::OptionalDeviceGuard guard(x.device());
-  auto d = gated_grads(dh, gated_rows(x), gated_rows(wg), gated_rows(wu), g, u, act, x.size(-1), true, true, has_bg, has_bu);
-  for (int i = 3; i < 5; ++i)
-    if (!d[i].defined()) d[i] = at::empty({0}, x.options());
+  auto d = gated_grads(dh, gated_rows(x), gated_rows(wg), gated_rows(wu), g, u, act, x.size(-1), need_x, need_w, has_bg, has_bu);
+  for (Tensor& t : d)
+    if (!t.defined()) t = at::empty({0}, x.options());
   return {d[0], d[1], d[2], d[3], d[4]};
 }
 
@@ -1320,7 +1321,7 @@ TORCH_LIBRARY(sparton_eager, m) {
   m.def("gated_fwd(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int activation) "
         "-> (Tensor, Tensor, Tensor)");
   m.def("gated_bwd(Tensor dh, Tensor x, Tensor w_gate, Tensor w_up, Tensor gate, Tensor up, int activation, "
-        "bool has_b_gate, bool has_b_up) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+        "bool has_b_gate, bool has_b_up, bool need_x=True, bool need_w=True) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("gated_8bit(Tensor x, Tensor x_scale, Tensor w_gate, Tensor gate_scale, Tensor w_up, Tensor up_scale, "
         "int activation, ScalarType out_dtype) -> Tensor");
 }

@@ -10,7 +10,7 @@ in e4m3 with a scale a row take the matrix cores' 8-bit rate.
 
     sparton::gated_infer(x, w_gate, w_up, b_gate?, b_up?, activation) -> h
     sparton::gated_fwd(x, w_gate, w_up, b_gate?, b_up?, activation) -> (h, gate, up)
-    sparton::gated_bwd(dh, x, w_gate, w_up, gate, up, activation, has_b_gate, has_b_up)
+    sparton::gated_bwd(dh, x, w_gate, w_up, gate, up, activation, has_b_gate, has_b_up, need_x=True, need_w=True)
         -> (dx, d_w_gate, d_w_up, d_b_gate, d_b_up)
     sparton::gated_8bit(x, x_scale, w_gate, gate_scale, w_up, up_scale, activation, out_dtype) -> h
 
@@ -109,8 +109,10 @@ def _(x, w_gate, w_up, b_gate, b_up, activation):
 
 @torch.library.custom_op("sparton::gated_bwd", mutates_args=())
 def gated_bwd(dh: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, gate: Tensor, up: Tensor, activation: str,
-              has_b_gate: bool, has_b_up: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """(dx, d_w_gate, d_w_up, d_b_gate, d_b_up) in x's dtype; the biases' are empty where there are none."""
+              has_b_gate: bool, has_b_up: bool, need_x: bool = True,
+              need_w: bool = True) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(dx, d_w_gate, d_w_up, d_b_gate, d_b_up) in x's dtype; those that are not asked for are empty, as the biases' are
+    where there are none."""
     op = "sparton::gated_bwd"
     code = _code(activation, op)
     _check(x, w_gate, w_up, None, None, op)
@@ -121,13 +123,13 @@ def gated_bwd(dh: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, gate: Tensor,
         if tuple(t.shape) != (x.numel() // D, width) or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError(f"{op}: gate and up must be contiguous float32 [{x.numel() // D}, {width}]")
     _require_device(x, (dh, gate, up), op)
-    return _eager.load().gated_bwd(dh, x, w_gate, w_up, gate, up, code, has_b_gate, has_b_up)
+    return _eager.load().gated_bwd(dh, x, w_gate, w_up, gate, up, code, has_b_gate, has_b_up, need_x, need_w)
 
 
 @gated_bwd.register_fake
-def _(dh, x, w_gate, w_up, gate, up, activation, has_b_gate, has_b_up):
+def _(dh, x, w_gate, w_up, gate, up, activation, has_b_gate, has_b_up, need_x=True, need_w=True):
     width = w_gate.shape[0]
-    return (x.new_empty(x.shape), w_gate.new_empty(w_gate.shape), w_up.new_empty(w_up.shape),
+    return (x.new_empty(x.shape if need_x else (0,)), *(w.new_empty(w.shape if need_w else (0,)) for w in (w_gate, w_up)),
             x.new_empty((width if has_b_gate else 0,)), x.new_empty((width if has_b_up else 0,)))
 
 
@@ -143,9 +145,10 @@ def _setup_context(ctx, inputs, output):
 def _backward(ctx, dh, _d_gate, _d_up):
     if dh is None:  # h did not reach the loss
         return (None,) * 6
-    dx, dwg, dwu, dbg, dbu = torch.ops.sparton.gated_bwd(dh, *ctx.saved_tensors, ctx.activation, ctx.has_b_gate,
-                                                         ctx.has_b_up)
-    return dx, dwg, dwu, dbg if ctx.has_b_gate else None, dbu if ctx.has_b_up else None, None
+    x, wg, wu, bg, bu = ctx.needs_input_grad[:5]
+    bg, bu = bg and ctx.has_b_gate, bu and ctx.has_b_up
+    grads = torch.ops.sparton.gated_bwd(dh, *ctx.saved_tensors, ctx.activation, bg, bu, x, wg or wu)
+    return (*(g if need else None for g, need in zip(grads, (x, wg, wu, bg, bu))), None)
 
 
 gated_fwd.register_autograd(_backward, setup_context=_setup_context)

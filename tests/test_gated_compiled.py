@@ -50,3 +50,37 @@ def test_a_compiled_forward(asked, device):
         assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(*args), want)
     got = torch.compile(f, backend="aot_eager", fullgraph=True)(*args)
     assert torch.equal(got.detach(), want) and got.requires_grad == bool(asked)
+
+
+ASKED = [["x"], ["w_up"], ["w_gate", "b_up"], ["b_gate"], ["b_gate", "b_up"], ["x", "b_up"], NAMES]
+
+
+@pytest.mark.parametrize("asked", ASKED)
+def test_a_backward_computes_what_is_asked_for(asked):
+    with FakeTensorMode(), Calls() as calls:
+        args = inputs(asked)
+        leaves = [t for t in args if t.requires_grad]
+        grads = torch.autograd.grad(gated_linear(*args).sum(), leaves)
+    assert [g.shape for g in grads] == [t.shape for t in leaves]
+    (name, args), = calls.seen[1:]
+    flags = [*args[7:], True, True][:4]  # the last two have defaults
+    assert name == "gated_bwd" and flags == ["b_gate" in asked, "b_up" in asked, "x" in asked,
+                                             bool({"w_gate", "w_up"} & set(asked))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("asked", ASKED)
+def test_a_compiled_backward(asked, device):
+    say(f"compiled backward of {asked}")
+    args = inputs(asked, device, torch.randn)
+    leaves = [t for t in args if t.requires_grad]
+    dh = torch.randn(20, 48, device=device)
+    f = lambda *t: gated_linear(*t) * 2
+    want = torch.autograd.grad(f(*args), leaves, dh)
+    got = torch.autograd.grad(torch.compile(f, backend="aot_eager", fullgraph=True)(*args), leaves, dh)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    every = torch.ops.sparton.gated_bwd(dh, *args[:3], *torch.ops.sparton.gated_fwd(*args, "silu")[1:], "silu", True, True)
+    some = torch.ops.sparton.gated_bwd(dh, *args[:3], *torch.ops.sparton.gated_fwd(*args, "silu")[1:], "silu",
+                                       "b_gate" in asked, "b_up" in asked, "x" in asked, "w_gate" in asked)
+    here = ["x" in asked, "w_gate" in asked, "w_gate" in asked, "b_gate" in asked, "b_up" in asked]
+    assert all(torch.equal(a, b) if h else a.numel() == 0 for a, b, h in zip(some, every, here))
