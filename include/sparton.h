@@ -394,7 +394,8 @@ int sparton_rms_norm_bwd(const void* dy, const void* dh, const void* h, const vo
  *     out[i] = scale table[ids[i]];   d_table[v] = scale sum of d_out[i] over ids[i] == v, ascending in i
  * ids: `ids_dtype` SPARTON_MASK_I64 or SPARTON_MASK_I32. An id outside [0, V) reads nothing, gives a row of
  * NaN and has no gradient; the id padding_idx (-1: none) has a row and no gradient. Any alignment of whole
- * elements; N, V < 2^31 - 1024, D <= 2^20.
+ * elements; N, V < 2^31 - 1024, D <= 2^20, N rows below 2^34 vectors of 16 bytes, a table below 2 TB; backward, N times D
+ * rounded up to 256 below 2^37 (SPARTON_EUNSUPPORTED past them).
  */
 int sparton_embedding_fwd(const void* ids, int ids_dtype, const void* table, float scale, void* out, int64_t N,
                           int64_t V, int64_t D, int dtype, void* stream);

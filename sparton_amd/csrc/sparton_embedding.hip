@@ -380,15 +380,17 @@ int zero_rows(int64_t D, int dtype) {
 size_t list_bytes(int64_t N) { return (size_t)round_up(N * 4, 256); }
 size_t part_bytes(int64_t N, int64_t D) { return (size_t)(cdiv(N, kChunk) * 2 * D * 4); }
 
-int check(int64_t N, int64_t V, int64_t D, int dtype, int ids_dtype) {
+int check(int64_t N, int64_t V, int64_t D, int dtype, int ids_dtype, bool backward) {
   if (N < 0 || V < 0 || D <= 0 || dtype < SPARTON_F32 || dtype > SPARTON_F16) return SPARTON_EINVAL;
   if (ids_dtype != SPARTON_MASK_I64 && ids_dtype != SPARTON_MASK_I32) return SPARTON_EINVAL;
   if (D > kMaxD || N > INT32_MAX - kTile || V >= (int64_t)kNone) return SPARTON_EUNSUPPORTED;
   const int64_t nv = cdiv(D, vec_of(D, dtype));
   if ((uint64_t)cdiv(N * nv, kThreads * kUnroll) * kThreads >= kMaxThreads) return SPARTON_EUNSUPPORTED;
-  const uint64_t waves = (uint64_t)(cdiv(N, kChunk) * cdiv(nv, 64) + cdiv(V, zero_rows(D, dtype)));
-  if (waves * 64 + kThreads >= kMaxThreads || (uint64_t)cdiv(N, kChunk) * cdiv(D, 256) * 64 * kJoinWaves >= kMaxThreads)
-    return SPARTON_EUNSUPPORTED;
+  // The backward's launches: a wave for each run of table rows (a table of 2 TB, also refused forward), for a chunk's
+  // columns, and the workgroups of the join.
+  const uint64_t zeros = (uint64_t)cdiv(V, zero_rows(D, dtype)), sums = backward ? (uint64_t)(cdiv(N, kChunk) * cdiv(nv, 64)) : 0;
+  if ((sums + zeros) * 64 + kThreads >= kMaxThreads) return SPARTON_EUNSUPPORTED;
+  if (backward && (uint64_t)cdiv(N, kChunk) * cdiv(D, 256) * 64 * kJoinWaves >= kMaxThreads) return SPARTON_EUNSUPPORTED;
   return SPARTON_OK;
 }
 
@@ -417,7 +419,7 @@ using namespace sparton;
 
 SPARTON_EXPORT int sparton_embedding_fwd(const void* ids, int ids_dtype, const void* table, float scale, void* out,
                                          int64_t N, int64_t V, int64_t D, int dtype, void* stream) {
-  const int rc = emb::check(N, V, D, dtype, ids_dtype);
+  const int rc = emb::check(N, V, D, dtype, ids_dtype, false);
   if (rc != SPARTON_OK) return rc;
   if (N == 0) return SPARTON_OK;
   if (ids == nullptr || out == nullptr || (table == nullptr && V > 0)) return SPARTON_EINVAL;
@@ -439,14 +441,14 @@ SPARTON_EXPORT int sparton_embedding_fwd(const void* ids, int ids_dtype, const v
 }
 
 SPARTON_EXPORT size_t sparton_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype) {
-  if (emb::check(N, V, D, dtype, SPARTON_MASK_I64) != SPARTON_OK || N == 0) return 0;
+  if (emb::check(N, V, D, dtype, SPARTON_MASK_I64, true) != SPARTON_OK || N == 0) return 0;
   return 4 * emb::list_bytes(N) + emb::part_bytes(N, D);
 }
 
 SPARTON_EXPORT int sparton_embedding_bwd(const void* ids, int ids_dtype, const void* d_out, float scale, int64_t padding_idx,
                                          void* d_table, void* workspace, size_t workspace_bytes, int64_t N, int64_t V,
                                          int64_t D, int dtype, void* stream) {
-  const int rc = emb::check(N, V, D, dtype, ids_dtype);
+  const int rc = emb::check(N, V, D, dtype, ids_dtype, true);
   if (rc != SPARTON_OK) return rc;
   if (V == 0) return SPARTON_OK;
   if (d_table == nullptr || (N > 0 && (ids == nullptr || d_out == nullptr))) return SPARTON_EINVAL;

@@ -1115,6 +1115,9 @@ struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
     at::AutoDispatchBelowADInplaceOrView below;
     c10::OptionalDeviceGuard guard(w.device());
     Tensor ids = ids_in.contiguous();
+    const int64_t N = ids.numel(), V = w.size(0), D = w.size(1);
+    TORCH_CHECK(N == 0 || V == 0 || sparton_embedding_workspace_bytes(N, V, D, dtype_code(w.scalar_type())) > 0,
+                "sparton: embedding: ", N, " ids of rows of ", D, " are too many for a gradient");
     ctx->save_for_backward({ids});
     ctx->saved_data["rows"] = w.size(0);
     ctx->saved_data["scale"] = scale;

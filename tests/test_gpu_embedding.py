@@ -207,3 +207,17 @@ def test_embedding_opcheck_and_compile(device):
     cf = torch.compile(f, backend="aot_eager", fullgraph=True)
     a, b = (torch.autograd.grad(c(leaf), leaf, dy)[0] for c in (cf, f))
     assert torch.equal(a, b)
+
+
+def test_embedding_of_more_ids_than_a_gradient_takes(device):
+    """2^29 narrow rows: looked up, and refused before the lookup where a gradient is asked for."""
+    say("2^29 ids")
+    N, D = 2 ** 29, 8
+    ids = torch.zeros(N, dtype=torch.int32, device=device)
+    places = torch.tensor([0, 1, 7, N // 2, N - 2, N - 1], device=device)
+    ids[places] = torch.tensor([3, 1, 2, 3, 1, 2], dtype=torch.int32, device=device)
+    w = torch.randn(4, D, device=device).bfloat16()
+    out = embedding(ids, w)
+    assert torch.equal(out[places], w[ids[places].long()]) and torch.equal(out[N // 3], w[0])
+    with pytest.raises(RuntimeError, match="too many for a gradient"):
+        embedding(ids, w.requires_grad_())

@@ -139,6 +139,16 @@ def test_embedding_checks_of_one():
     assert ebwd(ws=None) == -4 and ebwd(ws_bytes=64) == -4 and ebwd(ws=P + 16) == -2 and ebwd(V=0, dw=None) == 0
 
 
+def test_embedding_forward_has_its_own_limits():
+    """The join's workgroups, 256 threads for each 32 ids, bound the backward: 2^37 / 256 ids of narrow rows."""
+    N = 2 ** 29
+    assert ebwd(N=N, dy=None) == -3 and efwd(N=N, out=None) == -1  # accepted as far as the missing address
+    assert ebwd(N=N - 32, dy=None) == -1
+    size = _lib.load().sparton_embedding_workspace_bytes
+    assert size(N, 100, 64, 1) == 0 and size(N - 32, 100, 64, 1) > 0
+    assert efwd(N=2 ** 31 - 1025, D=64, out=None) == -1 and efwd(N=2 ** 31 - 1025, D=72, out=None) == -3
+
+
 def test_embedding_workspace():
     size = _lib.load().sparton_embedding_workspace_bytes
     assert size(0, 100, 64, 1) == 0 and size(8, 100, 0, 1) == 0 and size(8, 100, 64, 7) == 0
