@@ -199,8 +199,13 @@ template <typename T, bool KM, int R, int NW, bool PAIR> struct Copy {
     r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(from >> 32));
     r[2] = 0x80000000u;
     r[3] = 0x00020000u;
-    // The compiler would wait for a copy it knows of before any LDS read; these are waited for at the slab's end.
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(o), "s"(r));
+    // The compiler would wait for a copy it knows of before any LDS read; these are waited for at the slab's end. It
+    // allocates m0 to nothing and warns of it as a reserved register; named here, what it may write there itself right
+    // before an instruction of its own keeps clear of this.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(o), "s"(r) : "m0");
+#pragma clang diagnostic pop
   }
 };
 
