@@ -84,3 +84,31 @@ def test_a_compiled_backward(asked, device):
                                        "b_gate" in asked, "b_up" in asked, "x" in asked, "w_gate" in asked)
     here = ["x" in asked, "w_gate" in asked, "w_gate" in asked, "b_gate" in asked, "b_up" in asked]
     assert all(torch.equal(a, b) if h else a.numel() == 0 for a, b, h in zip(some, every, here))
+
+
+@pytest.mark.gpu
+def test_a_compiled_backbone(device):
+    """A gated encoder, switched whole, as one graph, with and without gradients; tolerances of test_backbone_gated.py."""
+    import copy
+    from transformers import EuroBertConfig, EuroBertModel
+    from sparton_amd.backbone import use_in_backbone
+    say("compiled backbone")
+    torch.manual_seed(0)
+    ref = EuroBertModel(EuroBertConfig(vocab_size=300, hidden_size=128, num_hidden_layers=2, num_attention_heads=4,
+                                       num_key_value_heads=2, intermediate_size=256, attn_implementation="eager",
+                                       pad_token_id=0)).to(device).eval()
+    ours = use_in_backbone(copy.deepcopy(ref), rms_norm=True, feed_forward=True, embedding=True)
+    ids = (torch.arange(12).reshape(2, 6) + 5).to(device)
+    mask = torch.ones_like(ids)
+    mask[1, 4:] = 0
+    on = mask.bool()
+    compiled = torch.compile(ours, backend="aot_eager", fullgraph=True)
+    want = ref(ids, mask).last_hidden_state[on]
+    got = compiled(ids, mask).last_hidden_state[on]
+    torch.testing.assert_close(got, want, rtol=1e-4, atol=1e-5)
+    a, b = (dict(zip(dict(m.named_parameters()), torch.autograd.grad(out.square().sum(), list(m.parameters()))))
+            for m, out in ((ref, want), (ours, got)))
+    floor = 1e-4 * max(g.abs().max().item() for g in a.values())
+    assert max((b[n] - g).abs().max().item() / max(g.abs().max().item(), floor) for n, g in a.items()) <= 1e-3
+    with torch.no_grad():
+        torch.testing.assert_close(compiled(ids, mask).last_hidden_state[on], want, rtol=1e-4, atol=1e-5)

@@ -305,3 +305,17 @@ def test_rms_norm_leaves_do_not_share_a_gradient(through, device):
     before = r.grad.clone()
     x.grad.mul_(2.0)
     assert torch.equal(r.grad, before)
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_rms_norm_changed_before_its_backward(residual, device):
+    """The backward reads h, or x where there is no residual: changed in place in between, autograd raises."""
+    say(f"changed in place, residual={residual}")
+    x, r = (torch.randn(4, 96, device=device, requires_grad=True) for _ in range(2))
+    w = torch.ones(96, device=device, requires_grad=True)
+    a = x * 1.0
+    y, h = rms_norm(a, w, 1e-6, r) if residual else (rms_norm(a, w), a)
+    with torch.no_grad():
+        h.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
