@@ -16,7 +16,6 @@ would wait for the device). Device tensors only, like the head.
 from __future__ import annotations
 
 import copy
-import math
 from typing import Optional
 
 import torch
@@ -25,6 +24,7 @@ from torch import Tensor, nn
 from . import _eager, _lib
 
 MAX_WIDTH = 1 << 20
+MAX_SCALE = torch.finfo(torch.float32).max
 ID_DTYPES = (torch.int64, torch.int32)
 _FLOAT_DTYPES = tuple(_lib.DTYPE_CODE)
 
@@ -37,8 +37,8 @@ def _check(ids: Tensor, table: Tensor, rows: int, scale: float, op: str) -> None
         raise TypeError(f"{op}: the table must be float32, bfloat16 or float16, got {table.dtype}")
     if not 1 <= table.shape[-1] <= MAX_WIDTH:
         raise ValueError(f"{op}: row width {table.shape[-1]} must be between 1 and {MAX_WIDTH}")
-    if not math.isfinite(scale):
-        raise ValueError(f"{op}: scale must be finite, got {scale}")
+    if not abs(scale) <= MAX_SCALE:
+        raise ValueError(f"{op}: scale must be finite in float32, got {scale}")
     if rows >= 2 ** 31 - 1 or ids.numel() > 2 ** 31 - 1025:
         raise ValueError(f"{op}: {ids.numel()} ids of {rows} rows are too many")
     if ids.device != table.device:

@@ -177,6 +177,15 @@ def test_embedding_refusals(args, kw, error):
         embedding(*args, **kw)
 
 
+@pytest.mark.parametrize("scale", [1e39, -1e39, 1e308])
+def test_an_embeddings_scale_past_fp32_is_refused(scale):
+    """The kernel's factor is fp32: it would be infinite."""
+    with pytest.raises(ValueError, match="finite"):
+        embedding(IDS, TABLE, scale=scale)
+    with pytest.raises(ValueError, match="finite"):
+        torch.ops.sparton.embedding_bwd(TABLE[:3], IDS, 5, scale, -1)
+
+
 def test_embedding_module_surface():
     m = nn.Embedding(10, 8, padding_idx=2)
     ours = SpartonEmbedding.of(m)
