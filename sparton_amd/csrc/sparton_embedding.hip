@@ -10,9 +10,10 @@
 // and the sorted list is cut into chunks of kChunk entries. A wave takes a chunk and 64 vectors of 16 bytes of the
 // row width, keeps the sum of the running id in fp32, and writes a table row where an id's entries end. The sum of
 // an id whose entries go on in a neighbouring chunk is left in fp32 in the workspace, and a second launch adds such
-// sums in order: an id that half of the batch has is then summed by as many waves as any other entries. Rows
-// without a token are zeroed by other waves of the first launch, so every row is written once and d table needs no
-// clearing. No atomics: results are bitwise reproducible.
+// sums in order: in the first launch an id that half of the batch has is summed by as many waves as any other entries.
+// The second has four waves for 256 columns of an id, whatever its chunks: all ids the same take 33 us in all at 8192 x 768
+// bf16 and 123 at 65536, random ones of 30522 34 and 80. Rows without a token are zeroed by other waves of the first launch,
+// so every row is written once and d table needs no clearing. No atomics: results are bitwise reproducible.
 //
 // The sort ranks each key among its wave's 64, then among 4 x 64 and 4 x 256, in a second launch among 32 x 1024 (all in
 // LDS), and in further ones among 16 x 32768, ... (memory): a key's rank is its own place in its list and, by binary

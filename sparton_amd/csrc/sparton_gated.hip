@@ -730,10 +730,11 @@ struct Split {
 //     16 bits   1.45                     1.3       0.9                      0.5
 //     fp32      7.3                      7.3       3.6                      1.95
 //     around    10                                 6
-// and a join writes and reads 6 MB a microsecond; what is split has to promise 3% more than that. bf16, dx of
-// 8192 x 768 x 2048: tiles of 256 80 us, in two parts 72; of 128 59, in two parts 80. dx of 5000 x 1024 x 3000: 113 and in
-// three parts 80; 94 and 93. dx of 300 x 768 x 2048: of 128 31, in four parts 14. dx of 8192 x 4096 x 11264: 1098 and 1485;
-// its dW, 1408 tiles of 256, 1218, the last 128 in two parts 1183.
+// `around` is silu's, without g and u: a tile of 256 x 256 with gelu takes about 14 around, and the forward of 8192 x 768 x
+// 2048 with both 73 us where this says 55. A join writes and reads 6 MB a microsecond; what is split has to promise 3% more
+// than that. bf16, dx of 8192 x 768 x 2048: tiles of 256 80 us, in two parts 72; of 128 59, in two parts 80. dx of 5000 x
+// 1024 x 3000: 113 and in three parts 80; 94 and 93. dx of 300 x 768 x 2048: of 128 31, in four parts 14. dx of 8192 x 4096
+// x 11264: 1098 and 1485; its dW, 1408 tiles of 256, 1218, the last 128 in two parts 1183.
 Split split_of(int64_t rows, int64_t cols, int64_t turns, int64_t slabs, int64_t es, bool may_split) {
   Split best = {};
   double least = -1.0;

@@ -14,7 +14,7 @@
 // Measured: 8192 x 4096 bf16 with a residual, forward 42 us (268 MB, 6.4 TB/s: more than a large copy's 5.1, as
 // repeated runs probably find part of it cached), backward 45 and 4 for the columns' sums (201 MB, 4.1 TB/s), forward in e4m3
 // 38. A few rows take 2.6, a launch. The backward of rows past 8192 spills 10 registers a lane in fp16 and 200 in
-// fp32.
+// fp32: 4096 x 16384 takes 86 us in bf16 (6.3 TB/s), 101 in fp16 and 508 in fp32 (2.1 TB/s).
 
 #include <math.h>
 

@@ -4,8 +4,8 @@
     d_weight[v] = scale * sum of d_out over the places where ids == v, in their order
 
 The first operator of a backbone (the reference runs torch's, training/model.py:88-139). The gradient
-sorts the tokens and adds each one's rows in order, so it is bitwise reproducible, and a token that half
-of the batch has (a padding or separator token) is summed by as many waves as any others.
+sorts the tokens and adds each one's rows in order, so it is bitwise reproducible; a token that half of
+the batch has (a padding or separator token) is summed in chunks by many waves, and the chunks by few.
 
     sparton::embedding_fwd(ids, weight, scale) -> out
     sparton::embedding_bwd(d_out, ids, rows, scale, padding) -> d_weight [rows, D]
