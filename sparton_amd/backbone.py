@@ -119,12 +119,13 @@ def _gated_block(self, *args, **kwargs) -> Tensor:
     return self.down_proj(h)
 
 
-def _pre_norm_layer(self, params, *args, **kwargs) -> Tensor:
-    """params: the names and defaults of what the layer's own forward takes. All but the hidden states go to the
-    attention by their names, as they do there."""
+def _pre_norm_layer(self, params, more, *args, **kwargs) -> Tensor:
+    """params: the names and defaults of what the layer's own forward takes; more: whether it takes other names too. All
+    but the hidden states go to the attention by their names, as they do there."""
     given = dict(zip((name for name, _ in params), args))
     call = {**dict(params), **given, **kwargs}
-    if len(args) > len(params) or given.keys() & kwargs.keys() or any(v is _REQUIRED for v in call.values()):
+    if (len(args) > len(params) or given.keys() & kwargs.keys() or any(v is _REQUIRED for v in call.values())
+            or not more and len(call) > len(params)):
         return type(self).forward(self, *args, **kwargs)  # which refuses the call
     hidden_states = call.pop(params[0][0])
     attended = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **call)[0]
@@ -175,13 +176,15 @@ def _is_gated_block(m: nn.Module) -> bool:
 
 
 def _params(m: nn.Module) -> Optional[tuple]:
-    """((name, default or _REQUIRED), ...) of what m's class's forward takes, or None if names alone do not say it."""
+    """((name, default or _REQUIRED), ...) of what m's class's forward takes, and whether it takes other names too; None
+    if names alone do not say it."""
     ps = list(inspect.signature(type(m).forward).parameters.values())[1:]
-    if ps and ps[-1].kind is ps[-1].VAR_KEYWORD:
+    more = bool(ps) and ps[-1].kind is ps[-1].VAR_KEYWORD
+    if more:
         ps.pop()
     if not ps or any(p.kind is not p.POSITIONAL_OR_KEYWORD for p in ps):
         return None
-    return tuple((p.name, p.default) for p in ps)
+    return tuple((p.name, p.default) for p in ps), more
 
 
 def _is_pre_norm_layer(m: nn.Module) -> bool:
@@ -190,11 +193,14 @@ def _is_pre_norm_layer(m: nn.Module) -> bool:
     names = ("input_layernorm", "self_attn", "post_attention_layernorm", "mlp")
     if set(m._modules) != set(names) or m._parameters or m._buffers:
         return False
-    params = _params(m)
-    if params is None:
+    found = _params(m)
+    if found is None:
         return False
+    params, more = found
     # flags keep their defaults; what may be None is something here, to be seen again in the attention
     others = {n: object() if default is None or default is _REQUIRED else default for n, default in params[1:]}
+    if more:
+        others["another_name"] = object()
     x = torch.linspace(-1, 1, 12, **PLAIN).view(1, 3, 4)
     children = dict(zip(names, (_Times(2.0), _Attended(others), _Times(5.0), _Times(7.0))))
     return computes(m, children, x, lambda: 36.0 * (x * 7.0), **others)  # x + 3 * 2 x, and 1 + 5 * 7 times that
@@ -224,7 +230,7 @@ def use_in_backbone(model: nn.Module, *, rms_norm: bool = False, feed_forward: b
             raise ValueError(f"{type(model).__name__} has no root-mean-square norm that the kernels compute")
         norms += found
         ours = {id(c) for _, _, c in children if isinstance(c, SpartonRMSNorm) or id(c) in made}
-        forwards += [(m, _pre_norm_layer, _params(m)) for m in modules if "forward" not in m.__dict__ and _is_pre_norm_layer(m)
+        forwards += [(m, _pre_norm_layer, *_params(m)) for m in modules if "forward" not in m.__dict__ and _is_pre_norm_layer(m)
                      and id(m.post_attention_layernorm) in ours]
     if feed_forward:
         blocks = [m for m in modules if _is_gated_block(m)]

@@ -289,13 +289,14 @@ class OtherCall(DropoutLayer):
         calls = dict(same=lambda: self.self_attn(hidden_states=x, mask=mask, flag=flag, **kwargs),
                      position=lambda: self.self_attn(x, mask=mask, flag=flag, **kwargs),
                      dropped=lambda: self.self_attn(hidden_states=x, mask=mask, **kwargs),
+                     rest_dropped=lambda: self.self_attn(hidden_states=x, mask=mask, flag=flag),
                      other=lambda: self.self_attn(hidden_states=x, mask=1, flag=flag, **kwargs),
                      more=lambda: self.self_attn(hidden_states=x, mask=mask, flag=flag, more=1, **kwargs))
         h = hidden_states + calls[self.kind]()[0]
         return h + self.mlp(self.post_attention_layernorm(h))
 
 
-@pytest.mark.parametrize("kind", ["same", "position", "dropped", "other", "more"])
+@pytest.mark.parametrize("kind", ["same", "position", "dropped", "rest_dropped", "other", "more"])
 def test_a_layer_that_calls_its_attention_in_another_way_keeps_its_forward(kind):
     assert _is_pre_norm_layer(OtherCall(kind)) == (kind == "same")
 
@@ -476,3 +477,33 @@ def test_modules_are_known_whatever_torchs_defaults_are(where, plain):  # noqa: 
     with torch.no_grad():
         same(ours(IDS).last_hidden_state, ref(IDS).last_hidden_state)
     assert plain == dict(rms=5, added=2, gated=2, embedding=1)
+
+
+def test_a_name_that_the_layer_does_not_take_is_refused(plain):  # noqa: F811
+    ref = decoder()
+
+    class Passing(nn.Module):
+        """The layer's steps, without other names."""
+
+        def __init__(self, layer):
+            super().__init__()
+            for n, c in layer.named_children():
+                setattr(self, n, c)
+
+        def forward(self, hidden_states, position_embeddings=None, attention_mask=None):
+            h = self.self_attn(hidden_states=self.input_layernorm(hidden_states), position_embeddings=position_embeddings,
+                               attention_mask=attention_mask)[0]
+            h = hidden_states + h
+            return h + self.mlp(self.post_attention_layernorm(h))
+
+    ref.layers[0] = Passing(ref.layers[0])
+    ours = use_in_backbone(copy.deepcopy(ref), **ALL)
+    x = torch.randn(1, 6, 128)
+    rope = ref.rotary_emb(x, torch.arange(6)[None])
+    with torch.no_grad():
+        want = ref.layers[0](x, rope, torch.full((6, 6), -1e30).triu(1)[None, None])
+        same(ours.layers[0](x, rope, torch.ones(1, 6)), want)
+    assert plain["added"] == 1
+    for m in (ref, ours):
+        with pytest.raises(TypeError):
+            m.layers[0](x, rope, use_cache=False)
